@@ -1,0 +1,135 @@
+// Device helpers shared by the feed-forward kernels: element types, matrix
+// instructions by type, the activations and their slopes.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/sdxl_hip/feed_forward.h"
+#include "sublayer_device.hpp"
+
+namespace sdxl_hip {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct FfType;
+template <>
+struct FfType<_Float16> {
+    static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) { return mfma32(a, b, c); }
+    // two values rounded to nearest even
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const f16x2 v{(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+    static __device__ __forceinline__ float lo(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[0]; }
+    static __device__ __forceinline__ float hi(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[1]; }
+    // four E4M3 codes, every one exact in the type
+    static __device__ __forceinline__ uint2 decode(uint32_t codes) { return e4m3x4_to_f16(codes); }
+};
+template <>
+struct FfType<__bf16> {
+    static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const bf16x2 v{(__bf16)a, (__bf16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+    static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
+    static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+    static __device__ __forceinline__ uint2 decode(uint32_t codes) {
+        const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false);
+        const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true);
+        return uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+    }
+};
+
+// ---- activations. Three families share the kernels, chosen once per
+// workgroup (the activation is uniform): z and relu; z sigmoid(z (c0 + c1
+// z^2)), which is silu, quick gelu and the tanh form of gelu (1 + tanh u = 2
+// sigmoid(2u)); and gelu. Infinite z takes the limit, NaN stays NaN.
+struct FfAct {
+    float lo, kink;  // z < lo becomes lo; slope 0 at z <= kink (NaN: nowhere)
+    float c0, c1;    // of the sigmoid's argument
+};
+
+enum FfFamily { kFamLinear = 0, kFamSigmoid = 1, kFamErf = 2 };
+
+__device__ __forceinline__ FfFamily ff_family(int32_t activation) {
+    return activation == SDXL_ACT_GELU ? kFamErf : activation <= SDXL_ACT_RELU ? kFamLinear : kFamSigmoid;
+}
+
+__device__ __forceinline__ FfAct ff_act(int32_t activation) {
+    FfAct a;
+    const bool relu = activation == SDXL_ACT_RELU;
+    a.lo = relu ? 0.0f : -__builtin_inff();
+    a.kink = relu ? 0.0f : __builtin_nanf("");
+    const float tanh_c = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+    a.c0 = activation == SDXL_ACT_QUICK_GELU ? 1.702f : activation == SDXL_ACT_GELU_TANH ? tanh_c : 1.0f;
+    a.c1 = activation == SDXL_ACT_GELU_TANH ? tanh_c * 0.044715f : 0.0f;
+    return a;
+}
+
+// Upper tail of the normal distribution, Q(x) = erfc(|x| / sqrt 2) / 2 =
+// e^(-x^2 / 2) R(|x|): R is a degree-6 polynomial without constant term in
+// t = 1 / (1 + 0.32 |x|), fitted to erfcx(|x| / sqrt 2) / 2 (reweighted least
+// squares towards the smallest relative error). Relative error 1.1e-5 for
+// every |x|, a fortieth of an fp16 half-step, so that gelu keeps its relative
+// precision in the negative tail; e is e^(-x^2 / 2), ax = min(|x|, 40).
+__device__ __forceinline__ float ff_tail(float x, float& e, float& ax) {
+    ax = __builtin_fminf(__builtin_fabsf(x), 40.0f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.32f, ax, 1.0f));
+    e = __builtin_amdgcn_exp2f(x * x * -0.7213475204444817f);
+    float r = __builtin_fmaf(t, -0.06677360087633133f, 0.13958339393138885f);
+    r = __builtin_fmaf(t, r, 0.04961634799838066f);
+    r = __builtin_fmaf(t, r, 0.12305037677288055f);
+    r = __builtin_fmaf(t, r, 0.12682831287384033f);
+    r = __builtin_fmaf(t, r, 0.12768970429897308f);
+    return e * (t * r);
+}
+
+template <FfFamily kFam>
+__device__ __forceinline__ float ff_value(const FfAct& a, float z) {
+    if constexpr (kFam == kFamLinear) {
+        return z < a.lo ? a.lo : z;
+    } else if constexpr (kFam == kFamSigmoid) {
+        const float z2 = __builtin_fminf(z * z, 1.0e30f);
+        const float s = __builtin_amdgcn_rcpf(
+            1.0f + __builtin_amdgcn_exp2f(z * __builtin_fmaf(a.c1, z2, a.c0) * -1.4426950408889634f));
+        return __builtin_fmaxf(z, -1.0e30f) * s;
+    } else {
+        float e, ax;
+        const float q = ff_tail(z, e, ax);
+        return __builtin_fmaf(-ax, q, __builtin_fmaxf(z, 0.0f));  // z Phi(z) = max(z, 0) - |z| Q(|z|)
+    }
+}
+
+// act(z) and act'(z)
+template <FfFamily kFam>
+__device__ __forceinline__ float ff_slope(const FfAct& a, float z, float& value) {
+    if constexpr (kFam == kFamLinear) {
+        value = z < a.lo ? a.lo : z;
+        return z <= a.kink ? 0.0f : 1.0f;
+    } else if constexpr (kFam == kFamSigmoid) {
+        const float z2 = __builtin_fminf(z * z, 1.0e30f);
+        const float s = __builtin_amdgcn_rcpf(
+            1.0f + __builtin_amdgcn_exp2f(z * __builtin_fmaf(a.c1, z2, a.c0) * -1.4426950408889634f));
+        value = __builtin_fmaxf(z, -1.0e30f) * s;
+        const float zc = __builtin_amdgcn_fmed3f(z, -1.0e30f, 1.0e30f);
+        return __builtin_fmaf((zc * s) * (1.0f - s), __builtin_fmaf(3.0f * a.c1, z2, a.c0), s);
+    } else {
+        float e, ax;
+        const float q = ff_tail(z, e, ax);
+        value = __builtin_fmaf(-ax, q, __builtin_fmaxf(z, 0.0f));
+        const float zc = __builtin_amdgcn_fmed3f(z, -40.0f, 40.0f);
+        return __builtin_fmaf(zc * 0.3989422804014327f, e, z > 0.0f ? 1.0f - q : q);
+    }
+}
+
+}  // namespace
+}  // namespace sdxl_hip

@@ -1,0 +1,44 @@
+// Internal launch interface of the feed-forward kernels (feed_forward.hip,
+// feed_forward_general.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace sdxl_hip {
+
+// What a product's epilogue makes of its sums.
+enum FfEpilogue : int32_t {
+    kFfLinear = 0,    // out = act(z) + residual
+    kFfGated = 1,     // out = value * act(gate)
+    kFfLinearDz = 2,  // out (dz) = dout * act'(z)
+    kFfGatedDz = 3,   // out (dz) = [dout * act(gate) | dout * value * act'(gate)]
+    kFfStore = 4      // out = the sums (dx, dw); optional row sums of the I operand (dbias)
+};
+
+// C[i, j] = sum_r I(i, r) J(j, r), then the epilogue. Operand X(i, r) is
+// element i * ld + r of its tensor, or r * ld + i where it is transposed. The
+// forward projections are I = x, J = w; dx is I = dz, J = w transposed; dw is
+// I = dz transposed, J = x transposed. J holds E4M3 codes if j_fp8.
+struct FfParams {
+    const void* ip;
+    const void* jp;
+    int64_t ld_i, ld_j;       // elements (E4M3: bytes)
+    const float* j_scale;     // nullable: fp32 scale of every J row
+    const void* bias;         // nullable, by J rows
+    const void* residual;     // nullable (kFfLinear)
+    const void* dout;         // kFfLinearDz, kFfGatedDz
+    void* out;                // nullable with row_sums
+    void* row_sums;           // nullable (kFfStore): sums over r of every I row
+    int64_t ld_res, ld_dout, ld_out;
+    int64_t rows, cols, depth;  // of C before the gating: gated products have 2 n J rows, cols = n
+    int64_t out_cols_padded;    // dz: columns up to here are written, zeros past the last one
+    int32_t activation;         // sdxl_activation
+    int32_t gate_first;
+};
+
+// The general kernel: any size, stride and alignment.
+hipError_t launch_ff_general(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool bf16,
+                             bool j_fp8, hipStream_t stream);
+
+}  // namespace sdxl_hip

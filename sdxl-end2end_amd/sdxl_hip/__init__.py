@@ -1,4 +1,4 @@
-"""Python harness binding of the sdxl_hip C ABI (include/sdxl_hip/attention.h, sublayer.h).
+"""Python harness binding of the sdxl_hip C ABI (include/sdxl_hip/attention.h, sublayer.h, feed_forward.h).
 
 This is a thin ctypes layer used by the test suite, the smoke check and bench.py.
 Device memory and streams come from PyTorch (plumbing only); every computation
@@ -18,6 +18,8 @@ LIB_PATH = os.environ.get("SDXL_HIP_LIB") or os.path.join(PKG_ROOT, "lib", "libs
 OK, INVALID_ARGUMENT, INVALID_SHAPE, UNSUPPORTED, LAUNCH_FAILED, DEVICE_ERROR = range(6)
 # sdxl_dtype
 F16, BF16, F32, E4M3 = 0, 1, 2, 3
+# sdxl_activation
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "quick_gelu": 4, "silu": 5}
 # sdxl_attn_backend (values of the reference's AttentionBackend, runtime.hpp:53-58)
 AUTO, CUDNN_SDPA, FLASH_SM80, WARP_ONLINE = 0, 1, 2, 3
 
@@ -43,6 +45,17 @@ EXPORTED_SYMBOLS = (
     "sdxl_attn_sublayer",
     "sdxl_cross_attn_sublayer_workspace_bytes",
     "sdxl_cross_attn_sublayer",
+)
+# of feed_forward.h
+FEED_FORWARD_SYMBOLS = (
+    "sdxl_linear_act",
+    "sdxl_gated_linear",
+    "sdxl_linear_act_backward_workspace_bytes",
+    "sdxl_gated_linear_backward_workspace_bytes",
+    "sdxl_linear_act_backward",
+    "sdxl_gated_linear_backward",
+    "sdxl_ff_sublayer_workspace_bytes",
+    "sdxl_ff_sublayer",
 )
 
 
@@ -91,12 +104,31 @@ class CrossSublayerDesc(ctypes.Structure):
                 ("ln_eps", ctypes.c_float), ("q_activations", ctypes.c_int32)]
 
 
+class FfDesc(ctypes.Structure):
+    """Mirror of struct sdxl_ff_desc."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("m", "n", "k", "x_row_stride", "w_row_stride", "out_row_stride",
+                                              "residual_row_stride", "dx_row_stride", "dw_row_stride")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "w_dtype", "activation", "gate_first", "reserved")]
+
+
+class FfSublayerDesc(ctypes.Structure):
+    """Mirror of struct sdxl_ff_sublayer_desc."""
+
+    _fields_ = [("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("inner", ctypes.c_int64),
+                ("w_in_dtype", ctypes.c_int32), ("w_out_dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+                ("gate_first", ctypes.c_int32), ("ln_eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
 # The descriptors as packed bytes (native alignment, as the structures above) and prototypes that
 # take them: on the call path one struct.pack costs a third of filling a ctypes structure.
 _ATTN_DESC = struct.Struct("9q4if4x")
 _LINEAR_DESC = struct.Struct("7q2i")
 _SUBLAYER_DESC = struct.Struct("3q2if2i4x")
 _CROSS_SUBLAYER_DESC = struct.Struct("4q2ifi")
+_FF_DESC = struct.Struct("9q5i4x")
+_FF_SUBLAYER_DESC = struct.Struct("3q4ifi")
+assert _FF_DESC.size == ctypes.sizeof(FfDesc) and _FF_SUBLAYER_DESC.size == ctypes.sizeof(FfSublayerDesc)
 assert _ATTN_DESC.size == ctypes.sizeof(AttnDesc) and _LINEAR_DESC.size == ctypes.sizeof(LinearDesc)
 assert _SUBLAYER_DESC.size == ctypes.sizeof(SublayerDesc) and _CROSS_SUBLAYER_DESC.size == ctypes.sizeof(CrossSublayerDesc)
 
@@ -167,10 +199,33 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.sdxl_cross_attn_sublayer.restype = ctypes.c_int
     lib.sdxl_cross_attn_sublayer.argtypes = [ctypes.POINTER(CrossSublayerDesc), vp, vp, vp, vp, vp, vp, i64, vp, vp,
                                              vp, vp, ctypes.c_size_t, vp]
-    for name in ("sdxl_attn_fwd", "sdxl_linear", "sdxl_attn_sublayer", "sdxl_cross_attn_sublayer"):
+    lib.sdxl_linear_act.restype = ctypes.c_int
+    lib.sdxl_linear_act.argtypes = [ctypes.POINTER(FfDesc), vp, vp, vp, vp, vp, vp, vp]
+    lib.sdxl_gated_linear.restype = ctypes.c_int
+    lib.sdxl_gated_linear.argtypes = [ctypes.POINTER(FfDesc), vp, vp, vp, vp, vp, vp]
+    for name in ("sdxl_linear_act_backward", "sdxl_gated_linear_backward"):
+        fn = getattr(lib, name + "_workspace_bytes")
+        fn.restype = ctypes.c_size_t
+        fn.argtypes = [ctypes.POINTER(FfDesc)]
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(FfDesc), vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.sdxl_ff_sublayer_workspace_bytes.restype = ctypes.c_size_t
+    lib.sdxl_ff_sublayer_workspace_bytes.argtypes = [ctypes.POINTER(FfSublayerDesc)]
+    lib.sdxl_ff_sublayer.restype = ctypes.c_int
+    lib.sdxl_ff_sublayer.argtypes = [ctypes.POINTER(FfSublayerDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                     ctypes.c_size_t, vp]
+    for name in ("sdxl_attn_fwd", "sdxl_linear", "sdxl_attn_sublayer", "sdxl_cross_attn_sublayer", "sdxl_linear_act",
+                 "sdxl_gated_linear", "sdxl_linear_act_backward", "sdxl_gated_linear_backward", "sdxl_ff_sublayer"):
         fn = lib[name]  # a function object of its own, with its own prototype
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_char_p] + getattr(lib, name).argtypes[1:]
+        setattr(lib, "packed_" + name, fn)
+    for name in ("sdxl_linear_act_backward_workspace_bytes", "sdxl_gated_linear_backward_workspace_bytes",
+                 "sdxl_ff_sublayer_workspace_bytes"):
+        fn = lib[name]
+        fn.restype = ctypes.c_size_t
+        fn.argtypes = [ctypes.c_char_p]
         setattr(lib, "packed_" + name, fn)
     _LIB = lib
     return lib
@@ -469,6 +524,216 @@ def cross_attn_sublayer(x, ln_gamma, ln_beta, w_q, w_q_scale, kv, w_out, b_out, 
         desc, x.data_ptr(), _ptr(ln_gamma), _ptr(ln_beta), _ptr(w_q), _ptr(w_q_scale), kv.data_ptr(),
         kv.stride(1), _ptr(w_out), _ptr(b_out), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
         t.raw_stream(index) if index >= 0 else None))
+    return out
+
+
+# ---------------------------------------------------------------- feed-forward
+# (include/sdxl_hip/feed_forward.h; reference src/cuda/unet.cpp:98-149)
+
+class _Guard:
+    """Makes a tensor's device current for a call where it is not (the library launches on the current one)."""
+
+    def __init__(self, index):
+        import torch
+        self.device = torch.cuda.device(index) if index >= 0 and index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.device is not None:
+            self.device.__enter__()
+
+    def __exit__(self, *exc):
+        if self.device is not None:
+            self.device.__exit__(*exc)
+
+
+def _ff_rows(name, what, t, rows, cols, like) -> int:
+    """The row stride of a 2-D tensor (0 where there is at most one row), after its checks."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise SdxlError(INVALID_SHAPE, f"{name}: {what} must be [{rows}, {cols}]")
+    if t.device != like.device:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: {what} must be on {like.device}")
+    row, col = t.stride()
+    if cols > 1 and col != 1:
+        raise SdxlError(INVALID_SHAPE, f"{name}: {what} must have unit column stride")
+    if rows <= 1 or cols == 0:
+        return 0
+    if row < cols:
+        raise SdxlError(INVALID_SHAPE, f"{name}: row stride smaller than the row")
+    return row
+
+
+def _ff_vector(name, what, t, size, dtype, like) -> int:
+    if t is None:
+        return 0
+    if t.dim() != 1 or t.shape[0] != size or t.dtype != dtype or (size > 1 and t.stride(0) != 1):
+        raise SdxlError(INVALID_SHAPE, f"{name}: {what} must be contiguous {dtype} [{size}]")
+    if t.device != like.device:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: {what} must be on {like.device}")
+    return t.data_ptr()
+
+
+def _ff_call(name, x, w, activation, gated):
+    """(torch lookups, M, N, K, dtype code, weight dtype code, activation code) after the common checks."""
+    t = _Torch.loaded or _Torch()
+    code = t.codes.get(x.dtype, F32)
+    if code == F32:
+        raise SdxlError(INVALID_SHAPE, f"{name}: tensors must be fp16 or bf16")
+    if w.dtype != x.dtype and w.dtype != t.uint8:
+        raise SdxlError(INVALID_SHAPE, f"{name}: weights must have the tensors' type or be E4M3")
+    if activation not in ACTIVATIONS:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: activation must be one of {', '.join(ACTIVATIONS)}")
+    if x.dim() != 2 or w.dim() != 2 or (gated and w.shape[0] % 2 != 0):
+        raise SdxlError(INVALID_SHAPE, f"{name}: x must be [M, K] and w [{'2N' if gated else 'N'}, K]")
+    features = w.shape[0]
+    return (t, x.shape[0], features // 2 if gated else features, x.shape[1], code,
+            E4M3 if w.dtype == t.uint8 else code, ACTIVATIONS[activation])
+
+
+def _ff_forward(name, gated, x, w, bias, w_scale, activation, gate_first, residual, out):
+    t, M, N, K, code, w_code, act = _ff_call(name, x, w, activation, gated)
+    features = 2 * N if gated else N
+    ldx = _ff_rows(name, "x", x, M, K, x)
+    ldw = _ff_rows(name, "w", w, features, K, x)
+    import torch
+    scale_ptr = _ff_vector(name, "w_scale", w_scale, features, torch.float32, x)
+    bias_ptr = _ff_vector(name, "bias", bias, features, x.dtype, x)
+    ldr = 0
+    if residual is not None:
+        if residual.dtype != x.dtype:
+            raise SdxlError(INVALID_SHAPE, f"{name}: residual must have x's type")
+        ldr = _ff_rows(name, "residual", residual, M, N, x)
+    ldo = 0
+    if out is None:
+        out = x.new_empty((M, N))
+    else:
+        if out.dtype != x.dtype:
+            raise SdxlError(INVALID_SHAPE, f"{name}: out must have x's type")
+        ldo = _ff_rows(name, "out", out, M, N, x)
+    desc = _FF_DESC.pack(M, N, K, ldx, ldw, ldo, ldr, 0, 0, code, w_code, act, 1 if gate_first else 0, 0)
+    index = x.get_device()
+    lib = load()
+    with _Guard(index):
+        stream = t.raw_stream(index) if index >= 0 else None
+        if gated:
+            status = lib.packed_sdxl_gated_linear(desc, x.data_ptr(), w.data_ptr(), scale_ptr, bias_ptr,
+                                                  out.data_ptr(), stream)
+        else:
+            status = lib.packed_sdxl_linear_act(desc, x.data_ptr(), w.data_ptr(), scale_ptr, bias_ptr,
+                                                residual.data_ptr() if residual is not None else None,
+                                                out.data_ptr(), stream)
+    _check_packed(status)
+    return out
+
+
+def gated_linear(x, w, bias=None, w_scale=None, activation: str = "gelu", gate_first: bool = False, out=None):
+    """value * act(gate) with [value | gate] = x . w^T + bias as one kernel (sdxl_gated_linear; the
+    reference's GEGLU projection, src/cuda/unet.cpp:98-149): x [M, K] fp16 or bf16, w [2N, K] of its
+    type or uint8 E4M3 codes (with w_scale [2N] fp32), bias [2N]; gate_first: [gate | value]. Rows may be
+    strided. Returns [M, N]."""
+    return _ff_forward("sdxl_gated_linear", True, x, w, bias, w_scale, activation, gate_first, None, out)
+
+
+def linear_act(x, w, bias=None, residual=None, w_scale=None, activation: str = "none", out=None):
+    """act(x . w^T + bias) + residual (sdxl_linear_act): x [M, K] fp16 or bf16, w [N, K] of its type or
+    uint8 E4M3 codes (with w_scale [N] fp32), bias [N], residual [M, N] (may be out). Returns [M, N]."""
+    return _ff_forward("sdxl_linear_act", False, x, w, bias, w_scale, activation, False, residual, out)
+
+
+def _ff_backward(name, gated, dout, x, w, bias, activation, gate_first, need_dx, need_dw, need_dbias, workspace):
+    t, M, N, K, code, w_code, act = _ff_call(name, x, w, activation, gated)
+    features = 2 * N if gated else N
+    if dout.dtype != x.dtype:
+        raise SdxlError(INVALID_SHAPE, f"{name}: dout must have x's type")
+    ldx = _ff_rows(name, "x", x, M, K, x)
+    ldw = _ff_rows(name, "w", w, features, K, x)
+    ldo = _ff_rows(name, "dout", dout, M, N, x)
+    bias_ptr = _ff_vector(name, "bias", bias, features, x.dtype, x)
+    dx = x.new_empty((M, K)) if need_dx else None
+    dw = x.new_empty((features, K)) if need_dw else None
+    dbias = x.new_empty((features,)) if (bias is not None if need_dbias is None else need_dbias) else None
+    desc = _FF_DESC.pack(M, N, K, ldx, ldw, ldo, 0, 0, 0, code, w_code, act, 1 if gate_first else 0, 0)
+    index = x.get_device()
+    lib = load()
+    with _Guard(index):
+        if workspace is None:
+            size = (lib.packed_sdxl_gated_linear_backward_workspace_bytes if gated else
+                    lib.packed_sdxl_linear_act_backward_workspace_bytes)(desc)
+            workspace = t.empty((size,), dtype=t.uint8, device=x.device)
+        elif workspace.device != x.device:
+            raise SdxlError(INVALID_ARGUMENT, f"{name}: workspace must be on {x.device}")
+        fn = lib.packed_sdxl_gated_linear_backward if gated else lib.packed_sdxl_linear_act_backward
+        status = fn(desc, dout.data_ptr(), x.data_ptr(), w.data_ptr(), bias_ptr, _ptr(dx), _ptr(dw), _ptr(dbias),
+                    workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                    t.raw_stream(index) if index >= 0 else None)
+    _check_packed(status)
+    return dx, dw, dbias
+
+
+def gated_linear_backward(dout, x, w, bias=None, activation: str = "gelu", gate_first: bool = False,
+                          need_dx: bool = True, need_dw: bool = True, need_dbias=None, workspace=None):
+    """Gradients (dx [M, K], dw [2N, K], dbias [2N]) of gated_linear for dout [M, N]; value and gate are
+    formed again from x, w and bias. What is not needed is None (dbias by default without a bias).
+    workspace: a contiguous tensor of ff_backward_workspace_bytes, else one is allocated."""
+    return _ff_backward("sdxl_gated_linear_backward", True, dout, x, w, bias, activation, gate_first, need_dx, need_dw,
+                        need_dbias, workspace)
+
+
+def linear_act_backward(dout, x, w, bias=None, activation: str = "none", need_dx: bool = True, need_dw: bool = True,
+                        need_dbias=None, workspace=None):
+    """Gradients (dx [M, K], dw [N, K], dbias [N]) of linear_act for dout [M, N]; the residual's gradient
+    is dout. Arguments as gated_linear_backward."""
+    return _ff_backward("sdxl_linear_act_backward", False, dout, x, w, bias, activation, False, need_dx, need_dw,
+                        need_dbias, workspace)
+
+
+def ff_backward_workspace_bytes(M: int, N: int, K: int, gated: bool, activation: str, dtype: int = F16) -> int:
+    """Workspace of gated_linear_backward / linear_act_backward."""
+    desc = FfDesc(m=M, n=N, k=K, dtype=dtype, w_dtype=dtype, activation=ACTIVATIONS[activation])
+    lib = load()
+    return int((lib.sdxl_gated_linear_backward_workspace_bytes if gated else
+                lib.sdxl_linear_act_backward_workspace_bytes)(ctypes.byref(desc)))
+
+
+def ff_sublayer(x, ln_gamma, ln_beta, w_in, w_in_scale, b_in, w_out, w_out_scale, b_out, activation: str = "gelu",
+                gate_first: bool = False, out=None, workspace=None, eps: float = 0.0):
+    """x + gated_linear(LN(x), w_in, b_in) . w_out^T + b_out for hidden x [B, S, W] fp16, the feed-forward
+    half of the reference's transformer block (src/cuda/unet.cpp:98-149) after attn_sublayer and
+    cross_attn_sublayer: w_in [2I, W], w_out [W, I], each fp16 or uint8 E4M3 with its scales, all contiguous."""
+    import torch
+    t = _Torch.loaded or _Torch()
+    name = "sdxl_ff_sublayer"
+    if x.dim() != 3 or x.dtype != t.f16:
+        raise SdxlError(INVALID_SHAPE, f"{name}: hidden must be [B, S, W] fp16")
+    if activation not in ACTIVATIONS:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: activation must be one of {', '.join(ACTIVATIONS)}")
+    B, S, W = x.shape
+    inner = w_in.shape[0] // 2
+    if out is None:
+        out = t.empty_like(x)
+    for what, tensor, shape, types in (("hidden", x, (B, S, W), (t.f16,)), ("out", out, (B, S, W), (t.f16,)),
+                                       ("w_in", w_in, (2 * inner, W), (t.f16, t.uint8)),
+                                       ("w_out", w_out, (W, inner), (t.f16, t.uint8)),
+                                       ("norm weight", ln_gamma, (W,), (t.f16,)), ("norm bias", ln_beta, (W,), (t.f16,)),
+                                       ("b_in", b_in, (2 * inner,), (t.f16,)), ("b_out", b_out, (W,), (t.f16,)),
+                                       ("w_in_scale", w_in_scale, (2 * inner,), (torch.float32,)),
+                                       ("w_out_scale", w_out_scale, (W,), (torch.float32,))):
+        if tensor is not None and (tensor.shape != shape or tensor.dtype not in types or not tensor.is_contiguous()
+                                   or tensor.device != x.device):
+            raise SdxlError(INVALID_SHAPE, f"{name}: {what} must be contiguous {list(shape)} on {x.device}")
+    desc = _FF_SUBLAYER_DESC.pack(B * S, W, inner, E4M3 if w_in.dtype == t.uint8 else F16,
+                                  E4M3 if w_out.dtype == t.uint8 else F16, ACTIVATIONS[activation],
+                                  1 if gate_first else 0, _f32(eps), 0)
+    index = x.get_device()
+    lib = load()
+    with _Guard(index):
+        if workspace is None:
+            workspace = t.empty((lib.packed_sdxl_ff_sublayer_workspace_bytes(desc),), dtype=t.uint8, device=x.device)
+        status = lib.packed_sdxl_ff_sublayer(desc, x.data_ptr(), _ptr(ln_gamma), _ptr(ln_beta), _ptr(w_in),
+                                             _ptr(w_in_scale), _ptr(b_in), _ptr(w_out), _ptr(w_out_scale), _ptr(b_out),
+                                             out.data_ptr(), workspace.data_ptr(),
+                                             workspace.numel() * workspace.element_size(),
+                                             t.raw_stream(index) if index >= 0 else None)
+    _check_packed(status)
     return out
 
 
