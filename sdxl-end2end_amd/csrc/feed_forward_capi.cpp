@@ -74,6 +74,8 @@ sdxl_status resolve(const sdxl_ff_desc* d, bool gated, bool backward, const char
 
 sdxl_status product(const FfParams& p, sdxl_hip::FfEpilogue epilogue, bool it, bool jt, const Call& c, bool w_fp8,
                     hipStream_t stream, const char* name) {
+    if (sdxl_hip::ff_tiled_supported(p, epilogue, it, jt, w_fp8))
+        return launch_status(sdxl_hip::launch_ff_tiled(p, epilogue, it, c.bf16, w_fp8, stream), name);
     return launch_status(sdxl_hip::launch_ff_general(p, epilogue, it, jt, c.bf16, w_fp8, stream), name);
 }
 
@@ -177,6 +179,7 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
         p.out = want_dw ? dw : nullptr;
         p.ld_out = c.lddw;
         p.row_sums = want_db ? dbias : nullptr;
+        if (dz_needed) p.i_row = lddz;
         st = product(p, sdxl_hip::kFfStore, true, true, c, false, stream, name);
         if (st != SDXL_STATUS_OK) return st;
     }
@@ -189,6 +192,7 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
         p.rows = c.m;
         p.cols = c.k;
         p.depth = c.features;
+        if (dz_needed) p.i_row = lddz;
         p.out = dx;
         p.ld_out = c.lddx;
         st = product(p, sdxl_hip::kFfStore, false, true, c, false, stream, name);

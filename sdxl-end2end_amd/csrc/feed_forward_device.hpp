@@ -27,6 +27,10 @@ struct FfType<_Float16> {
     }
     static __device__ __forceinline__ float lo(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[0]; }
     static __device__ __forceinline__ float hi(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[1]; }
+    // the sum of two packed values and s
+    static __device__ __forceinline__ float dot_ones(uint32_t v, float s) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, v), f16x2{(_Float16)1.0f, (_Float16)1.0f}, s, false);
+    }
     // four E4M3 codes, every one exact in the type
     static __device__ __forceinline__ uint2 decode(uint32_t codes) { return e4m3x4_to_f16(codes); }
 };
@@ -42,6 +46,9 @@ struct FfType<__bf16> {
     }
     static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
     static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+    static __device__ __forceinline__ float dot_ones(uint32_t v, float s) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, s, false);
+    }
     static __device__ __forceinline__ uint2 decode(uint32_t codes) {
         const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false);
         const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true);

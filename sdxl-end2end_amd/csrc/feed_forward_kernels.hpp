@@ -32,13 +32,23 @@ struct FfParams {
     void* row_sums;           // nullable (kFfStore): sums over r of every I row
     int64_t ld_res, ld_dout, ld_out;
     int64_t rows, cols, depth;  // of C before the gating: gated products have 2 n J rows, cols = n
+    // I's row as it may be read, where its columns are padded with zeros up to a multiple of 8 (dz): the row's
+    // depth, or its columns where I is transposed; 0: as given
+    int64_t i_row;
     int64_t out_cols_padded;    // dz: columns up to here are written, zeros past the last one
     int32_t activation;         // sdxl_activation
     int32_t gate_first;
+    // filled by the tiled kernel's launcher: wide epilogue accesses, tiles of C, row blocks per task group
+    int32_t vec, i_blocks, j_blocks, group_i;
 };
 
 // The general kernel: any size, stride and alignment.
 hipError_t launch_ff_general(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool bf16,
                              bool j_fp8, hipStream_t stream);
+
+// The tiled kernel: operands whose rows 16-byte accesses divide.
+bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);
+hipError_t launch_ff_tiled(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
+                           hipStream_t stream);
 
 }  // namespace sdxl_hip
