@@ -1,0 +1,679 @@
+// The tiled product kernel of the feed-forward operators
+// (include/sdxl_hip/feed_forward.h), for gfx950 (MI355X, CDNA4).
+//
+// C[i, j] = sum_r I(i, r) J(j, r), with the epilogue of FfEpilogue on the fp32
+// sums: the projections (I = x, J = w), dx (I = dz, J = w by columns) and dw
+// (I = dz by columns, J = x by columns). A workgroup of kWI x kWJ waves owns
+// (32 kMI kWI) x (32 kMJ kWJ) tiles of C, each wave a (32 kMI) x (32 kMJ) block
+// as kMI x kMJ v_mfma_f32_32x32x16 tiles with the J rows as the A operand, so
+// that a lane ends up with 4 consecutive columns of one row of C.
+//
+// Depth goes in stages of 64 through two LDS buffers, filled by
+// buffer_load_dwordx4 ... lds (1 KiB per wave and instruction, no registers).
+// Rows with contiguous depth lie as 128-byte rows whose 16-byte chunks are
+// XOR-swizzled (conflict-free 16-byte operand reads); operands taken by columns
+// lie as panels of 64 columns x 64 depth rows in the same layout and reach the
+// registers through the transposing ds_read_b64_tr_b16. E4M3 rows stay as codes
+// (64-byte rows) and are decoded on the way to the matrix cores. What lies
+// outside an operand (rows past the end, depth past the end) is read as zero:
+// the descriptor's size cuts the rows off, and the last stage's chunks past the
+// depth get an offset beyond it.
+//
+// Schedule: the operands of depth step k + 1 are read while step k's matrix
+// instructions run (two register sets), across the stage boundary too: the
+// barrier that frees a buffer stands before the stage's last step, whose
+// operands are in registers by then, so that its matrix instructions cover the
+// barrier, the next stage's first reads and the issue of the transfers.
+//
+// Gated products put 16 value rows and the 16 gate rows of the same columns
+// into every 32-row J tile: a lane holds value and gate of its columns and the
+// product needs no exchange.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <utility>
+
+#include "feed_forward_device.hpp"
+#include "feed_forward_kernels.hpp"
+
+namespace sdxl_hip {
+namespace {
+
+typedef __attribute__((address_space(3))) i16x8 lds_op;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+typedef __attribute__((address_space(3))) float lds_float;
+
+// An operand's window as a buffer descriptor (raw, byte offsets): reads at or
+// past `size` return zero.
+struct Window {
+    const char* base;
+    uint32_t size;
+};
+
+__device__ __forceinline__ u32x4 window_rsrc(Window w) {
+    const uint64_t b = (uint64_t)(uintptr_t)w.base;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32) & 0xFFFFu),
+                 (uint32_t)__builtin_amdgcn_readfirstlane(w.size), 0x00020000u};
+}
+
+// 1-KiB transfer: lane l's 16 bytes at offset voff of the window go to lds +
+// 16 l. Ordered by explicit waits and barriers, as the attention kernel's.
+__device__ __forceinline__ void window_to_lds(u32x4 rsrc, uint32_t voff, uint32_t lds) {
+    lds = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile(
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %0, %1, 0 offen lds"
+        :
+        : "v"(voff), "s"(rsrc), "{m0}"(lds));
+}
+
+constexpr uint32_t kOutside = 0x80000000u;  // past every window (their sizes stay below 2^31)
+
+__device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
+
+// Exchanges the halves so that lanes 0-31 hold 8 consecutive columns made of
+// both halves' a, lanes 32-63 those of b (a, b: two values each, packed).
+__device__ __forceinline__ void join_halves(uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
+// A tile: kWI x kWJ waves of (32 kMI) x (32 kMJ) blocks, kWK such groups of
+// waves that share every stage's depth, kRing stages in LDS.
+template <int kWI_, int kWJ_, int kWK_, int kMI_, int kMJ_, int kRing_, int kSpread_ = 1>
+struct FfTile {
+    static constexpr int kWI = kWI_, kWJ = kWJ_, kWK = kWK_, kMI = kMI_, kMJ = kMJ_, kRing = kRing_, kSpread = kSpread_;
+    static constexpr int kWaves = kWI * kWJ * kWK, kBI = 32 * kMI * kWI, kBJ = 32 * kMJ * kWJ;
+    static constexpr int stage_bytes(bool j_fp8) { return kBI * 128 + kBJ * (j_fp8 ? 64 : 128); }
+    // workgroups that one CU's LDS and registers (512 per lane and SIMD) hold
+    static constexpr int waves_per_simd(bool j_fp8) {
+        const int by_lds = kWaves / 4 * (160 * 1024 / (kRing * stage_bytes(j_fp8)));
+        const int by_regs = kMI * kMJ <= 4 ? 4 : kMI * kMJ <= 10 ? 2 : 1;
+        return by_lds < by_regs ? by_lds : by_regs;
+    }
+};
+
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
+__global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) void ff_tile_kernel(FfParams p) {
+    constexpr int kWI = Tile::kWI, kWJ = Tile::kWJ, kWK = Tile::kWK, kMI = Tile::kMI, kMJ = Tile::kMJ, kRing = Tile::kRing;
+    using F = FfType<T>;
+    constexpr bool kGated = kEpi == kFfGated || kEpi == kFfGatedDz;
+    constexpr int kWaves = Tile::kWaves, kBI = Tile::kBI, kBJ = Tile::kBJ;
+    constexpr int kCols = kGated ? kBJ / 2 : kBJ;  // columns of C per tile
+    constexpr int kSteps = 4 / kWK;                // depth steps (of 16) per wave and stage
+    constexpr int kSpread = Tile::kSpread;         // steps that a stage's requests are spread over
+    static_assert(kSpread <= kSteps, "steps");
+    constexpr int kIBytes = kBI * 128, kStage = Tile::stage_bytes(kJFp8), kJBytes = kStage - kIBytes;
+    constexpr int kIXfers = kIBytes / 1024, kJXfers = kJBytes / 1024;
+    constexpr int kIX = (kIXfers + kWaves - 1) / kWaves, kXfers = kIX + (kJXfers + kWaves - 1) / kWaves;
+    static_assert(kWaves % 4 == 0, "the waves' transfers keep their parity and their half of the gating");
+    // waves below kMore have kXfers transfers a stage, the others one less
+    constexpr int kMore = kIXfers % kWaves + kJXfers % kWaves;
+    static_assert(kIXfers % kWaves == 0 || kJXfers % kWaves == 0, "one operand's transfers come out even");
+    static_assert((kRing - 1) * kXfers < 64, "vmcnt range");
+    static_assert(kWK == 1 || (kWK == 2 && !kJFp8), "depth shares");
+    static_assert(!kGated || (!kIT && !kJT), "gated products are projections");
+    static_assert(!kJFp8 || !kJT, "E4M3: by rows");
+    // sums of the other depth shares, one round of tiles at a time
+    constexpr int kExchange = kWK > 1 ? kWI * kWJ * kWK * (kWK - 1) * 4096 : 0;
+    constexpr int kSmem = kRing * kStage > kExchange ? kRing * kStage : kExchange;
+    static_assert(kSmem <= 160 * 1024, "LDS of one CU");
+    __shared__ __attribute__((aligned(1024))) char smem[kSmem];
+
+    const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave % kWI, wj = wave / kWI % kWJ, wk = kWK > 1 ? wave / (kWI * kWJ) : 0;
+    const int64_t value_row = p.gate_first ? p.cols : 0, gate_row = p.gate_first ? 0 : p.cols;
+    const int n_stages = (int)((p.depth + 63) / 64);
+    const int64_t ldi_b = p.ld_i * 2, ldj_b = p.ld_j * (kJFp8 ? 1 : 2);
+
+    // ---- task: each XCD takes one contiguous range of them, in groups of
+    // group_i row blocks (rows fastest, then columns), so that its workgroups
+    // share I rows and J rows in its L2
+    int64_t i0, j0;
+    {
+        const int n = p.i_blocks * p.j_blocks;
+        const int id = blockIdx.x, xcd = id & 7, slot = id >> 3;
+        const int per = n >> 3, extra = n & 7;
+        const int task = xcd * per + (xcd < extra ? xcd : extra) + slot;
+        const int in_group = p.group_i * p.j_blocks;
+        const int first = (task / in_group) * p.group_i;
+        const int rows = min(p.i_blocks - first, p.group_i);
+        const int r = task % in_group;
+        i0 = (int64_t)(first + r % rows) * kBI;
+        j0 = (int64_t)(r / rows) * kCols;
+    }
+
+    // ---- transfers. Transfer n of an operand is 8 rows (E4M3: 16) of 128 (64)
+    // bytes of its region; wave w takes n = w, w + kWaves, ..: the swizzle and,
+    // for gated J tiles, value or gate follow from the wave.
+    const int row8 = lane >> 3, chunk8 = (lane & 7) ^ swz(8 * (wave & 1) + row8);
+    const int row16 = lane >> 2, chunk16 = (lane & 3) ^ ((row16 >> 2) & 3);
+    Window iw, jw;
+    uint32_t i_lane, j_lane;  // the lane's offset in a transfer
+    if constexpr (kIT) {
+        iw.base = (const char*)p.ip + i0 * 2;
+        i_lane = (uint32_t)(row8 * ldi_b) + chunk8 * 16;
+    } else {
+        iw.base = (const char*)p.ip + i0 * ldi_b;
+        i_lane = (uint32_t)(row8 * ldi_b) + chunk8 * 16;
+    }
+    const int64_t j_first = kGated ? j0 + ((kJFp8 ? wave & 1 : wave & 2) ? gate_row : value_row) : j0;
+    if constexpr (kJT) jw.base = (const char*)p.jp + j0 * 2;
+    else jw.base = (const char*)p.jp + j_first * ldj_b;
+    j_lane = kJFp8 ? (uint32_t)(row16 * ldj_b) + chunk16 * 16 : (uint32_t)(row8 * ldj_b) + chunk8 * 16;
+    const int64_t i_rows = min64(p.rows - i0, kBI), j_rows = min64(p.cols - j0, kGated ? kCols : kBJ);
+    // window of stage st: everything from its first byte to the last valid one
+    // (past the last stage: nothing, its transfers write zeros that nobody reads)
+    auto i_window = [&](int st) __attribute__((always_inline)) {
+        const int64_t left = p.depth - (int64_t)st * 64;
+        const char* base = iw.base + (kIT ? (int64_t)st * 64 * ldi_b : (int64_t)st * 128);
+        const int64_t size = kIT ? (min64(left, 64) - 1) * ldi_b + min64(p.i_row - i0, kBI) * 2
+                                 : (i_rows - 1) * ldi_b + (p.i_row - (int64_t)st * 64) * 2;
+        return window_rsrc({base, left > 0 ? (uint32_t)size : 0u});
+    };
+    auto j_window = [&](int st) __attribute__((always_inline)) {
+        const int64_t left = p.depth - (int64_t)st * 64;
+        const char* base = jw.base + (kJT ? (int64_t)st * 64 * ldj_b : (int64_t)st * (kJFp8 ? 64 : 128));
+        const int64_t size = kJT ? (min64(left, 64) - 1) * ldj_b + j_rows * 2 : (j_rows - 1) * ldj_b + left * (kJFp8 ? 1 : 2);
+        return window_rsrc({base, left > 0 ? (uint32_t)size : 0u});
+    };
+    const uint32_t lds0 = lds_addr(smem);
+    // one of the wave's kXfers transfers of stage st
+    auto issue = [&](int st, int buffer, int x, u32x4 irsrc, u32x4 jrsrc) __attribute__((always_inline)) {
+        const uint32_t buf = lds0 + buffer * kStage;
+        // depth of the stage, by I's rows and by J's
+        const int i_left = (int)min64(p.i_row - (int64_t)st * 64, 64), left = (int)min64(p.depth - (int64_t)st * 64, 64);
+        if (x < kIX) {
+            const int n = x * kWaves + wave;
+            if (kIXfers % kWaves != 0 && n >= kIXfers) return;
+            uint32_t off;
+            if constexpr (kIT) {
+                off = (uint32_t)((8 * (n & 7)) * ldi_b) + (n >> 3) * 128 + i_lane;
+            } else {
+                off = (uint32_t)(8 * n * ldi_b) + i_lane;
+                if (8 * chunk8 >= i_left) off = kOutside;
+            }
+            window_to_lds(irsrc, off, buf + n * 1024);
+        } else {
+            const int n = (x - kIX) * kWaves + wave;
+            if (kJXfers % kWaves != 0 && n >= kJXfers) return;
+            uint32_t off;
+            if constexpr (kJT) {
+                off = (uint32_t)((8 * (n & 7)) * ldj_b) + (n >> 3) * 128 + j_lane;
+            } else if constexpr (kJFp8) {
+                off = (uint32_t)(16 * (kGated ? n >> 1 : n) * ldj_b) + j_lane;
+                if (16 * chunk16 >= left) off = kOutside;
+            } else {
+                off = (uint32_t)((kGated ? 16 * (n >> 2) + 8 * (n & 1) : 8 * n) * ldj_b) + j_lane;
+                if (8 * chunk8 >= left) off = kOutside;
+            }
+            window_to_lds(jrsrc, off, buf + kIBytes + n * 1024);
+        }
+    };
+
+    // ---- operand reads. Depth order inside a stage: step ks = 2 pp + q has lane
+    // half hf supply depth 32 pp + 16 hf + 8 q .. + 7 of its row (any order that
+    // both operands share gives the same sum), so that a lane's E4M3 codes of two
+    // steps are 16 consecutive bytes.
+    // With the depth shared, group wk of the waves takes steps kSteps wk ...
+    int row_off[kSteps];  // by rows: chunk 4 pp + 2 hf + q of row col
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        const int ks = kSteps * wk + k;
+        row_off[k] = col * 128 + (((4 * (ks >> 1) + 2 * hf + (ks & 1)) ^ swz(col)) << 4);
+    }
+    // by columns: [q][depth group of 4][half of the panel]; the half is the wave's
+    // where an even number of waves share the operand, else the tile's
+    constexpr int kQ = kSteps > 1 ? 2 : 1, kHalfI = kWI == 1 ? 2 : 1, kHalfJ = kWJ == 1 ? 2 : 1;
+    int tr_i[kQ][2][kHalfI], tr_j[kQ][2][kHalfJ];
+    if constexpr (kIT || kJT) {
+        const int s = lane & 15, g = lane >> 4, pp = kSteps * wk >> 1;
+#pragma unroll
+        for (int k = 0; k < kQ; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int q = kQ == 2 ? k : wk & 1;
+                const int row = 16 * (g >> 1) + 8 * q + 4 * h + (s >> 2);
+                const int c = 2 * (g & 1) + ((s & 3) >> 1), at = pp * 4096 + row * 128 + (s & 1) * 8;
+#pragma unroll
+                for (int b = 0; b < kHalfI; ++b) tr_i[k][h][b] = at + (((c + 4 * (kWI == 1 ? b : wi & 1)) ^ swz(row)) << 4);
+#pragma unroll
+                for (int b = 0; b < kHalfJ; ++b) tr_j[k][h][b] = at + (((c + 4 * (kWJ == 1 ? b : wj & 1)) ^ swz(row)) << 4);
+            }
+    }
+    // The wave's tile t is tile kW t + w of the region (kW waves share the
+    // operand): by columns it is half w % 2 of panel (kW t + w) / 2.
+    static_assert((!kIT || kWI == 1 || kWI % 2 == 0) && (!kJT || kWJ == 1 || kWJ % 2 == 0), "half panels by wave or by tile");
+    auto read_rows = [&](const char* region, int t, int k) __attribute__((always_inline)) {
+        return *(const lds_op*)(region + t * 4096 + row_off[k]);
+    };
+    auto read_columns = [&](const char* region, int panel, int lo_off, int hi_off, int k) __attribute__((always_inline)) {
+        const char* base = region + panel * 8192 + (k >> 1) * 4096;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + lo_off));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + hi_off));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    const int i_base = kIT ? (wi >> 1) * 8192 : wi * 4096;
+    const int j_base = kIBytes + (kJT ? (wj >> 1) * 8192 : wj * (kJFp8 ? 2048 : 4096));
+    i16x8 iop[2][kMI];
+    u32x4 jop[2][kMJ];  // E4M3: the codes of two steps, read at the first
+    auto read_ops = [&](int buffer, int k, int set) __attribute__((always_inline)) {
+        const char* buf = smem + buffer * kStage;
+#pragma unroll
+        for (int t = 0; t < kMJ; ++t) {
+            if constexpr (kJFp8) {
+                if ((k & 1) == 0)
+                    jop[(k >> 1) & 1][t] = *(const lds_u32x4*)(buf + j_base + t * kWJ * 2048 + col * 64 +
+                                                              (((2 * (k >> 1) + hf) ^ ((col >> 2) & 3)) << 4));
+            } else {
+                if constexpr (kJT) jop[set][t] = __builtin_bit_cast(u32x4, read_columns(buf + j_base, t * kWJ / 2, tr_j[k & (kQ - 1)][0][t & (kHalfJ - 1)],
+                                                                                     tr_j[k & (kQ - 1)][1][t & (kHalfJ - 1)], k));
+                else jop[set][t] = __builtin_bit_cast(u32x4, read_rows(buf + j_base, t * kWJ, k));
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kMI; ++t) {
+            if constexpr (kIT) iop[set][t] = read_columns(buf + i_base, t * kWI / 2, tr_i[k & (kQ - 1)][0][t & (kHalfI - 1)],
+                                                          tr_i[k & (kQ - 1)][1][t & (kHalfI - 1)], k);
+            else iop[set][t] = read_rows(buf + i_base, t * kWI, k);
+        }
+    };
+
+    f32x16 acc[kMJ][kMI];
+#pragma unroll
+    for (int j = 0; j < kMJ; ++j)
+#pragma unroll
+        for (int i = 0; i < kMI; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
+    float sums[kMI] = {};  // row sums of the I operand (dbias)
+
+    // at most kFlying of the wave's transfers are still on their way, and no wave reads LDS any more
+    // at most kFlying stages' transfers of the wave are still on their way, and no wave reads LDS any more
+    auto land = [&]<int kFlying>() __attribute__((always_inline)) {
+        if (kFlying == 0 || kMore == 0 || wave < kMore) wait_vmem<kFlying * kXfers>();
+        else wait_vmem<kFlying * (kXfers - 1)>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto main_loop = [&]<bool kSums>() __attribute__((always_inline)) {
+        // step k's matrix instructions, with part kPart of the transfers of stage `next` between them (-1: none)
+        auto step = [&]<int kPart>(int k, int next, int buffer) __attribute__((always_inline)) {
+            constexpr int kFrom = kPart < 0 ? 0 : kPart * kXfers / kSpread, kTo = kPart < 0 ? 0 : (kPart + 1) * kXfers / kSpread;
+            const int set = k & 1;
+            u32x4 irsrc{}, jrsrc{};
+            if constexpr (kTo > kFrom) {
+                irsrc = i_window(next);
+                jrsrc = j_window(next);
+            }
+            i16x8 w[kMJ];
+#pragma unroll
+            for (int t = 0; t < kMJ; ++t) {
+                if constexpr (kJFp8) {
+                    const u32x4 codes = jop[(k >> 1) & 1][t];
+                    const uint2 lo = F::decode(codes[2 * (k & 1)]), hi = F::decode(codes[2 * (k & 1) + 1]);
+                    w[t] = __builtin_bit_cast(i16x8, u32x4{lo.x, lo.y, hi.x, hi.y});
+                } else {
+                    w[t] = __builtin_bit_cast(i16x8, jop[set][t]);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < kMI * kMJ; ++q) {
+                const int j = q / kMI, i = q % kMI;
+                acc[j][i] = F::mfma(w[j], iop[set][i], acc[j][i]);
+                if (kFrom + q < kTo) issue(next, buffer, kFrom + q, irsrc, jrsrc);
+            }
+#pragma unroll
+            for (int x = kFrom + kMI * kMJ; x < kTo; ++x) issue(next, buffer, x, irsrc, jrsrc);
+            if constexpr (kSums) {
+#pragma unroll
+                for (int i = 0; i < kMI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sums[i] = F::dot_ones(__builtin_bit_cast(u32x4, iop[set][i])[e], sums[i]);
+            }
+        };
+        // Stage st in `buffer`: part 0 of the requests of stage st + kRing follows the barrier that frees
+        // the buffer, the other parts the next stage's first steps.
+        auto stage = [&](int st, int buffer) __attribute__((always_inline)) {
+            const int before = buffer == 0 ? kRing - 1 : buffer - 1;
+            [&]<int... k>(std::integer_sequence<int, k...>) __attribute__((always_inline)) {
+                ((read_ops(buffer, k + 1, (k + 1) & 1), __builtin_amdgcn_sched_barrier(0),
+                  step.template operator()<(k + 1 < kSpread ? k + 1 : -1)>(k, st - 1 + kRing, before),
+                  __builtin_amdgcn_sched_barrier(0)), ...);
+            }(std::make_integer_sequence<int, kSteps - 1>{});
+            land.template operator()<kRing - 2>();  // stage st + 1 is there, and nobody reads stage st any more
+            read_ops(buffer + 1 == kRing ? 0 : buffer + 1, 0, 0);  // (past the last stage: unused)
+            __builtin_amdgcn_sched_barrier(0);
+            step.template operator()<0>(kSteps - 1, st + kRing, buffer);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int st = 0; st < kRing; ++st) {
+            const u32x4 ir = i_window(st), jr = j_window(st);
+#pragma unroll
+            for (int x = 0; x < (st == kRing - 1 ? kXfers / kSpread : kXfers); ++x) issue(st, st, x, ir, jr);
+        }
+        land.template operator()<kRing - 2>();
+        read_ops(0, 0, 0);
+        for (int st = 0, buffer = 0; st < n_stages; ++st, buffer = buffer + 1 == kRing ? 0 : buffer + 1) stage(st, buffer);
+        wait_vmem<0>();  // LDS outlives the transfers
+    };
+    const bool with_sums = kEpi == kFfStore && kIT && p.row_sums != nullptr && j0 == 0 && wj == 0;  // (every depth share)
+    if constexpr (kEpi == kFfStore && kIT) {
+        if (with_sums) main_loop.template operator()<true>();
+        else main_loop.template operator()<false>();
+    } else {
+        main_loop.template operator()<false>();
+    }
+
+    // ---- epilogue. acc[t][s][4u + q]: row i0 + 32 (kWI s + wi) + col, tile column
+    // 32 (kWJ t + wj) + 8u + 4hf + q. Two groups of 4 columns are rounded, packed
+    // and exchanged between the lane halves, so that every lane stores 16 bytes.
+    // Everything goes through windows of the tile's rows: rows past the end lie
+    // outside them, columns past the end get an offset that does (loads give 0,
+    // stores nothing), so that no access branches.
+    const bool vec = p.vec != 0;
+    const int wave_row = 32 * wi + col;             // + 32 kWI s: the lane's row in the tile
+    const int wave_col = (kGated ? 16 : 32) * wj;   // + (16 | 32) kWJ t: columns of C in the tile
+    const int cols = (int)min64(p.cols - j0, 1 << 16);         // columns of C from j0 on
+    auto rows_window = [&](const void* base, int64_t ld, int64_t first) __attribute__((always_inline)) {
+        // [i_rows, ..] of a row-major 16-bit tensor, from column `first` to the end of C's columns
+        const uint64_t b = (uint64_t)(uintptr_t)base + (uint64_t)((i0 * ld + first) * 2);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)b, 0, (int)(base == nullptr ? 0 : ((i_rows - 1) * ld + cols) * 2),
+                                                 0x00020000);
+    };
+    auto load4 = [&](__amdgpu_buffer_rsrc_t r, uint32_t row_b, int c, float (&v)[4]) __attribute__((always_inline)) {
+        if (vec) {
+            const u32x2 d = __builtin_amdgcn_raw_buffer_load_b64(r, c < cols ? row_b + 2 * c : kOutside, 0, 0);
+            v[0] = F::lo(d[0]), v[1] = F::hi(d[0]), v[2] = F::lo(d[1]), v[3] = F::hi(d[1]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                v[q] = F::lo((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, c + q < cols ? row_b + 2 * (c + q) : kOutside, 0, 0));
+        }
+    };
+    auto load4f = [&](__amdgpu_buffer_rsrc_t r, int c, float (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            v[q] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, c + q < cols ? 4 * (c + q) : kOutside, 0, 0));
+    };
+    auto store8 = [&](__amdgpu_buffer_rsrc_t r, uint32_t row_b, int c, const float (&a)[4], const float (&b)[4]) __attribute__((always_inline)) {
+        // a: columns c + 4hf .., b: c + 8 + 4hf ..
+        uint32_t a0 = F::pack(a[0], a[1]), a1 = F::pack(a[2], a[3]), b0 = F::pack(b[0], b[1]), b1 = F::pack(b[2], b[3]);
+        join_halves(a0, b0);
+        join_halves(a1, b1);
+        const int at = c + 8 * hf;
+        const u32x4 d{a0, a1, b0, b1};
+        if (vec) {
+            __builtin_amdgcn_raw_buffer_store_b128(d, r, at < cols ? row_b + 2 * at : kOutside, 0, 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(d[e >> 1] >> (16 * (e & 1))), r,
+                                                      at + e < cols ? row_b + 2 * (at + e) : kOutside, 0, 0);
+        }
+    };
+    auto vector_window = [&](const void* base, int64_t first, int elem) __attribute__((always_inline)) {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)((uintptr_t)base + (uintptr_t)(first * elem)), 0,
+                                                 base == nullptr ? 0 : cols * elem, 0x00020000);
+    };
+    // dz: zeros behind the last column, up to the padded row
+    auto zero_pad = [&](uint32_t row, int64_t first) __attribute__((always_inline)) {
+        if (j0 + kCols >= p.cols && wj == 0 && hf == 0 && (int64_t)row < i_rows)
+            for (int64_t z = first; z < p.out_cols_padded; ++z) ((T*)p.out)[(i0 + row) * p.ld_out + z] = (T)0.0f;
+    };
+    const FfAct act = ff_act(p.activation);
+    const uint32_t ldo_b = (uint32_t)(p.ld_out * 2), ldd_b = (uint32_t)(p.ld_dout * 2), ldr_b = (uint32_t)(p.ld_res * 2);
+    const auto dout = rows_window(p.dout, p.ld_dout, j0), residual = rows_window(p.residual, p.ld_res, j0);
+    const auto out = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? value_row : 0) + j0);
+    const auto out_g = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? gate_row : 0) + j0);
+    constexpr int kHalves = kGated ? 2 : 4;  // groups of 4 columns of a lane: value (and gate) columns 8u + 4hf ..
+    float bias[kHalves][4], scale[kHalves][4], bias_g[2][4], scale_g[2][4];
+    // the columns' constants of the tile from column c0 of C's tile on
+    auto constants = [&](int c0) __attribute__((always_inline)) {
+        if constexpr (kEpi == kFfStore) return;
+        const int64_t first = kGated ? value_row : 0;
+        const auto b = vector_window(p.bias, first + j0, 2), sc = vector_window(p.j_scale, first + j0, 4);
+        const auto bg = vector_window(p.bias, gate_row + j0, 2), sg = vector_window(p.j_scale, gate_row + j0, 4);
+#pragma unroll
+        for (int u = 0; u < kHalves; ++u) {
+            const int c = c0 + 8 * u + 4 * hf;
+            load4(b, 0, c, bias[u]);
+            if constexpr (kGated) load4(bg, 0, c, bias_g[u]);
+            if (p.j_scale != nullptr) {
+                load4f(sc, c, scale[u]);
+                if constexpr (kGated) load4f(sg, c, scale_g[u]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    scale[u][q] = 1.0f;
+                    if constexpr (kGated) scale_g[u][q] = 1.0f;
+                }
+            }
+        }
+    };
+    // one 32 x 32 tile of sums: the lane's row of C's tile, first column c0
+    auto finish = [&]<FfFamily kFam>(const f32x16& z, uint32_t row, int c0) __attribute__((always_inline)) {
+        if constexpr (kGated) {
+            float va[2][4], vb[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float d[4];
+                if constexpr (kEpi == kFfGatedDz) load4(dout, row * ldd_b, c0 + 8 * u + 4 * hf, d);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float v = __builtin_fmaf(z[4 * u + q], scale[u][q], bias[u][q]);
+                    const float g = __builtin_fmaf(z[8 + 4 * u + q], scale_g[u][q], bias_g[u][q]);
+                    if constexpr (kEpi == kFfGated) {
+                        va[u][q] = v * ff_value<kFam>(act, g);
+                    } else {
+                        float a;
+                        const float sl = ff_slope<kFam>(act, g, a);
+                        va[u][q] = d[q] * a;
+                        vb[u][q] = d[q] * v * sl;
+                    }
+                }
+            }
+            store8(out, row * ldo_b, c0, va[0], va[1]);
+            if constexpr (kEpi == kFfGatedDz) store8(out_g, row * ldo_b, c0, vb[0], vb[1]);
+        } else {
+            float v[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float d[4] = {};
+                if constexpr (kEpi == kFfLinearDz) {
+                    load4(dout, row * ldd_b, c0 + 8 * u + 4 * hf, d);
+                } else if constexpr (kEpi == kFfLinear) {
+                    if (p.residual != nullptr) load4(residual, row * ldr_b, c0 + 8 * u + 4 * hf, d);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float sum = z[4 * u + q];
+                    if constexpr (kEpi == kFfStore) {
+                        v[u][q] = sum;
+                    } else if constexpr (kEpi == kFfLinear) {
+                        v[u][q] = ff_value<kFam>(act, __builtin_fmaf(sum, scale[u][q], bias[u][q])) + d[q];
+                    } else {
+                        float a;
+                        v[u][q] = ff_slope<kFam>(act, __builtin_fmaf(sum, scale[u][q], bias[u][q]), a) * d[q];
+                    }
+                }
+            }
+            store8(out, row * ldo_b, c0, v[0], v[1]);
+            store8(out, row * ldo_b, c0 + 16, v[2], v[3]);
+        }
+    };
+    auto epilogue = [&]<FfFamily kFam>() __attribute__((always_inline)) {
+        if constexpr (kWK == 1) {
+#pragma unroll
+            for (int t = 0; t < kMJ; ++t) {
+                const int c0 = wave_col + (kGated ? 16 : 32) * kWJ * t;
+                constants(c0);
+#pragma unroll
+                for (int s = 0; s < kMI; ++s) finish.template operator()<kFam>(acc[t][s], wave_row + 32 * kWI * s, c0);
+            }
+        } else {
+            // The depth shares' sums meet in LDS, kWK tiles a round: group wk of the
+            // waves finishes tile kWK r + wk of round r, adding the shares in their order.
+            char* mine = smem + (wi + kWI * wj) * (kWK * (kWK - 1) * 4096) + lane * 16;
+            auto slot = [&](int owner, int from) __attribute__((always_inline)) {
+                return mine + (owner * (kWK - 1) + (from < owner ? from : from - 1)) * 4096;
+            };
+            constexpr int kTiles = kMI * kMJ;
+#pragma unroll
+            for (int r = 0; r < (kTiles + kWK - 1) / kWK; ++r) {
+                land.template operator()<0>();  // the stage buffers, or the last round's sums, are free
+                f32x16 own{};
+#pragma unroll
+                for (int o = 0; o < kWK; ++o) {
+                    const int q = r * kWK + o;
+                    if (q >= kTiles) continue;
+                    if (o == wk) {
+                        own = acc[q / kMI][q % kMI];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *(lds_f32x4*)(slot(o, wk) + e * 1024) = f32x4{acc[q / kMI][q % kMI][4 * e], acc[q / kMI][q % kMI][4 * e + 1],
+                                                                         acc[q / kMI][q % kMI][4 * e + 2], acc[q / kMI][q % kMI][4 * e + 3]};
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                const int q = r * kWK + wk;
+                if (q < kTiles) {
+                    f32x16 sum{};
+#pragma unroll
+                    for (int from = 0; from < kWK; ++from) {
+                        f32x16 part = own;
+                        if (from != wk) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const f32x4 v = *(const lds_f32x4*)(slot(wk, from) + e * 1024);
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) part[4 * e + x] = v[x];
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) sum[x] += part[x];
+                    }
+                    const int c0 = wave_col + (kGated ? 16 : 32) * kWJ * (q / kMI);
+                    constants(c0);
+                    finish.template operator()<kFam>(sum, wave_row + 32 * kWI * (q % kMI), c0);
+                }
+            }
+        }
+        if constexpr (kEpi == kFfLinearDz || kEpi == kFfGatedDz) {
+            if (wk == 0)
+#pragma unroll
+                for (int s = 0; s < kMI; ++s) zero_pad(wave_row + 32 * kWI * s, kGated ? 2 * p.cols : p.cols);
+        }
+    };
+    if constexpr (kEpi == kFfStore) {
+        epilogue.template operator()<kFamLinear>();
+        if constexpr (kIT) {
+            const bool tile_sums = p.row_sums != nullptr && j0 == 0;
+            if constexpr (kWK > 1) {
+                if (tile_sums) {
+                    land.template operator()<0>();
+                    float* part = (float*)smem + lane;  // [kMI][kWI][kWK][64]
+                    if (wj == 0)
+#pragma unroll
+                        for (int s = 0; s < kMI; ++s) *(lds_float*)(part + 64 * (kWK * (kWI * s + wi) + wk)) = sums[s];
+                    land.template operator()<0>();
+#pragma unroll
+                    for (int s = 0; s < kMI; ++s) {
+                        sums[s] = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < kWK; ++w) sums[s] += *(const lds_float*)(part + 64 * (kWK * (kWI * s + wi) + w));
+                    }
+                }
+            }
+            if (with_sums && wk == 0) {
+#pragma unroll
+                for (int s = 0; s < kMI; ++s) {
+                    const int64_t i = i0 + 32 * (kWI * s + wi) + col;
+                    const float v = sums[s] + __shfl_xor(sums[s], 32);
+                    if (hf == 0 && i < p.rows) ((T*)p.row_sums)[i] = (T)v;
+                }
+            }
+        }
+    } else {
+        const FfFamily fam = ff_family(p.activation);
+        if (fam == kFamErf) epilogue.template operator()<kFamErf>();
+        else if (fam == kFamSigmoid) epilogue.template operator()<kFamSigmoid>();
+        else epilogue.template operator()<kFamLinear>();
+    }
+}
+
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
+hipError_t ff_launch(FfParams p, hipStream_t stream) {
+    constexpr int cols = Tile::kBJ / (kEpi == kFfGated || kEpi == kFfGatedDz ? 2 : 1);
+    p.i_blocks = (int32_t)((p.rows + Tile::kBI - 1) / Tile::kBI);
+    p.j_blocks = (int32_t)((p.cols + cols - 1) / cols);
+    p.group_i = p.i_blocks < 8 ? p.i_blocks : 8;
+    hipLaunchKernelGGL((ff_tile_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks)),
+                       dim3(64 * Tile::kWaves), 0, stream, p);
+    return hipGetLastError();
+}
+
+// The tiles that the launcher chooses from (feed_forward.hip), and their products by direction.
+typedef FfTile<4, 2, 1, 2, 5, 2, 2> FfTile256x320;
+typedef FfTile<4, 2, 1, 2, 4, 2, 2> FfTile256x256;
+typedef FfTile<2, 4, 1, 2, 2, 3, 2> FfTile128x256;
+typedef FfTile<2, 2, 2, 2, 2, 4, 2> FfTile128x128;
+typedef FfTile<2, 2, 1, 1, 2, 3, 3> FfTile64x128;
+typedef FfTile<2, 2, 1, 1, 1, 4, 4> FfTile64x64;
+
+template <typename T, typename Tile>
+hipError_t ff_forward_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, hipStream_t stream) {
+    if constexpr (Tile::kWK == 1) {
+        if (j_fp8)
+            return epilogue == kFfGated ? ff_launch<T, false, false, true, Tile, kFfGated>(p, stream)
+                                        : ff_launch<T, false, false, true, Tile, kFfLinear>(p, stream);
+    }
+    return j_fp8 ? hipErrorInvalidValue
+           : epilogue == kFfGated ? ff_launch<T, false, false, false, Tile, kFfGated>(p, stream)
+                                  : ff_launch<T, false, false, false, Tile, kFfLinear>(p, stream);
+}
+
+template <typename T, typename Tile>
+hipError_t ff_backward_tile(const FfParams& p, FfEpilogue epilogue, bool i_transposed, hipStream_t stream) {
+    if (epilogue == kFfGatedDz) return ff_launch<T, false, false, false, Tile, kFfGatedDz>(p, stream);
+    if (epilogue == kFfLinearDz) return ff_launch<T, false, false, false, Tile, kFfLinearDz>(p, stream);
+    return i_transposed ? ff_launch<T, true, true, false, Tile, kFfStore>(p, stream)
+                        : ff_launch<T, false, true, false, Tile, kFfStore>(p, stream);
+}
+
+template <typename T>
+hipError_t ff_forward(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int tile, hipStream_t stream) {
+    switch (tile) {
+    case kFf256x320: return ff_forward_tile<T, FfTile256x320>(p, epilogue, j_fp8, stream);
+    case kFf256x256: return ff_forward_tile<T, FfTile256x256>(p, epilogue, j_fp8, stream);
+    case kFf128x256: return ff_forward_tile<T, FfTile128x256>(p, epilogue, j_fp8, stream);
+    case kFf128x128: return ff_forward_tile<T, FfTile128x128>(p, epilogue, j_fp8, stream);
+    case kFf64x128: return ff_forward_tile<T, FfTile64x128>(p, epilogue, j_fp8, stream);
+    case kFf64x64: return ff_forward_tile<T, FfTile64x64>(p, epilogue, j_fp8, stream);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <typename T>
+hipError_t ff_backward(const FfParams& p, FfEpilogue epilogue, bool i_transposed, int tile, hipStream_t stream) {
+    switch (tile) {
+    case kFf256x320: return ff_backward_tile<T, FfTile256x320>(p, epilogue, i_transposed, stream);
+    case kFf256x256: return ff_backward_tile<T, FfTile256x256>(p, epilogue, i_transposed, stream);
+    case kFf128x256: return ff_backward_tile<T, FfTile128x256>(p, epilogue, i_transposed, stream);
+    case kFf128x128: return ff_backward_tile<T, FfTile128x128>(p, epilogue, i_transposed, stream);
+    case kFf64x128: return ff_backward_tile<T, FfTile64x128>(p, epilogue, i_transposed, stream);
+    case kFf64x64: return ff_backward_tile<T, FfTile64x64>(p, epilogue, i_transposed, stream);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+}  // namespace sdxl_hip

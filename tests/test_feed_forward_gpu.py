@@ -206,6 +206,47 @@ def test_backward_every_activation(activation, dtype):
                    False)
 
 
+# rows and columns of sums that each tile of the tiled kernel takes at a depth of 328 (six stages, the last one
+# ragged), largest tile last, every edge ragged
+TILES = [(200, 4104), (4100, 520), (4100, 1032), (4100, 2056), (4100, 4104)]
+
+
+@pytest.mark.parametrize("rows,cols", TILES)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_every_tile_forward(rows, cols, dtype):
+    x, w = values(1, rows, 328, dtype=dtype), values(2, cols, 328, std=0.055, dtype=dtype)
+    bias, residual = values(3, cols, std=0.3, dtype=dtype), values(4, rows, cols, dtype=dtype)
+    check_forward(x, w.double(), bias, "gelu", sh.gated_linear(x, w, bias=bias), True)
+    got = sh.linear_act(x, w, bias=bias, residual=residual, activation="silu")
+    check_forward(x, w.double(), bias, "silu", got, False, residual=residual)
+
+
+@pytest.mark.parametrize("rows,cols", TILES)
+def test_every_tile_forward_e4m3(rows, cols):
+    x = values(1, rows, 336)
+    codes, scale, w64 = e4m3(2, cols, 336)
+    check_forward(x, w64, None, "gelu", sh.gated_linear(x, codes, w_scale=scale), True)
+    check_forward(x, w64, None, "none", sh.linear_act(x, codes, w_scale=scale), False)
+
+
+@pytest.mark.parametrize("rows,cols", TILES)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_every_tile_backward(rows, cols, dtype):
+    """dz on the tile, then dx with few features, then dw with few rows"""
+    x, w = values(1, rows, 328, dtype=dtype), values(2, cols, 328, std=0.055, dtype=dtype)
+    bias = values(3, cols, std=0.3, dtype=dtype)
+    dout = values(4, rows, cols // 2, std=0.3, dtype=dtype)
+    check_backward(dout, x, w, bias, "gelu", sh.gated_linear_backward(dout, x, w, bias=bias), True)
+    dout = values(5, rows, cols, std=0.3, dtype=dtype)
+    grads = sh.linear_act_backward(dout, x, w, bias=bias, activation="silu")
+    check_backward(dout, x, w, bias, "silu", grads, False)
+    x, w, dout = values(6, rows, cols, dtype=dtype), values(7, 328, cols, std=0.05, dtype=dtype), values(8, rows, 328, dtype=dtype)
+    check_backward(dout, x, w, None, "none", sh.linear_act_backward(dout, x, w, need_dw=False), False)
+    x, w, dout = values(6, 328, cols, dtype=dtype), values(7, rows, cols, std=0.05, dtype=dtype), values(8, 328, rows, dtype=dtype)
+    grads = sh.linear_act_backward(dout, x, w, need_dx=False, need_dbias=True)
+    check_backward(dout, x, w, None, "none", grads, False)
+
+
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("activation", ["none", "gelu"])
 def test_backward_parts(gated, activation):
