@@ -1,5 +1,5 @@
-// Which tile a product of the feed-forward operators runs on, and which calls
-// the tiled kernel takes (feed_forward_tiles.hpp).
+// Which kernel and tile a product of the feed-forward operators runs on whose
+// rows 16-byte accesses divide (feed_forward_tiles.hpp, feed_forward_deep.hip).
 #include <hip/hip_runtime.h>
 
 #include "feed_forward_kernels.hpp"
@@ -10,6 +10,7 @@ hipError_t ff_forward_f16(const FfParams& p, FfEpilogue epilogue, bool j_fp8, in
 hipError_t ff_forward_bf16(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int tile, hipStream_t stream);
 hipError_t ff_backward_f16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, int tile, hipStream_t stream);
 hipError_t ff_backward_bf16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, int tile, hipStream_t stream);
+hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool one_per_cu, hipStream_t stream);
 
 namespace {
 
@@ -32,14 +33,23 @@ struct TileCost {
 };
 constexpr TileCost kTiles[kFfTiles] = {{256, 320, 1.60f, 0.0f, 15.0f}, {256, 256, 1.32f, 0.0f, 10.5f},
                                        {128, 256, 0.76f, 0.0f, 7.2f},  {128, 128, 0.45f, 0.0f, 5.5f},
-                                       {64, 128, 0.35f, 0.58f, 5.0f},  {64, 64, 0.30f, 0.46f, 5.0f}};
+                                       {64, 128, 0.35f, 0.58f, 5.0f},  {64, 64, 0.30f, 0.46f, 4.5f}};
 
-int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int compute_units) {
-    const int64_t cus = compute_units > 0 ? compute_units : 256;
+// The same for the 32 x 32 tiles whose waves share the depth (feed_forward_deep.hip): 0.095 us a 64-deep block
+// where every CU has at most one tile, else 0.33 us per two tiles of a CU (0.25 where the caches hold w).
+float deep_time(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool& one_per_cu) {
+    const int64_t cols = epilogue == kFfGated ? 2 * p.cols : p.cols;
+    const int64_t tiles = ((p.rows + 31) / 32) * ((cols + 31) / 32);
+    const float blocks = (float)((p.depth + 63) / 64);
+    one_per_cu = tiles <= cus;
+    const float shared = 0.33f * (float)tiles / (float)(2 * cus);
+    return 3.0f + blocks * (one_per_cu ? 0.095f : shared > 0.19f ? shared : 0.19f);
+}
+
+int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus, float& best_time) {
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
     const float stages = (float)((p.depth + 63) / 64);
     int best = 0;
-    float best_time = 0.0f;
     for (int t = 0; t < kFfTiles; ++t) {
         if (j_fp8 && t == kFf128x128) continue;  // its waves share a stage's depth, E4M3 codes come in pairs of steps
         const TileCost& c = kTiles[t];
@@ -81,9 +91,14 @@ hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_t
     // 16-byte stores and 8-byte loads in the epilogue
     p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 8) &&
             aligned(p.dout, 8) && (p.residual == nullptr || p.ld_res % 4 == 0) && (p.dout == nullptr || p.ld_dout % 4 == 0);
-    const int tile = choose_tile(p, epilogue, j_fp8, compute_units);
-    if (epilogue == kFfLinear || epilogue == kFfGated)
+    const int64_t cus = compute_units > 0 ? compute_units : 256;
+    float time = 0.0f;
+    const int tile = choose_tile(p, epilogue, j_fp8, cus, time);
+    if (epilogue == kFfLinear || epilogue == kFfGated) {
+        bool one_per_cu;
+        if (deep_time(p, epilogue, cus, one_per_cu) < time) return ff_deep(p, epilogue, bf16, j_fp8, one_per_cu, stream);
         return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, tile, stream);
+    }
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);
 }
 

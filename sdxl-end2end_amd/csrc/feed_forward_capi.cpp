@@ -74,6 +74,8 @@ sdxl_status resolve(const sdxl_ff_desc* d, bool gated, bool backward, const char
 
 sdxl_status product(const FfParams& p, sdxl_hip::FfEpilogue epilogue, bool it, bool jt, const Call& c, bool w_fp8,
                     hipStream_t stream, const char* name) {
+    if (sdxl_hip::ff_rows_supported(p, epilogue, w_fp8))
+        return launch_status(sdxl_hip::launch_ff_rows(p, epilogue, c.bf16, w_fp8, stream), name);
     if (sdxl_hip::ff_tiled_supported(p, epilogue, it, jt, w_fp8))
         return launch_status(sdxl_hip::launch_ff_tiled(p, epilogue, it, c.bf16, w_fp8, sdxl_hip_compute_units(), stream), name);
     return launch_status(sdxl_hip::launch_ff_general(p, epilogue, it, jt, c.bf16, w_fp8, stream), name);

@@ -1,0 +1,188 @@
+// Projections of few tiles and much depth (some tens to hundreds of rows, few
+// columns: the down projections of short batches). Tiles of the tiled kernel
+// that fill the CUs there are so small that a stage's barrier costs more than
+// its work (64 x 64: 0.3 us a 64-deep stage, 650 clocks for 64 of matrix
+// instructions per wave), so here the waves of a 32 x 32 tile share the depth
+// and never meet before the end: wave v takes the 64-deep blocks v, v + kWaves,
+// .., brings both operands' rows of a block into LDS of its own (8 KiB, the
+// tiled kernel's layouts) through a ring of two blocks, and multiplies all of
+// the tile. The waves' sums are added in LDS in the waves' order. Eight waves
+// where every CU has at most one tile, else four and two tiles a CU: [64, 5120] x
+// [1280, 5120] 10.3 us with eight, 13.5 with four, 31 on 64 x 64 tiles; [600, 640]
+// x [640, 640] 6.4, 4.9 and 8.
+#include <hip/hip_runtime.h>
+
+#include "feed_forward_device.hpp"
+#include "feed_forward_kernels.hpp"
+
+namespace sdxl_hip {
+namespace {
+
+typedef __attribute__((address_space(3))) i16x8 lds_op;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+
+template <typename T, bool kJFp8, int kWaves, FfEpilogue kEpi>
+__global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
+    using F = FfType<T>;
+    constexpr bool kGated = kEpi == kFfGated;
+    constexpr int kRing = 2, kCols = kGated ? 16 : 32;
+    constexpr int kIBytes = 32 * 128, kBlock = kIBytes + 32 * (kJFp8 ? 64 : 128), kXfers = kBlock / 1024;
+    __shared__ __attribute__((aligned(1024))) char smem[kWaves * kRing * kBlock];  // then the sums
+
+    const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t value_row = p.gate_first ? p.cols : 0, gate_row = p.gate_first ? 0 : p.cols;
+    const int64_t ldi_b = p.ld_i * 2, ldj_b = p.ld_j * (kJFp8 ? 1 : 2);
+    // tasks by XCD, rows fastest: an XCD's workgroups share their J rows in its L2
+    int64_t i0, j0;
+    {
+        const int n = p.i_blocks * p.j_blocks;
+        const int id = blockIdx.x, xcd = id & 7, slot = id >> 3;
+        const int per = n >> 3, extra = n & 7;
+        const int task = xcd * per + (xcd < extra ? xcd : extra) + slot;
+        i0 = (int64_t)(task % p.i_blocks) * 32;
+        j0 = (int64_t)(task / p.i_blocks) * kCols;
+    }
+    const int64_t i_rows = min(p.rows - i0, (int64_t)32), j_rows = min(p.cols - j0, (int64_t)kCols);
+    const int blocks = (int)((p.depth + 63) / 64);
+    const int mine = (blocks - wave + kWaves - 1) / kWaves;  // blocks of the wave
+
+    // the lane's part of a transfer: 8 rows (by the parity of its number) or, of E4M3 rows, 16
+    const int row8 = lane >> 3, row16 = lane >> 2;
+    const int chunk8[2] = {(lane & 7) ^ swz(row8), (lane & 7) ^ swz(8 + row8)}, chunk16 = (lane & 3) ^ ((row16 >> 2) & 3);
+    const uint32_t lds0 = lds_addr(smem) + wave * kRing * kBlock;
+    auto request = [&](int it, int slot) __attribute__((always_inline)) {
+        const int64_t at = (int64_t)(it * kWaves + wave) * 64, left = p.depth - at, i_left = p.i_row - at;
+        const uint32_t buf = lds0 + slot * kBlock;
+        const u32x4 ir = window_rsrc({(const char*)p.ip + i0 * ldi_b + at * 2, (uint32_t)((i_rows - 1) * ldi_b + i_left * 2)});
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            window_to_lds(ir, 8 * chunk8[n & 1] < i_left ? (uint32_t)((8 * n + row8) * ldi_b) + 16 * chunk8[n & 1] : kOutside, buf + n * 1024);
+        const char* base = (const char*)p.jp + at * (kJFp8 ? 1 : 2);
+        const uint32_t size = (uint32_t)((j_rows - 1) * ldj_b + left * (kJFp8 ? 1 : 2));
+        const u32x4 jv = window_rsrc({base + (kGated ? value_row + j0 : j0) * ldj_b, size});
+        const u32x4 jg = window_rsrc({base + (kGated ? gate_row + j0 : j0) * ldj_b, size});
+#pragma unroll
+        for (int n = 0; n < (kJFp8 ? 2 : 4); ++n) {
+            const bool gate = kGated && (kJFp8 ? n & 1 : n & 2);
+            uint32_t off;
+            if constexpr (kJFp8)
+                off = 16 * chunk16 < left ? (uint32_t)(((kGated ? 0 : 16 * n) + row16) * ldj_b) + 16 * chunk16 : kOutside;
+            else
+                off = 8 * chunk8[n & 1] < left ? (uint32_t)(((kGated ? 8 * (n & 1) : 8 * n) + row8) * ldj_b) + 16 * chunk8[n & 1]
+                                               : kOutside;
+            window_to_lds(gate ? jg : jv, off, buf + kIBytes + n * 1024);
+        }
+    };
+    // operand reads: depth step ks = 2 pp + q has lane half hf supply depth 32 pp + 16 hf + 8 q .. + 7
+    int row_off[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) row_off[ks] = col * 128 + (((4 * (ks >> 1) + 2 * hf + (ks & 1)) ^ swz(col)) << 4);
+    f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+    auto multiply = [&](int slot) __attribute__((always_inline)) {
+        const char* buf = smem + (wave * kRing + slot) * kBlock;
+        u32x4 codes;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const i16x8 iop = *(const lds_op*)(buf + row_off[ks]);
+            i16x8 jop;
+            if constexpr (kJFp8) {
+                if ((ks & 1) == 0)
+                    codes = *(const lds_u32x4*)(buf + kIBytes + col * 64 + (((2 * (ks >> 1) + hf) ^ ((col >> 2) & 3)) << 4));
+                const uint2 lo = F::decode(codes[2 * (ks & 1)]), hi = F::decode(codes[2 * (ks & 1) + 1]);
+                jop = __builtin_bit_cast(i16x8, u32x4{lo.x, lo.y, hi.x, hi.y});
+            } else {
+                jop = *(const lds_op*)(buf + kIBytes + row_off[ks]);
+            }
+            acc = F::mfma(jop, iop, acc);
+        }
+    };
+#pragma unroll
+    for (int it = 0; it < kRing; ++it)
+        if (it < mine) request(it, it);
+    for (int it = 0; it < mine; ++it) {
+        const int slot = it & 1;
+        if (it + 1 < mine) wait_vmem<kXfers>();  // the next block's transfers may still be on their way
+        else wait_vmem<0>();
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(slot);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is read
+        if (it + kRing < mine) request(it + kRing, slot);
+    }
+    __syncthreads();
+    // the sums: [wave][4][lane] f32x4; acc[4u + q]: row col, tile column 8u + 4hf + q
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        *(lds_f32x4*)(smem + ((wave * 4 + u) * 64 + lane) * 16) = f32x4{acc[4 * u], acc[4 * u + 1], acc[4 * u + 2], acc[4 * u + 3]};
+    __syncthreads();
+
+    const FfAct act = ff_act(p.activation);
+    const FfFamily fam = ff_family(p.activation);
+    auto act_of = [&](float z) {
+        return fam == kFamErf ? ff_value<kFamErf>(act, z) : fam == kFamSigmoid ? ff_value<kFamSigmoid>(act, z) : ff_value<kFamLinear>(act, z);
+    };
+    auto sum_of = [&](int u) {
+        f32x4 s{};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) s += *(const lds_f32x4*)(smem + ((w * 4 + u) * 64 + lane) * 16);
+        return s;
+    };
+    auto z_of = [&](float sum, int64_t j) {
+        if (p.j_scale != nullptr) sum *= p.j_scale[j];
+        if (p.bias != nullptr) sum += (float)((const T*)p.bias)[j];
+        return sum;
+    };
+    const int64_t i = i0 + col;
+    // one group of 4 columns per wave (gated: of the first two waves)
+    if (wave < (kGated ? 2 : 4)) {
+        const int64_t c = j0 + 8 * wave + 4 * hf;
+        const f32x4 a = sum_of(wave);
+        f32x4 b{};
+        if constexpr (kGated) b = sum_of(wave + 2);
+        if (i >= p.rows) return;
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            v[q] = 0.0f;
+            if (c + q >= p.cols) continue;
+            if constexpr (kGated) v[q] = z_of(a[q], value_row + c + q) * act_of(z_of(b[q], gate_row + c + q));
+            else v[q] = act_of(z_of(a[q], c + q)) + (p.residual != nullptr ? (float)((const T*)p.residual)[i * p.ld_res + c + q] : 0.0f);
+        }
+        T* out = (T*)p.out + i * p.ld_out + c;
+        if (p.vec && c < p.cols) {
+            *(u32x2*)out = u32x2{F::pack(v[0], v[1]), F::pack(v[2], v[3])};
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < p.cols) out[q] = (T)v[q];
+        }
+    }
+}
+
+template <typename T, bool kJFp8, int kWaves>
+hipError_t launch(FfParams p, FfEpilogue epilogue, hipStream_t stream) {
+    const bool gated = epilogue == kFfGated;
+    p.i_blocks = (int32_t)((p.rows + 31) / 32);
+    p.j_blocks = (int32_t)(gated ? (p.cols + 15) / 16 : (p.cols + 31) / 32);
+    const dim3 grid((unsigned)(p.i_blocks * p.j_blocks)), block(64 * kWaves);
+    if (gated) hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfGated>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfLinear>), grid, block, 0, stream, p);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_type(const FfParams& p, FfEpilogue epilogue, bool j_fp8, bool one_per_cu, hipStream_t stream) {
+    if (one_per_cu) return j_fp8 ? launch<T, true, 8>(p, epilogue, stream) : launch<T, false, 8>(p, epilogue, stream);
+    return j_fp8 ? launch<T, true, 4>(p, epilogue, stream) : launch<T, false, 4>(p, epilogue, stream);
+}
+
+}  // namespace
+
+hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool one_per_cu, hipStream_t stream) {
+    return bf16 ? launch_type<__bf16>(p, epilogue, j_fp8, one_per_cu, stream)
+                : launch_type<_Float16>(p, epilogue, j_fp8, one_per_cu, stream);
+}
+
+}  // namespace sdxl_hip

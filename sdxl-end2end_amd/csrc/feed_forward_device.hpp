@@ -56,6 +56,33 @@ struct FfType<__bf16> {
     }
 };
 
+// An operand's window as a buffer descriptor (raw, byte offsets): reads at or
+// past `size` return zero.
+struct Window {
+    const char* base;
+    uint32_t size;
+};
+
+__device__ __forceinline__ u32x4 window_rsrc(Window w) {
+    const uint64_t b = (uint64_t)(uintptr_t)w.base;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32) & 0xFFFFu),
+                 (uint32_t)__builtin_amdgcn_readfirstlane(w.size), 0x00020000u};
+}
+
+// 1-KiB transfer: lane l's 16 bytes at offset voff of the window go to lds +
+// 16 l. Ordered by explicit waits and barriers, as the attention kernel's.
+__device__ __forceinline__ void window_to_lds(u32x4 rsrc, uint32_t voff, uint32_t lds) {
+    lds = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile(
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %0, %1, 0 offen lds"
+        :
+        : "v"(voff), "s"(rsrc), "{m0}"(lds));
+}
+
+constexpr uint32_t kOutside = 0x80000000u;  // past every window (their sizes stay below 2^31)
+
 // ---- activations. Three families share the kernels, chosen once per
 // workgroup (the activation is uniform): z and relu; z sigmoid(z (c0 + c1
 // z^2)), which is silu, quick gelu and the tanh form of gelu (1 + tanh u = 2

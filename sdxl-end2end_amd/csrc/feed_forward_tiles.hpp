@@ -44,33 +44,6 @@ typedef __attribute__((address_space(3))) i16x8 lds_op;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 typedef __attribute__((address_space(3))) float lds_float;
 
-// An operand's window as a buffer descriptor (raw, byte offsets): reads at or
-// past `size` return zero.
-struct Window {
-    const char* base;
-    uint32_t size;
-};
-
-__device__ __forceinline__ u32x4 window_rsrc(Window w) {
-    const uint64_t b = (uint64_t)(uintptr_t)w.base;
-    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b),
-                 (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32) & 0xFFFFu),
-                 (uint32_t)__builtin_amdgcn_readfirstlane(w.size), 0x00020000u};
-}
-
-// 1-KiB transfer: lane l's 16 bytes at offset voff of the window go to lds +
-// 16 l. Ordered by explicit waits and barriers, as the attention kernel's.
-__device__ __forceinline__ void window_to_lds(u32x4 rsrc, uint32_t voff, uint32_t lds) {
-    lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile(
-        "s_nop 4\n\t"
-        "buffer_load_dwordx4 %0, %1, 0 offen lds"
-        :
-        : "v"(voff), "s"(rsrc), "{m0}"(lds));
-}
-
-constexpr uint32_t kOutside = 0x80000000u;  // past every window (their sizes stay below 2^31)
-
 __device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
 // Exchanges the halves so that lanes 0-31 hold 8 consecutive columns made of

@@ -276,7 +276,10 @@ class _Torch:
     def __init__(self):
         import torch
         self.codes = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
-        self.f16, self.int32, self.uint8 = torch.float16, torch.int32, torch.uint8
+        self.half_codes = {torch.float16: F16, torch.bfloat16: BF16}
+        self.f16, self.f32, self.int32, self.uint8 = torch.float16, torch.float32, torch.int32, torch.uint8
+        self.device = torch.cuda.device
+        self.current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         self.empty, self.empty_like = torch.empty, torch.empty_like
         # the handle of the current stream without a Stream object around it
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
@@ -530,98 +533,89 @@ def cross_attn_sublayer(x, ln_gamma, ln_beta, w_q, w_q_scale, kv, w_out, b_out, 
 # ---------------------------------------------------------------- feed-forward
 # (include/sdxl_hip/feed_forward.h; reference src/cuda/unet.cpp:98-149)
 
-class _Guard:
-    """Makes a tensor's device current for a call where it is not (the library launches on the current one)."""
-
-    def __init__(self, index):
-        import torch
-        self.device = torch.cuda.device(index) if index >= 0 and index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.device is not None:
-            self.device.__enter__()
-
-    def __exit__(self, *exc):
-        if self.device is not None:
-            self.device.__exit__(*exc)
+def _ff_call(fn, index, t, *args) -> None:
+    """fn(*args, stream) on the tensors' device, which is made current where it is not."""
+    if index < 0:
+        status = fn(*args, None)
+    elif index == t.current_device():
+        status = fn(*args, t.raw_stream(index))
+    else:
+        with t.device(index):
+            status = fn(*args, t.raw_stream(index))
+    if status != OK:
+        _check(status)
 
 
-def _ff_rows(name, what, t, rows, cols, like) -> int:
-    """The row stride of a 2-D tensor (0 where there is at most one row), after its checks."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise SdxlError(INVALID_SHAPE, f"{name}: {what} must be [{rows}, {cols}]")
-    if t.device != like.device:
-        raise SdxlError(INVALID_ARGUMENT, f"{name}: {what} must be on {like.device}")
+def _ff_stride(name, what, t) -> int:
+    """The row stride of a 2-D tensor that is not contiguous, after its checks."""
     row, col = t.stride()
-    if cols > 1 and col != 1:
+    if t.shape[1] > 1 and col != 1:
         raise SdxlError(INVALID_SHAPE, f"{name}: {what} must have unit column stride")
-    if rows <= 1 or cols == 0:
+    if t.shape[0] <= 1 or t.shape[1] == 0:
         return 0
-    if row < cols:
+    if row < t.shape[1]:
         raise SdxlError(INVALID_SHAPE, f"{name}: row stride smaller than the row")
     return row
 
 
-def _ff_vector(name, what, t, size, dtype, like) -> int:
-    if t is None:
-        return 0
-    if t.dim() != 1 or t.shape[0] != size or t.dtype != dtype or (size > 1 and t.stride(0) != 1):
-        raise SdxlError(INVALID_SHAPE, f"{name}: {what} must be contiguous {dtype} [{size}]")
-    if t.device != like.device:
-        raise SdxlError(INVALID_ARGUMENT, f"{name}: {what} must be on {like.device}")
-    return t.data_ptr()
+def _ff_like(name, what, t, shape, dtype, index) -> None:
+    """Checks of a tensor beside x: its shape, type and device (and that a vector is contiguous)."""
+    if t.shape != shape or t.dtype != dtype or (len(shape) == 1 and not t.is_contiguous()):
+        raise SdxlError(INVALID_SHAPE, f"{name}: {what} must be {dtype} {list(shape)}")
+    if t.get_device() != index:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: {what} must be on x's device")
 
 
-def _ff_call(name, x, w, activation, gated):
-    """(torch lookups, M, N, K, dtype code, weight dtype code, activation code) after the common checks."""
+def _ff_common(name, x, w, bias, activation, gated):
+    """(torch lookups, M, K, rows of w, type code, weights' type code, activation code, device index)"""
     t = _Torch.loaded or _Torch()
-    code = t.codes.get(x.dtype, F32)
-    if code == F32:
+    code = t.half_codes.get(x.dtype)
+    if code is None:
         raise SdxlError(INVALID_SHAPE, f"{name}: tensors must be fp16 or bf16")
-    if w.dtype != x.dtype and w.dtype != t.uint8:
-        raise SdxlError(INVALID_SHAPE, f"{name}: weights must have the tensors' type or be E4M3")
-    if activation not in ACTIVATIONS:
+    w_code = code
+    if w.dtype != x.dtype:
+        if w.dtype != t.uint8:
+            raise SdxlError(INVALID_SHAPE, f"{name}: weights must have the tensors' type or be E4M3")
+        w_code = E4M3
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise SdxlError(INVALID_ARGUMENT, f"{name}: activation must be one of {', '.join(ACTIVATIONS)}")
-    if x.dim() != 2 or w.dim() != 2 or (gated and w.shape[0] % 2 != 0):
+    x_shape, w_shape = x.shape, w.shape
+    if len(x_shape) != 2 or len(w_shape) != 2 or w_shape[1] != x_shape[1] or (gated and w_shape[0] % 2 != 0):
         raise SdxlError(INVALID_SHAPE, f"{name}: x must be [M, K] and w [{'2N' if gated else 'N'}, K]")
-    features = w.shape[0]
-    return (t, x.shape[0], features // 2 if gated else features, x.shape[1], code,
-            E4M3 if w.dtype == t.uint8 else code, ACTIVATIONS[activation])
+    index = x.get_device()
+    if w.get_device() != index:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: w must be on x's device")
+    if bias is not None:
+        _ff_like(name, "bias", bias, w_shape[:1], x.dtype, index)
+    return t, x_shape[0], x_shape[1], w_shape[0], code, w_code, act, index
 
 
 def _ff_forward(name, gated, x, w, bias, w_scale, activation, gate_first, residual, out):
-    t, M, N, K, code, w_code, act = _ff_call(name, x, w, activation, gated)
-    features = 2 * N if gated else N
-    ldx = _ff_rows(name, "x", x, M, K, x)
-    ldw = _ff_rows(name, "w", w, features, K, x)
-    import torch
-    scale_ptr = _ff_vector(name, "w_scale", w_scale, features, torch.float32, x)
-    bias_ptr = _ff_vector(name, "bias", bias, features, x.dtype, x)
-    ldr = 0
+    t, M, K, features, code, w_code, act, index = _ff_common(name, x, w, bias, activation, gated)
+    N = features // 2 if gated else features
+    ldr = ldo = 0
+    if w_scale is not None:
+        _ff_like(name, "w_scale", w_scale, (features,), t.f32, index)
     if residual is not None:
-        if residual.dtype != x.dtype:
-            raise SdxlError(INVALID_SHAPE, f"{name}: residual must have x's type")
-        ldr = _ff_rows(name, "residual", residual, M, N, x)
-    ldo = 0
+        _ff_like(name, "residual", residual, (M, N), x.dtype, index)
+        ldr = 0 if residual.is_contiguous() else _ff_stride(name, "residual", residual)
     if out is None:
         out = x.new_empty((M, N))
     else:
-        if out.dtype != x.dtype:
-            raise SdxlError(INVALID_SHAPE, f"{name}: out must have x's type")
-        ldo = _ff_rows(name, "out", out, M, N, x)
-    desc = _FF_DESC.pack(M, N, K, ldx, ldw, ldo, ldr, 0, 0, code, w_code, act, 1 if gate_first else 0, 0)
-    index = x.get_device()
-    lib = load()
-    with _Guard(index):
-        stream = t.raw_stream(index) if index >= 0 else None
-        if gated:
-            status = lib.packed_sdxl_gated_linear(desc, x.data_ptr(), w.data_ptr(), scale_ptr, bias_ptr,
-                                                  out.data_ptr(), stream)
-        else:
-            status = lib.packed_sdxl_linear_act(desc, x.data_ptr(), w.data_ptr(), scale_ptr, bias_ptr,
-                                                residual.data_ptr() if residual is not None else None,
-                                                out.data_ptr(), stream)
-    _check_packed(status)
+        _ff_like(name, "out", out, (M, N), x.dtype, index)
+        ldo = 0 if out.is_contiguous() else _ff_stride(name, "out", out)
+    desc = _FF_DESC.pack(M, N, K, 0 if x.is_contiguous() else _ff_stride(name, "x", x),
+                         0 if w.is_contiguous() else _ff_stride(name, "w", w), ldo, ldr, 0, 0, code, w_code, act,
+                         1 if gate_first else 0, 0)
+    scale_ptr = w_scale.data_ptr() if w_scale is not None else None
+    bias_ptr = bias.data_ptr() if bias is not None else None
+    if gated:
+        _ff_call(load().packed_sdxl_gated_linear, index, t, desc, x.data_ptr(), w.data_ptr(), scale_ptr, bias_ptr,
+                 out.data_ptr())
+    else:
+        _ff_call(load().packed_sdxl_linear_act, index, t, desc, x.data_ptr(), w.data_ptr(), scale_ptr, bias_ptr,
+                 residual.data_ptr() if residual is not None else None, out.data_ptr())
     return out
 
 
@@ -640,32 +634,26 @@ def linear_act(x, w, bias=None, residual=None, w_scale=None, activation: str = "
 
 
 def _ff_backward(name, gated, dout, x, w, bias, activation, gate_first, need_dx, need_dw, need_dbias, workspace):
-    t, M, N, K, code, w_code, act = _ff_call(name, x, w, activation, gated)
-    features = 2 * N if gated else N
-    if dout.dtype != x.dtype:
-        raise SdxlError(INVALID_SHAPE, f"{name}: dout must have x's type")
-    ldx = _ff_rows(name, "x", x, M, K, x)
-    ldw = _ff_rows(name, "w", w, features, K, x)
-    ldo = _ff_rows(name, "dout", dout, M, N, x)
-    bias_ptr = _ff_vector(name, "bias", bias, features, x.dtype, x)
+    t, M, K, features, code, w_code, act, index = _ff_common(name, x, w, bias, activation, gated)
+    N = features // 2 if gated else features
+    _ff_like(name, "dout", dout, (M, N), x.dtype, index)
+    desc = _FF_DESC.pack(M, N, K, 0 if x.is_contiguous() else _ff_stride(name, "x", x),
+                         0 if w.is_contiguous() else _ff_stride(name, "w", w),
+                         0 if dout.is_contiguous() else _ff_stride(name, "dout", dout), 0, 0, 0, code, w_code, act,
+                         1 if gate_first else 0, 0)
+    lib = load()
+    if workspace is None:
+        size = (lib.packed_sdxl_gated_linear_backward_workspace_bytes if gated else
+                lib.packed_sdxl_linear_act_backward_workspace_bytes)(desc)
+        workspace = t.empty((size,), dtype=t.uint8, device=x.device)
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: workspace must be contiguous and on x's device")
     dx = x.new_empty((M, K)) if need_dx else None
     dw = x.new_empty((features, K)) if need_dw else None
     dbias = x.new_empty((features,)) if (bias is not None if need_dbias is None else need_dbias) else None
-    desc = _FF_DESC.pack(M, N, K, ldx, ldw, ldo, 0, 0, 0, code, w_code, act, 1 if gate_first else 0, 0)
-    index = x.get_device()
-    lib = load()
-    with _Guard(index):
-        if workspace is None:
-            size = (lib.packed_sdxl_gated_linear_backward_workspace_bytes if gated else
-                    lib.packed_sdxl_linear_act_backward_workspace_bytes)(desc)
-            workspace = t.empty((size,), dtype=t.uint8, device=x.device)
-        elif workspace.device != x.device:
-            raise SdxlError(INVALID_ARGUMENT, f"{name}: workspace must be on {x.device}")
-        fn = lib.packed_sdxl_gated_linear_backward if gated else lib.packed_sdxl_linear_act_backward
-        status = fn(desc, dout.data_ptr(), x.data_ptr(), w.data_ptr(), bias_ptr, _ptr(dx), _ptr(dw), _ptr(dbias),
-                    workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                    t.raw_stream(index) if index >= 0 else None)
-    _check_packed(status)
+    _ff_call(lib.packed_sdxl_gated_linear_backward if gated else lib.packed_sdxl_linear_act_backward, index, t, desc,
+             dout.data_ptr(), x.data_ptr(), w.data_ptr(), bias.data_ptr() if bias is not None else None, _ptr(dx),
+             _ptr(dw), _ptr(dbias), workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return dx, dw, dbias
 
 
@@ -699,7 +687,6 @@ def ff_sublayer(x, ln_gamma, ln_beta, w_in, w_in_scale, b_in, w_out, w_out_scale
     """x + gated_linear(LN(x), w_in, b_in) . w_out^T + b_out for hidden x [B, S, W] fp16, the feed-forward
     half of the reference's transformer block (src/cuda/unet.cpp:98-149) after attn_sublayer and
     cross_attn_sublayer: w_in [2I, W], w_out [W, I], each fp16 or uint8 E4M3 with its scales, all contiguous."""
-    import torch
     t = _Torch.loaded or _Torch()
     name = "sdxl_ff_sublayer"
     if x.dim() != 3 or x.dtype != t.f16:
@@ -715,25 +702,22 @@ def ff_sublayer(x, ln_gamma, ln_beta, w_in, w_in_scale, b_in, w_out, w_out_scale
                                        ("w_out", w_out, (W, inner), (t.f16, t.uint8)),
                                        ("norm weight", ln_gamma, (W,), (t.f16,)), ("norm bias", ln_beta, (W,), (t.f16,)),
                                        ("b_in", b_in, (2 * inner,), (t.f16,)), ("b_out", b_out, (W,), (t.f16,)),
-                                       ("w_in_scale", w_in_scale, (2 * inner,), (torch.float32,)),
-                                       ("w_out_scale", w_out_scale, (W,), (torch.float32,))):
+                                       ("w_in_scale", w_in_scale, (2 * inner,), (t.f32,)),
+                                       ("w_out_scale", w_out_scale, (W,), (t.f32,))):
         if tensor is not None and (tensor.shape != shape or tensor.dtype not in types or not tensor.is_contiguous()
                                    or tensor.device != x.device):
             raise SdxlError(INVALID_SHAPE, f"{name}: {what} must be contiguous {list(shape)} on {x.device}")
     desc = _FF_SUBLAYER_DESC.pack(B * S, W, inner, E4M3 if w_in.dtype == t.uint8 else F16,
                                   E4M3 if w_out.dtype == t.uint8 else F16, ACTIVATIONS[activation],
                                   1 if gate_first else 0, _f32(eps), 0)
-    index = x.get_device()
     lib = load()
-    with _Guard(index):
-        if workspace is None:
-            workspace = t.empty((lib.packed_sdxl_ff_sublayer_workspace_bytes(desc),), dtype=t.uint8, device=x.device)
-        status = lib.packed_sdxl_ff_sublayer(desc, x.data_ptr(), _ptr(ln_gamma), _ptr(ln_beta), _ptr(w_in),
-                                             _ptr(w_in_scale), _ptr(b_in), _ptr(w_out), _ptr(w_out_scale), _ptr(b_out),
-                                             out.data_ptr(), workspace.data_ptr(),
-                                             workspace.numel() * workspace.element_size(),
-                                             t.raw_stream(index) if index >= 0 else None)
-    _check_packed(status)
+    if workspace is None:
+        workspace = t.empty((lib.packed_sdxl_ff_sublayer_workspace_bytes(desc),), dtype=t.uint8, device=x.device)
+    elif workspace.device != x.device or not workspace.is_contiguous():
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: workspace must be contiguous and on {x.device}")
+    _ff_call(lib.packed_sdxl_ff_sublayer, x.get_device(), t, desc, x.data_ptr(), _ptr(ln_gamma), _ptr(ln_beta),
+             _ptr(w_in), _ptr(w_in_scale), _ptr(b_in), _ptr(w_out), _ptr(w_out_scale), _ptr(b_out), out.data_ptr(),
+             workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return out
 
 

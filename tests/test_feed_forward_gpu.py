@@ -206,6 +206,27 @@ def test_backward_every_activation(activation, dtype):
                    False)
 
 
+# few rows: one token to 16 rows (depths below a block, of one step and of several steps of 2048), then tens of
+# rows with much depth, with at most one 32 x 32 tile of sums per CU and with more; ragged edges
+FEW_ROWS = [(1, 1283, 2120), (2, 1280, 320), (16, 40, 4112), (5, 2056, 80), (9, 20, 16), (17, 72, 1304), (64, 643, 1296),
+            (150, 650, 528), (33, 3001, 336), (63, 16, 9000)]
+
+
+@pytest.mark.parametrize("m,n,k", FEW_ROWS)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_few_rows(m, n, k, dtype):
+    x, w = values(1, m, k, dtype=dtype), values(2, 2 * n, k, std=k ** -0.5, dtype=dtype)
+    bias, residual = values(3, 2 * n, std=0.3, dtype=dtype), values(4, m, n, dtype=dtype)
+    check_forward(x, w.double(), bias, "gelu", sh.gated_linear(x, w, bias=bias, gate_first=True), True, True)
+    got = sh.linear_act(x, w[:n], bias=bias[:n].clone(), residual=residual, activation="silu")
+    check_forward(x, w[:n].double(), bias[:n], "silu", got, False, residual=residual)
+    codes, scale, w64 = e4m3(5, 2 * n, k)
+    if k % 16 == 0:
+        check_forward(x, w64, bias, "silu", sh.gated_linear(x, codes, bias=bias, w_scale=scale, activation="silu"), True)
+        got = sh.linear_act(x, codes[:n], w_scale=scale[:n], residual=residual)
+        check_forward(x, w64[:n], None, "none", got, False, residual=residual)
+
+
 # rows and columns of sums that each tile of the tiled kernel takes at a depth of 328 (six stages, the last one
 # ragged), largest tile last, every edge ragged
 TILES = [(200, 4104), (4100, 520), (4100, 1032), (4100, 2056), (4100, 4104)]
