@@ -10,6 +10,8 @@ hipError_t ff_forward_f16(const FfParams& p, FfEpilogue epilogue, bool j_fp8, in
 hipError_t ff_forward_bf16(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int tile, hipStream_t stream);
 hipError_t ff_backward_f16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, int tile, hipStream_t stream);
 hipError_t ff_backward_bf16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, int tile, hipStream_t stream);
+hipError_t ff_pair_f16(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream);
+hipError_t ff_pair_bf16(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream);
 hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool one_per_cu, hipStream_t stream);
 
 namespace {
@@ -34,6 +36,37 @@ struct TileCost {
 constexpr TileCost kTiles[kFfTiles] = {{256, 320, 1.60f, 0.0f, 15.0f}, {256, 256, 1.32f, 0.0f, 10.5f},
                                        {128, 256, 0.76f, 0.0f, 7.2f},  {128, 128, 0.45f, 0.0f, 5.5f},
                                        {64, 128, 0.35f, 0.58f, 5.0f},  {64, 64, 0.30f, 0.46f, 4.5f}};
+
+// Time of two kinds of tasks, a tasks of a_time each before b of b_time, on CUs that take the next task when
+// they are free: the CUs as groups that become free together.
+float list_time(int64_t a, float a_time, int64_t b, float b_time, int64_t cus) {
+    // after the a tasks: `late` CUs free at a_end, the others one a_time earlier
+    const int64_t rounds = a / cus, late = a % cus;
+    float early_at = (float)rounds * a_time, late_at = early_at + a_time;
+    if (b == 0) return late > 0 ? late_at : early_at;
+    // b tasks go round by round to whichever group is free first; a group moves as one
+    int64_t early_cus = cus - late, late_cus = late;
+    float end = late > 0 ? late_at : early_at;
+    while (b > 0) {
+        const bool to_early = late_cus == 0 || (early_cus > 0 && early_at <= late_at);
+        float& at = to_early ? early_at : late_at;
+        const int64_t n = to_early ? early_cus : late_cus;
+        // as many rounds at once as stay ahead of the other group
+        int64_t times = 1;
+        if (early_cus > 0 && late_cus > 0) {
+            const float gap = (to_early ? late_at : early_at) - at;
+            times = gap > b_time ? (int64_t)(gap / b_time) : 1;
+        } else {
+            times = (b + n - 1) / n;
+        }
+        const int64_t needed = (b + n - 1) / n;
+        if (times > needed) times = needed;
+        at += (float)times * b_time;
+        b -= times * n;
+        if (at > end) end = at;
+    }
+    return end;
+}
 
 // The same for the 32 x 32 tiles whose waves share the depth (feed_forward_deep.hip): 0.095 us a 64-deep block
 // where every CU has at most one tile, else 0.33 us per two tiles of a CU (0.25 where the caches hold w).
@@ -70,6 +103,16 @@ int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus,
     return best;
 }
 
+// Fills in what the tiled kernels' launchers leave to the dispatch.
+FfParams prepared(const FfParams& params, bool i_transposed) {
+    FfParams p = params;
+    if (p.i_row == 0) p.i_row = i_transposed ? p.rows : p.depth;
+    // 16-byte stores and 8-byte loads in the epilogue
+    p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 8) &&
+            aligned(p.dout, 8) && (p.residual == nullptr || p.ld_res % 4 == 0) && (p.dout == nullptr || p.ld_dout % 4 == 0);
+    return p;
+}
+
 }  // namespace
 
 bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8) {
@@ -86,11 +129,7 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
 
 hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
                            int compute_units, hipStream_t stream) {
-    FfParams p = params;
-    if (p.i_row == 0) p.i_row = i_transposed ? p.rows : p.depth;
-    // 16-byte stores and 8-byte loads in the epilogue
-    p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 8) &&
-            aligned(p.dout, 8) && (p.residual == nullptr || p.ld_res % 4 == 0) && (p.dout == nullptr || p.ld_dout % 4 == 0);
+    const FfParams p = prepared(params, i_transposed);
     const int64_t cus = compute_units > 0 ? compute_units : 256;
     float time = 0.0f;
     const int tile = choose_tile(p, epilogue, j_fp8, cus, time);
@@ -100,6 +139,41 @@ hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_t
         return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, tile, stream);
     }
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);
+}
+
+hipError_t launch_ff_pair(const FfParams& dw, const FfParams& dx, bool bf16, int compute_units, hipStream_t stream) {
+    const FfParams w = prepared(dw, true), x = prepared(dx, false);
+    const int64_t cus = compute_units > 0 ? compute_units : 256;
+    // apart, or together on the best pair of tiles that take a CU each. Together was measured against apart on
+    // an MI355X at [2048, 1280] x [10240, 1280] 142 -> 107 us, [8192, 1280] x [10240, 1280] 459 -> 360.
+    float apart_w, apart_x;
+    choose_tile(w, kFfStore, false, cus, apart_w);
+    choose_tile(x, kFfStore, false, cus, apart_x);
+    float best = apart_w + apart_x;
+    int best_w = -1, best_x = -1;
+    bool w_first = true;
+    constexpr int kPairTiles[3] = {kFf256x256, kFf128x256, kFf128x128};
+    for (int tw : kPairTiles) {
+        const TileCost& cw = kTiles[tw];
+        const int64_t nw = ((w.rows + cw.rows - 1) / cw.rows) * ((w.cols + cw.cols - 1) / cw.cols);
+        const float time_w = (float)((w.depth + 63) / 64) * cw.alone + cw.ends - 2.0f;
+        for (int tx : kPairTiles) {
+            const TileCost& cx = kTiles[tx];
+            const int64_t nx = ((x.rows + cx.rows - 1) / cx.rows) * ((x.cols + cx.cols - 1) / cx.cols);
+            const float time_x = (float)((x.depth + 63) / 64) * cx.alone + cx.ends - 2.0f;
+            const bool first = time_w >= time_x;
+            const float time = 2.0f + (first ? list_time(nw, time_w, nx, time_x, cus) : list_time(nx, time_x, nw, time_w, cus));
+            if (time < best && nw + nx <= (1 << 23)) {
+                best = time;
+                best_w = tw;
+                best_x = tx;
+                w_first = first;
+            }
+        }
+    }
+    if (best_w >= 0) return (bf16 ? ff_pair_bf16 : ff_pair_f16)(w, x, best_w, best_x, w_first, stream);
+    const hipError_t err = launch_ff_tiled(dw, kFfStore, true, bf16, false, compute_units, stream);
+    return err != hipSuccess ? err : launch_ff_tiled(dx, kFfStore, false, bf16, false, compute_units, stream);
 }
 
 }  // namespace sdxl_hip

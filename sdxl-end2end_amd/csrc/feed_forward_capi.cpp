@@ -169,36 +169,35 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
         dz = workspace;
         lddz = dz_stride(c);
     }
+    FfParams pw{}, px{};
+    pw.ip = dz;
+    pw.jp = x;
+    pw.ld_i = lddz;
+    pw.ld_j = c.ldx;
+    pw.rows = c.features;
+    pw.cols = want_dw ? c.k : 1;  // the row sums alone: one tile of columns
+    pw.depth = c.m;
+    pw.out = want_dw ? dw : nullptr;
+    pw.ld_out = c.lddw;
+    pw.row_sums = want_db ? dbias : nullptr;
+    px.ip = dz;
+    px.jp = w;
+    px.ld_i = lddz;
+    px.ld_j = c.ldw;
+    px.rows = c.m;
+    px.cols = c.k;
+    px.depth = c.features;
+    px.out = dx;
+    px.ld_out = c.lddx;
+    if (dz_needed) pw.i_row = px.i_row = lddz;
+    if (want_dw && want_dx && sdxl_hip::ff_tiled_supported(pw, sdxl_hip::kFfStore, true, true, false) &&
+        sdxl_hip::ff_tiled_supported(px, sdxl_hip::kFfStore, false, true, false))
+        return launch_status(sdxl_hip::launch_ff_pair(pw, px, c.bf16, sdxl_hip_compute_units(), stream), name);
     if (want_dw || want_db) {
-        FfParams p{};
-        p.ip = dz;
-        p.jp = x;
-        p.ld_i = lddz;
-        p.ld_j = c.ldx;
-        p.rows = c.features;
-        p.cols = want_dw ? c.k : 1;  // the row sums alone: one tile of columns
-        p.depth = c.m;
-        p.out = want_dw ? dw : nullptr;
-        p.ld_out = c.lddw;
-        p.row_sums = want_db ? dbias : nullptr;
-        if (dz_needed) p.i_row = lddz;
-        st = product(p, sdxl_hip::kFfStore, true, true, c, false, stream, name);
+        st = product(pw, sdxl_hip::kFfStore, true, true, c, false, stream, name);
         if (st != SDXL_STATUS_OK) return st;
     }
-    if (want_dx) {
-        FfParams p{};
-        p.ip = dz;
-        p.jp = w;
-        p.ld_i = lddz;
-        p.ld_j = c.ldw;
-        p.rows = c.m;
-        p.cols = c.k;
-        p.depth = c.features;
-        if (dz_needed) p.i_row = lddz;
-        p.out = dx;
-        p.ld_out = c.lddx;
-        st = product(p, sdxl_hip::kFfStore, false, true, c, false, stream, name);
-    }
+    if (want_dx) st = product(px, sdxl_hip::kFfStore, false, true, c, false, stream, name);
     return st;
 }
 

@@ -54,6 +54,9 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
 hipError_t launch_ff_tiled(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
                            int compute_units, hipStream_t stream);
 
+// dw (I transposed) and dx, both of which the tiled kernel supports: in one launch where that is faster.
+hipError_t launch_ff_pair(const FfParams& dw, const FfParams& dx, bool bf16, int compute_units, hipStream_t stream);
+
 // Projections of at most 16 rows whose rows 16-byte accesses divide.
 bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8);
 hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, hipStream_t stream);

@@ -61,16 +61,22 @@ struct FfTile {
     static constexpr int kWI = kWI_, kWJ = kWJ_, kWK = kWK_, kMI = kMI_, kMJ = kMJ_, kRing = kRing_, kSpread = kSpread_;
     static constexpr int kWaves = kWI * kWJ * kWK, kBI = 32 * kMI * kWI, kBJ = 32 * kMJ * kWJ;
     static constexpr int stage_bytes(bool j_fp8) { return kBI * 128 + kBJ * (j_fp8 ? 64 : 128); }
+    // the stages, or the sums of the other depth shares (one round of tiles at a time)
+    static constexpr int smem_bytes(bool j_fp8) {
+        const int stages = kRing * stage_bytes(j_fp8), exchange = kWI * kWJ * kWK * (kWK - 1) * 4096;
+        return stages > exchange ? stages : exchange;
+    }
     // workgroups that one CU's LDS and registers (512 per lane and SIMD) hold
     static constexpr int waves_per_simd(bool j_fp8) {
-        const int by_lds = kWaves / 4 * (160 * 1024 / (kRing * stage_bytes(j_fp8)));
+        const int by_lds = kWaves / 4 * (160 * 1024 / smem_bytes(j_fp8));
         const int by_regs = kMI * kMJ <= 4 ? 4 : kMI * kMJ <= 10 ? 2 : 1;
         return by_lds < by_regs ? by_lds : by_regs;
     }
 };
 
+// Task `id` of a product whose tasks' numbers modulo 8 are their XCDs; smem: Tile::smem_bytes.
 template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
-__global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) void ff_tile_kernel(FfParams p) {
+__device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
     constexpr int kWI = Tile::kWI, kWJ = Tile::kWJ, kWK = Tile::kWK, kMI = Tile::kMI, kMJ = Tile::kMJ, kRing = Tile::kRing;
     using F = FfType<T>;
     constexpr bool kGated = kEpi == kFfGated || kEpi == kFfGatedDz;
@@ -90,11 +96,7 @@ __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) voi
     static_assert(kWK == 1 || (kWK == 2 && !kJFp8), "depth shares");
     static_assert(!kGated || (!kIT && !kJT), "gated products are projections");
     static_assert(!kJFp8 || !kJT, "E4M3: by rows");
-    // sums of the other depth shares, one round of tiles at a time
-    constexpr int kExchange = kWK > 1 ? kWI * kWJ * kWK * (kWK - 1) * 4096 : 0;
-    constexpr int kSmem = kRing * kStage > kExchange ? kRing * kStage : kExchange;
-    static_assert(kSmem <= 160 * 1024, "LDS of one CU");
-    __shared__ __attribute__((aligned(1024))) char smem[kSmem];
+    static_assert(Tile::smem_bytes(kJFp8) <= 160 * 1024, "LDS of one CU");
 
     const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) voi
     int64_t i0, j0;
     {
         const int n = p.i_blocks * p.j_blocks;
-        const int id = blockIdx.x, xcd = id & 7, slot = id >> 3;
+        const int xcd = id & 7, slot = id >> 3;
         const int per = n >> 3, extra = n & 7;
         const int task = xcd * per + (xcd < extra ? xcd : extra) + slot;
         const int in_group = p.group_i * p.j_blocks;
@@ -584,13 +586,49 @@ __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) voi
 }
 
 template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
-hipError_t ff_launch(FfParams p, hipStream_t stream) {
-    constexpr int cols = Tile::kBJ / (kEpi == kFfGated || kEpi == kFfGatedDz ? 2 : 1);
+__global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) void ff_tile_kernel(FfParams p) {
+    __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
+    ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi>(p, blockIdx.x, smem);
+}
+
+// dw and dx in one launch, one workgroup per CU at a time: the tasks of the
+// product with the longer ones first, so that the shorter ones fill the CUs
+// that the last round of the longer ones leaves idle.
+template <typename T, typename TileW, typename TileX>
+__global__ __launch_bounds__(512, 2) void ff_pair_kernel(FfParams w, FfParams x, int w_first) {
+    static_assert(TileW::kWaves == 8 && TileX::kWaves == 8, "waves");
+    constexpr int kW = TileW::smem_bytes(false), kX = TileX::smem_bytes(false);
+    __shared__ __attribute__((aligned(1024))) char smem[kW > kX ? kW : kX];
+    const int w_tasks = w.i_blocks * w.j_blocks, x_tasks = x.i_blocks * x.j_blocks;
+    const int id = blockIdx.x;
+    if (w_first ? id < w_tasks : id >= x_tasks) ff_tile<T, true, true, false, TileW, kFfStore>(w, w_first ? id : id - x_tasks, smem);
+    else ff_tile<T, false, true, false, TileX, kFfStore>(x, w_first ? id - w_tasks : id, smem);
+}
+
+// Tiles of C and the tasks' groups.
+template <typename Tile>
+void ff_blocks(FfParams& p, bool gated) {
+    const int cols = Tile::kBJ / (gated ? 2 : 1);
     p.i_blocks = (int32_t)((p.rows + Tile::kBI - 1) / Tile::kBI);
     p.j_blocks = (int32_t)((p.cols + cols - 1) / cols);
     p.group_i = p.i_blocks < 8 ? p.i_blocks : 8;
+}
+
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
+hipError_t ff_launch(FfParams p, hipStream_t stream) {
+    ff_blocks<Tile>(p, kEpi == kFfGated || kEpi == kFfGatedDz);
     hipLaunchKernelGGL((ff_tile_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks)),
                        dim3(64 * Tile::kWaves), 0, stream, p);
+    return hipGetLastError();
+}
+
+template <typename T, typename TileW, typename TileX>
+hipError_t ff_launch_pair(FfParams w, FfParams x, bool w_first, hipStream_t stream) {
+    ff_blocks<TileW>(w, false);
+    ff_blocks<TileX>(x, false);
+    hipLaunchKernelGGL((ff_pair_kernel<T, TileW, TileX>),
+                       dim3((unsigned)((int64_t)w.i_blocks * w.j_blocks + (int64_t)x.i_blocks * x.j_blocks)), dim3(512), 0, stream, w, x,
+                       w_first ? 1 : 0);
     return hipGetLastError();
 }
 
@@ -620,6 +658,22 @@ hipError_t ff_backward_tile(const FfParams& p, FfEpilogue epilogue, bool i_trans
     if (epilogue == kFfLinearDz) return ff_launch<T, false, false, false, Tile, kFfLinearDz>(p, stream);
     return i_transposed ? ff_launch<T, true, true, false, Tile, kFfStore>(p, stream)
                         : ff_launch<T, false, true, false, Tile, kFfStore>(p, stream);
+}
+
+template <typename T, typename TileW>
+hipError_t ff_pair_tile(const FfParams& w, const FfParams& x, int x_tile, bool w_first, hipStream_t stream) {
+    return x_tile == kFf256x256   ? ff_launch_pair<T, TileW, FfTile256x256>(w, x, w_first, stream)
+           : x_tile == kFf128x256 ? ff_launch_pair<T, TileW, FfTile128x256>(w, x, w_first, stream)
+           : x_tile == kFf128x128 ? ff_launch_pair<T, TileW, FfTile128x128>(w, x, w_first, stream)
+                                  : hipErrorInvalidValue;
+}
+
+template <typename T>
+hipError_t ff_pair(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream) {
+    return w_tile == kFf256x256   ? ff_pair_tile<T, FfTile256x256>(w, x, x_tile, w_first, stream)
+           : w_tile == kFf128x256 ? ff_pair_tile<T, FfTile128x256>(w, x, x_tile, w_first, stream)
+           : w_tile == kFf128x128 ? ff_pair_tile<T, FfTile128x128>(w, x, x_tile, w_first, stream)
+                                  : hipErrorInvalidValue;
 }
 
 template <typename T>

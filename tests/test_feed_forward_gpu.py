@@ -116,7 +116,7 @@ def check_backward(dout, x, w, bias, activation, grads, gated, gate_first=False)
     dz, edz = dz_of(dout, x, w.double(), bias, activation, gated, gate_first)
     h, tiny = HALF[x.dtype], TINY[x.dtype]
     x64, w64 = x.double(), w.double()
-    for what, got, want, mass, err, terms in (
+    for what, got, want, mass, err, terms in (  # (got None: not asked for)
         ("dx", dx, dz @ w64, dz.abs() @ w64.abs(), edz @ w64.abs(), w.shape[0]),
         ("dw", dw, dz.t() @ x64, dz.abs().t() @ x64.abs(), edz.t() @ x64.abs(), x.shape[0]),
         ("db", db, dz.sum(0), dz.abs().sum(0), edz.sum(0), x.shape[0]),
@@ -268,10 +268,22 @@ def test_every_tile_backward(rows, cols, dtype):
     check_backward(dout, x, w, None, "none", grads, False)
 
 
+# dw and dx in one launch, either one's tasks first, on every pair of their tiles that the sizes of a call lead to
+# (rows, columns, features)
+@pytest.mark.parametrize("m,n,k", [(2056, 1283, 328), (328, 2056, 1288), (2400, 200, 1800), (200, 2400, 1800), (4100, 648, 2056),
+                                   (648, 4100, 2056), (1111, 640, 640), (4104, 2056, 264), (70, 6001, 136)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_backward_in_one_launch(m, n, k, dtype):
+    x, w = values(1, m, k, dtype=dtype), values(2, n, k, std=k ** -0.5, dtype=dtype)
+    dout, bias = values(3, m, n, std=0.3, dtype=dtype), values(4, n, std=0.3, dtype=dtype)
+    check_backward(dout, x, w, bias, "gelu", sh.linear_act_backward(dout, x, w, bias=bias, activation="gelu"), False)
+
+
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("activation", ["none", "gelu"])
 def test_backward_parts(gated, activation):
-    """Each gradient alone is the one of the whole call; a bias gradient without a bias; nothing asked."""
+    """Each gradient alone (its product may run on another tile than in the whole call, so its sums' order may
+    differ); a bias gradient without a bias; nothing asked."""
     x, w = values(1, 100, 64), values(2, 80, 64, std=0.125)
     dout = values(3, 100, 40 if gated else 80)
     fn = sh.gated_linear_backward if gated else sh.linear_act_backward
@@ -281,7 +293,7 @@ def test_backward_parts(gated, activation):
         need = dict(zip(("need_dx", "need_dw", "need_dbias"), (part == 0, part == 1, part == 2)))
         alone = fn(dout, x, w, activation=activation, **need)
         assert [g is not None for g in alone] == [part == i for i in range(3)]
-        assert torch.equal(alone[part], whole[part])
+        check_backward(dout, x, w, None, activation, alone, gated)
     assert fn(dout, x, w, activation=activation, need_dx=False, need_dw=False, need_dbias=False) == (None, None, None)
 
 
