@@ -107,9 +107,9 @@ int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus,
 FfParams prepared(const FfParams& params, bool i_transposed) {
     FfParams p = params;
     if (p.i_row == 0) p.i_row = i_transposed ? p.rows : p.depth;
-    // 16-byte stores and 8-byte loads in the epilogue
-    p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 8) &&
-            aligned(p.dout, 8) && (p.residual == nullptr || p.ld_res % 4 == 0) && (p.dout == nullptr || p.ld_dout % 4 == 0);
+    // 16-byte accesses in the epilogue (bias: 8)
+    p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 16) &&
+            aligned(p.dout, 16) && (p.residual == nullptr || p.ld_res % 8 == 0) && (p.dout == nullptr || p.ld_dout % 8 == 0);
     return p;
 }
 

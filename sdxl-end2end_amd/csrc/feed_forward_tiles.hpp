@@ -372,6 +372,24 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
                 v[q] = F::lo((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, c + q < cols ? row_b + 2 * (c + q) : kOutside, 0, 0));
         }
     };
+    // 16 columns from c on of the lane's row: as loaded, 8 a lane, and as the sums lie (columns 8u + 4hf ..)
+    auto load16 = [&](__amdgpu_buffer_rsrc_t r, uint32_t row_b, int c) __attribute__((always_inline)) {
+        const int at = c + 8 * hf;
+        if (vec) return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at < cols ? row_b + 2 * at : kOutside, 0, 0));
+        u32x4 d{};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            d[e >> 1] |= (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at + e < cols ? row_b + 2 * (at + e) : kOutside, 0, 0)
+                         << (16 * (e & 1));
+        return d;
+    };
+    auto values16 = [&](u32x4 d, float (&v)[2][4]) __attribute__((always_inline)) {
+        uint32_t a0 = d[0], a1 = d[1], b0 = d[2], b1 = d[3];
+        join_halves(a0, b0);
+        join_halves(a1, b1);
+        v[0][0] = F::lo(a0), v[0][1] = F::hi(a0), v[0][2] = F::lo(a1), v[0][3] = F::hi(a1);
+        v[1][0] = F::lo(b0), v[1][1] = F::hi(b0), v[1][2] = F::lo(b1), v[1][3] = F::hi(b1);
+    };
     auto load4f = [&](__amdgpu_buffer_rsrc_t r, int c, float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -402,11 +420,35 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
         if (j0 + kCols >= p.cols && wj == 0 && hf == 0 && (int64_t)row < i_rows)
             for (int64_t z = first; z < p.out_cols_padded; ++z) ((T*)p.out)[(i0 + row) * p.ld_out + z] = (T)0.0f;
     };
-    const FfAct act = ff_act(p.activation);
     const uint32_t ldo_b = (uint32_t)(p.ld_out * 2), ldd_b = (uint32_t)(p.ld_dout * 2), ldr_b = (uint32_t)(p.ld_res * 2);
     const auto dout = rows_window(p.dout, p.ld_dout, j0), residual = rows_window(p.residual, p.ld_res, j0);
     const auto out = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? value_row : 0) + j0);
     const auto out_g = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? gate_row : 0) + j0);
+    // What the epilogue reads of a tile (dout, or the residual): requested for all of the wave's tiles first where the
+    // registers hold that, so that its latency passes once (256 x 256, dz [8192, 10240] 258 -> 239 us), else tile by tile.
+    constexpr int kSets = kGated ? 1 : 2;  // of 16 columns
+    constexpr bool kReads = kEpi == kFfLinear || kEpi == kFfLinearDz || kEpi == kFfGatedDz;
+    constexpr bool kAhead = kReads && kWK == 1 && kMI * kMJ * kSets <= 8;
+    u32x4 ahead[kAhead ? kMJ : 1][kAhead ? kMI : 1][kSets];
+    auto read_tile = [&](uint32_t row, int c0, u32x4 (&d)[kSets]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < kSets; ++h) {
+            if constexpr (kEpi == kFfLinear) {
+                if (p.residual != nullptr) d[h] = load16(residual, row * ldr_b, c0 + 16 * h);
+                else d[h] = u32x4{};
+            } else {
+                d[h] = load16(dout, row * ldd_b, c0 + 16 * h);
+            }
+        }
+    };
+    if constexpr (kAhead) {
+#pragma unroll
+        for (int t = 0; t < kMJ; ++t)
+#pragma unroll
+            for (int s = 0; s < kMI; ++s) read_tile(wave_row + 32 * kWI * s, wave_col + (kGated ? 16 : 32) * kWJ * t, ahead[t][s]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    const FfAct act = ff_act(p.activation);
     constexpr int kHalves = kGated ? 2 : 4;  // groups of 4 columns of a lane: value (and gate) columns 8u + 4hf ..
     float bias[kHalves][4], scale[kHalves][4], bias_g[2][4], scale_g[2][4];
     // the columns' constants of the tile from column c0 of C's tile on
@@ -432,14 +474,13 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
             }
         }
     };
-    // one 32 x 32 tile of sums: the lane's row of C's tile, first column c0
-    auto finish = [&]<FfFamily kFam>(const f32x16& z, uint32_t row, int c0) __attribute__((always_inline)) {
+    // one 32 x 32 tile of sums: the lane's row of C's tile, first column c0, what read_tile gave
+    auto finish = [&]<FfFamily kFam>(const f32x16& z, uint32_t row, int c0, const u32x4 (&in)[kSets]) __attribute__((always_inline)) {
         if constexpr (kGated) {
-            float va[2][4], vb[2][4];
+            float va[2][4], vb[2][4], d[2][4];
+            if constexpr (kEpi == kFfGatedDz) values16(in[0], d);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float d[4];
-                if constexpr (kEpi == kFfGatedDz) load4(dout, row * ldd_b, c0 + 8 * u + 4 * hf, d);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float v = __builtin_fmaf(z[4 * u + q], scale[u][q], bias[u][q]);
@@ -449,33 +490,31 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
                     } else {
                         float a;
                         const float sl = ff_slope<kFam>(act, g, a);
-                        va[u][q] = d[q] * a;
-                        vb[u][q] = d[q] * v * sl;
+                        va[u][q] = d[u][q] * a;
+                        vb[u][q] = d[u][q] * v * sl;
                     }
                 }
             }
             store8(out, row * ldo_b, c0, va[0], va[1]);
             if constexpr (kEpi == kFfGatedDz) store8(out_g, row * ldo_b, c0, vb[0], vb[1]);
         } else {
-            float v[4][4];
+            float v[4][4], d[2][2][4] = {};
+            if (kEpi == kFfLinearDz || (kEpi == kFfLinear && p.residual != nullptr)) {
+                values16(in[0], d[0]);
+                values16(in[kSets - 1], d[1]);
+            }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                float d[4] = {};
-                if constexpr (kEpi == kFfLinearDz) {
-                    load4(dout, row * ldd_b, c0 + 8 * u + 4 * hf, d);
-                } else if constexpr (kEpi == kFfLinear) {
-                    if (p.residual != nullptr) load4(residual, row * ldr_b, c0 + 8 * u + 4 * hf, d);
-                }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float sum = z[4 * u + q];
                     if constexpr (kEpi == kFfStore) {
                         v[u][q] = sum;
                     } else if constexpr (kEpi == kFfLinear) {
-                        v[u][q] = ff_value<kFam>(act, __builtin_fmaf(sum, scale[u][q], bias[u][q])) + d[q];
+                        v[u][q] = ff_value<kFam>(act, __builtin_fmaf(sum, scale[u][q], bias[u][q])) + d[u >> 1][u & 1][q];
                     } else {
                         float a;
-                        v[u][q] = ff_slope<kFam>(act, __builtin_fmaf(sum, scale[u][q], bias[u][q]), a) * d[q];
+                        v[u][q] = ff_slope<kFam>(act, __builtin_fmaf(sum, scale[u][q], bias[u][q]), a) * d[u >> 1][u & 1][q];
                     }
                 }
             }
@@ -490,7 +529,16 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
                 const int c0 = wave_col + (kGated ? 16 : 32) * kWJ * t;
                 constants(c0);
 #pragma unroll
-                for (int s = 0; s < kMI; ++s) finish.template operator()<kFam>(acc[t][s], wave_row + 32 * kWI * s, c0);
+                for (int s = 0; s < kMI; ++s) {
+                    const uint32_t row = wave_row + 32 * kWI * s;
+                    if constexpr (kAhead) {
+                        finish.template operator()<kFam>(acc[t][s], row, c0, ahead[t][s]);
+                    } else {
+                        u32x4 in[kSets];
+                        if constexpr (kReads) read_tile(row, c0, in);
+                        finish.template operator()<kFam>(acc[t][s], row, c0, in);
+                    }
+                }
             }
         } else {
             // The depth shares' sums meet in LDS, kWK tiles a round: group wk of the
@@ -538,7 +586,10 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
                     }
                     const int c0 = wave_col + (kGated ? 16 : 32) * kWJ * (q / kMI);
                     constants(c0);
-                    finish.template operator()<kFam>(sum, wave_row + 32 * kWI * (q % kMI), c0);
+                    const uint32_t row = wave_row + 32 * kWI * (q % kMI);
+                    u32x4 in[kSets];
+                    if constexpr (kReads) read_tile(row, c0, in);
+                    finish.template operator()<kFam>(sum, row, c0, in);
                 }
             }
         }
