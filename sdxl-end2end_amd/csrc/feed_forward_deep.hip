@@ -120,9 +120,6 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
 
     const FfAct act = ff_act(p.activation);
     const FfFamily fam = ff_family(p.activation);
-    auto act_of = [&](float z) {
-        return fam == kFamErf ? ff_value<kFamErf>(act, z) : fam == kFamSigmoid ? ff_value<kFamSigmoid>(act, z) : ff_value<kFamLinear>(act, z);
-    };
     auto sum_of = [&](int u) {
         f32x4 s{};
 #pragma unroll
@@ -147,8 +144,8 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
         for (int q = 0; q < 4; ++q) {
             v[q] = 0.0f;
             if (c + q >= p.cols) continue;
-            if constexpr (kGated) v[q] = z_of(a[q], value_row + c + q) * act_of(z_of(b[q], gate_row + c + q));
-            else v[q] = act_of(z_of(a[q], c + q)) + (p.residual != nullptr ? (float)((const T*)p.residual)[i * p.ld_res + c + q] : 0.0f);
+            if constexpr (kGated) v[q] = z_of(a[q], value_row + c + q) * ff_value_of(act, fam, z_of(b[q], gate_row + c + q));
+            else v[q] = ff_value_of(act, fam, z_of(a[q], c + q)) + (p.residual != nullptr ? (float)((const T*)p.residual)[i * p.ld_res + c + q] : 0.0f);
         }
         T* out = (T*)p.out + i * p.ld_out + c;
         if (p.vec && c < p.cols) {

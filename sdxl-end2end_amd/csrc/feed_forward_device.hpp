@@ -83,19 +83,19 @@ __device__ __forceinline__ void window_to_lds(u32x4 rsrc, uint32_t voff, uint32_
 
 constexpr uint32_t kOutside = 0x80000000u;  // past every window (their sizes stay below 2^31)
 
-// ---- activations. Three families share the kernels, chosen once per
-// workgroup (the activation is uniform): z and relu; z sigmoid(z (c0 + c1
-// z^2)), which is silu, quick gelu and the tanh form of gelu (1 + tanh u = 2
+// ---- activations, in families that a workgroup chooses from once (the
+// activation is uniform): z and relu; z sigmoid(c0 z), which is silu and quick
+// gelu; z sigmoid(z (c0 + c1 z^2)), the tanh form of gelu (1 + tanh u = 2
 // sigmoid(2u)); and gelu. Infinite z takes the limit, NaN stays NaN.
 struct FfAct {
     float lo, kink;  // z < lo becomes lo; slope 0 at z <= kink (NaN: nowhere)
     float c0, c1;    // of the sigmoid's argument
 };
 
-enum FfFamily { kFamLinear = 0, kFamSigmoid = 1, kFamErf = 2 };
+enum FfFamily { kFamLinear, kFamSigmoid, kFamTanh, kFamErf };
 
 __device__ __forceinline__ FfFamily ff_family(int32_t activation) {
-    return activation == SDXL_ACT_GELU ? kFamErf : activation <= SDXL_ACT_RELU ? kFamLinear : kFamSigmoid;
+    return activation == SDXL_ACT_GELU ? kFamErf : activation <= SDXL_ACT_RELU ? kFamLinear : activation == SDXL_ACT_GELU_TANH ? kFamTanh : kFamSigmoid;
 }
 
 __device__ __forceinline__ FfAct ff_act(int32_t activation) {
@@ -105,7 +105,7 @@ __device__ __forceinline__ FfAct ff_act(int32_t activation) {
     a.kink = relu ? 0.0f : __builtin_nanf("");
     const float tanh_c = 1.5957691216057308f;  // 2 sqrt(2 / pi)
     a.c0 = activation == SDXL_ACT_QUICK_GELU ? 1.702f : activation == SDXL_ACT_GELU_TANH ? tanh_c : 1.0f;
-    a.c1 = activation == SDXL_ACT_GELU_TANH ? tanh_c * 0.044715f : 0.0f;
+    a.c1 = tanh_c * 0.044715f;
     return a;
 }
 
@@ -127,15 +127,19 @@ __device__ __forceinline__ float ff_tail(float x, float& e, float& ax) {
     return e * (t * r);
 }
 
+// sigmoid of the two families' argument; z2 (tanh form): min(z^2, 1e30), so that c1 z^2 stays finite
+template <FfFamily kFam>
+__device__ __forceinline__ float ff_sigmoid(const FfAct& a, float z, float z2) {
+    const float c = kFam == kFamTanh ? __builtin_fmaf(a.c1, z2, a.c0) : a.c0;
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * (c * -1.4426950408889634f)));
+}
+
 template <FfFamily kFam>
 __device__ __forceinline__ float ff_value(const FfAct& a, float z) {
     if constexpr (kFam == kFamLinear) {
         return z < a.lo ? a.lo : z;
-    } else if constexpr (kFam == kFamSigmoid) {
-        const float z2 = __builtin_fminf(z * z, 1.0e30f);
-        const float s = __builtin_amdgcn_rcpf(
-            1.0f + __builtin_amdgcn_exp2f(z * __builtin_fmaf(a.c1, z2, a.c0) * -1.4426950408889634f));
-        return __builtin_fmaxf(z, -1.0e30f) * s;
+    } else if constexpr (kFam != kFamErf) {
+        return __builtin_fmaxf(z, -1.0e30f) * ff_sigmoid<kFam>(a, z, __builtin_fminf(z * z, 1.0e30f));
     } else {
         float e, ax;
         const float q = ff_tail(z, e, ax);
@@ -149,19 +153,39 @@ __device__ __forceinline__ float ff_slope(const FfAct& a, float z, float& value)
     if constexpr (kFam == kFamLinear) {
         value = z < a.lo ? a.lo : z;
         return z <= a.kink ? 0.0f : 1.0f;
-    } else if constexpr (kFam == kFamSigmoid) {
+    } else if constexpr (kFam != kFamErf) {
         const float z2 = __builtin_fminf(z * z, 1.0e30f);
-        const float s = __builtin_amdgcn_rcpf(
-            1.0f + __builtin_amdgcn_exp2f(z * __builtin_fmaf(a.c1, z2, a.c0) * -1.4426950408889634f));
+        const float s = ff_sigmoid<kFam>(a, z, z2);
         value = __builtin_fmaxf(z, -1.0e30f) * s;
         const float zc = __builtin_amdgcn_fmed3f(z, -1.0e30f, 1.0e30f);
-        return __builtin_fmaf((zc * s) * (1.0f - s), __builtin_fmaf(3.0f * a.c1, z2, a.c0), s);
+        return __builtin_fmaf((zc * s) * (1.0f - s), kFam == kFamTanh ? __builtin_fmaf(3.0f * a.c1, z2, a.c0) : a.c0, s);
     } else {
         float e, ax;
         const float q = ff_tail(z, e, ax);
         value = __builtin_fmaf(-ax, q, __builtin_fmaxf(z, 0.0f));
         const float zc = __builtin_amdgcn_fmed3f(z, -40.0f, 40.0f);
         return __builtin_fmaf(zc * 0.3989422804014327f, e, z > 0.0f ? 1.0f - q : q);
+    }
+}
+
+// act(z) where the family is not a constant
+__device__ __forceinline__ float ff_value_of(const FfAct& a, FfFamily fam, float z) {
+    switch (fam) {
+    case kFamErf: return ff_value<kFamErf>(a, z);
+    case kFamTanh: return ff_value<kFamTanh>(a, z);
+    case kFamSigmoid: return ff_value<kFamSigmoid>(a, z);
+    default: return ff_value<kFamLinear>(a, z);
+    }
+}
+
+// f.operator()<family>() of the activation
+template <typename Fn>
+__device__ __forceinline__ void ff_with_family(int32_t activation, Fn&& f) {
+    switch (ff_family(activation)) {
+    case kFamErf: f.template operator()<kFamErf>(); break;
+    case kFamTanh: f.template operator()<kFamTanh>(); break;
+    case kFamSigmoid: f.template operator()<kFamSigmoid>(); break;
+    default: f.template operator()<kFamLinear>(); break;
     }
 }
 

@@ -35,7 +35,6 @@ __global__ __launch_bounds__(256) void ff_general_kernel(FfParams p) {
     const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, col = lane & 31;
     const int wi = tid >> 7, wj = (tid >> 6) & 1;
     const FfAct act = ff_act(p.activation);
-    const FfFamily fam = ff_family(p.activation);
     const int64_t value_row = p.gate_first ? p.cols : 0, gate_row = p.gate_first ? 0 : p.cols;
     const int64_t i_blocks = (p.rows + kGTile - 1) / kGTile, j_blocks = (p.cols + kCols - 1) / kCols;
 
@@ -141,9 +140,7 @@ __global__ __launch_bounds__(256) void ff_general_kernel(FfParams p) {
             }
         };
         if constexpr (kEpi == kFfStore) epilogue.template operator()<kFamLinear>();
-        else if (fam == kFamErf) epilogue.template operator()<kFamErf>();
-        else if (fam == kFamSigmoid) epilogue.template operator()<kFamSigmoid>();
-        else epilogue.template operator()<kFamLinear>();
+        else ff_with_family(p.activation, epilogue);
     }
 }
 

@@ -126,9 +126,6 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
         if (p.bias != nullptr) sum += (float)((const T*)p.bias)[row];
         return sum;
     };
-    auto act_of = [&](float z) {
-        return fam == kFamErf ? ff_value<kFamErf>(act, z) : fam == kFamSigmoid ? ff_value<kFamSigmoid>(act, z) : ff_value<kFamLinear>(act, z);
-    };
     if (threadIdx.x < (kGated ? 32 : 64)) {
         const int64_t i = r16;
         if (i >= p.rows) return;
@@ -141,9 +138,9 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
             const int64_t n = c0 + 4 * g + e;
             if (n >= p.cols) continue;
             if constexpr (kGated) {
-                out[n] = (T)(z_of(a[e], value_row + n) * act_of(z_of(b[e], gate_row + n)));
+                out[n] = (T)(z_of(a[e], value_row + n) * ff_value_of(act, fam, z_of(b[e], gate_row + n)));
             } else {
-                float v = act_of(z_of(a[e], n));
+                float v = ff_value_of(act, fam, z_of(a[e], n));
                 if (p.residual != nullptr) v += (float)((const T*)p.residual)[i * p.ld_res + n];
                 out[n] = (T)v;
             }

@@ -629,10 +629,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
             }
         }
     } else {
-        const FfFamily fam = ff_family(p.activation);
-        if (fam == kFamErf) epilogue.template operator()<kFamErf>();
-        else if (fam == kFamSigmoid) epilogue.template operator()<kFamSigmoid>();
-        else epilogue.template operator()<kFamLinear>();
+        ff_with_family(p.activation, epilogue);
     }
 }
 
