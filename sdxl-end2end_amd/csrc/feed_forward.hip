@@ -2,6 +2,7 @@
 // rows 16-byte accesses divide (feed_forward_tiles.hpp, feed_forward_deep.hip).
 #include <hip/hip_runtime.h>
 
+#include "feed_forward_device.hpp"
 #include "feed_forward_kernels.hpp"
 
 namespace sdxl_hip {
@@ -108,9 +109,79 @@ FfParams prepared(const FfParams& params, bool i_transposed) {
     FfParams p = params;
     if (p.i_row == 0) p.i_row = i_transposed ? p.rows : p.depth;
     // 16-byte accesses in the epilogue (bias: 8)
+    p.splits = 1;
     p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 16) &&
             aligned(p.dout, 16) && (p.residual == nullptr || p.ld_res % 8 == 0) && (p.dout == nullptr || p.ld_dout % 8 == 0);
     return p;
+}
+
+// ---- dw and dx in one launch. A side of it: a product on a tile, its depth in so many shares.
+constexpr int kPairTiles = 3, kPairTile[kPairTiles] = {kFf256x256, kFf128x256, kFf128x128};
+constexpr int kSplitSteps = 4, kMaxSplits = 1 << (kSplitSteps - 1);
+constexpr size_t kMaxPartial = 32 << 20;  // partial sums of a call, bytes
+// the joining pass
+constexpr float kJoinStart = 3.0f, kJoinPerByte = 0.4e-6f;
+
+struct PairSide {
+    int64_t tasks, partial;  // bytes
+    float time;              // of a task
+};
+
+int share_stages(const FfParams& p, int splits) { return (int)(((p.depth + 63) / 64 + splits - 1) / splits); }
+
+PairSide pair_side(const FfParams& p, int tile, int splits) {
+    const TileCost& c = kTiles[tile];
+    const int64_t tiles = ((p.rows + c.rows - 1) / c.rows) * ((p.cols + c.cols - 1) / c.cols);
+    const int stages = share_stages(p, splits);
+    // (no share may be empty, and few stages are not worth a start)
+    const bool ok = splits == 1 || (stages >= 8 && (int64_t)stages * 64 * (splits - 1) < p.depth);
+    const int64_t sums = splits == 1 ? 0 : splits * p.rows * (p.cols + (p.row_sums != nullptr ? 1 : 0));
+    return {ok ? tiles * splits : (int64_t)1 << 30, (sums * 4 + 255) / 256 * 256, (float)stages * c.alone + c.ends - 2.0f};
+}
+
+void set_splits(FfParams& p, int splits, float* partial) {
+    p.splits = splits;
+    p.share_stages = share_stages(p, splits);
+    p.partial = partial;
+}
+
+FfJoin join_of(const FfParams& p) {
+    if (p.splits == 1) return {};
+    const int64_t threads = p.rows * (p.cols / 8) + (p.row_sums != nullptr ? p.rows : 0);
+    return {p.partial, p.out, p.row_sums, p.ld_out, (int32_t)p.rows, (int32_t)p.cols, p.splits, p.vec, (int32_t)((threads + 255) / 256)};
+}
+
+// Adds the shares in their order, 8 columns a thread (or one row sum), and rounds once. Bound by the reads, which come
+// out of the Infinity Cache.
+template <typename T>
+__global__ __launch_bounds__(256) void ff_join_kernel(FfJoin a, FfJoin b) {
+    using F = FfType<T>;
+    const bool second = (int)blockIdx.x >= a.blocks;
+    const FfJoin& p = second ? b : a;
+    const uint32_t at = (blockIdx.x - (second ? a.blocks : 0)) * 256 + threadIdx.x;
+    const uint32_t chunks = p.cols / 8, all = p.rows * chunks;
+    const size_t share = (size_t)p.rows * p.cols;
+    if (at < all) {
+        float v[8] = {};
+        for (int s = 0; s < p.splits; ++s) {
+            const f32x4* from = (const f32x4*)(p.partial + s * share + (size_t)at * 8);
+            const f32x4 lo = from[0], hi = from[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
+        }
+        T* out = (T*)p.out + (int64_t)(at / chunks) * p.ld_out + (at % chunks) * 8;
+        if (p.vec) {
+            *(u32x4*)out = u32x4{F::pack(v[0], v[1]), F::pack(v[2], v[3]), F::pack(v[4], v[5]), F::pack(v[6], v[7])};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = (T)v[e];
+        }
+    } else if (p.row_sums != nullptr && at - all < (uint32_t)p.rows) {
+        const float* sums = p.partial + p.splits * share + (at - all);
+        float v = 0.0f;
+        for (int s = 0; s < p.splits; ++s) v += sums[(size_t)s * p.rows];
+        ((T*)p.row_sums)[at - all] = (T)v;
+    }
 }
 
 }  // namespace
@@ -141,37 +212,61 @@ hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_t
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);
 }
 
-hipError_t launch_ff_pair(const FfParams& dw, const FfParams& dx, bool bf16, int compute_units, hipStream_t stream) {
-    const FfParams w = prepared(dw, true), x = prepared(dx, false);
+size_t ff_partial_bytes(int64_t m, int64_t features, int64_t k) {
+    const double all = 4.0 * kMaxSplits * ((double)m * (double)k + (double)features * (double)(k + 1)) + 1024.0;
+    return m <= 0 || features <= 0 || k <= 0 ? 0 : all < (double)kMaxPartial ? ((size_t)all + 255) / 256 * 256 : kMaxPartial;
+}
+
+hipError_t launch_ff_pair(const FfParams& dw, const FfParams& dx, bool bf16, float* partial, size_t partial_bytes,
+                          int compute_units, hipStream_t stream) {
+    FfParams w = prepared(dw, true), x = prepared(dx, false);
     const int64_t cus = compute_units > 0 ? compute_units : 256;
-    // apart, or together on the best pair of tiles that take a CU each. Together was measured against apart on
-    // an MI355X at [2048, 1280] x [10240, 1280] 142 -> 107 us, [8192, 1280] x [10240, 1280] 459 -> 360.
+    // apart, or together on the best pair of tiles that take a CU each, of whole depths or of shares of them.
+    // Measured on an MI355X, dw and dx of x [m, k], w [f, k]: m 2048, k 1280, f 10240 apart 142 us, together 117;
+    // m 8192 apart 459, together 368; m 1111, k 640, f 5120 (two tasks in five CUs) together 42, with dx's depth in
+    // 2 shares 28.6 and 4 for the joining pass.
     float apart_w, apart_x;
     choose_tile(w, kFfStore, false, cus, apart_w);
     choose_tile(x, kFfStore, false, cus, apart_x);
     float best = apart_w + apart_x;
-    int best_w = -1, best_x = -1;
+    int best_w = -1, best_x = -1, w_splits = 1, x_splits = 1;
     bool w_first = true;
-    constexpr int kPairTiles[3] = {kFf256x256, kFf128x256, kFf128x128};
-    for (int tw : kPairTiles) {
-        const TileCost& cw = kTiles[tw];
-        const int64_t nw = ((w.rows + cw.rows - 1) / cw.rows) * ((w.cols + cw.cols - 1) / cw.cols);
-        const float time_w = (float)((w.depth + 63) / 64) * cw.alone + cw.ends - 2.0f;
-        for (int tx : kPairTiles) {
-            const TileCost& cx = kTiles[tx];
-            const int64_t nx = ((x.rows + cx.rows - 1) / cx.rows) * ((x.cols + cx.cols - 1) / cx.cols);
-            const float time_x = (float)((x.depth + 63) / 64) * cx.alone + cx.ends - 2.0f;
-            const bool first = time_w >= time_x;
-            const float time = 2.0f + (first ? list_time(nw, time_w, nx, time_x, cus) : list_time(nx, time_x, nw, time_w, cus));
-            if (time < best && nw + nx <= (1 << 23)) {
-                best = time;
-                best_w = tw;
-                best_x = tx;
-                w_first = first;
-            }
+    PairSide sides[2][kPairTiles][kSplitSteps];
+    for (int side = 0; side < 2; ++side)
+        for (int t = 0; t < kPairTiles; ++t)
+            for (int s = 0; s < kSplitSteps; ++s) sides[side][t][s] = pair_side(side == 0 ? w : x, kPairTile[t], 1 << s);
+    for (int i = 0; i < kPairTiles * kSplitSteps * kPairTiles * kSplitSteps; ++i) {
+        const int tw = i / (kSplitSteps * kPairTiles * kSplitSteps), tx = i / kSplitSteps % kPairTiles;
+        const int sw = i / (kPairTiles * kSplitSteps) % kSplitSteps, sx = i % kSplitSteps;
+        const PairSide &a = sides[0][tw][sw], &b = sides[1][tx][sx];
+        const int64_t partial_size = a.partial + b.partial;
+        if (a.tasks + b.tasks > (1 << 23) || partial_size > (int64_t)partial_bytes) continue;
+        const float join = partial_size == 0 ? 0.0f : kJoinStart + (float)partial_size * kJoinPerByte;
+        const float least = ((float)a.tasks * a.time + (float)b.tasks * b.time) / (float)cus;
+        if (2.0f + join + least >= best) continue;
+        const bool first = a.time >= b.time;
+        const float time = 2.0f + join + (first ? list_time(a.tasks, a.time, b.tasks, b.time, cus)
+                                                : list_time(b.tasks, b.time, a.tasks, a.time, cus));
+        if (time < best) {
+            best = time;
+            best_w = kPairTile[tw];
+            best_x = kPairTile[tx];
+            w_splits = 1 << sw;
+            x_splits = 1 << sx;
+            w_first = first;
         }
     }
-    if (best_w >= 0) return (bf16 ? ff_pair_bf16 : ff_pair_f16)(w, x, best_w, best_x, w_first, stream);
+    if (best_w >= 0) {
+        set_splits(w, w_splits, partial);
+        set_splits(x, x_splits, partial + (size_t)pair_side(w, best_w, w_splits).partial / 4);
+        const hipError_t err = (bf16 ? ff_pair_bf16 : ff_pair_f16)(w, x, best_w, best_x, w_first, stream);
+        if (err != hipSuccess || (w.splits == 1 && x.splits == 1)) return err;
+        const FfJoin jw = join_of(w), jx = join_of(x);
+        const dim3 grid((unsigned)(jw.blocks + jx.blocks));
+        if (bf16) hipLaunchKernelGGL(ff_join_kernel<__bf16>, grid, dim3(256), 0, stream, jw, jx);
+        else hipLaunchKernelGGL(ff_join_kernel<_Float16>, grid, dim3(256), 0, stream, jw, jx);
+        return hipGetLastError();
+    }
     const hipError_t err = launch_ff_tiled(dw, kFfStore, true, bf16, false, compute_units, stream);
     return err != hipSuccess ? err : launch_ff_tiled(dx, kFfStore, false, bf16, false, compute_units, stream);
 }

@@ -120,13 +120,18 @@ sdxl_status forward(const sdxl_ff_desc* d, bool gated, const char* name, const v
                    reinterpret_cast<hipStream_t>(stream), name);
 }
 
+size_t round256(size_t v) { return (v + 255) / 256 * 256; }
+
 // Backward workspace: dz [m, features] with rows of a multiple of 8 elements
 // (16 bytes), unless the product can take dout itself (no activation).
 int64_t dz_stride(const Call& c) { return (c.features + 7) / 8 * 8; }
 bool needs_dz(const Call& c) { return c.gated || c.activation != SDXL_ACT_NONE; }
 size_t dz_bytes(const Call& c) { return needs_dz(c) ? (size_t)c.m * (size_t)dz_stride(c) * 2 : 0; }
 
-size_t backward_workspace(const Call& c) { return dz_bytes(c); }
+// then the partial sums of products whose depth is split
+size_t backward_workspace(const Call& c) {
+    return round256(dz_bytes(c)) + sdxl_hip::ff_partial_bytes(c.m, c.features, c.k);
+}
 
 size_t workspace_of(const sdxl_ff_desc* d, bool gated, const char* name) {
     Call c;
@@ -190,9 +195,11 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     px.out = dx;
     px.ld_out = c.lddx;
     if (dz_needed) pw.i_row = px.i_row = lddz;
+    float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(dz_bytes(c)));
     if (want_dw && want_dx && sdxl_hip::ff_tiled_supported(pw, sdxl_hip::kFfStore, true, true, false) &&
         sdxl_hip::ff_tiled_supported(px, sdxl_hip::kFfStore, false, true, false))
-        return launch_status(sdxl_hip::launch_ff_pair(pw, px, c.bf16, sdxl_hip_compute_units(), stream), name);
+        return launch_status(sdxl_hip::launch_ff_pair(pw, px, c.bf16, partial, sdxl_hip::ff_partial_bytes(c.m, c.features, c.k),
+                                                      sdxl_hip_compute_units(), stream), name);
     if (want_dw || want_db) {
         st = product(pw, sdxl_hip::kFfStore, true, true, c, false, stream, name);
         if (st != SDXL_STATUS_OK) return st;
@@ -200,9 +207,6 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     if (want_dx) st = product(px, sdxl_hip::kFfStore, false, true, c, false, stream, name);
     return st;
 }
-
-// The sublayer's workspace: the normalised rows, then the gated activations.
-size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 
 sdxl_status sublayer_shape(const sdxl_ff_sublayer_desc* d) {
     const char* name = "sdxl_ff_sublayer";
@@ -222,6 +226,7 @@ sdxl_status sublayer_shape(const sdxl_ff_sublayer_desc* d) {
     return SDXL_STATUS_OK;
 }
 
+// The sublayer's workspace: the normalised rows, then the gated activations.
 size_t sublayer_workspace(const sdxl_ff_sublayer_desc* d) {
     return round256((size_t)d->rows * (size_t)d->width * 2) + round256((size_t)d->rows * (size_t)d->inner * 2);
 }

@@ -80,8 +80,8 @@ struct FfTile {
 };
 
 // Task `id` of a product whose tasks' numbers modulo 8 are their XCDs; smem: Tile::smem_bytes.
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
-__device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false>
+__device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* smem) {
     constexpr int kWI = Tile::kWI, kWJ = Tile::kWJ, kWK = Tile::kWK, kMI = Tile::kMI, kMJ = Tile::kMJ, kRing = Tile::kRing;
     using F = FfType<T>;
     constexpr bool kGated = kEpi == kFfGated || kEpi == kFfGatedDz;
@@ -107,17 +107,22 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave % kWI, wj = wave / kWI % kWJ, wk = kWK > 1 ? wave / (kWI * kWJ) : 0;
     const int64_t value_row = p.gate_first ? p.cols : 0, gate_row = p.gate_first ? 0 : p.cols;
-    const int n_stages = (int)((p.depth + 63) / 64);
     const int64_t ldi_b = p.ld_i * 2, ldj_b = p.ld_j * (kJFp8 ? 1 : 2);
+    // the workgroup's share of the depth: from depth0 on
+    static_assert(!kSplit || kEpi == kFfStore, "shares are joined before an epilogue");
+    const int n_tiles = p.i_blocks * p.j_blocks, share = kSplit ? task_id / n_tiles : 0, id = kSplit ? task_id % n_tiles : task_id;
+    const int64_t depth0 = kSplit ? (int64_t)share * p.share_stages * 64 : 0;
+    const int64_t depth = kSplit ? min64(p.depth - depth0, (int64_t)p.share_stages * 64) : p.depth;
+    const int64_t i_row = kIT ? p.i_row : p.i_row - depth0;  // (by columns the row runs along C)
+    const int n_stages = (int)((depth + 63) / 64);
 
     // ---- task: each XCD takes one contiguous range of them, in groups of
     // group_i row blocks (rows fastest, then columns), so that its workgroups
     // share I rows and J rows in its L2
     int64_t i0, j0;
     {
-        const int n = p.i_blocks * p.j_blocks;
         const int xcd = id & 7, slot = id >> 3;
-        const int per = n >> 3, extra = n & 7;
+        const int per = n_tiles >> 3, extra = n_tiles & 7;
         const int task = xcd * per + (xcd < extra ? xcd : extra) + slot;
         const int in_group = p.group_i * p.j_blocks;
         const int first = (task / in_group) * p.group_i;
@@ -135,28 +140,28 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
     Window iw, jw;
     uint32_t i_lane, j_lane;  // the lane's offset in a transfer
     if constexpr (kIT) {
-        iw.base = (const char*)p.ip + i0 * 2;
+        iw.base = (const char*)p.ip + i0 * 2 + depth0 * ldi_b;
         i_lane = (uint32_t)(row8 * ldi_b) + chunk8 * 16;
     } else {
-        iw.base = (const char*)p.ip + i0 * ldi_b;
+        iw.base = (const char*)p.ip + i0 * ldi_b + depth0 * 2;
         i_lane = (uint32_t)(row8 * ldi_b) + chunk8 * 16;
     }
     const int64_t j_first = kGated ? j0 + ((kJFp8 ? wave & 1 : wave & 2) ? gate_row : value_row) : j0;
-    if constexpr (kJT) jw.base = (const char*)p.jp + j0 * 2;
-    else jw.base = (const char*)p.jp + j_first * ldj_b;
+    if constexpr (kJT) jw.base = (const char*)p.jp + j0 * 2 + depth0 * ldj_b;
+    else jw.base = (const char*)p.jp + j_first * ldj_b + depth0 * (kJFp8 ? 1 : 2);
     j_lane = kJFp8 ? (uint32_t)(row16 * ldj_b) + chunk16 * 16 : (uint32_t)(row8 * ldj_b) + chunk8 * 16;
     const int64_t i_rows = min64(p.rows - i0, kBI), j_rows = min64(p.cols - j0, kGated ? kCols : kBJ);
     // window of stage st: everything from its first byte to the last valid one
     // (past the last stage: nothing, its transfers write zeros that nobody reads)
     auto i_window = [&](int st) __attribute__((always_inline)) {
-        const int64_t left = p.depth - (int64_t)st * 64;
+        const int64_t left = depth - (int64_t)st * 64;
         const char* base = iw.base + (kIT ? (int64_t)st * 64 * ldi_b : (int64_t)st * 128);
-        const int64_t size = kIT ? (min64(left, 64) - 1) * ldi_b + min64(p.i_row - i0, kBI) * 2
-                                 : (i_rows - 1) * ldi_b + (p.i_row - (int64_t)st * 64) * 2;
+        const int64_t size = kIT ? (min64(left, 64) - 1) * ldi_b + min64(i_row - i0, kBI) * 2
+                                 : (i_rows - 1) * ldi_b + (i_row - (int64_t)st * 64) * 2;
         return window_rsrc({base, left > 0 ? (uint32_t)size : 0u});
     };
     auto j_window = [&](int st) __attribute__((always_inline)) {
-        const int64_t left = p.depth - (int64_t)st * 64;
+        const int64_t left = depth - (int64_t)st * 64;
         const char* base = jw.base + (kJT ? (int64_t)st * 64 * ldj_b : (int64_t)st * (kJFp8 ? 64 : 128));
         const int64_t size = kJT ? (min64(left, 64) - 1) * ldj_b + j_rows * 2 : (j_rows - 1) * ldj_b + left * (kJFp8 ? 1 : 2);
         return window_rsrc({base, left > 0 ? (uint32_t)size : 0u});
@@ -166,7 +171,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
     auto issue = [&](int st, int buffer, int x, u32x4 irsrc, u32x4 jrsrc) __attribute__((always_inline)) {
         const uint32_t buf = lds0 + buffer * kStage;
         // depth of the stage, by I's rows and by J's
-        const int i_left = (int)min64(p.i_row - (int64_t)st * 64, 64), left = (int)min64(p.depth - (int64_t)st * 64, 64);
+        const int i_left = (int)min64(i_row - (int64_t)st * 64, 64), left = (int)min64(depth - (int64_t)st * 64, 64);
         if (x < kIX) {
             const int n = x * kWaves + wave;
             if (kIXfers % kWaves != 0 && n >= kIXfers) return;
@@ -529,7 +534,18 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
             store8(out, row * ldo_b, c0 + 16, v[2], v[3]);
         }
     };
-    auto epilogue = [&]<FfFamily kFam>() __attribute__((always_inline)) {
+    // a share's sums, 4 columns a lane
+    auto store_share = [&](const f32x16& z, uint32_t row, int c0) __attribute__((always_inline)) {
+        const uint64_t b = (uint64_t)(uintptr_t)p.partial + (uint64_t)(((share * p.rows + i0) * p.cols + j0) * 4);
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)b, 0, (int)(((i_rows - 1) * p.cols + cols) * 4), 0x00020000);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = c0 + 8 * u + 4 * hf;
+            const f32x4 v{z[4 * u], z[4 * u + 1], z[4 * u + 2], z[4 * u + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, c < cols ? (uint32_t)(row * p.cols + c) * 4 : kOutside, 0, 0);
+        }
+    };
+    auto epilogue = [&]<FfFamily kFam, bool kShare = false>() __attribute__((always_inline)) {
         if constexpr (kWK == 1) {
 #pragma unroll
             for (int t = 0; t < kMJ; ++t) {
@@ -538,7 +554,9 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
 #pragma unroll
                 for (int s = 0; s < kMI; ++s) {
                     const uint32_t row = wave_row + 32 * kWI * s;
-                    if constexpr (kAhead) {
+                    if constexpr (kShare) {
+                        store_share(acc[t][s], row, c0);
+                    } else if constexpr (kAhead) {
                         finish.template operator()<kFam>(acc[t][s], row, c0, ahead[t][s]);
                     } else {
                         u32x4 in[kSets];
@@ -594,9 +612,13 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
                     const int c0 = wave_col + (kGated ? 16 : 32) * kWJ * (q / kMI);
                     constants(c0);
                     const uint32_t row = wave_row + 32 * kWI * (q % kMI);
-                    u32x4 in[kSets];
-                    if constexpr (kReads) read_tile(row, c0, in);
-                    finish.template operator()<kFam>(sum, row, c0, in);
+                    if constexpr (kShare) {
+                        store_share(sum, row, c0);
+                    } else {
+                        u32x4 in[kSets];
+                        if constexpr (kReads) read_tile(row, c0, in);
+                        finish.template operator()<kFam>(sum, row, c0, in);
+                    }
                 }
             }
         }
@@ -607,7 +629,8 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
         }
     };
     if constexpr (kEpi == kFfStore) {
-        epilogue.template operator()<kFamLinear>();
+        if (kSplit && p.splits > 1) epilogue.template operator()<kFamLinear, kSplit>();
+        else epilogue.template operator()<kFamLinear>();
         if constexpr (kIT) {
             const bool tile_sums = p.row_sums != nullptr && j0 == 0;
             if constexpr (kWK > 1) {
@@ -631,7 +654,10 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
                 for (int s = 0; s < kMI; ++s) {
                     const int64_t i = i0 + 32 * (kWI * s + wi) + col;
                     const float v = sums[s] + __shfl_xor(sums[s], 32);
-                    if (hf == 0 && i < p.rows) ((T*)p.row_sums)[i] = (T)v;
+                    if (hf == 0 && i < p.rows) {
+                        if (kSplit && p.splits > 1) p.partial[(p.splits * p.cols + share) * p.rows + i] = v;
+                        else ((T*)p.row_sums)[i] = (T)v;
+                    }
                 }
             }
         }
@@ -640,7 +666,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int id, char* smem) {
     }
 }
 
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false>
 __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) void ff_tile_kernel(FfParams p) {
     __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
     ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi>(p, blockIdx.x, smem);
@@ -654,10 +680,10 @@ __global__ __launch_bounds__(512, 2) void ff_pair_kernel(FfParams w, FfParams x,
     static_assert(TileW::kWaves == 8 && TileX::kWaves == 8, "waves");
     constexpr int kW = TileW::smem_bytes(false), kX = TileX::smem_bytes(false);
     __shared__ __attribute__((aligned(1024))) char smem[kW > kX ? kW : kX];
-    const int w_tasks = w.i_blocks * w.j_blocks, x_tasks = x.i_blocks * x.j_blocks;
+    const int w_tasks = w.i_blocks * w.j_blocks * w.splits, x_tasks = x.i_blocks * x.j_blocks * x.splits;
     const int id = blockIdx.x;
-    if (w_first ? id < w_tasks : id >= x_tasks) ff_tile<T, true, true, false, TileW, kFfStore>(w, w_first ? id : id - x_tasks, smem);
-    else ff_tile<T, false, true, false, TileX, kFfStore>(x, w_first ? id - w_tasks : id, smem);
+    if (w_first ? id < w_tasks : id >= x_tasks) ff_tile<T, true, true, false, TileW, kFfStore, true>(w, w_first ? id : id - x_tasks, smem);
+    else ff_tile<T, false, true, false, TileX, kFfStore, true>(x, w_first ? id - w_tasks : id, smem);
 }
 
 // Tiles of C and the tasks' groups.
@@ -669,7 +695,7 @@ void ff_blocks(FfParams& p, bool gated) {
     p.group_i = p.i_blocks < 8 ? p.i_blocks : 8;
 }
 
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false>
 hipError_t ff_launch(FfParams p, hipStream_t stream) {
     ff_blocks<Tile>(p, kEpi == kFfGated || kEpi == kFfGatedDz);
     hipLaunchKernelGGL((ff_tile_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks)),
@@ -682,7 +708,7 @@ hipError_t ff_launch_pair(FfParams w, FfParams x, bool w_first, hipStream_t stre
     ff_blocks<TileW>(w, false);
     ff_blocks<TileX>(x, false);
     hipLaunchKernelGGL((ff_pair_kernel<T, TileW, TileX>),
-                       dim3((unsigned)((int64_t)w.i_blocks * w.j_blocks + (int64_t)x.i_blocks * x.j_blocks)), dim3(512), 0, stream, w, x,
+                       dim3((unsigned)(w.i_blocks * w.j_blocks * w.splits + x.i_blocks * x.j_blocks * x.splits)), dim3(512), 0, stream, w, x,
                        w_first ? 1 : 0);
     return hipGetLastError();
 }

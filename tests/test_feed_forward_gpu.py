@@ -279,6 +279,22 @@ def test_backward_in_one_launch(m, n, k, dtype):
     check_backward(dout, x, w, bias, "gelu", sh.linear_act_backward(dout, x, w, bias=bias, activation="gelu"), False)
 
 
+# few tiles and a long sum: the depth of dx, of dw or of both in shares that do not come out even, joined afterwards
+@pytest.mark.parametrize("m,n,k,gated,activation", [(300, 2571, 136, True, "gelu"), (4100, 72, 264, False, "none"),
+                                                    (8192, 136, 128, True, "silu"), (2200, 1288, 648, False, "gelu"),
+                                                    (90, 6000, 1000, False, "relu"), (1100, 1099, 72, False, "silu")])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_backward_of_split_sums(m, n, k, gated, activation, dtype):
+    features = 2 * n if gated else n
+    x, w = values(1, m, k, dtype=dtype), values(2, features, k, std=k ** -0.5, dtype=dtype)
+    dout, bias = values(3, m, n, std=0.3, dtype=dtype), values(4, features, std=0.3, dtype=dtype)
+    fn = sh.gated_linear_backward if gated else sh.linear_act_backward
+    grads = fn(dout, x, w, bias=bias, activation=activation)
+    check_backward(dout, x, w, bias, activation, grads, gated)
+    for a, b in zip(grads, fn(dout, x, w, bias=bias, activation=activation)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("activation", ["none", "gelu"])
 def test_backward_parts(gated, activation):
