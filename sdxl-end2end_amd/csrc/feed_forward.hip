@@ -26,7 +26,8 @@ bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0;
 // products of 160, 128 and 32 stages on 40 to 2752 tiles:
 //   256 x 320  dx [8192, 1280] deep 10240 234 us, [2048, 10240] deep 1280 gated 51
 //   256 x 256  dx 200, dw [10240, 1280] deep 8192 178 (1200 TFLOP/s), gated 71
-//   128 x 256  dw 208, [8192, 640] deep 2560 38 (256 x 256: 55)
+//   128 x 256  dw [5120, 1280] deep 2464 39 (256 x 256: 55, 128 x 128: 48)
+//   128 x 192  [8192, 640] deep 2560 39 (128 x 256: 42), [512, 10240] deep 1280 gated 21 (128 x 256: 23, 128 x 128: 32)
 //   128 x 128  dx [2048, 1280] deep 10240 69 (256 x 256: 207, 128 x 256: 116)
 //    64 x 128  dw [640, 2560] deep 8192 51 (128 x 128: 56, 128 x 256: 95)
 //    64 x  64  [154, 5120] deep 1280 10 (128 x 128: 15, 256 x 256: 32)
@@ -35,7 +36,8 @@ struct TileCost {
     float alone, pair, ends;
 };
 constexpr TileCost kTiles[kFfTiles] = {{256, 320, 1.60f, 0.0f, 15.0f}, {256, 256, 1.32f, 0.0f, 10.5f},
-                                       {128, 256, 0.76f, 0.0f, 7.2f},  {128, 128, 0.45f, 0.0f, 5.5f},
+                                       {128, 256, 0.76f, 0.0f, 7.2f},  {128, 192, 0.62f, 0.0f, 6.5f},
+                                       {128, 128, 0.45f, 0.0f, 5.5f},
                                        {64, 128, 0.35f, 0.58f, 5.0f},  {64, 64, 0.30f, 0.46f, 4.5f}};
 
 // Time of two kinds of tasks, a tasks of a_time each before b of b_time, on CUs that take the next task when

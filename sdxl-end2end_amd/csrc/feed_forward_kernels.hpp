@@ -59,7 +59,7 @@ hipError_t launch_ff_general(const FfParams& p, FfEpilogue epilogue, bool i_tran
                              bool j_fp8, hipStream_t stream);
 
 // Tiles of the tiled kernel, rows x columns of sums.
-enum FfTileId : int { kFf256x320, kFf256x256, kFf128x256, kFf128x128, kFf64x128, kFf64x64, kFfTiles };
+enum FfTileId : int { kFf256x320, kFf256x256, kFf128x256, kFf128x192, kFf128x128, kFf64x128, kFf64x64, kFfTiles };
 
 // The tiled kernel: operands whose rows 16-byte accesses divide.
 bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);

@@ -717,6 +717,7 @@ hipError_t ff_launch_pair(FfParams w, FfParams x, bool w_first, hipStream_t stre
 typedef FfTile<4, 2, 1, 2, 5, 2, 2> FfTile256x320;
 typedef FfTile<4, 2, 1, 2, 4, 2, 2> FfTile256x256;
 typedef FfTile<2, 4, 1, 2, 2, 3, 2> FfTile128x256;
+typedef FfTile<4, 2, 1, 1, 3, 3, 2> FfTile128x192;
 typedef FfTile<2, 2, 2, 2, 2, 4, 2> FfTile128x128;
 typedef FfTile<2, 2, 1, 1, 2, 3, 3> FfTile64x128;
 typedef FfTile<2, 2, 1, 1, 1, 4, 4> FfTile64x64;
@@ -763,6 +764,7 @@ hipError_t ff_forward(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int ti
     case kFf256x320: return ff_forward_tile<T, FfTile256x320>(p, epilogue, j_fp8, stream);
     case kFf256x256: return ff_forward_tile<T, FfTile256x256>(p, epilogue, j_fp8, stream);
     case kFf128x256: return ff_forward_tile<T, FfTile128x256>(p, epilogue, j_fp8, stream);
+    case kFf128x192: return ff_forward_tile<T, FfTile128x192>(p, epilogue, j_fp8, stream);
     case kFf128x128: return ff_forward_tile<T, FfTile128x128>(p, epilogue, j_fp8, stream);
     case kFf64x128: return ff_forward_tile<T, FfTile64x128>(p, epilogue, j_fp8, stream);
     case kFf64x64: return ff_forward_tile<T, FfTile64x64>(p, epilogue, j_fp8, stream);
@@ -776,6 +778,7 @@ hipError_t ff_backward(const FfParams& p, FfEpilogue epilogue, bool i_transposed
     case kFf256x320: return ff_backward_tile<T, FfTile256x320>(p, epilogue, i_transposed, stream);
     case kFf256x256: return ff_backward_tile<T, FfTile256x256>(p, epilogue, i_transposed, stream);
     case kFf128x256: return ff_backward_tile<T, FfTile128x256>(p, epilogue, i_transposed, stream);
+    case kFf128x192: return ff_backward_tile<T, FfTile128x192>(p, epilogue, i_transposed, stream);
     case kFf128x128: return ff_backward_tile<T, FfTile128x128>(p, epilogue, i_transposed, stream);
     case kFf64x128: return ff_backward_tile<T, FfTile64x128>(p, epilogue, i_transposed, stream);
     case kFf64x64: return ff_backward_tile<T, FfTile64x64>(p, epilogue, i_transposed, stream);

@@ -229,7 +229,7 @@ def test_few_rows(m, n, k, dtype):
 
 # rows and columns of sums that each tile of the tiled kernel takes at a depth of 328 (six stages, the last one
 # ragged), largest tile last, every edge ragged
-TILES = [(200, 4104), (4100, 520), (4100, 1032), (4100, 2056), (4100, 4104)]
+TILES = [(200, 4104), (4100, 520), (4100, 744), (4100, 1032), (4100, 1496), (4100, 2056), (4100, 4104)]
 
 
 @pytest.mark.parametrize("rows,cols", TILES)
