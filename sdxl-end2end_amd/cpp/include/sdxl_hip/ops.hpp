@@ -1,8 +1,9 @@
 // Operator layer of the sdxl_hip C++20 host API: the attention entry point of
 // the reference's Ops (include/sdxl/cuda/ops.hpp:92-97) and the operators of
 // the UNet transformer block's attention sublayer (layer_norm, linear with
-// fp16 or FP8 E4M3 weights, FP8 weight packing), implemented over the C ABI
-// (include/sdxl_hip/attention.h, sublayer.h).
+// fp16 or FP8 E4M3 weights, FP8 weight packing) and of its feed-forward half
+// (gated projection, linear with an activation), implemented over the C ABI
+// (include/sdxl_hip/attention.h, sublayer.h, feed_forward.h).
 #pragma once
 
 #include "sdxl_hip/runtime.hpp"
@@ -11,6 +12,9 @@
 #include <cstddef>
 
 namespace sdxl::hip {
+
+// Activations of the feed-forward operators (sdxl_activation in feed_forward.h).
+enum class Activation { None, Relu, Gelu, GeluTanh, QuickGelu, Silu };
 
 class Ops final {
 public:
@@ -78,6 +82,26 @@ public:
     void cross_attention_sublayer(Tensor& hidden, const Tensor& norm_weight, const Tensor& norm_bias,
                                   const Tensor& q_weight, const Tensor& context_kv, const Tensor& out_weight,
                                   const Tensor& out_bias, std::size_t heads, bool fp8_activations = false) const;
+
+    // value * act(gate) with [value | gate] = input . weight^T + bias (the reference's GEGLU
+    // projection, unet.cpp:98-149, both halves and their product in one kernel): input [..., K]
+    // fp16 or bf16, weight [2N, K] of its type or Float8E4M3 with attached scales, optional bias
+    // [2N]; gate_first: [gate | value]. Any sizes. Returns [..., N].
+    [[nodiscard]] Tensor gated_linear(const Tensor& input, const Tensor& weight, const Tensor* bias = nullptr,
+                                      Activation activation = Activation::Gelu, bool gate_first = false) const;
+
+    // act(input . weight^T + bias) + residual in one kernel (the text encoder's MLP, the time
+    // embedding): weight [N, K] as above, optional bias [N] and residual [..., N]. Any sizes.
+    [[nodiscard]] Tensor linear_activation(const Tensor& input, const Tensor& weight, const Tensor* bias,
+                                           Activation activation, const Tensor* residual = nullptr) const;
+
+    // hidden += gated(LN(hidden), in_weight, in_bias) . out_weight^T + out_bias in place: the
+    // feed-forward half of the reference's transformer block (src/cuda/unet.cpp:133-147). hidden
+    // fp16 [..., W]; in_weight [2I, W] and out_weight [W, I] fp16 or packed E4M3; biases optional.
+    void feed_forward_sublayer(Tensor& hidden, const Tensor& norm_weight, const Tensor& norm_bias,
+                               const Tensor& in_weight, const Tensor* in_bias, const Tensor& out_weight,
+                               const Tensor* out_bias, Activation activation = Activation::Gelu,
+                               float epsilon = 1.0e-5F) const;
 
 private:
     const Runtime* runtime_ = nullptr;

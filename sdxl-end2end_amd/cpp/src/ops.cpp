@@ -5,6 +5,7 @@
 #include "sdxl_hip/ops.hpp"
 
 #include "sdxl_hip/attention.h"
+#include "sdxl_hip/feed_forward.h"
 #include "sdxl_hip/sublayer.h"
 
 #include <sstream>
@@ -305,6 +306,128 @@ void Ops::attention_sublayer(Tensor& hidden, const Tensor& norm_weight, const Te
     check(st);
     // The workspace is released when `workspace` goes out of scope; hipFree
     // waits for the work queued on it.
+}
+
+namespace {
+
+std::int32_t activation_code(Activation activation) {
+    switch (activation) {
+    case Activation::None: return SDXL_ACT_NONE;
+    case Activation::Relu: return SDXL_ACT_RELU;
+    case Activation::Gelu: return SDXL_ACT_GELU;
+    case Activation::GeluTanh: return SDXL_ACT_GELU_TANH;
+    case Activation::QuickGelu: return SDXL_ACT_QUICK_GELU;
+    case Activation::Silu: return SDXL_ACT_SILU;
+    }
+    throw HipError("feed-forward: unknown activation");
+}
+
+// E4M3 weights need a scale per row.
+const float* weight_scales(const Tensor& weight) {
+    if (weight.type() != ScalarType::Float8E4M3) return nullptr;
+    if (!weight.has_dequant_scale() || weight.dequant_scale_count() != weight.size(0))
+        throw HipError("FP8 weight has invalid scaling metadata");
+    return weight.dequant_scale_data();
+}
+
+sdxl_ff_desc feed_forward_desc(const Tensor& input, const Tensor& weight, const Tensor* bias, bool gated,
+                               Activation activation, bool gate_first) {
+    if ((input.type() != ScalarType::Float16 && input.type() != ScalarType::BFloat16) || input.rank() < 2 ||
+        weight.rank() != 2 || (weight.type() != input.type() && weight.type() != ScalarType::Float8E4M3))
+        throw HipError("feed-forward requires an fp16 or bf16 input and a rank-2 weight of its type or FP8 E4M3");
+    if (weight.size(1) != input.shape().back() || (gated && weight.size(0) % 2 != 0))
+        throw HipError("feed-forward feature mismatch");
+    if (bias != nullptr && (bias->type() != input.type() || bias->rank() != 1 || bias->size(0) != weight.size(0)))
+        throw HipError("feed-forward bias mismatch");
+    sdxl_ff_desc d{};
+    d.m = 1;  // rows: also where the input has no columns
+    for (std::size_t i = 0; i + 1 < input.rank(); ++i) d.m *= static_cast<std::int64_t>(input.size(i));
+    d.n = static_cast<std::int64_t>(gated ? weight.size(0) / 2 : weight.size(0));
+    d.k = static_cast<std::int64_t>(weight.size(1));
+    d.dtype = dtype_code(input.type());
+    d.w_dtype = weight.type() == ScalarType::Float8E4M3 ? SDXL_DTYPE_E4M3 : d.dtype;
+    d.activation = activation_code(activation);
+    d.gate_first = gate_first ? 1 : 0;
+    return d;
+}
+
+std::string feed_forward_label(const char* name, const sdxl_ff_desc& d) {
+    std::ostringstream label;
+    label << "ops/" << name << '/'
+          << (d.w_dtype == SDXL_DTYPE_E4M3 ? "e4m3" : d.w_dtype == SDXL_DTYPE_BF16 ? "bf16" : "f16") << "/m" << d.m
+          << "_n" << d.n << "_k" << d.k;
+    return label.str();
+}
+
+}  // namespace
+
+Tensor Ops::gated_linear(const Tensor& input, const Tensor& weight, const Tensor* bias, Activation activation,
+                         bool gate_first) const {
+    const sdxl_ff_desc d = feed_forward_desc(input, weight, bias, true, activation, gate_first);
+    const float* scales = weight_scales(weight);
+    std::vector<std::size_t> shape = input.shape();
+    shape.back() = weight.size(0) / 2;
+    Tensor output = Tensor::allocate(*runtime_, shape, input.type());
+    const int scope = runtime_->begin_profile(feed_forward_label("gated_linear", d));
+    const sdxl_status st = sdxl_gated_linear(&d, input.data(), weight.data(), scales, bias ? bias->data() : nullptr,
+                                             output.data(), runtime_->stream());
+    runtime_->end_profile(scope);
+    check(st);
+    return output;
+}
+
+Tensor Ops::linear_activation(const Tensor& input, const Tensor& weight, const Tensor* bias, Activation activation,
+                              const Tensor* residual) const {
+    const sdxl_ff_desc d = feed_forward_desc(input, weight, bias, false, activation, false);
+    const float* scales = weight_scales(weight);
+    std::vector<std::size_t> shape = input.shape();
+    shape.back() = weight.size(0);
+    if (residual != nullptr && (residual->type() != input.type() || residual->shape() != shape))
+        throw HipError("feed-forward residual mismatch");
+    Tensor output = Tensor::allocate(*runtime_, shape, input.type());
+    const int scope = runtime_->begin_profile(feed_forward_label("linear_activation", d));
+    const sdxl_status st = sdxl_linear_act(&d, input.data(), weight.data(), scales, bias ? bias->data() : nullptr,
+                                           residual ? residual->data() : nullptr, output.data(), runtime_->stream());
+    runtime_->end_profile(scope);
+    check(st);
+    return output;
+}
+
+void Ops::feed_forward_sublayer(Tensor& hidden, const Tensor& norm_weight, const Tensor& norm_bias,
+                                const Tensor& in_weight, const Tensor* in_bias, const Tensor& out_weight,
+                                const Tensor* out_bias, Activation activation, float epsilon) const {
+    if (hidden.type() != ScalarType::Float16 || hidden.rank() < 2)
+        throw HipError("feed-forward sublayer requires fp16 hidden [..., W]");
+    const sdxl_ff_desc in = feed_forward_desc(hidden, in_weight, in_bias, true, activation, false);
+    const std::size_t W = hidden.shape().back(), inner = in_weight.size(0) / 2;
+    if (out_weight.rank() != 2 || out_weight.size(0) != W || out_weight.size(1) != inner ||
+        (out_weight.type() != ScalarType::Float16 && out_weight.type() != ScalarType::Float8E4M3) ||
+        (out_bias != nullptr &&
+         (out_bias->type() != ScalarType::Float16 || out_bias->rank() != 1 || out_bias->size(0) != W)) ||
+        norm_weight.type() != ScalarType::Float16 || norm_bias.type() != ScalarType::Float16 ||
+        norm_weight.elements() != W || norm_bias.elements() != W)
+        throw HipError("feed-forward sublayer weight mismatch");
+    sdxl_ff_sublayer_desc d{};
+    d.rows = in.m;
+    d.width = static_cast<std::int64_t>(W);
+    d.inner = static_cast<std::int64_t>(inner);
+    d.w_in_dtype = in.w_dtype;
+    d.w_out_dtype = out_weight.type() == ScalarType::Float8E4M3 ? SDXL_DTYPE_E4M3 : SDXL_DTYPE_F16;
+    d.activation = in.activation;
+    d.ln_eps = epsilon;
+    const float *in_scales = weight_scales(in_weight), *out_scales = weight_scales(out_weight);
+    const std::size_t ws_bytes = sdxl_ff_sublayer_workspace_bytes(&d);
+    Tensor workspace = Tensor::allocate(*runtime_, {ws_bytes}, ScalarType::Float8E4M3);  // raw bytes
+    std::ostringstream label;
+    label << "unet/feed_forward_sublayer/m" << d.rows << "_w" << W << "_i" << inner
+          << (in_scales != nullptr ? "_e4m3" : "_f16");
+    const int scope = runtime_->begin_profile(label.str());
+    const sdxl_status st = sdxl_ff_sublayer(
+        &d, hidden.data(), norm_weight.data(), norm_bias.data(), in_weight.data(), in_scales,
+        in_bias ? in_bias->data() : nullptr, out_weight.data(), out_scales, out_bias ? out_bias->data() : nullptr,
+        hidden.data(), workspace.data(), ws_bytes, runtime_->stream());
+    runtime_->end_profile(scope);
+    check(st);
 }
 
 }  // namespace sdxl::hip

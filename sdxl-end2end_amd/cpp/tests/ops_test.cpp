@@ -355,6 +355,77 @@ void graph_capture_cases() {
     std::cout << "graph capture cases passed\n";
 }
 
+// The feed-forward operators against float64 on the host. Inputs are exact in fp16, so the bound is half a step of the
+// rounded output (2^-11) with a small allowance for the fp32 sums and activations.
+void feed_forward_cases() {
+    Runtime runtime;
+    Ops ops(runtime);
+    const auto half_exact = [](float v) { return half_to_float(float_to_half(v)); };
+    const std::size_t M = 37, K = 72, N = 40;
+    const auto xh = filled({1, M, K}, [&](std::size_t i) { return half_exact(std::sin(static_cast<float>(i) * 0.37F)); });
+    const auto wh = filled({2 * N, K}, [&](std::size_t i) { return half_exact(std::cos(static_cast<float>(i) * 0.11F) * 0.25F); });
+    const auto bh = filled({2 * N}, [&](std::size_t i) { return half_exact(std::sin(static_cast<float>(i))); });
+    const auto x = Tensor::from_host_f32(runtime, xh), w = Tensor::from_host_f32(runtime, wh), b = Tensor::from_host_f32(runtime, bh);
+    const auto z = [&](std::size_t r, std::size_t c) {
+        double s = bh.values[c];
+        for (std::size_t k = 0; k < K; ++k) s += (double)xh.values[r * K + k] * wh.values[c * K + k];
+        return s;
+    };
+    const auto near = [](float got, double want, const char* what) {
+        require_close(got, static_cast<float>(want), static_cast<float>(std::ldexp(std::fabs(want), -11) + 1e-5 * (1.0 + std::fabs(want))), what);
+    };
+    const auto gelu = [](double v) { return 0.5 * v * (1.0 + std::erf(v / std::sqrt(2.0))); };
+    const auto silu = [](double v) { return v / (1.0 + std::exp(-v)); };
+    const auto gated = ops.gated_linear(x, w, &b).to_host_f32(runtime);
+    const auto swapped = ops.gated_linear(x, w, &b, Activation::Silu, true).to_host_f32(runtime);
+    require(gated.shape == std::vector<std::size_t>({1, M, N}), "gated shape");
+    for (std::size_t r = 0; r < M; ++r)
+        for (std::size_t c = 0; c < N; ++c) {
+            near(gated.values[r * N + c], z(r, c) * gelu(z(r, N + c)), "gated linear");
+            near(swapped.values[r * N + c], z(r, N + c) * silu(z(r, c)), "gate first");
+        }
+    const auto rh = filled({1, M, 2 * N}, [&](std::size_t i) { return half_exact(std::cos(static_cast<float>(i) * 0.7F)); });
+    const auto residual = Tensor::from_host_f32(runtime, rh);
+    const auto act = ops.linear_activation(x, w, &b, Activation::Silu, &residual).to_host_f32(runtime);
+    for (std::size_t r = 0; r < M; ++r)
+        for (std::size_t c = 0; c < 2 * N; ++c)
+            near(act.values[r * 2 * N + c], silu(z(r, c)) + rh.values[r * 2 * N + c], "linear activation");
+    // bf16 takes the same path: the plain product of one row
+    const auto xb = Tensor::from_host_f32(runtime, filled({1, 8}, [](std::size_t) { return 1.0F; }), ScalarType::BFloat16);
+    const auto wb = Tensor::from_host_f32(runtime, filled({3, 8}, [](std::size_t i) { return static_cast<float>(i / 8); }), ScalarType::BFloat16);
+    const auto plain = ops.linear_activation(xb, wb, nullptr, Activation::None).to_host_f32(runtime);
+    for (std::size_t c = 0; c < 3; ++c) require_close(plain.values[c], 8.0F * static_cast<float>(c), 0.0F, "bf16 linear");
+    // the sublayer gives what its three steps give, with fp16 and with packed weights
+    const std::size_t W = 64, I = 96;
+    const auto hh = filled({2, 33, W}, [](std::size_t i) { return std::sin(static_cast<float>(i) * 0.61F); });
+    const auto ones = Tensor::from_host_f32(runtime, filled({W}, [](std::size_t) { return 1.0F; }));
+    const auto zeros = Tensor::from_host_f32(runtime, filled({W}, [](std::size_t) { return 0.0F; }));
+    const auto in_bias = Tensor::from_host_f32(runtime, filled({2 * I}, [](std::size_t i) { return std::cos(static_cast<float>(i)) * 0.1F; }));
+    Tensor w_in = Tensor::from_host_f32(runtime, filled({2 * I, W}, [](std::size_t i) { return std::sin(static_cast<float>(i) * 0.19F) * 0.2F; }));
+    Tensor w_out = Tensor::from_host_f32(runtime, filled({W, I}, [](std::size_t i) { return std::cos(static_cast<float>(i) * 0.23F) * 0.2F; }));
+    for (int packed = 0; packed < 2; ++packed) {
+        if (packed == 1) {
+            w_in = ops.pack_e4m3(w_in);
+            w_out = ops.pack_e4m3(w_out);
+        }
+        Tensor hidden = Tensor::from_host_f32(runtime, hh);
+        const auto steps =
+            ops.linear_activation(ops.gated_linear(ops.layer_norm(hidden, ones, zeros), w_in, &in_bias), w_out, nullptr,
+                                  Activation::None, &hidden).to_host_f32(runtime);
+        ops.feed_forward_sublayer(hidden, ones, zeros, w_in, &in_bias, w_out, nullptr);
+        const auto whole = hidden.to_host_f32(runtime);
+        for (std::size_t i = 0; i < whole.values.size(); ++i) require_close(whole.values[i], steps.values[i], 0.0F, "sublayer");
+    }
+    require_throws([&] { (void)ops.gated_linear(x, Tensor::from_host_f32(runtime, filled({3, K}, [](std::size_t) { return 0.0F; }))); },
+                   "feature mismatch", "odd gated rows");
+    require_throws([&] { (void)ops.linear_activation(x, w, &zeros, Activation::Relu); }, "bias mismatch", "bias");
+    require_throws([&] { (void)ops.linear_activation(x, w, &b, Activation::Relu, &x); }, "residual mismatch", "residual");
+    require_throws([&] { (void)ops.gated_linear(x, wb); }, "rank-2 weight of its type", "weight type");
+    Tensor odd = Tensor::from_host_f32(runtime, hh);
+    require_throws([&] { ops.feed_forward_sublayer(odd, ones, zeros, w_in, &in_bias, w_in, nullptr); }, "weight mismatch", "out weight");
+    std::cout << "feed-forward cases passed\n";
+}
+
 void device_cases() {
     Runtime runtime;
     Ops ops(runtime);
@@ -457,6 +528,7 @@ void device_cases() {
     std::cout << "device cases passed\n";
     sublayer_cases();
     out_projection_cases();
+    feed_forward_cases();
 }
 
 }  // namespace

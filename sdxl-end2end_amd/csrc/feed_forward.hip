@@ -13,6 +13,8 @@ hipError_t ff_backward_f16(const FfParams& p, FfEpilogue epilogue, bool i_transp
 hipError_t ff_backward_bf16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, int tile, hipStream_t stream);
 hipError_t ff_pair_f16(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream);
 hipError_t ff_pair_bf16(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream);
+hipError_t ff_staged_f16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
+hipError_t ff_staged_bf16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
 hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool one_per_cu, hipStream_t stream);
 
 namespace {
@@ -188,16 +190,30 @@ __global__ __launch_bounds__(256) void ff_join_kernel(FfJoin a, FfJoin b) {
 
 }  // namespace
 
-bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8) {
+bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8) {
     if (p.depth <= 0 || (epilogue == kFfStore && (!j_transposed || p.out == nullptr))) return false;
+    // rows of 16 bytes or more: a row's last chunk is read as its last 16 bytes
+    if ((i_transposed ? p.rows : p.depth) < 8 || (j_transposed ? p.cols : p.depth) < (j_fp8 ? 16 : 8)) return false;
+    // a window (at most 320 rows) stays below 2^31 bytes, the threads of a launch below 2^32
+    if (p.ld_i > (1 << 20) || p.ld_j > (1 << 20) || p.ld_out > (1 << 20) || p.ld_dout > (1 << 20) || p.ld_res > (1 << 20))
+        return false;
+    return ((p.rows + 63) / 64) * ((p.cols + 31) / 32) <= (1 << 23);
+}
+
+bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8) {
+    if (!ff_staged_supported(p, epilogue, i_transposed, j_transposed, j_fp8)) return false;
     // rows in whole 16-byte chunks: the depth, or the columns of an operand that is read by columns
     const int64_t i_row = p.i_row != 0 ? p.i_row : i_transposed ? p.rows : p.depth;
     if (!aligned(p.ip, 16) || !aligned(p.jp, 16) || p.ld_i % 8 != 0 || p.ld_j % (j_fp8 ? 16 : 8) != 0) return false;
-    if (i_row % 8 != 0 || (j_transposed ? p.cols % 8 != 0 : p.depth % (j_fp8 ? 16 : 8) != 0)) return false;
-    // a window (at most 320 rows) stays below 2^31 bytes, the tasks below 2^31
-    if (p.ld_i > (1 << 20) || p.ld_j > (1 << 20) || p.ld_out > (1 << 20) || p.ld_dout > (1 << 20) || p.ld_res > (1 << 20))
-        return false;
-    return ((p.rows + 63) / 64) * ((p.cols + 31) / 32) <= (1 << 24);
+    return i_row % 8 == 0 && (j_transposed ? p.cols % 8 == 0 : p.depth % (j_fp8 ? 16 : 8) == 0);
+}
+
+hipError_t launch_ff_staged(const FfParams& params, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
+                            int compute_units, hipStream_t stream) {
+    const FfParams p = prepared(params, i_transposed);
+    const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
+    const bool large = ((p.rows + 127) / 128) * ((cols + 127) / 128) >= (compute_units > 0 ? compute_units : 256);
+    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, i_transposed, j_fp8, large, stream);
 }
 
 hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
@@ -208,7 +224,8 @@ hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_t
     const int tile = choose_tile(p, epilogue, j_fp8, cus, time);
     if (epilogue == kFfLinear || epilogue == kFfGated) {
         bool one_per_cu;
-        if (deep_time(p, epilogue, cus, one_per_cu) < time) return ff_deep(p, epilogue, bf16, j_fp8, one_per_cu, stream);
+        if (deep_time(p, epilogue, cus, one_per_cu) < time)
+            return ff_deep(p, epilogue, bf16, j_fp8, one_per_cu, stream);
         return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, tile, stream);
     }
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);

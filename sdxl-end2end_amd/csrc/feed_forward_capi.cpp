@@ -78,6 +78,8 @@ sdxl_status product(const FfParams& p, sdxl_hip::FfEpilogue epilogue, bool it, b
         return launch_status(sdxl_hip::launch_ff_rows(p, epilogue, c.bf16, w_fp8, stream), name);
     if (sdxl_hip::ff_tiled_supported(p, epilogue, it, jt, w_fp8))
         return launch_status(sdxl_hip::launch_ff_tiled(p, epilogue, it, c.bf16, w_fp8, sdxl_hip_compute_units(), stream), name);
+    if (sdxl_hip::ff_staged_supported(p, epilogue, it, jt, w_fp8))
+        return launch_status(sdxl_hip::launch_ff_staged(p, epilogue, it, c.bf16, w_fp8, sdxl_hip_compute_units(), stream), name);
     return launch_status(sdxl_hip::launch_ff_general(p, epilogue, it, jt, c.bf16, w_fp8, stream), name);
 }
 

@@ -66,6 +66,11 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
 hipError_t launch_ff_tiled(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
                            int compute_units, hipStream_t stream);
 
+// The same through registers: rows of any length and alignment.
+bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);
+hipError_t launch_ff_staged(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
+                            int compute_units, hipStream_t stream);
+
 // dw (I transposed) and dx, both of which the tiled kernel supports: in one launch where that is faster, with the
 // depth split as far as `partial` (256-byte aligned) holds the shares' sums: ff_partial_bytes is enough for any split
 // that is taken.

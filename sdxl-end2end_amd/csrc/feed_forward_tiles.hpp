@@ -49,6 +49,12 @@ typedef __attribute__((address_space(3))) i16x8 lds_op;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 typedef __attribute__((address_space(3))) float lds_float;
 
+// 16 bytes at any element's address
+template <int kAlign>
+struct __attribute__((packed, aligned(kAlign))) Unaligned {
+    u32x4 v;
+};
+
 __device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
 // Exchanges the halves so that lanes 0-31 hold 8 consecutive columns made of
@@ -80,7 +86,7 @@ struct FfTile {
 };
 
 // Task `id` of a product whose tasks' numbers modulo 8 are their XCDs; smem: Tile::smem_bytes.
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false>
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false, bool kStaged = false>
 __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* smem) {
     constexpr int kWI = Tile::kWI, kWJ = Tile::kWJ, kWK = Tile::kWK, kMI = Tile::kMI, kMJ = Tile::kMJ, kRing = Tile::kRing;
     using F = FfType<T>;
@@ -167,6 +173,86 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         return window_rsrc({base, left > 0 ? (uint32_t)size : 0u});
     };
     const uint32_t lds0 = lds_addr(smem);
+    // Staged: rows that 16-byte accesses do not divide come through registers, to the places that the transfers give
+    // them: the wave's parts of the next stage are fetched over a stage before they are needed. A chunk that its row
+    // ends in is fetched as the row's last 16 bytes and shifted when it is put down.
+    static_assert(!kStaged || (kRing == 2 && kSpread == 1 && kMore == 0), "staged: one stage in LDS, one in registers");
+    u32x4 held[kStaged ? kXfers : 1];
+    // part x of stage st: its address, and how many of the chunk's elements its row has (none: 0 or less)
+    auto part = [&](int st, int x, const char*& from) __attribute__((always_inline)) {
+        const int64_t d_left = depth - (int64_t)st * 64;
+        const int left = (int)min64(d_left, 64);
+        int64_t off;
+        int valid;
+        if (x < kIX) {
+            const int n = x * kWaves + wave;
+            if constexpr (kIT) {
+                off = (int64_t)st * 64 * ldi_b + (int64_t)(8 * (n & 7)) * ldi_b + (n >> 3) * 128 + i_lane;
+                valid = 8 * (n & 7) + row8 < left ? (int)min64(i_row - i0, kBI) - 64 * (n >> 3) - 8 * chunk8 : 0;
+            } else {
+                off = (int64_t)st * 128 + (int64_t)(8 * n) * ldi_b + i_lane;
+                valid = 8 * n + row8 < i_rows ? (int)min64(i_row - (int64_t)st * 64, 64) - 8 * chunk8 : 0;
+            }
+            from = iw.base + off;
+        } else {
+            const int n = (x - kIX) * kWaves + wave;
+            if constexpr (kJT) {
+                off = (int64_t)st * 64 * ldj_b + (int64_t)(8 * (n & 7)) * ldj_b + (n >> 3) * 128 + j_lane;
+                valid = 8 * (n & 7) + row8 < left ? (int)j_rows - 64 * (n >> 3) - 8 * chunk8 : 0;
+            } else {
+                const int first = kJFp8 ? 16 * (kGated ? n >> 1 : n) : kGated ? 16 * (n >> 2) + 8 * (n & 1) : 8 * n;
+                off = (int64_t)st * (kJFp8 ? 64 : 128) + (int64_t)first * ldj_b + j_lane;
+                valid = first + (kJFp8 ? row16 : row8) < j_rows ? left - (kJFp8 ? 16 * chunk16 : 8 * chunk8) : 0;
+            }
+            from = jw.base + off;
+        }
+        return valid;
+    };
+    const bool inner_tile = i_rows == kBI && j_rows == (kGated ? kCols : kBJ) && (!kIT || i_row - i0 >= kBI);
+    auto whole = [&](int st) __attribute__((always_inline)) { return inner_tile && depth - (int64_t)st * 64 >= 64; };
+    auto read16 = [&](int x, const char* from) __attribute__((always_inline)) {
+        return kJFp8 && x >= kIX ? ((const Unaligned<1>*)from)->v : ((const Unaligned<2>*)from)->v;
+    };
+    auto fetch = [&](int st) __attribute__((always_inline)) {
+        const char* from;
+        if (whole(st)) {
+#pragma unroll
+            for (int x = 0; x < kXfers; ++x) {
+                part(st, x, from);
+                held[x] = read16(x, from);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < kXfers; ++x) {
+                const int all = kJFp8 && x >= kIX ? 16 : 8, valid = part(st, x, from);
+                held[x] = u32x4{};
+                if (valid > 0) held[x] = read16(x, from - (valid < all ? all - valid : 0) * (16 / all));
+            }
+        }
+    };
+    auto put = [&](int st, int buffer) __attribute__((always_inline)) {
+        char* buf = smem + buffer * kStage + lane * 16;
+        if (!whole(st)) {
+#pragma unroll
+            for (int x = 0; x < kXfers; ++x) {
+                const char* from;
+                const int all = kJFp8 && x >= kIX ? 16 : 8, valid = part(st, x, from);
+                const int bits = valid < all && valid > 0 ? (all - valid) * (128 / all) : 0;
+                uint64_t lo = held[x][0] | (uint64_t)held[x][1] << 32, hi = held[x][2] | (uint64_t)held[x][3] << 32;
+                if (bits >= 64) {
+                    lo = hi >> (bits - 64);
+                    hi = 0;
+                } else if (bits > 0) {
+                    lo = lo >> bits | hi << (64 - bits);
+                    hi >>= bits;
+                }
+                held[x] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < kXfers; ++x)
+            *(lds_u32x4*)(buf + (x < kIX ? 0 : kIBytes) + ((x < kIX ? x : x - kIX) * kWaves + wave) * 1024) = held[x];
+    };
     // one of the wave's kXfers transfers of stage st
     auto issue = [&](int st, int buffer, int x, u32x4 irsrc, u32x4 jrsrc) __attribute__((always_inline)) {
         const uint32_t buf = lds0 + buffer * kStage;
@@ -334,15 +420,23 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                 ((step.template operator()<(k + 1 < kSpread ? k + 1 : -1)>(k, buffer, k + 1, st - 1 + kRing, before),
                   __builtin_amdgcn_sched_barrier(0)), ...);
             }(std::make_integer_sequence<int, kSteps - 1>{});
+            if constexpr (kStaged) put(st + 1, before);
             land.template operator()<kRing - 2>();  // stage st + 1 is there, and nobody reads stage st any more
-            step.template operator()<0>(kSteps - 1, after, 0, st + kRing, buffer);  // (past the last stage: reads unused)
+            if constexpr (kStaged) fetch(st + kRing);
+            step.template operator()<kStaged ? -1 : 0>(kSteps - 1, after, 0, st + kRing, buffer);  // (past the last stage: reads unused)
             __builtin_amdgcn_sched_barrier(0);
         };
+        if constexpr (kStaged) {
+            fetch(0);
+            put(0, 0);
+            fetch(1);
+        } else {
 #pragma unroll
-        for (int st = 0; st < kRing; ++st) {
-            const u32x4 ir = i_window(st), jr = j_window(st);
+            for (int st = 0; st < kRing; ++st) {
+                const u32x4 ir = i_window(st), jr = j_window(st);
 #pragma unroll
-            for (int x = 0; x < (st == kRing - 1 ? kXfers / kSpread : kXfers); ++x) issue(st, st, x, ir, jr);
+                for (int x = 0; x < (st == kRing - 1 ? kXfers / kSpread : kXfers); ++x) issue(st, st, x, ir, jr);
+            }
         }
         land.template operator()<kRing - 2>();
 #pragma unroll
@@ -666,10 +760,17 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     }
 }
 
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false>
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false, bool kStaged = false>
 __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) void ff_tile_kernel(FfParams p) {
     __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
     ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi>(p, blockIdx.x, smem);
+}
+
+// Rows that 16-byte accesses do not divide.
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
+__global__ __launch_bounds__(64 * Tile::kWaves, Tile::kMI * Tile::kMJ > 1 ? 2 : 4) void ff_staged_kernel(FfParams p) {
+    __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
+    ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi, false, true>(p, blockIdx.x, smem);
 }
 
 // dw and dx in one launch, one workgroup per CU at a time: the tasks of the
@@ -695,10 +796,18 @@ void ff_blocks(FfParams& p, bool gated) {
     p.group_i = p.i_blocks < 8 ? p.i_blocks : 8;
 }
 
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false>
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false, bool kStaged = false>
 hipError_t ff_launch(FfParams p, hipStream_t stream) {
     ff_blocks<Tile>(p, kEpi == kFfGated || kEpi == kFfGatedDz);
     hipLaunchKernelGGL((ff_tile_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks)),
+                       dim3(64 * Tile::kWaves), 0, stream, p);
+    return hipGetLastError();
+}
+
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
+hipError_t ff_launch_staged(FfParams p, hipStream_t stream) {
+    ff_blocks<Tile>(p, kEpi == kFfGated || kEpi == kFfGatedDz);
+    hipLaunchKernelGGL((ff_staged_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks)),
                        dim3(64 * Tile::kWaves), 0, stream, p);
     return hipGetLastError();
 }
@@ -784,6 +893,34 @@ hipError_t ff_backward(const FfParams& p, FfEpilogue epilogue, bool i_transposed
     case kFf64x64: return ff_backward_tile<T, FfTile64x64>(p, epilogue, i_transposed, stream);
     }
     return hipErrorInvalidValue;
+}
+
+// The tiles of rows that come through registers.
+typedef FfTile<2, 2, 1, 2, 2, 2, 1> FfStaged128x128;
+typedef FfTile<2, 2, 1, 1, 1, 2, 1> FfStaged64x64;
+
+template <typename T, typename Tile>
+hipError_t ff_staged_tile(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, hipStream_t stream) {
+    switch (epilogue) {
+    case kFfLinear:
+        return j_fp8 ? ff_launch_staged<T, false, false, true, Tile, kFfLinear>(p, stream)
+                     : ff_launch_staged<T, false, false, false, Tile, kFfLinear>(p, stream);
+    case kFfGated:
+        return j_fp8 ? ff_launch_staged<T, false, false, true, Tile, kFfGated>(p, stream)
+                     : ff_launch_staged<T, false, false, false, Tile, kFfGated>(p, stream);
+    case kFfLinearDz: return ff_launch_staged<T, false, false, false, Tile, kFfLinearDz>(p, stream);
+    case kFfGatedDz: return ff_launch_staged<T, false, false, false, Tile, kFfGatedDz>(p, stream);
+    case kFfStore:
+        return i_transposed ? ff_launch_staged<T, true, true, false, Tile, kFfStore>(p, stream)
+                            : ff_launch_staged<T, false, true, false, Tile, kFfStore>(p, stream);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <typename T>
+hipError_t ff_staged(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream) {
+    return large ? ff_staged_tile<T, FfStaged128x128>(p, epilogue, i_transposed, j_fp8, stream)
+                 : ff_staged_tile<T, FfStaged64x64>(p, epilogue, i_transposed, j_fp8, stream);
 }
 
 }  // namespace

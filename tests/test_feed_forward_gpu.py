@@ -9,6 +9,8 @@ at 0 is 0.851, silu's 0.5, gelu's 0.798); the backward's dz is rounded to the ty
 """
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 
@@ -16,6 +18,7 @@ import sdxl_hip as sh
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 DEV = "cuda:0"
 F16, BF16 = torch.float16, torch.bfloat16
 HALF = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
@@ -352,6 +355,43 @@ def test_row_strides(m, n, k, pad):
     check_backward(dout, x, w[:n], None, "none", sh.linear_act_backward(dout, x, w[:n]), False)
 
 
+# rows that no 16-byte access divides, on 64 x 64 and on 128 x 128 tiles: the last chunk of a row of 8 elements or more is
+# its last 16 bytes; E4M3 rows of 16 codes or more
+@pytest.mark.parametrize("m,n,k", [(1, 1283, 321), (40, 9, 8), (77, 100, 9), (130, 331, 71), (301, 257, 645), (2200, 1091, 133),
+                                   (4100, 1543, 68)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_odd_rows(m, n, k, dtype):
+    x, w = values(1, m, k, dtype=dtype), values(2, 2 * n, k, std=k ** -0.5, dtype=dtype)
+    bias, residual, dout = values(3, 2 * n, std=0.3, dtype=dtype), values(4, m, n, dtype=dtype), values(5, m, n, std=0.3, dtype=dtype)
+    check_forward(x, w.double(), bias, "gelu", sh.gated_linear(x, w, bias=bias), True)
+    got = sh.linear_act(x, w[:n], bias=bias[:n].clone(), residual=residual, activation="silu")
+    check_forward(x, w[:n].double(), bias[:n], "silu", got, False, residual=residual)
+    check_backward(dout, x, w, bias, "silu", sh.gated_linear_backward(dout, x, w, bias=bias, activation="silu"), True)
+    check_backward(dout, x, w[:n], None, "none", sh.linear_act_backward(dout, x, w[:n]), False)
+    if k >= 16:
+        codes, scale, w64 = e4m3(6, 2 * n, k)
+        check_forward(x, w64, bias, "gelu_tanh", sh.gated_linear(x, codes, bias=bias, w_scale=scale, activation="gelu_tanh"), True)
+        check_forward(x, w64[:n], None, "relu", sh.linear_act(x, codes[:n], w_scale=scale[:n], activation="relu"), False)
+
+
+@pytest.mark.parametrize("m,n,k,pad,shift", [(70, 136, 72, 8, 0), (70, 136, 72, 5, 0), (70, 136, 75, 8, 0), (70, 137, 72, 8, 1),
+                                             (9, 72, 64, 8, 0), (2100, 1032, 88, 8, 0), (2100, 1033, 91, 3, 2), (80, 640, 648, 8, 0)])
+def test_what_lies_beside_the_rows_is_not_read_into_them(m, n, k, pad, shift):
+    """x, w, dout and the residual are column slices of tensors that are NaN everywhere else."""
+    def slice_of(seed, rows, cols, std=1.0):
+        t = torch.full((rows + 2, cols + pad + shift), float("nan"), dtype=F16, device=DEV)
+        part = t[1:rows + 1, shift:cols + shift]
+        part.copy_(values(seed, rows, cols, std=std))
+        return part
+
+    x, w, dout, residual = slice_of(1, m, k), slice_of(2, 2 * n, k, k ** -0.5), slice_of(3, m, n, 0.3), slice_of(4, m, n)
+    check_forward(x, w.double(), None, "gelu", sh.gated_linear(x, w), True)
+    got = sh.linear_act(x, w[:n], residual=residual, activation="silu")
+    check_forward(x, w[:n].double(), None, "silu", got, False, residual=residual)
+    check_backward(dout, x, w, None, "gelu", sh.gated_linear_backward(dout, x, w, need_dbias=True), True)
+    check_backward(dout, x, w[:n], None, "none", sh.linear_act_backward(dout, x, w[:n], need_dbias=True), False)
+
+
 def test_strided_gradients_through_the_c_abi():
     m, n, k = 40, 24, 72
     x, w, dout = values(1, m, k), values(2, n, k, std=0.12), values(3, m, n)
@@ -564,3 +604,10 @@ def test_transformer_block_halves_in_a_row():
     h = sh.gated_linear(normed, ff[2], bias=ff[4])
     check_forward(normed, ff[2].double(), ff[4], "gelu", h, True)
     check_forward(h, ff[5].double(), ff[7], "none", c.view(B * S, W), False, residual=b.view(B * S, W))
+
+
+def test_cpp_host_api():
+    """The C++ Ops on the same kernels, against 64 bits on the host."""
+    exe = os.path.join(ROOT, "sdxl-end2end_amd", "bin", "sdxl_hip_ops_test")
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "feed-forward cases passed" in r.stdout, r.stdout + r.stderr
