@@ -462,6 +462,8 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     const int wave_row = 32 * wi + col;             // + 32 kWI s: the lane's row in the tile
     const int wave_col = (kGated ? 16 : 32) * wj;   // + (16 | 32) kWJ t: columns of C in the tile
     const int cols = (int)min64(p.cols - j0, 1 << 16);         // columns of C from j0 on
+    const uint32_t ldo_b = (uint32_t)(p.ld_out * 2), ldd_b = (uint32_t)(p.ld_dout * 2), ldr_b = (uint32_t)(p.ld_res * 2);
+    auto rows_at = [&](const void* base, int64_t ld, int64_t first) __attribute__((always_inline)) { return (char*)base + (i0 * ld + first) * 2; };
     auto rows_window = [&](const void* base, int64_t ld, int64_t first) __attribute__((always_inline)) {
         // [i_rows, ..] of a row-major 16-bit tensor, from column `first` to the end of C's columns
         const uint64_t b = (uint64_t)(uintptr_t)base + (uint64_t)((i0 * ld + first) * 2);
@@ -478,10 +480,14 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                 v[q] = F::lo((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, c + q < cols ? row_b + 2 * (c + q) : kOutside, 0, 0));
         }
     };
-    // 16 columns from c on of the lane's row: as loaded, 8 a lane, and as the sums lie (columns 8u + 4hf ..)
-    auto load16 = [&](__amdgpu_buffer_rsrc_t r, uint32_t row_b, int c) __attribute__((always_inline)) {
+    // 16 columns from c on of the lane's row: as loaded, 8 a lane, and as the sums lie (columns 8u + 4hf ..).
+    // Rows that 16 bytes do not divide: 16 bytes at any address where the row has them, elements at its end
+    // (elements alone: gated [2048, 2 x 5123] deep 1280 96 us, dw [10240, 1283] of one row 240).
+    auto load16 = [&](__amdgpu_buffer_rsrc_t r, const char* base, uint32_t row, uint32_t ld_b, int c) __attribute__((always_inline)) {
         const int at = c + 8 * hf;
+        const uint32_t row_b = row * ld_b;
         if (vec) return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at < cols ? row_b + 2 * at : kOutside, 0, 0));
+        if ((int64_t)row < i_rows && at + 8 <= cols) return ((const Unaligned<2>*)(base + row_b + 2 * at))->v;
         u32x4 d{};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -501,15 +507,18 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         for (int q = 0; q < 4; ++q)
             v[q] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, c + q < cols ? 4 * (c + q) : kOutside, 0, 0));
     };
-    auto store8 = [&](__amdgpu_buffer_rsrc_t r, uint32_t row_b, int c, const float (&a)[4], const float (&b)[4]) __attribute__((always_inline)) {
+    auto store8 = [&](__amdgpu_buffer_rsrc_t r, char* base, uint32_t row, int c, const float (&a)[4], const float (&b)[4]) __attribute__((always_inline)) {
         // a: columns c + 4hf .., b: c + 8 + 4hf ..
         uint32_t a0 = F::pack(a[0], a[1]), a1 = F::pack(a[2], a[3]), b0 = F::pack(b[0], b[1]), b1 = F::pack(b[2], b[3]);
         join_halves(a0, b0);
         join_halves(a1, b1);
         const int at = c + 8 * hf;
         const u32x4 d{a0, a1, b0, b1};
+        const uint32_t row_b = row * ldo_b;
         if (vec) {
             __builtin_amdgcn_raw_buffer_store_b128(d, r, at < cols ? row_b + 2 * at : kOutside, 0, 0);
+        } else if ((int64_t)row < i_rows && at + 8 <= cols) {
+            ((Unaligned<2>*)(base + row_b + 2 * at))->v = d;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -526,10 +535,12 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         if (j0 + kCols >= p.cols && wj == 0 && hf == 0 && (int64_t)row < i_rows)
             for (int64_t z = first; z < p.out_cols_padded; ++z) ((T*)p.out)[(i0 + row) * p.ld_out + z] = (T)0.0f;
     };
-    const uint32_t ldo_b = (uint32_t)(p.ld_out * 2), ldd_b = (uint32_t)(p.ld_dout * 2), ldr_b = (uint32_t)(p.ld_res * 2);
     const auto dout = rows_window(p.dout, p.ld_dout, j0), residual = rows_window(p.residual, p.ld_res, j0);
     const auto out = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? value_row : 0) + j0);
     const auto out_g = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? gate_row : 0) + j0);
+    const char *dout_at = rows_at(p.dout, p.ld_dout, j0), *residual_at = rows_at(p.residual, p.ld_res, j0);
+    char *out_at = rows_at(p.out, p.ld_out, (kEpi == kFfGatedDz ? value_row : 0) + j0);
+    char *out_g_at = rows_at(p.out, p.ld_out, (kEpi == kFfGatedDz ? gate_row : 0) + j0);
     // What the epilogue reads of a tile (dout, or the residual): requested for all of the wave's tiles first where the
     // registers hold that, so that its latency passes once (256 x 256, dz [8192, 10240] 258 -> 239 us), else tile by tile.
     constexpr int kSets = kGated ? 1 : 2;  // of 16 columns
@@ -540,10 +551,10 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
 #pragma unroll
         for (int h = 0; h < kSets; ++h) {
             if constexpr (kEpi == kFfLinear) {
-                if (p.residual != nullptr) d[h] = load16(residual, row * ldr_b, c0 + 16 * h);
+                if (p.residual != nullptr) d[h] = load16(residual, residual_at, row, ldr_b, c0 + 16 * h);
                 else d[h] = u32x4{};
             } else {
-                d[h] = load16(dout, row * ldd_b, c0 + 16 * h);
+                d[h] = load16(dout, dout_at, row, ldd_b, c0 + 16 * h);
             }
         }
     };
@@ -601,8 +612,8 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     }
                 }
             }
-            store8(out, row * ldo_b, c0, va[0], va[1]);
-            if constexpr (kEpi == kFfGatedDz) store8(out_g, row * ldo_b, c0, vb[0], vb[1]);
+            store8(out, out_at, row, c0, va[0], va[1]);
+            if constexpr (kEpi == kFfGatedDz) store8(out_g, out_g_at, row, c0, vb[0], vb[1]);
         } else {
             float v[4][4], d[2][2][4] = {};
             if (kEpi == kFfLinearDz || (kEpi == kFfLinear && p.residual != nullptr)) {
@@ -624,8 +635,8 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     }
                 }
             }
-            store8(out, row * ldo_b, c0, v[0], v[1]);
-            store8(out, row * ldo_b, c0 + 16, v[2], v[3]);
+            store8(out, out_at, row, c0, v[0], v[1]);
+            store8(out, out_at, row, c0 + 16, v[2], v[3]);
         }
     };
     // a share's sums, 4 columns a lane
