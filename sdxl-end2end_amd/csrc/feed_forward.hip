@@ -74,14 +74,15 @@ float list_time(int64_t a, float a_time, int64_t b, float b_time, int64_t cus) {
 }
 
 // The same for the 32 x 32 tiles whose waves share the depth (feed_forward_deep.hip): 0.095 us a 64-deep block
-// where every CU has at most one tile, else 0.33 us per two tiles of a CU (0.25 where the caches hold w).
+// where every CU has at most one tile, else 0.33 us per two tiles of a CU (0.25 where the caches hold w), and 2.2 us
+// for the start and end of every two more (gated [8192, 64] -> 2 x 5120, 160 rounds of them: 420 us, on 256 x 320 tiles 58).
 float deep_time(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool& one_per_cu) {
     const int64_t cols = epilogue == kFfGated ? 2 * p.cols : p.cols;
     const int64_t tiles = ((p.rows + 31) / 32) * ((cols + 31) / 32);
-    const float blocks = (float)((p.depth + 63) / 64);
+    const float blocks = (float)((p.depth + 63) / 64), rounds = (float)tiles / (float)(2 * cus);
     one_per_cu = tiles <= cus;
-    const float shared = 0.33f * (float)tiles / (float)(2 * cus);
-    return 3.0f + blocks * (one_per_cu ? 0.095f : shared > 0.19f ? shared : 0.19f);
+    if (one_per_cu) return 3.0f + blocks * 0.095f;
+    return 3.0f + blocks * (0.33f * rounds > 0.19f ? 0.33f * rounds : 0.19f) + (rounds > 1.0f ? 2.2f * (rounds - 1.0f) : 0.0f);
 }
 
 int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus, float& best_time) {
@@ -114,9 +115,17 @@ FfParams prepared(const FfParams& params, bool i_transposed) {
     if (p.i_row == 0) p.i_row = i_transposed ? p.rows : p.depth;
     // 16-byte accesses in the epilogue (bias: 8)
     p.splits = 1;
+    p.share_stages = (int32_t)((p.depth + 63) / 64);
+    p.ld_partial = (p.cols + 7) / 8 * 8;
     p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 16) &&
             aligned(p.dout, 16) && (p.residual == nullptr || p.ld_res % 8 == 0) && (p.dout == nullptr || p.ld_dout % 8 == 0);
     return p;
+}
+
+// 128 x 128 tiles where every CU gets one, else 64 x 64 (gated [1024, 323] -> 2 x 1280 on 160 of the large tiles 18 us, 11 on
+// small ones).
+bool staged_large(const FfParams& p, int64_t cols, int compute_units) {
+    return ((p.rows + 127) / 128) * ((cols + 127) / 128) >= (compute_units > 0 ? compute_units : 256);
 }
 
 // ---- dw and dx in one launch. A side of it: a product on a tile, its depth in so many shares.
@@ -139,7 +148,7 @@ PairSide pair_side(const FfParams& p, int tile, int splits) {
     const int stages = share_stages(p, splits);
     // (no share may be empty, and few stages are not worth a start)
     const bool ok = splits == 1 || (stages >= 8 && (int64_t)stages * 64 * (splits - 1) < p.depth);
-    const int64_t sums = splits == 1 ? 0 : splits * p.rows * (p.cols + (p.row_sums != nullptr ? 1 : 0));
+    const int64_t sums = splits == 1 ? 0 : splits * p.rows * (p.ld_partial + (p.row_sums != nullptr ? 1 : 0));
     return {ok ? tiles * splits : (int64_t)1 << 30, (sums * 4 + 255) / 256 * 256, (float)stages * c.alone + c.ends - 2.0f};
 }
 
@@ -151,8 +160,9 @@ void set_splits(FfParams& p, int splits, float* partial) {
 
 FfJoin join_of(const FfParams& p) {
     if (p.splits == 1) return {};
-    const int64_t threads = p.rows * (p.cols / 8) + (p.row_sums != nullptr ? p.rows : 0);
-    return {p.partial, p.out, p.row_sums, p.ld_out, (int32_t)p.rows, (int32_t)p.cols, p.splits, p.vec, (int32_t)((threads + 255) / 256)};
+    const int64_t threads = p.rows * (p.ld_partial / 8) + (p.row_sums != nullptr ? p.rows : 0);
+    return {p.partial, p.out, p.row_sums, p.ld_out, (int32_t)p.rows, (int32_t)p.cols, (int32_t)p.ld_partial, p.splits, p.vec,
+            (int32_t)((threads + 255) / 256)};
 }
 
 // Adds the shares in their order, 8 columns a thread (or one row sum), and rounds once. Bound by the reads, which come
@@ -163,8 +173,8 @@ __global__ __launch_bounds__(256) void ff_join_kernel(FfJoin a, FfJoin b) {
     const bool second = (int)blockIdx.x >= a.blocks;
     const FfJoin& p = second ? b : a;
     const uint32_t at = (blockIdx.x - (second ? a.blocks : 0)) * 256 + threadIdx.x;
-    const uint32_t chunks = p.cols / 8, all = p.rows * chunks;
-    const size_t share = (size_t)p.rows * p.cols;
+    const uint32_t chunks = p.ld / 8, all = p.rows * chunks;
+    const size_t share = (size_t)p.rows * p.ld;
     if (at < all) {
         float v[8] = {};
         for (int s = 0; s < p.splits; ++s) {
@@ -173,12 +183,14 @@ __global__ __launch_bounds__(256) void ff_join_kernel(FfJoin a, FfJoin b) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
         }
-        T* out = (T*)p.out + (int64_t)(at / chunks) * p.ld_out + (at % chunks) * 8;
+        const int c = (at % chunks) * 8;
+        T* out = (T*)p.out + (int64_t)(at / chunks) * p.ld_out + c;
         if (p.vec) {
             *(u32x4*)out = u32x4{F::pack(v[0], v[1]), F::pack(v[2], v[3]), F::pack(v[4], v[5]), F::pack(v[6], v[7])};
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out[e] = (T)v[e];
+            for (int e = 0; e < 8; ++e)
+                if (c + e < p.cols) out[e] = (T)v[e];
         }
     } else if (p.row_sums != nullptr && at - all < (uint32_t)p.rows) {
         const float* sums = p.partial + p.splits * share + (at - all);
@@ -208,12 +220,11 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
     return i_row % 8 == 0 && (j_transposed ? p.cols % 8 == 0 : p.depth % (j_fp8 ? 16 : 8) == 0);
 }
 
-hipError_t launch_ff_staged(const FfParams& params, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
-                            int compute_units, hipStream_t stream) {
-    const FfParams p = prepared(params, i_transposed);
+hipError_t launch_ff_staged(const FfParams& params, FfEpilogue epilogue, bool bf16, bool j_fp8, int compute_units,
+                            hipStream_t stream) {
+    const FfParams p = prepared(params, false);
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
-    const bool large = ((p.rows + 127) / 128) * ((cols + 127) / 128) >= (compute_units > 0 ? compute_units : 256);
-    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, i_transposed, j_fp8, large, stream);
+    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, staged_large(p, cols, compute_units), stream);
 }
 
 hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
@@ -236,8 +247,20 @@ size_t ff_partial_bytes(int64_t m, int64_t features, int64_t k) {
     return m <= 0 || features <= 0 || k <= 0 ? 0 : all < (double)kMaxPartial ? ((size_t)all + 255) / 256 * 256 : kMaxPartial;
 }
 
-hipError_t launch_ff_pair(const FfParams& dw, const FfParams& dx, bool bf16, float* partial, size_t partial_bytes,
-                          int compute_units, hipStream_t stream) {
+namespace {
+
+hipError_t launch_join(const FfParams& w, const FfParams& x, bool bf16, hipStream_t stream) {
+    if (w.splits == 1 && x.splits == 1) return hipSuccess;
+    const FfJoin jw = join_of(w), jx = join_of(x);
+    const dim3 grid((unsigned)(jw.blocks + jx.blocks));
+    if (bf16) hipLaunchKernelGGL(ff_join_kernel<__bf16>, grid, dim3(256), 0, stream, jw, jx);
+    else hipLaunchKernelGGL(ff_join_kernel<_Float16>, grid, dim3(256), 0, stream, jw, jx);
+    return hipGetLastError();
+}
+
+// Both gradients on the tiled kernel.
+hipError_t launch_pair(const FfParams& dw, const FfParams& dx, bool bf16, float* partial, size_t partial_bytes,
+                       int compute_units, hipStream_t stream) {
     FfParams w = prepared(dw, true), x = prepared(dx, false);
     const int64_t cus = compute_units > 0 ? compute_units : 256;
     // apart, or together on the best pair of tiles that take a CU each, of whole depths or of shares of them.
@@ -279,15 +302,55 @@ hipError_t launch_ff_pair(const FfParams& dw, const FfParams& dx, bool bf16, flo
         set_splits(w, w_splits, partial);
         set_splits(x, x_splits, partial + (size_t)pair_side(w, best_w, w_splits).partial / 4);
         const hipError_t err = (bf16 ? ff_pair_bf16 : ff_pair_f16)(w, x, best_w, best_x, w_first, stream);
-        if (err != hipSuccess || (w.splits == 1 && x.splits == 1)) return err;
-        const FfJoin jw = join_of(w), jx = join_of(x);
-        const dim3 grid((unsigned)(jw.blocks + jx.blocks));
-        if (bf16) hipLaunchKernelGGL(ff_join_kernel<__bf16>, grid, dim3(256), 0, stream, jw, jx);
-        else hipLaunchKernelGGL(ff_join_kernel<_Float16>, grid, dim3(256), 0, stream, jw, jx);
-        return hipGetLastError();
+        return err != hipSuccess ? err : launch_join(w, x, bf16, stream);
     }
     const hipError_t err = launch_ff_tiled(dw, kFfStore, true, bf16, false, compute_units, stream);
     return err != hipSuccess ? err : launch_ff_tiled(dx, kFfStore, false, bf16, false, compute_units, stream);
+}
+
+// One gradient through registers; p becomes what was launched, for the joining pass.
+hipError_t launch_staged_gradient(FfParams& p, bool i_transposed, bool bf16, float*& partial, size_t& partial_bytes,
+                                  int compute_units, hipStream_t stream) {
+    const int64_t cus = compute_units > 0 ? compute_units : 256;
+    const bool large = staged_large(p, p.cols, compute_units);
+    // few tiles: shares of at least 16 stages until every CU has one (gradients of one row, w [10240, 1283]: 212 us, 76 so)
+    int splits = 1;
+    if (!large) {
+        const int64_t tiles = ((p.rows + 63) / 64) * ((p.cols + 63) / 64);
+        while (splits < kMaxSplits && tiles * splits < cus && share_stages(p, 2 * splits) >= 16 &&
+               pair_side(p, kFf64x64, 2 * splits).partial <= (int64_t)partial_bytes)
+            splits *= 2;
+    }
+    if (splits > 1) {
+        const size_t bytes = (size_t)pair_side(p, kFf64x64, splits).partial;
+        set_splits(p, splits, partial);
+        partial += bytes / 4;
+        partial_bytes -= bytes;
+    }
+    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, kFfStore, i_transposed, false, large, stream);
+}
+
+}  // namespace
+
+hipError_t launch_ff_gradients(const FfParams* dw, const FfParams* dx, bool bf16, float* partial, size_t partial_bytes,
+                               int compute_units, hipStream_t stream) {
+    const bool w_tiled = dw != nullptr && ff_tiled_supported(*dw, kFfStore, true, true, false);
+    const bool x_tiled = dx != nullptr && ff_tiled_supported(*dx, kFfStore, false, true, false);
+    if (w_tiled && x_tiled) return launch_pair(*dw, *dx, bf16, partial, partial_bytes, compute_units, stream);
+    FfParams w{}, x{};
+    w.splits = x.splits = 1;
+    hipError_t err = hipSuccess;
+    if (dw != nullptr) {
+        w = prepared(*dw, true);
+        err = w_tiled ? launch_ff_tiled(*dw, kFfStore, true, bf16, false, compute_units, stream)
+                      : launch_staged_gradient(w, true, bf16, partial, partial_bytes, compute_units, stream);
+    }
+    if (err == hipSuccess && dx != nullptr) {
+        x = prepared(*dx, false);
+        err = x_tiled ? launch_ff_tiled(*dx, kFfStore, false, bf16, false, compute_units, stream)
+                      : launch_staged_gradient(x, false, bf16, partial, partial_bytes, compute_units, stream);
+    }
+    return err != hipSuccess ? err : launch_join(w, x, bf16, stream);
 }
 
 }  // namespace sdxl_hip

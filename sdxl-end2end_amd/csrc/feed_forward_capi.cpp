@@ -72,15 +72,20 @@ sdxl_status resolve(const sdxl_ff_desc* d, bool gated, bool backward, const char
     return SDXL_STATUS_OK;
 }
 
-sdxl_status product(const FfParams& p, sdxl_hip::FfEpilogue epilogue, bool it, bool jt, const Call& c, bool w_fp8,
-                    hipStream_t stream, const char* name) {
+// A projection, or dz.
+sdxl_status product(const FfParams& p, sdxl_hip::FfEpilogue epilogue, const Call& c, bool w_fp8, hipStream_t stream,
+                    const char* name) {
+    const int cus = sdxl_hip_compute_units();
+    hipError_t err;
     if (sdxl_hip::ff_rows_supported(p, epilogue, w_fp8))
-        return launch_status(sdxl_hip::launch_ff_rows(p, epilogue, c.bf16, w_fp8, stream), name);
-    if (sdxl_hip::ff_tiled_supported(p, epilogue, it, jt, w_fp8))
-        return launch_status(sdxl_hip::launch_ff_tiled(p, epilogue, it, c.bf16, w_fp8, sdxl_hip_compute_units(), stream), name);
-    if (sdxl_hip::ff_staged_supported(p, epilogue, it, jt, w_fp8))
-        return launch_status(sdxl_hip::launch_ff_staged(p, epilogue, it, c.bf16, w_fp8, sdxl_hip_compute_units(), stream), name);
-    return launch_status(sdxl_hip::launch_ff_general(p, epilogue, it, jt, c.bf16, w_fp8, stream), name);
+        err = sdxl_hip::launch_ff_rows(p, epilogue, c.bf16, w_fp8, stream);
+    else if (sdxl_hip::ff_tiled_supported(p, epilogue, false, false, w_fp8))
+        err = sdxl_hip::launch_ff_tiled(p, epilogue, false, c.bf16, w_fp8, cus, stream);
+    else if (sdxl_hip::ff_staged_supported(p, epilogue, false, false, w_fp8))
+        err = sdxl_hip::launch_ff_staged(p, epilogue, c.bf16, w_fp8, cus, stream);
+    else
+        err = sdxl_hip::launch_ff_general(p, epilogue, false, false, c.bf16, w_fp8, stream);
+    return launch_status(err, name);
 }
 
 // The projections and their epilogue's inputs, shared by both directions.
@@ -118,7 +123,7 @@ sdxl_status forward(const sdxl_ff_desc* d, bool gated, const char* name, const v
     p.ld_res = c.ldr;
     p.out = out;
     p.ld_out = c.ldo;
-    return product(p, gated ? sdxl_hip::kFfGated : sdxl_hip::kFfLinear, false, false, c, c.w_fp8,
+    return product(p, gated ? sdxl_hip::kFfGated : sdxl_hip::kFfLinear, c, c.w_fp8,
                    reinterpret_cast<hipStream_t>(stream), name);
 }
 
@@ -171,7 +176,7 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
         p.ld_dout = c.ldo;
         p.out = workspace;
         p.ld_out = p.out_cols_padded = dz_stride(c);
-        st = product(p, gated ? sdxl_hip::kFfGatedDz : sdxl_hip::kFfLinearDz, false, false, c, false, stream, name);
+        st = product(p, gated ? sdxl_hip::kFfGatedDz : sdxl_hip::kFfLinearDz, c, false, stream, name);
         if (st != SDXL_STATUS_OK) return st;
         dz = workspace;
         lddz = dz_stride(c);
@@ -198,15 +203,19 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     px.ld_out = c.lddx;
     if (dz_needed) pw.i_row = px.i_row = lddz;
     float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(dz_bytes(c)));
-    if (want_dw && want_dx && sdxl_hip::ff_tiled_supported(pw, sdxl_hip::kFfStore, true, true, false) &&
-        sdxl_hip::ff_tiled_supported(px, sdxl_hip::kFfStore, false, true, false))
-        return launch_status(sdxl_hip::launch_ff_pair(pw, px, c.bf16, partial, sdxl_hip::ff_partial_bytes(c.m, c.features, c.k),
-                                                      sdxl_hip_compute_units(), stream), name);
-    if (want_dw || want_db) {
-        st = product(pw, sdxl_hip::kFfStore, true, true, c, false, stream, name);
+    // the gradients that the tiled kernels take, then the others
+    const bool w_fast = want_dw && sdxl_hip::ff_staged_supported(pw, sdxl_hip::kFfStore, true, true, false);
+    const bool x_fast = want_dx && sdxl_hip::ff_staged_supported(px, sdxl_hip::kFfStore, false, true, false);
+    if (w_fast || x_fast) {
+        st = launch_status(sdxl_hip::launch_ff_gradients(w_fast ? &pw : nullptr, x_fast ? &px : nullptr, c.bf16, partial,
+                                                         sdxl_hip::ff_partial_bytes(c.m, c.features, c.k),
+                                                         sdxl_hip_compute_units(), stream), name);
         if (st != SDXL_STATUS_OK) return st;
     }
-    if (want_dx) st = product(px, sdxl_hip::kFfStore, false, true, c, false, stream, name);
+    if ((want_dw || want_db) && !w_fast)
+        st = launch_status(sdxl_hip::launch_ff_general(pw, sdxl_hip::kFfStore, true, true, c.bf16, false, stream), name);
+    if (st == SDXL_STATUS_OK && want_dx && !x_fast)
+        st = launch_status(sdxl_hip::launch_ff_general(px, sdxl_hip::kFfStore, false, true, c.bf16, false, stream), name);
     return st;
 }
 

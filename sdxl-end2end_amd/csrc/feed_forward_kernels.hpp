@@ -40,9 +40,10 @@ struct FfParams {
     int32_t gate_first;
     // filled by the tiled kernel's launcher: wide epilogue accesses, tiles of C, row blocks per task group
     int32_t vec, i_blocks, j_blocks, group_i;
-    // The depth in `splits` shares of 64 * share_stages (ff_pair_kernel): share s leaves its sums in partial
-    // [splits][rows][cols], its row sums behind them in [splits][rows]; one share: as ever.
+    // kFfStore: the depth in `splits` shares of 64 * share_stages: share s leaves its sums in partial
+    // [splits][rows][ld_partial], its row sums behind them in [splits][rows]; one share: as ever.
     int32_t splits, share_stages;
+    int64_t ld_partial;  // cols, up to a multiple of 8
     float* partial;
 };
 
@@ -51,7 +52,7 @@ struct FfJoin {
     const float* partial;
     void *out, *row_sums;
     int64_t ld_out;
-    int32_t rows, cols, splits, vec, blocks;
+    int32_t rows, cols, ld, splits, vec, blocks;
 };
 
 // The general kernel: any size, stride and alignment.
@@ -66,17 +67,17 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
 hipError_t launch_ff_tiled(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
                            int compute_units, hipStream_t stream);
 
-// The same through registers: rows of any length and alignment.
+// Projections and dz through registers: rows of any alignment.
 bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);
-hipError_t launch_ff_staged(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
-                            int compute_units, hipStream_t stream);
+hipError_t launch_ff_staged(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, int compute_units,
+                            hipStream_t stream);
 
-// dw (I transposed) and dx, both of which the tiled kernel supports: in one launch where that is faster, with the
-// depth split as far as `partial` (256-byte aligned) holds the shares' sums: ff_partial_bytes is enough for any split
-// that is taken.
+// dw (I transposed) and dx (nullable, each; both writing) of operands that ff_staged_supported takes: in one launch where
+// both are tiled and that is faster, with the depth split where tiles are few, as far as `partial` (256-byte aligned)
+// holds the shares' sums: ff_partial_bytes is enough for any split that is taken.
 size_t ff_partial_bytes(int64_t m, int64_t features, int64_t k);
-hipError_t launch_ff_pair(const FfParams& dw, const FfParams& dx, bool bf16, float* partial, size_t partial_bytes,
-                          int compute_units, hipStream_t stream);
+hipError_t launch_ff_gradients(const FfParams* dw, const FfParams* dx, bool bf16, float* partial, size_t partial_bytes,
+                               int compute_units, hipStream_t stream);
 
 // Projections of at most 16 rows whose rows 16-byte accesses divide.
 bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8);

@@ -641,13 +641,13 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     };
     // a share's sums, 4 columns a lane
     auto store_share = [&](const f32x16& z, uint32_t row, int c0) __attribute__((always_inline)) {
-        const uint64_t b = (uint64_t)(uintptr_t)p.partial + (uint64_t)(((share * p.rows + i0) * p.cols + j0) * 4);
-        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)b, 0, (int)(((i_rows - 1) * p.cols + cols) * 4), 0x00020000);
+        const uint64_t b = (uint64_t)(uintptr_t)p.partial + (uint64_t)(((share * p.rows + i0) * p.ld_partial + j0) * 4);
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)b, 0, (int)((i_rows * p.ld_partial - j0) * 4), 0x00020000);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int c = c0 + 8 * u + 4 * hf;
             const f32x4 v{z[4 * u], z[4 * u + 1], z[4 * u + 2], z[4 * u + 3]};
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, c < cols ? (uint32_t)(row * p.cols + c) * 4 : kOutside, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, c < cols ? (uint32_t)(row * p.ld_partial + c) * 4 : kOutside, 0, 0);
         }
     };
     auto epilogue = [&]<FfFamily kFam, bool kShare = false>() __attribute__((always_inline)) {
@@ -760,7 +760,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     const int64_t i = i0 + 32 * (kWI * s + wi) + col;
                     const float v = sums[s] + __shfl_xor(sums[s], 32);
                     if (hf == 0 && i < p.rows) {
-                        if (kSplit && p.splits > 1) p.partial[(p.splits * p.cols + share) * p.rows + i] = v;
+                        if (kSplit && p.splits > 1) p.partial[(p.splits * p.ld_partial + share) * p.rows + i] = v;
                         else ((T*)p.row_sums)[i] = (T)v;
                     }
                 }
@@ -781,7 +781,7 @@ __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) voi
 template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
 __global__ __launch_bounds__(64 * Tile::kWaves, Tile::kMI * Tile::kMJ > 1 ? 2 : 4) void ff_staged_kernel(FfParams p) {
     __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
-    ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi, false, true>(p, blockIdx.x, smem);
+    ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi, kEpi == kFfStore, true>(p, blockIdx.x, smem);
 }
 
 // dw and dx in one launch, one workgroup per CU at a time: the tasks of the
@@ -818,7 +818,7 @@ hipError_t ff_launch(FfParams p, hipStream_t stream) {
 template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
 hipError_t ff_launch_staged(FfParams p, hipStream_t stream) {
     ff_blocks<Tile>(p, kEpi == kFfGated || kEpi == kFfGatedDz);
-    hipLaunchKernelGGL((ff_staged_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks)),
+    hipLaunchKernelGGL((ff_staged_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks * p.splits)),
                        dim3(64 * Tile::kWaves), 0, stream, p);
     return hipGetLastError();
 }

@@ -285,7 +285,9 @@ def test_backward_in_one_launch(m, n, k, dtype):
 # few tiles and a long sum: the depth of dx, of dw or of both in shares that do not come out even, joined afterwards
 @pytest.mark.parametrize("m,n,k,gated,activation", [(300, 2571, 136, True, "gelu"), (4100, 72, 264, False, "none"),
                                                     (8192, 136, 128, True, "silu"), (2200, 1288, 648, False, "gelu"),
-                                                    (90, 6000, 1000, False, "relu"), (1100, 1099, 72, False, "silu")])
+                                                    (90, 6000, 1000, False, "relu"), (1100, 1099, 72, False, "silu"),
+                                                    (2, 2571, 141, True, "gelu"), (4100, 72, 261, False, "none"), (4101, 71, 72, False, "silu"),
+                                                    (300, 4000, 137, True, "silu")])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_backward_of_split_sums(m, n, k, gated, activation, dtype):
     features = 2 * n if gated else n
