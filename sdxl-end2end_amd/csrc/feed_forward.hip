@@ -1,5 +1,6 @@
 // Which kernel and tile a product of the feed-forward operators runs on whose
-// rows 16-byte accesses divide (feed_forward_tiles.hpp, feed_forward_deep.hip).
+// rows have 16 bytes (feed_forward_tiles.hpp, feed_forward_deep.hip), and what goes
+// with the gradients: shares of a depth, their joining pass, row sums alone.
 #include <hip/hip_runtime.h>
 
 #include "feed_forward_device.hpp"
@@ -200,10 +201,51 @@ __global__ __launch_bounds__(256) void ff_join_kernel(FfJoin a, FfJoin b) {
     }
 }
 
+// Sums of I's rows alone (a bias gradient without its weights'): I = dz by columns, depth x rows. 8 columns a thread, 4 rows
+// of them a workgroup at a time, the depth in shares of `span`; one share writes the sums, more their parts. Bound by
+// the read: [8192, 5120] in 32 shares 24 us with the joining pass (316 as a product's by-product on the general kernel).
+constexpr int kSumsMaxShares = 32;
+
+template <typename T>
+__global__ __launch_bounds__(256) void ff_row_sums_kernel(FfParams p, int64_t span) {
+    using F = FfType<T>;
+    __shared__ float part[4][64][8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 8, first = (int64_t)blockIdx.y * span;
+    const int64_t last = first + span < p.depth ? first + span : p.depth;
+    const int n = (int)(p.rows - c < 8 ? p.rows - c : 8);
+    float v[8] = {};
+    const char* from = (const char*)p.ip + c * 2;
+    if (n == 8) {
+#pragma unroll 8
+        for (int64_t r = first + wave; r < last; r += 4) {
+            const u32x4 d = ((const Unaligned<2>*)(from + r * p.ld_i * 2))->v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[2 * e] += F::lo(d[e]), v[2 * e + 1] += F::hi(d[e]);
+        }
+    } else {
+        for (int64_t r = first + wave; r < last; r += 4)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < n) v[e] += (float)((const T*)(from + r * p.ld_i * 2))[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[wave][lane][e] = v[e];
+    __syncthreads();
+    for (int at = threadIdx.x; at < 512; at += 256) {
+        const int64_t i = (int64_t)blockIdx.x * 512 + at;
+        if (i >= p.rows) continue;
+        const float* x = &part[0][0][0] + at;
+        const float sum = (x[0] + x[512]) + (x[1024] + x[1536]);
+        if (gridDim.y > 1) p.partial[blockIdx.y * p.rows + i] = sum;
+        else ((T*)p.row_sums)[i] = (T)sum;
+    }
+}
+
 }  // namespace
 
 bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8) {
-    if (p.depth <= 0 || (epilogue == kFfStore && (!j_transposed || p.out == nullptr))) return false;
+    if (p.depth <= 0 || (epilogue == kFfStore && !j_transposed)) return false;
     // rows of 16 bytes or more: a row's last chunk is read as its last 16 bytes
     if ((i_transposed ? p.rows : p.depth) < 8 || (j_transposed ? p.cols : p.depth) < (j_fp8 ? 16 : 8)) return false;
     // a window (at most 320 rows) stays below 2^31 bytes, the threads of a launch below 2^32
@@ -351,6 +393,29 @@ hipError_t launch_ff_gradients(const FfParams* dw, const FfParams* dx, bool bf16
                       : launch_staged_gradient(x, false, bf16, partial, partial_bytes, compute_units, stream);
     }
     return err != hipSuccess ? err : launch_join(w, x, bf16, stream);
+}
+
+hipError_t launch_ff_row_sums(const FfParams& params, bool bf16, float* partial, size_t partial_bytes, int compute_units,
+                              hipStream_t stream) {
+    FfParams p = params;
+    const int64_t blocks = (p.rows + 511) / 512;
+    // shares of at least 64 rows until there are four workgroups a CU
+    int64_t shares = 1;
+    while (shares < kSumsMaxShares && blocks * shares < 4 * (int64_t)(compute_units > 0 ? compute_units : 256) &&
+           p.depth >= 128 * shares && 8 * shares * (size_t)p.rows <= partial_bytes)
+        shares *= 2;
+    const int64_t span = (p.depth + shares - 1) / shares;
+    p.partial = partial;
+    const dim3 grid((unsigned)blocks, (unsigned)shares);
+    if (bf16) hipLaunchKernelGGL(ff_row_sums_kernel<__bf16>, grid, dim3(256), 0, stream, p, span);
+    else hipLaunchKernelGGL(ff_row_sums_kernel<_Float16>, grid, dim3(256), 0, stream, p, span);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || shares == 1) return err;
+    FfParams none{};
+    none.splits = 1;
+    p.cols = p.ld_partial = 0;
+    p.splits = (int32_t)shares;
+    return launch_join(p, none, bf16, stream);
 }
 
 }  // namespace sdxl_hip

@@ -187,9 +187,9 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     pw.ld_i = lddz;
     pw.ld_j = c.ldx;
     pw.rows = c.features;
-    pw.cols = want_dw ? c.k : 1;  // the row sums alone: one tile of columns
+    pw.cols = c.k;
     pw.depth = c.m;
-    pw.out = want_dw ? dw : nullptr;
+    pw.out = dw;
     pw.ld_out = c.lddw;
     pw.row_sums = want_db ? dbias : nullptr;
     px.ip = dz;
@@ -203,16 +203,18 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     px.ld_out = c.lddx;
     if (dz_needed) pw.i_row = px.i_row = lddz;
     float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(dz_bytes(c)));
+    const size_t partial_bytes = sdxl_hip::ff_partial_bytes(c.m, c.features, c.k);
     // the gradients that the tiled kernels take, then the others
     const bool w_fast = want_dw && sdxl_hip::ff_staged_supported(pw, sdxl_hip::kFfStore, true, true, false);
     const bool x_fast = want_dx && sdxl_hip::ff_staged_supported(px, sdxl_hip::kFfStore, false, true, false);
     if (w_fast || x_fast) {
         st = launch_status(sdxl_hip::launch_ff_gradients(w_fast ? &pw : nullptr, x_fast ? &px : nullptr, c.bf16, partial,
-                                                         sdxl_hip::ff_partial_bytes(c.m, c.features, c.k),
-                                                         sdxl_hip_compute_units(), stream), name);
+                                                         partial_bytes, sdxl_hip_compute_units(), stream), name);
         if (st != SDXL_STATUS_OK) return st;
     }
-    if ((want_dw || want_db) && !w_fast)
+    if (want_db && !want_dw)
+        st = launch_status(sdxl_hip::launch_ff_row_sums(pw, c.bf16, partial, partial_bytes, sdxl_hip_compute_units(), stream), name);
+    else if (want_dw && !w_fast)
         st = launch_status(sdxl_hip::launch_ff_general(pw, sdxl_hip::kFfStore, true, true, c.bf16, false, stream), name);
     if (st == SDXL_STATUS_OK && want_dx && !x_fast)
         st = launch_status(sdxl_hip::launch_ff_general(px, sdxl_hip::kFfStore, false, true, c.bf16, false, stream), name);

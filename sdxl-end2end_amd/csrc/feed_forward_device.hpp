@@ -56,6 +56,12 @@ struct FfType<__bf16> {
     }
 };
 
+// 16 bytes at any element's address
+template <int kAlign>
+struct __attribute__((packed, aligned(kAlign))) Unaligned {
+    u32x4 v;
+};
+
 // An operand's window as a buffer descriptor (raw, byte offsets): reads at or
 // past `size` return zero.
 struct Window {

@@ -28,7 +28,7 @@ struct FfParams {
     const void* bias;         // nullable, by J rows
     const void* residual;     // nullable (kFfLinear)
     const void* dout;         // kFfLinearDz, kFfGatedDz
-    void* out;                // nullable with row_sums
+    void* out;
     void* row_sums;           // nullable (kFfStore): sums over r of every I row
     int64_t ld_res, ld_dout, ld_out;
     int64_t rows, cols, depth;  // of C before the gating: gated products have 2 n J rows, cols = n
@@ -78,6 +78,10 @@ hipError_t launch_ff_staged(const FfParams& p, FfEpilogue epilogue, bool bf16, b
 size_t ff_partial_bytes(int64_t m, int64_t features, int64_t k);
 hipError_t launch_ff_gradients(const FfParams* dw, const FfParams* dx, bool bf16, float* partial, size_t partial_bytes,
                                int compute_units, hipStream_t stream);
+
+// Row sums of I = dz by columns (row_sums) without a product.
+hipError_t launch_ff_row_sums(const FfParams& p, bool bf16, float* partial, size_t partial_bytes, int compute_units,
+                              hipStream_t stream);
 
 // Projections of at most 16 rows whose rows 16-byte accesses divide.
 bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8);

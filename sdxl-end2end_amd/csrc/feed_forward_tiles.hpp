@@ -49,12 +49,6 @@ typedef __attribute__((address_space(3))) i16x8 lds_op;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 typedef __attribute__((address_space(3))) float lds_float;
 
-// 16 bytes at any element's address
-template <int kAlign>
-struct __attribute__((packed, aligned(kAlign))) Unaligned {
-    u32x4 v;
-};
-
 __device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
 // Exchanges the halves so that lanes 0-31 hold 8 consecutive columns made of

@@ -318,6 +318,17 @@ def test_backward_parts(gated, activation):
     assert fn(dout, x, w, activation=activation, need_dx=False, need_dw=False, need_dbias=False) == (None, None, None)
 
 
+# the bias gradient without the weights': one share of the rows and many, whole and ragged groups of 8 columns, odd strides
+@pytest.mark.parametrize("m,n,pad", [(1, 3, 0), (127, 520, 0), (128, 512, 8), (5000, 1283, 0), (4097, 640, 3), (300, 10007, 1)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_bias_gradient_alone(m, n, pad, dtype):
+    x, w = values(1, m, 24, dtype=dtype), values(2, n, 24, std=0.2, dtype=dtype)
+    dout = values(3, m, n + pad, dtype=dtype)[:, :n]
+    for activation in ("none", "silu"):
+        got = sh.linear_act_backward(dout, x, w, activation=activation, need_dx=False, need_dw=False, need_dbias=True)
+        check_backward(dout, x, w, None, activation, got, False)
+
+
 @pytest.mark.parametrize("gated", [False, True])
 def test_empty_sums(gated):
     """No input features: the bias alone. No rows: gradients of zeros. No output features: dx of zeros."""
