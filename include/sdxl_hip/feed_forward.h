@@ -16,7 +16,8 @@
  * cores. Any m, n, k >= 0 and any row strides of at least a row; tensors need only their
  * element's alignment. Rows that 16-byte accesses divide (pointers and row strides
  * multiples of 16 bytes, k a multiple of 8 and with E4M3 weights of 16) run the fast
- * kernels, everything else the general one (the sums' order differs).
+ * kernels; other rows of 16 bytes or more take about twice as long, shorter ones and
+ * strides above 2^20 elements the general kernel (the sums' order differs).
  * An infinite pre-activation takes the activation's limit; NaN stays NaN.
  *
  * All calls are stream-ordered, allocate nothing, never synchronise and may be captured
@@ -75,8 +76,8 @@ sdxl_status sdxl_linear_act(const sdxl_ff_desc* desc, const void* x, const void*
 sdxl_status sdxl_gated_linear(const sdxl_ff_desc* desc, const void* x, const void* w, const float* w_scale,
                               const void* bias, void* out, void* stream);
 
-/* Workspace of the backward calls (dz, and partial sums where the rows are split), 256-byte
- * aligned; 0 for a descriptor that the call refuses. */
+/* Workspace of the backward calls (dz, and up to 32 MiB of partial sums where a product of few
+ * tiles splits its sum), 256-byte aligned; 0 for a descriptor that the call refuses. */
 size_t sdxl_linear_act_backward_workspace_bytes(const sdxl_ff_desc* desc);
 size_t sdxl_gated_linear_backward_workspace_bytes(const sdxl_ff_desc* desc);
 

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/sdxl_hip/feed_forward.h"
@@ -20,6 +21,13 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 sdxl_status fail(const char* name, sdxl_status status, const char* what) {
     return sdxl_hip_fail(status, std::string(name) + ": " + what);
+}
+
+// Outputs in place of an input that other workgroups still read: only the exact overlap is seen here.
+bool one_of(const void* out, std::initializer_list<const void*> inputs) {
+    for (const void* in : inputs)
+        if (out != nullptr && out == in) return true;
+    return false;
 }
 
 sdxl_status launch_status(hipError_t err, const char* name) {
@@ -118,6 +126,8 @@ sdxl_status forward(const sdxl_ff_desc* d, bool gated, const char* name, const v
     if (!aligned(x, 2) || !aligned(w, c.w_fp8 ? 1 : 2) || !aligned(w_scale, 4) || !aligned(bias, 2) ||
         !aligned(residual, 2) || !aligned(out, 2))
         return fail(name, SDXL_STATUS_UNSUPPORTED, "tensor not aligned to its elements");
+    if (one_of(out, {x, w, bias, w_scale}) || (out == residual && c.ldr != c.ldo))
+        return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "out overlaps an input");
     FfParams p = projection(c, x, w, w_scale, bias);
     p.residual = residual;
     p.ld_res = c.ldr;
@@ -166,6 +176,9 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     const size_t need = inputs ? backward_workspace(c) : 0;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");
+    for (const void* out : {want_dx ? dx : nullptr, want_dw ? dw : nullptr, want_db ? dbias : nullptr})
+        if (inputs && one_of(out, {dout, x, w, bias}))
+            return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "a gradient overlaps an input");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
 
     const void* dz = dout;

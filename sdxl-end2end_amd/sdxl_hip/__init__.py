@@ -536,8 +536,8 @@ def cross_attn_sublayer(x, ln_gamma, ln_beta, w_q, w_q_scale, kv, w_out, b_out, 
 def _ff_call(fn, index, t, *args) -> None:
     """fn(*args, stream) on the tensors' device, which is made current where it is not."""
     if index < 0:
-        status = fn(*args, None)
-    elif index == t.current_device():
+        raise SdxlError(INVALID_ARGUMENT, "feed-forward: tensors must be on a GPU")
+    if index == t.current_device():
         status = fn(*args, t.raw_stream(index))
     else:
         with t.device(index):

@@ -170,3 +170,30 @@ def test_torch_wrapper_refusals():
     ):
         with pytest.raises(sh.SdxlError):
             refused()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_outputs_in_place_of_inputs_are_refused(kind):
+    X, W, B, R, OUT = (P * i for i in range(1, 6))
+    if kind.endswith("backward"):
+        D, DX, DW, DB, WS = (P * i for i in range(6, 11))
+        given = dict(x=X, w=W, bias=B, dout=D, dx=DX, dw=DW, db=DB, ws=WS)
+        cases = [dict(given, **{out: given[i]}) for out in ("dx", "dw", "db") for i in ("x", "w", "dout", "bias")]
+    else:
+        given = dict(x=X, w=W, bias=B, out=OUT)
+        cases = [dict(given, out=given[i]) for i in ("x", "w", "bias")]
+    for case in cases:
+        assert call(kind, desc(), **case) == sh.INVALID_ARGUMENT
+        assert "overlaps" in sh.load().sdxl_last_error().decode()
+    if kind == "linear":  # the residual in place only row for row
+        d = desc(out_row_stride=16, residual_row_stride=24)
+        assert call(kind, d, x=X, w=W, res=R, out=R) == sh.INVALID_ARGUMENT
+
+
+def test_tensors_on_the_cpu_are_refused():
+    x, w = torch.zeros(4, 8, dtype=torch.float16), torch.zeros(6, 8, dtype=torch.float16)
+    for fn in (sh.linear_act, sh.gated_linear):
+        with pytest.raises(sh.SdxlError, match="on a GPU"):
+            fn(x, w)
+    with pytest.raises(sh.SdxlError, match="on a GPU"):
+        sh.linear_act_backward(torch.zeros(4, 6, dtype=torch.float16), x, w)

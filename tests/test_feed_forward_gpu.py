@@ -405,6 +405,20 @@ def test_what_lies_beside_the_rows_is_not_read_into_them(m, n, k, pad, shift):
     check_backward(dout, x, w[:n], None, "none", sh.linear_act_backward(dout, x, w[:n], need_dbias=True), False)
 
 
+# rows half a million elements apart (offsets past 32 bits at the last ones) and beyond the fast kernels' strides
+@pytest.mark.parametrize("m,ld", [(4600, 1 << 19), (4600, (1 << 19) + 1), (40, (1 << 20) + 8)])
+def test_rows_far_apart(m, ld):
+    n, k = 72, 136
+    wide = torch.empty(m, ld, dtype=F16, device=DEV)
+    x, out, dout = wide[:, 8:8 + k], wide[:, 1024:1024 + n], wide[:, 2048:2048 + n]
+    x.copy_(values(1, m, k))
+    dout.copy_(values(2, m, n, std=0.3))
+    w, bias = values(3, 2 * n, k, std=k ** -0.5), values(4, 2 * n, std=0.3)
+    sh.gated_linear(x, w, bias=bias, out=out)
+    check_forward(x, w.double(), bias, "gelu", out, True)
+    check_backward(dout, x, w, bias, "gelu", sh.gated_linear_backward(dout, x, w, bias=bias), True)
+
+
 def test_strided_gradients_through_the_c_abi():
     m, n, k = 40, 24, 72
     x, w, dout = values(1, m, k), values(2, n, k, std=0.12), values(3, m, n)
