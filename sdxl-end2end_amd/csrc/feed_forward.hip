@@ -16,7 +16,7 @@ hipError_t ff_pair_f16(const FfParams& w, const FfParams& x, int w_tile, int x_t
 hipError_t ff_pair_bf16(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream);
 hipError_t ff_staged_f16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
 hipError_t ff_staged_bf16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
-hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool one_per_cu, hipStream_t stream);
+hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool staged, bool one_per_cu, hipStream_t stream);
 
 namespace {
 
@@ -127,6 +127,22 @@ FfParams prepared(const FfParams& params, bool i_transposed) {
 // small ones).
 bool staged_large(const FfParams& p, int64_t cols, int compute_units) {
     return ((p.rows + 127) / 128) * ((cols + 127) / 128) >= (compute_units > 0 ? compute_units : 256);
+}
+
+// Rows through registers, on 64 x 64 tiles and on 32 x 32 ones whose waves share the depth, microseconds: a stage of the
+// first waits for its reads (0.85, more with over 256 tiles), the second have a block per wave under way. Measured in
+// bf16 [40, 5127] x [1280, 5127] 72 and 20, [600, 645] x [645, 645] 14.2 and 10.3, gated [1000, 323] -> 2 x 1280 12 and 33.
+float staged_time(const FfParams& p, int64_t cols) {
+    const int64_t tiles = ((p.rows + 63) / 64) * ((cols + 63) / 64);
+    return 4.5f + (float)((p.depth + 63) / 64) * (tiles > 256 ? 0.85f + 0.0012f * (float)(tiles - 256) : 0.85f);
+}
+
+float staged_deep_time(const FfParams& p, int64_t cols, int compute_units, bool& one_per_cu) {
+    const int64_t cus = compute_units > 0 ? compute_units : 256, tiles = ((p.rows + 31) / 32) * ((cols + 31) / 32);
+    const float blocks = (float)((p.depth + 63) / 64), rounds = (float)tiles / (float)(2 * cus);
+    one_per_cu = tiles <= cus;
+    if (one_per_cu) return 5.0f + 0.19f * blocks;
+    return rounds > 1.0f ? 3.0f + 0.6f * rounds * blocks + 2.2f * (rounds - 1.0f) : 3.0f + 0.6f * blocks;
 }
 
 // ---- dw and dx in one launch. A side of it: a product on a tile, its depth in so many shares.
@@ -266,7 +282,12 @@ hipError_t launch_ff_staged(const FfParams& params, FfEpilogue epilogue, bool bf
                             hipStream_t stream) {
     const FfParams p = prepared(params, false);
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
-    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, staged_large(p, cols, compute_units), stream);
+    const bool large = staged_large(p, cols, compute_units);
+    bool one_per_cu;
+    if (!large && (epilogue == kFfLinear || epilogue == kFfGated) &&
+        staged_deep_time(p, cols, compute_units, one_per_cu) < staged_time(p, cols))
+        return ff_deep(p, epilogue, bf16, j_fp8, true, one_per_cu, stream);
+    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, large, stream);
 }
 
 hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
@@ -278,7 +299,7 @@ hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_t
     if (epilogue == kFfLinear || epilogue == kFfGated) {
         bool one_per_cu;
         if (deep_time(p, epilogue, cus, one_per_cu) < time)
-            return ff_deep(p, epilogue, bf16, j_fp8, one_per_cu, stream);
+            return ff_deep(p, epilogue, bf16, j_fp8, false, one_per_cu, stream);
         return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, tile, stream);
     }
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);

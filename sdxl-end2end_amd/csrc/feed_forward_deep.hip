@@ -9,7 +9,8 @@
 // the tile. The waves' sums are added in LDS in the waves' order. Eight waves
 // where every CU has at most one tile, else four and two tiles a CU: [64, 5120] x
 // [1280, 5120] 10.3 us with eight, 13.5 with four, 31 on 64 x 64 tiles; [600, 640]
-// x [640, 640] 6.4, 4.9 and 8.
+// x [640, 640] 6.4, 4.9 and 8. Rows that 16-byte accesses do not divide come
+// through registers, two blocks ahead: [40, 5127] x [1280, 5127] 20 us.
 #include <hip/hip_runtime.h>
 
 #include "feed_forward_device.hpp"
@@ -21,7 +22,7 @@ namespace {
 typedef __attribute__((address_space(3))) i16x8 lds_op;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
-template <typename T, bool kJFp8, int kWaves, FfEpilogue kEpi>
+template <typename T, bool kJFp8, int kWaves, FfEpilogue kEpi, bool kStaged>
 __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     using F = FfType<T>;
     constexpr bool kGated = kEpi == kFfGated;
@@ -99,17 +100,63 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
             acc = F::mfma(jop, iop, acc);
         }
     };
+    if constexpr (kStaged) {
+        // through registers, two blocks ahead, and one place in LDS
+        u32x4 held[2][kXfers];
+        auto part = [&](int it, int n, const char*& at) __attribute__((always_inline)) {
+            const int64_t k0 = (int64_t)(it * kWaves + wave) * 64;
+            const int left = (int)min(p.depth - k0, (int64_t)64);
+            if (n < 4) {
+                at = (const char*)p.ip + (i0 + 8 * n + row8) * ldi_b + k0 * 2 + 16 * chunk8[n & 1];
+                return 8 * n + row8 < i_rows ? left - 8 * chunk8[n & 1] : 0;
+            }
+            n -= 4;
+            const bool gate = kGated && (kJFp8 ? n & 1 : n & 2);
+            const int row = kJFp8 ? (kGated ? 0 : 16 * n) + row16 : (kGated ? 8 * (n & 1) : 8 * n) + row8;
+            const int chunk = kJFp8 ? chunk16 : chunk8[n & 1];
+            at = (const char*)p.jp + ((kGated ? (gate ? gate_row : value_row) : 0) + j0 + row) * ldj_b + k0 * (kJFp8 ? 1 : 2) + 16 * chunk;
+            return row < j_rows ? left - (kJFp8 ? 16 : 8) * chunk : 0;
+        };
+        auto fetch = [&](int it, u32x4 (&to)[kXfers]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int it = 0; it < kRing; ++it)
-        if (it < mine) request(it, it);
-    for (int it = 0; it < mine; ++it) {
-        const int slot = it & 1;
-        if (it + 1 < mine) wait_vmem<kXfers>();  // the next block's transfers may still be on their way
-        else wait_vmem<0>();
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(slot);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is read
-        if (it + kRing < mine) request(it + kRing, slot);
+            for (int n = 0; n < kXfers; ++n) {
+                const char* at;
+                const int valid = it < mine ? part(it, n, at) : 0;
+                to[n] = kJFp8 && n >= 4 ? fetch_chunk<16>(at, valid) : fetch_chunk<8>(at, valid);
+            }
+        };
+        auto turn = [&](int it, u32x4 (&from)[kXfers]) __attribute__((always_inline)) {
+            char* buf = smem + wave * kRing * kBlock + lane * 16;
+#pragma unroll
+            for (int n = 0; n < kXfers; ++n) {
+                const char* at;
+                const int valid = part(it, n, at);
+                *(lds_u32x4*)(buf + n * 1024) = kJFp8 && n >= 4 ? settle_chunk<16>(from[n], valid) : settle_chunk<8>(from[n], valid);
+            }
+            fetch(it + 2, from);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            multiply(0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next block is put down
+        };
+        fetch(0, held[0]);
+        fetch(1, held[1]);
+        for (int it = 0; it < mine; it += 2) {
+            turn(it, held[0]);
+            if (it + 1 < mine) turn(it + 1, held[1]);
+        }
+    } else {
+#pragma unroll
+        for (int it = 0; it < kRing; ++it)
+            if (it < mine) request(it, it);
+        for (int it = 0; it < mine; ++it) {
+            const int slot = it & 1;
+            if (it + 1 < mine) wait_vmem<kXfers>();  // the next block's transfers may still be on their way
+            else wait_vmem<0>();
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(slot);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is read
+            if (it + kRing < mine) request(it + kRing, slot);
+        }
     }
     __syncthreads();
     // the sums: [wave][4][lane] f32x4; acc[4u + q]: row col, tile column 8u + 4hf + q
@@ -158,28 +205,31 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     }
 }
 
-template <typename T, bool kJFp8, int kWaves>
+template <typename T, bool kJFp8, int kWaves, bool kStaged>
 hipError_t launch(FfParams p, FfEpilogue epilogue, hipStream_t stream) {
     const bool gated = epilogue == kFfGated;
     p.i_blocks = (int32_t)((p.rows + 31) / 32);
     p.j_blocks = (int32_t)(gated ? (p.cols + 15) / 16 : (p.cols + 31) / 32);
     const dim3 grid((unsigned)(p.i_blocks * p.j_blocks)), block(64 * kWaves);
-    if (gated) hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfGated>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfLinear>), grid, block, 0, stream, p);
+    if (gated) hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfGated, kStaged>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfLinear, kStaged>), grid, block, 0, stream, p);
     return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool kStaged>
 hipError_t launch_type(const FfParams& p, FfEpilogue epilogue, bool j_fp8, bool one_per_cu, hipStream_t stream) {
-    if (one_per_cu) return j_fp8 ? launch<T, true, 8>(p, epilogue, stream) : launch<T, false, 8>(p, epilogue, stream);
-    return j_fp8 ? launch<T, true, 4>(p, epilogue, stream) : launch<T, false, 4>(p, epilogue, stream);
+    if (one_per_cu) return j_fp8 ? launch<T, true, 8, kStaged>(p, epilogue, stream) : launch<T, false, 8, kStaged>(p, epilogue, stream);
+    return j_fp8 ? launch<T, true, 4, kStaged>(p, epilogue, stream) : launch<T, false, 4, kStaged>(p, epilogue, stream);
 }
 
 }  // namespace
 
-hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool one_per_cu, hipStream_t stream) {
-    return bf16 ? launch_type<__bf16>(p, epilogue, j_fp8, one_per_cu, stream)
-                : launch_type<_Float16>(p, epilogue, j_fp8, one_per_cu, stream);
+hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool staged, bool one_per_cu, hipStream_t stream) {
+    if (staged)
+        return bf16 ? launch_type<__bf16, true>(p, epilogue, j_fp8, one_per_cu, stream)
+                    : launch_type<_Float16, true>(p, epilogue, j_fp8, one_per_cu, stream);
+    return bf16 ? launch_type<__bf16, false>(p, epilogue, j_fp8, one_per_cu, stream)
+                : launch_type<_Float16, false>(p, epilogue, j_fp8, one_per_cu, stream);
 }
 
 }  // namespace sdxl_hip

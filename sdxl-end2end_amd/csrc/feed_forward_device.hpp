@@ -62,6 +62,31 @@ struct __attribute__((packed, aligned(kAlign))) Unaligned {
     u32x4 v;
 };
 
+// A chunk of 16 bytes (kAll elements) of a row that 16-byte accesses do not divide, of which the row has `valid` elements
+// (none: 0 or less; rows have at least kAll). One that the row ends in is read as the row's last 16 bytes and shifted
+// by settle_chunk, which waits for the read.
+template <int kAll>
+__device__ __forceinline__ u32x4 fetch_chunk(const char* at, int valid) {
+    constexpr int kElem = 16 / kAll;
+    u32x4 d{};
+    if (valid > 0) d = ((const Unaligned<kElem>*)(at - (valid < kAll ? kAll - valid : 0) * kElem))->v;
+    return d;
+}
+
+template <int kAll>
+__device__ __forceinline__ u32x4 settle_chunk(u32x4 d, int valid) {
+    const int bits = valid < kAll && valid > 0 ? (kAll - valid) * (128 / kAll) : 0;
+    uint64_t lo = d[0] | (uint64_t)d[1] << 32, hi = d[2] | (uint64_t)d[3] << 32;
+    if (bits >= 64) {
+        lo = hi >> (bits - 64);
+        hi = 0;
+    } else if (bits > 0) {
+        lo = lo >> bits | hi << (64 - bits);
+        hi >>= bits;
+    }
+    return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
 // An operand's window as a buffer descriptor (raw, byte offsets): reads at or
 // past `size` return zero.
 struct Window {

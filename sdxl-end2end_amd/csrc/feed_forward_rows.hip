@@ -12,7 +12,9 @@
 // LDS in the waves' order. Up to 32 blocks (64 KiB; a depth of 2048) are on
 // their way at once; deeper products repeat that. (Weights loaded
 // straight into registers, 16 rows a load, took 9.5 us for [1, 1280] x [10240,
-// 1280], a plain read of those bytes 5.7.)
+// 1280], a plain read of those bytes 5.7, this 5.7 on the device.) Rows that 16-byte
+// accesses do not divide come through registers, as many blocks at once: [16,
+// 5127] x [1280, 5127] 20 us, [1, 1283] x [5120, 1283] 6.7.
 #include <hip/hip_runtime.h>
 
 #include "feed_forward_device.hpp"
@@ -31,7 +33,7 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, bool kJFp8, int kWaves, bool kGated>
+template <typename T, bool kJFp8, int kWaves, bool kGated, bool kStaged>
 __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
     using F = FfType<T>;
     constexpr int kBlocks = 32 / kWaves;  // of a wave at a time
@@ -64,30 +66,60 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
     f32x4 acc{};
     for (int first = 0; first < blocks; first += 32) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of the blocks' place are done
+        if constexpr (kStaged) {
+            // through registers: all reads first
+            constexpr int kAll = kJFp8 ? 16 : 8, kH = kJFp8 ? 1 : 2;
+            u32x4 held[kBlocks][kH];
+            auto x_valid = [&](int block, int q) { return r16 < p.rows ? depth - (64 * block + 32 * q + 8 * g) : 0; };
+            auto w_valid = [&](int block, int h) { return w_at[h] != kOutside ? depth - 64 * block - kAll * chunk_at[h] : 0; };
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            const int block = first + b * kWaves + wave;
-            if (block < blocks) {
+            for (int b = 0; b < kBlocks; ++b) {
+                const int block = first + b * kWaves + wave;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int k = 64 * block + 32 * q + 8 * g;
-                    x[b][q] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, k < depth && x_at != kOutside ? x_at + 2 * k : kOutside, 0, 0);
+                for (int q = 0; q < 2; ++q)
+                    x[b][q] = fetch_chunk<8>((const char*)p.ip + (r16 * p.ld_i + 64 * block + 32 * q + 8 * g) * 2, x_valid(block, q));
+#pragma unroll
+                for (int h = 0; h < kH; ++h)
+                    held[b][h] = fetch_chunk<kAll>((const char*)p.jp + w_at[h] + (int64_t)(64 * block + kAll * chunk_at[h]) * kElem, w_valid(block, h));
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const int block = first + b * kWaves + wave;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) x[b][q] = settle_chunk<8>(x[b][q], x_valid(block, q));
+                if (block < blocks) {  // (LDS holds no others)
+#pragma unroll
+                    for (int h = 0; h < kH; ++h)
+                        *(lds_u32x4*)(smem + (b * kWaves + wave) * kBlockBytes + 1024 * h + lane * 16) = settle_chunk<kAll>(held[b][h], w_valid(block, h));
                 }
             }
-        }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        } else {
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            const int block = first + b * kWaves + wave;
-            if (block < blocks) {
+            for (int b = 0; b < kBlocks; ++b) {
+                const int block = first + b * kWaves + wave;
+                if (block < blocks) {
 #pragma unroll
-                for (int h = 0; h < (kJFp8 ? 1 : 2); ++h) {
-                    const int k = 64 * block + (kJFp8 ? 16 : 8) * chunk_at[h];
-                    window_to_lds(w_rsrc, k < depth && w_at[h] != kOutside ? w_at[h] + kElem * k : kOutside,
-                                  lds0 + (b * kWaves + wave) * kBlockBytes + 1024 * h);
+                    for (int q = 0; q < 2; ++q) {
+                        const int k = 64 * block + 32 * q + 8 * g;
+                        x[b][q] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, k < depth && x_at != kOutside ? x_at + 2 * k : kOutside, 0, 0);
+                    }
                 }
             }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const int block = first + b * kWaves + wave;
+                if (block < blocks) {
+#pragma unroll
+                    for (int h = 0; h < (kJFp8 ? 1 : 2); ++h) {
+                        const int k = 64 * block + (kJFp8 ? 16 : 8) * chunk_at[h];
+                        window_to_lds(w_rsrc, k < depth && w_at[h] != kOutside ? w_at[h] + kElem * k : kOutside,
+                                      lds0 + (b * kWaves + wave) * kBlockBytes + 1024 * h);
+                    }
+                }
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
             if (first + b * kWaves + wave < blocks) {
@@ -148,23 +180,23 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
     }
 }
 
-template <typename T, bool kJFp8, int kWaves>
+template <typename T, bool kJFp8, int kWaves, bool kStaged>
 hipError_t launch(const FfParams& p, bool gated, hipStream_t stream) {
     const dim3 grid((unsigned)(gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16)), block(64 * kWaves);
     const int64_t blocks = (p.depth + 63) / 64, held = blocks < 32 ? (blocks + kWaves - 1) / kWaves * kWaves : 32;
     const size_t lds = (size_t)held * (kJFp8 ? 1024 : 2048);  // (the sums take 1 KiB a wave)
-    if (gated) hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, true>), grid, block, lds, stream, p);
-    else hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, false>), grid, block, lds, stream, p);
+    if (gated) hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, true, kStaged>), grid, block, lds, stream, p);
+    else hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, false, kStaged>), grid, block, lds, stream, p);
     return hipGetLastError();
 }
 
-template <typename T, bool kJFp8>
+template <typename T, bool kJFp8, bool kStaged>
 hipError_t launch_rows(const FfParams& p, bool gated, hipStream_t stream) {
     // waves of a workgroup: 2048 in all where there are blocks for them
     const int64_t groups = gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16, blocks = (p.depth + 63) / 64;
-    if (groups * 8 < 2048 && blocks > 8) return launch<T, kJFp8, 16>(p, gated, stream);
-    if (groups * 4 < 2048 && blocks > 4) return launch<T, kJFp8, 8>(p, gated, stream);
-    return launch<T, kJFp8, 4>(p, gated, stream);
+    if (groups * 8 < 2048 && blocks > 8) return launch<T, kJFp8, 16, kStaged>(p, gated, stream);
+    if (groups * 4 < 2048 && blocks > 4) return launch<T, kJFp8, 8, kStaged>(p, gated, stream);
+    return launch<T, kJFp8, 4, kStaged>(p, gated, stream);
 }
 
 }  // namespace
@@ -172,14 +204,17 @@ hipError_t launch_rows(const FfParams& p, bool gated, hipStream_t stream) {
 bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8) {
     // one window (below 2^31 bytes) holds w, one x
     const int64_t w_rows = epilogue == kFfGated ? 2 * p.cols : p.cols;
-    return (epilogue == kFfLinear || epilogue == kFfGated) && p.rows <= 16 && p.depth >= 8 &&
-           w_rows * p.ld_j * (j_fp8 ? 1 : 2) < (int64_t{1} << 31) && ff_tiled_supported(p, epilogue, false, false, j_fp8);
+    return (epilogue == kFfLinear || epilogue == kFfGated) && p.rows <= 16 &&
+           w_rows * p.ld_j * (j_fp8 ? 1 : 2) < (int64_t{1} << 31) && ff_staged_supported(p, epilogue, false, false, j_fp8);
 }
 
 hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, hipStream_t stream) {
-    const bool gated = epilogue == kFfGated;
-    if (bf16) return j_fp8 ? launch_rows<__bf16, true>(p, gated, stream) : launch_rows<__bf16, false>(p, gated, stream);
-    return j_fp8 ? launch_rows<_Float16, true>(p, gated, stream) : launch_rows<_Float16, false>(p, gated, stream);
+    const bool gated = epilogue == kFfGated, staged = !ff_tiled_supported(p, epilogue, false, false, j_fp8);
+    auto by_type = [&]<typename T>() {
+        if (staged) return j_fp8 ? launch_rows<T, true, true>(p, gated, stream) : launch_rows<T, false, true>(p, gated, stream);
+        return j_fp8 ? launch_rows<T, true, false>(p, gated, stream) : launch_rows<T, false, false>(p, gated, stream);
+    };
+    return bf16 ? by_type.template operator()<__bf16>() : by_type.template operator()<_Float16>();
 }
 
 }  // namespace sdxl_hip

@@ -218,9 +218,8 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         } else {
 #pragma unroll
             for (int x = 0; x < kXfers; ++x) {
-                const int all = kJFp8 && x >= kIX ? 16 : 8, valid = part(st, x, from);
-                held[x] = u32x4{};
-                if (valid > 0) held[x] = read16(x, from - (valid < all ? all - valid : 0) * (16 / all));
+                const int valid = part(st, x, from);
+                held[x] = kJFp8 && x >= kIX ? fetch_chunk<16>(from, valid) : fetch_chunk<8>(from, valid);
             }
         }
     };
@@ -230,17 +229,8 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
 #pragma unroll
             for (int x = 0; x < kXfers; ++x) {
                 const char* from;
-                const int all = kJFp8 && x >= kIX ? 16 : 8, valid = part(st, x, from);
-                const int bits = valid < all && valid > 0 ? (all - valid) * (128 / all) : 0;
-                uint64_t lo = held[x][0] | (uint64_t)held[x][1] << 32, hi = held[x][2] | (uint64_t)held[x][3] << 32;
-                if (bits >= 64) {
-                    lo = hi >> (bits - 64);
-                    hi = 0;
-                } else if (bits > 0) {
-                    lo = lo >> bits | hi << (64 - bits);
-                    hi >>= bits;
-                }
-                held[x] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+                const int valid = part(st, x, from);
+                held[x] = kJFp8 && x >= kIX ? settle_chunk<16>(held[x], valid) : settle_chunk<8>(held[x], valid);
             }
         }
 #pragma unroll

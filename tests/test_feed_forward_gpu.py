@@ -370,7 +370,8 @@ def test_row_strides(m, n, k, pad):
 
 # rows that no 16-byte access divides, on 64 x 64 and on 128 x 128 tiles: the last chunk of a row of 8 elements or more is
 # its last 16 bytes; E4M3 rows of 16 codes or more
-@pytest.mark.parametrize("m,n,k", [(1, 1283, 321), (40, 9, 8), (77, 100, 9), (130, 331, 71), (301, 257, 645), (2200, 1091, 133),
+@pytest.mark.parametrize("m,n,k", [(1, 1283, 321), (16, 1291, 2123), (7, 37, 4109), (5, 2056, 81), (19, 72, 1303), (63, 643, 1297),
+                                   (150, 651, 525), (33, 1501, 337), (40, 16, 9001), (40, 9, 8), (77, 100, 9), (130, 331, 71), (301, 257, 645), (2200, 1091, 133),
                                    (4100, 1543, 68)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_odd_rows(m, n, k, dtype):
