@@ -78,7 +78,7 @@ float list_time(int64_t a, float a_time, int64_t b, float b_time, int64_t cus) {
 // where every CU has at most one tile, else 0.33 us per two tiles of a CU (0.25 where the caches hold w), and 2.2 us
 // for the start and end of every two more (gated [8192, 64] -> 2 x 5120, 160 rounds of them: 420 us, on 256 x 320 tiles 58).
 float deep_time(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool& one_per_cu) {
-    const int64_t cols = epilogue == kFfGated ? 2 * p.cols : p.cols;
+    const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
     const int64_t tiles = ((p.rows + 31) / 32) * ((cols + 31) / 32);
     const float blocks = (float)((p.depth + 63) / 64), rounds = (float)tiles / (float)(2 * cus);
     one_per_cu = tiles <= cus;
@@ -114,17 +114,17 @@ int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus,
 FfParams prepared(const FfParams& params, bool i_transposed) {
     FfParams p = params;
     if (p.i_row == 0) p.i_row = i_transposed ? p.rows : p.depth;
-    // 16-byte accesses in the epilogue (bias: 8)
     p.splits = 1;
     p.share_stages = (int32_t)((p.depth + 63) / 64);
     p.ld_partial = (p.cols + 7) / 8 * 8;
+    // 16-byte accesses in the epilogue (bias: 8)
     p.vec = p.cols % 8 == 0 && p.ld_out % 8 == 0 && aligned(p.out, 16) && aligned(p.bias, 8) && aligned(p.residual, 16) &&
             aligned(p.dout, 16) && (p.residual == nullptr || p.ld_res % 8 == 0) && (p.dout == nullptr || p.ld_dout % 8 == 0);
     return p;
 }
 
-// 128 x 128 tiles where every CU gets one, else 64 x 64 (gated [1024, 323] -> 2 x 1280 on 160 of the large tiles 18 us, 11 on
-// small ones).
+// 128 x 128 tiles where every CU gets one, else 64 x 64: [8192, 2561] x [640, 2561], 320 of the large tiles, 62 us (small: 84);
+// [2632, 2567] x [640, 2567], 105, 66 (45); gated [2632, 2567] -> 2 x 640, 210, 68 (64).
 bool staged_large(const FfParams& p, int64_t cols, int compute_units) {
     return ((p.rows + 127) / 128) * ((cols + 127) / 128) >= (compute_units > 0 ? compute_units : 256);
 }
@@ -149,7 +149,7 @@ float staged_deep_time(const FfParams& p, int64_t cols, int compute_units, bool&
 constexpr int kPairTiles = 3, kPairTile[kPairTiles] = {kFf256x256, kFf128x256, kFf128x128};
 constexpr int kSplitSteps = 4, kMaxSplits = 1 << (kSplitSteps - 1);
 constexpr size_t kMaxPartial = 32 << 20;  // partial sums of a call, bytes
-// the joining pass
+// the joining pass: start and microseconds a byte
 constexpr float kJoinStart = 3.0f, kJoinPerByte = 0.4e-6f;
 
 struct PairSide {
@@ -183,7 +183,7 @@ FfJoin join_of(const FfParams& p) {
 }
 
 // Adds the shares in their order, 8 columns a thread (or one row sum), and rounds once. Bound by the reads, which come
-// out of the Infinity Cache.
+// out of the Infinity Cache: 5.7 MB 4.1 us.
 template <typename T>
 __global__ __launch_bounds__(256) void ff_join_kernel(FfJoin a, FfJoin b) {
     using F = FfType<T>;
@@ -284,8 +284,7 @@ hipError_t launch_ff_staged(const FfParams& params, FfEpilogue epilogue, bool bf
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
     const bool large = staged_large(p, cols, compute_units);
     bool one_per_cu;
-    if (!large && (epilogue == kFfLinear || epilogue == kFfGated) &&
-        staged_deep_time(p, cols, compute_units, one_per_cu) < staged_time(p, cols))
+    if (!large && staged_deep_time(p, cols, compute_units, one_per_cu) < staged_time(p, cols))
         return ff_deep(p, epilogue, bf16, j_fp8, true, one_per_cu, stream);
     return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, large, stream);
 }
@@ -296,12 +295,11 @@ hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_t
     const int64_t cus = compute_units > 0 ? compute_units : 256;
     float time = 0.0f;
     const int tile = choose_tile(p, epilogue, j_fp8, cus, time);
-    if (epilogue == kFfLinear || epilogue == kFfGated) {
-        bool one_per_cu;
-        if (deep_time(p, epilogue, cus, one_per_cu) < time)
-            return ff_deep(p, epilogue, bf16, j_fp8, false, one_per_cu, stream);
+    bool one_per_cu;
+    if (epilogue != kFfStore && deep_time(p, epilogue, cus, one_per_cu) < time)
+        return ff_deep(p, epilogue, bf16, j_fp8, false, one_per_cu, stream);
+    if (epilogue == kFfLinear || epilogue == kFfGated)
         return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, tile, stream);
-    }
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);
 }
 
@@ -328,8 +326,8 @@ hipError_t launch_pair(const FfParams& dw, const FfParams& dx, bool bf16, float*
     const int64_t cus = compute_units > 0 ? compute_units : 256;
     // apart, or together on the best pair of tiles that take a CU each, of whole depths or of shares of them.
     // Measured on an MI355X, dw and dx of x [m, k], w [f, k]: m 2048, k 1280, f 10240 apart 142 us, together 117;
-    // m 8192 apart 459, together 368; m 1111, k 640, f 5120 (two tasks in five CUs) together 42, with dx's depth in
-    // 2 shares 28.6 and 4 for the joining pass.
+    // m 8192 apart 459, together 368; m 1111, k 640, f 5120 together 42 (105 tasks for 256 CUs), with dx's depth in 2
+    // shares 28.6 and 4 for the joining pass.
     float apart_w, apart_x;
     choose_tile(w, kFfStore, false, cus, apart_w);
     choose_tile(x, kFfStore, false, cus, apart_x);

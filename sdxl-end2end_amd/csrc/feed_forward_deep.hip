@@ -1,4 +1,4 @@
-// Projections of few tiles and much depth (some tens to hundreds of rows, few
+// Projections, and dz, of few tiles and much depth (some tens to hundreds of rows, few
 // columns: the down projections of short batches). Tiles of the tiled kernel
 // that fill the CUs there are so small that a stage's barrier costs more than
 // its work (64 x 64: 0.3 us a 64-deep stage, 650 clocks for 64 of matrix
@@ -10,7 +10,8 @@
 // where every CU has at most one tile, else four and two tiles a CU: [64, 5120] x
 // [1280, 5120] 10.3 us with eight, 13.5 with four, 31 on 64 x 64 tiles; [600, 640]
 // x [640, 640] 6.4, 4.9 and 8. Rows that 16-byte accesses do not divide come
-// through registers, two blocks ahead: [40, 5127] x [1280, 5127] 20 us.
+// through registers, two blocks ahead: [40, 5127] x [1280, 5127] 20 us. dz of 19
+// rows, 2 x 736 deep 2048: 7.3 us here, 16 on 64 x 64 tiles.
 #include <hip/hip_runtime.h>
 
 #include "feed_forward_device.hpp"
@@ -25,7 +26,7 @@ typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 template <typename T, bool kJFp8, int kWaves, FfEpilogue kEpi, bool kStaged>
 __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     using F = FfType<T>;
-    constexpr bool kGated = kEpi == kFfGated;
+    constexpr bool kGated = kEpi == kFfGated || kEpi == kFfGatedDz, kDz = kEpi == kFfLinearDz || kEpi == kFfGatedDz;
     constexpr int kRing = 2, kCols = kGated ? 16 : 32;
     constexpr int kIBytes = 32 * 128, kBlock = kIBytes + 32 * (kJFp8 ? 64 : 128), kXfers = kBlock / 1024;
     __shared__ __attribute__((aligned(1024))) char smem[kWaves * kRing * kBlock];  // then the sums
@@ -186,33 +187,58 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
         f32x4 b{};
         if constexpr (kGated) b = sum_of(wave + 2);
         if (i >= p.rows) return;
-        float v[4];
+        if constexpr (kDz) {
+            const T* dout = (const T*)p.dout + i * p.ld_dout;
+            T* out = (T*)p.out + i * p.ld_out;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            v[q] = 0.0f;
-            if (c + q >= p.cols) continue;
-            if constexpr (kGated) v[q] = z_of(a[q], value_row + c + q) * ff_value_of(act, fam, z_of(b[q], gate_row + c + q));
-            else v[q] = ff_value_of(act, fam, z_of(a[q], c + q)) + (p.residual != nullptr ? (float)((const T*)p.residual)[i * p.ld_res + c + q] : 0.0f);
-        }
-        T* out = (T*)p.out + i * p.ld_out + c;
-        if (p.vec && c < p.cols) {
-            *(u32x2*)out = u32x2{F::pack(v[0], v[1]), F::pack(v[2], v[3])};
+            for (int q = 0; q < 4; ++q) {
+                if (c + q >= p.cols) continue;
+                const float d = (float)dout[c + q];
+                float value;
+                if constexpr (kGated) {
+                    const float s = ff_slope_of(act, fam, z_of(b[q], gate_row + c + q), value);
+                    out[value_row + c + q] = (T)(d * value);
+                    out[gate_row + c + q] = (T)(d * z_of(a[q], value_row + c + q) * s);
+                } else {
+                    out[c + q] = (T)(ff_slope_of(act, fam, z_of(a[q], c + q), value) * d);
+                }
+                if (c + q == p.cols - 1)  // up to the padded row
+                    for (int64_t z = kGated ? 2 * p.cols : p.cols; z < p.out_cols_padded; ++z) out[z] = (T)0.0f;
+            }
         } else {
+            float v[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (c + q < p.cols) out[q] = (T)v[q];
+            for (int q = 0; q < 4; ++q) {
+                v[q] = 0.0f;
+                if (c + q >= p.cols) continue;
+                if constexpr (kGated) v[q] = z_of(a[q], value_row + c + q) * ff_value_of(act, fam, z_of(b[q], gate_row + c + q));
+                else v[q] = ff_value_of(act, fam, z_of(a[q], c + q)) + (p.residual != nullptr ? (float)((const T*)p.residual)[i * p.ld_res + c + q] : 0.0f);
+            }
+            T* out = (T*)p.out + i * p.ld_out + c;
+            if (p.vec && c < p.cols) {
+                *(u32x2*)out = u32x2{F::pack(v[0], v[1]), F::pack(v[2], v[3])};
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (c + q < p.cols) out[q] = (T)v[q];
+            }
         }
     }
 }
 
 template <typename T, bool kJFp8, int kWaves, bool kStaged>
 hipError_t launch(FfParams p, FfEpilogue epilogue, hipStream_t stream) {
-    const bool gated = epilogue == kFfGated;
     p.i_blocks = (int32_t)((p.rows + 31) / 32);
-    p.j_blocks = (int32_t)(gated ? (p.cols + 15) / 16 : (p.cols + 31) / 32);
+    p.j_blocks = (int32_t)(epilogue == kFfGated || epilogue == kFfGatedDz ? (p.cols + 15) / 16 : (p.cols + 31) / 32);
     const dim3 grid((unsigned)(p.i_blocks * p.j_blocks)), block(64 * kWaves);
-    if (gated) hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfGated, kStaged>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfLinear, kStaged>), grid, block, 0, stream, p);
+    if (epilogue == kFfGated) {
+        hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfGated, kStaged>), grid, block, 0, stream, p);
+    } else if (epilogue == kFfLinear) {
+        hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kWaves, kFfLinear, kStaged>), grid, block, 0, stream, p);
+    } else if constexpr (!kJFp8) {
+        if (epilogue == kFfGatedDz) hipLaunchKernelGGL((ff_deep_kernel<T, false, kWaves, kFfGatedDz, kStaged>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((ff_deep_kernel<T, false, kWaves, kFfLinearDz, kStaged>), grid, block, 0, stream, p);
+    }
     return hipGetLastError();
 }
 

@@ -209,6 +209,16 @@ __device__ __forceinline__ float ff_value_of(const FfAct& a, FfFamily fam, float
     }
 }
 
+// the same of act'(z), with act(z)
+__device__ __forceinline__ float ff_slope_of(const FfAct& a, FfFamily fam, float z, float& value) {
+    switch (fam) {
+    case kFamErf: return ff_slope<kFamErf>(a, z, value);
+    case kFamTanh: return ff_slope<kFamTanh>(a, z, value);
+    case kFamSigmoid: return ff_slope<kFamSigmoid>(a, z, value);
+    default: return ff_slope<kFamLinear>(a, z, value);
+    }
+}
+
 // f.operator()<family>() of the activation
 template <typename Fn>
 __device__ __forceinline__ void ff_with_family(int32_t activation, Fn&& f) {
