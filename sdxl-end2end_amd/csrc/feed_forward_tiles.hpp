@@ -288,28 +288,23 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         const int ks = kSteps * wk + k;
         row_off[k] = col * 128 + (((4 * (ks >> 1) + 2 * hf + (ks & 1)) ^ swz(col)) << 4);
     }
-    // by columns: [q][depth group of 4][half of the panel]; the half is the wave's
-    // where an even number of waves share the operand, else the tile's
-    constexpr int kQ = kSteps > 1 ? 2 : 1, kHalfI = kWI == 1 ? 2 : 1, kHalfJ = kWJ == 1 ? 2 : 1;
-    int tr_i[kQ][2][kHalfI], tr_j[kQ][2][kHalfJ];
+    // by columns: [q][depth group of 4] in the wave's half of the panel
+    int tr_i[2][2], tr_j[2][2];
     if constexpr (kIT || kJT) {
         const int s = lane & 15, g = lane >> 4, pp = kSteps * wk >> 1;
 #pragma unroll
-        for (int k = 0; k < kQ; ++k)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int q = kQ == 2 ? k : wk & 1;
                 const int row = 16 * (g >> 1) + 8 * q + 4 * h + (s >> 2);
                 const int c = 2 * (g & 1) + ((s & 3) >> 1), at = pp * 4096 + row * 128 + (s & 1) * 8;
-#pragma unroll
-                for (int b = 0; b < kHalfI; ++b) tr_i[k][h][b] = at + (((c + 4 * (kWI == 1 ? b : wi & 1)) ^ swz(row)) << 4);
-#pragma unroll
-                for (int b = 0; b < kHalfJ; ++b) tr_j[k][h][b] = at + (((c + 4 * (kWJ == 1 ? b : wj & 1)) ^ swz(row)) << 4);
+                tr_i[q][h] = at + (((c + 4 * (wi & 1)) ^ swz(row)) << 4);
+                tr_j[q][h] = at + (((c + 4 * (wj & 1)) ^ swz(row)) << 4);
             }
     }
     // The wave's tile t is tile kW t + w of the region (kW waves share the
     // operand): by columns it is half w % 2 of panel (kW t + w) / 2.
-    static_assert((!kIT || kWI == 1 || kWI % 2 == 0) && (!kJT || kWJ == 1 || kWJ % 2 == 0), "half panels by wave or by tile");
+    static_assert(kWI % 2 == 0 && kWJ % 2 == 0 && kSteps % 2 == 0, "half panels by wave, both depth groups by step");
     auto read_rows = [&](const char* region, int t, int k) __attribute__((always_inline)) {
         return *(const lds_op*)(region + t * 4096 + row_off[k]);
     };
@@ -333,14 +328,12 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     jop[(k >> 1) & 1][t] = *(const lds_u32x4*)(buf + j_base + t * kWJ * 2048 + col * 64 +
                                                               (((2 * (k >> 1) + hf) ^ ((col >> 2) & 3)) << 4));
             } else {
-                if constexpr (kJT) jop[set][t] = __builtin_bit_cast(u32x4, read_columns(buf + j_base, t * kWJ / 2, tr_j[k & (kQ - 1)][0][t & (kHalfJ - 1)],
-                                                                                     tr_j[k & (kQ - 1)][1][t & (kHalfJ - 1)], k));
+                if constexpr (kJT) jop[set][t] = __builtin_bit_cast(u32x4, read_columns(buf + j_base, t * kWJ / 2, tr_j[k & 1][0], tr_j[k & 1][1], k));
                 else jop[set][t] = __builtin_bit_cast(u32x4, read_rows(buf + j_base, t * kWJ, k));
             }
         } else {
             const int t = x - 1;
-            if constexpr (kIT) iop[set][t] = read_columns(buf + i_base, t * kWI / 2, tr_i[k & (kQ - 1)][0][t & (kHalfI - 1)],
-                                                          tr_i[k & (kQ - 1)][1][t & (kHalfI - 1)], k);
+            if constexpr (kIT) iop[set][t] = read_columns(buf + i_base, t * kWI / 2, tr_i[k & 1][0], tr_i[k & 1][1], k);
             else iop[set][t] = read_rows(buf + i_base, t * kWI, k);
         }
     };
