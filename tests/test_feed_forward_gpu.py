@@ -596,6 +596,44 @@ def test_two_graphs_share_a_workspace():
         ws.fill_(255)
 
 
+# joined shares of a sum, rows through registers, few rows, a bias gradient alone: one graph each, over one workspace that
+# is overwritten between the replays, with another shape's eager call in between
+@pytest.mark.parametrize("m,n,k,parts", [(1111, 640, 320, "xwb"), (300, 2571, 136, "xwb"), (70, 643, 331, "xwb"), (2, 643, 645, "xw"),
+                                         (4100, 640, 72, "b")])
+def test_captured_gradients_of_every_kind(m, n, k, parts):
+    x, w, dout = values(1, m, k), values(2, 2 * n, k, std=k ** -0.5), values(3, m, n, std=0.3)
+    need = dict(need_dx="x" in parts, need_dw="w" in parts, need_dbias="b" in parts)
+    ws = torch.empty(sh.ff_backward_workspace_bytes(m, n, k, True, "gelu"), dtype=torch.uint8, device=DEV)
+    want = sh.gated_linear_backward(dout, x, w, workspace=ws, **need)
+    other = [values(4, 500, 72), values(5, 144, 72, std=0.1), values(6, 500, 144)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sh.gated_linear_backward(dout, x, w, workspace=ws, **need)
+    for _ in range(4):
+        for g in got:
+            if g is not None:
+                g.fill_(float("nan"))
+        ws.fill_(255)
+        sh.linear_act_backward(other[2], other[0], other[1], activation="gelu")
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got) if a is not None)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 72, 64), (70, 136, 72), (300, 331, 71), (2100, 1288, 136)])
+def test_vectors_off_alignment(m, n, k):
+    """bias and scales that begin anywhere: elements' alignment is all they need."""
+    x, w = values(1, m, k), values(2, 2 * n, k, std=k ** -0.5)
+    bias = values(3, 2 * n + 1, std=0.3)[1:]
+    scale = values(4, 2 * n + 1, dtype=torch.float32).abs()[1:]
+    w64 = w.double() * scale.double()[:, None]
+    check_forward(x, w64, bias, "gelu", sh.gated_linear(x, w, bias=bias, w_scale=scale), True)
+    check_forward(x, w64, bias, "silu", sh.linear_act(x, w, bias=bias, w_scale=scale, activation="silu"), False)
+    dout = values(5, m, n, std=0.3)
+    check_backward(dout, x, w, bias, "gelu", sh.gated_linear_backward(dout, x, w, bias=bias), True)
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("B,S,W", [(2, 50, 128), (1, 1, 640), (1, 77, 66)])
 def test_sublayer_is_its_steps(B, S, W, fp8):
