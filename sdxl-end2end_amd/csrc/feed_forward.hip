@@ -319,19 +319,27 @@ hipError_t launch_join(const FfParams& w, const FfParams& x, bool bf16, hipStrea
     return hipGetLastError();
 }
 
-// Both gradients on the tiled kernel.
-hipError_t launch_pair(const FfParams& dw, const FfParams& dx, bool bf16, float* partial, size_t partial_bytes,
+// Both gradients on the tiled kernel, or one (the other's pointer null).
+hipError_t launch_pair(const FfParams* dw, const FfParams* dx, bool bf16, float* partial, size_t partial_bytes,
                        int compute_units, hipStream_t stream) {
-    FfParams w = prepared(dw, true), x = prepared(dx, false);
+    FfParams w{}, x{};  // (no rows: no tasks)
+    w.splits = x.splits = 1;
     const int64_t cus = compute_units > 0 ? compute_units : 256;
     // apart, or together on the best pair of tiles that take a CU each, of whole depths or of shares of them.
     // Measured on an MI355X, dw and dx of x [m, k], w [f, k]: m 2048, k 1280, f 10240 apart 142 us, together 117;
     // m 8192 apart 459, together 368; m 1111, k 640, f 5120 together 42 (105 tasks for 256 CUs), with dx's depth in 2
-    // shares 28.6 and 4 for the joining pass.
-    float apart_w, apart_x;
-    choose_tile(w, kFfStore, false, cus, apart_w);
-    choose_tile(x, kFfStore, false, cus, apart_x);
-    float best = apart_w + apart_x;
+    // shares 28.6 and 4 for the joining pass; dx alone of m 154, k 1280, f 5120 whole 31, in shares 18.
+    float best = 0.0f, apart;
+    if (dw != nullptr) {
+        w = prepared(*dw, true);
+        choose_tile(w, kFfStore, false, cus, apart);
+        best += apart;
+    }
+    if (dx != nullptr) {
+        x = prepared(*dx, false);
+        choose_tile(x, kFfStore, false, cus, apart);
+        best += apart;
+    }
     int best_w = -1, best_x = -1, w_splits = 1, x_splits = 1;
     bool w_first = true;
     PairSide sides[2][kPairTiles][kSplitSteps];
@@ -341,13 +349,14 @@ hipError_t launch_pair(const FfParams& dw, const FfParams& dx, bool bf16, float*
     for (int i = 0; i < kPairTiles * kSplitSteps * kPairTiles * kSplitSteps; ++i) {
         const int tw = i / (kSplitSteps * kPairTiles * kSplitSteps), tx = i / kSplitSteps % kPairTiles;
         const int sw = i / (kPairTiles * kSplitSteps) % kSplitSteps, sx = i % kSplitSteps;
+        if ((dw == nullptr && (tw > 0 || sw > 0)) || (dx == nullptr && (tx > 0 || sx > 0))) continue;
         const PairSide &a = sides[0][tw][sw], &b = sides[1][tx][sx];
         const int64_t partial_size = a.partial + b.partial;
         if (a.tasks + b.tasks > (1 << 23) || partial_size > (int64_t)partial_bytes) continue;
         const float join = partial_size == 0 ? 0.0f : kJoinStart + (float)partial_size * kJoinPerByte;
         const float least = ((float)a.tasks * a.time + (float)b.tasks * b.time) / (float)cus;
         if (2.0f + join + least >= best) continue;
-        const bool first = a.time >= b.time;
+        const bool first = dx == nullptr || (dw != nullptr && a.time >= b.time);
         const float time = 2.0f + join + (first ? list_time(a.tasks, a.time, b.tasks, b.time, cus)
                                                 : list_time(b.tasks, b.time, a.tasks, a.time, cus));
         if (time < best) {
@@ -360,13 +369,15 @@ hipError_t launch_pair(const FfParams& dw, const FfParams& dx, bool bf16, float*
         }
     }
     if (best_w >= 0) {
-        set_splits(w, w_splits, partial);
-        set_splits(x, x_splits, partial + (size_t)pair_side(w, best_w, w_splits).partial / 4);
+        if (dw != nullptr) set_splits(w, w_splits, partial);
+        if (dx != nullptr) set_splits(x, x_splits, partial + (size_t)pair_side(w, best_w, w_splits).partial / 4);
         const hipError_t err = (bf16 ? ff_pair_bf16 : ff_pair_f16)(w, x, best_w, best_x, w_first, stream);
         return err != hipSuccess ? err : launch_join(w, x, bf16, stream);
     }
-    const hipError_t err = launch_ff_tiled(dw, kFfStore, true, bf16, false, compute_units, stream);
-    return err != hipSuccess ? err : launch_ff_tiled(dx, kFfStore, false, bf16, false, compute_units, stream);
+    hipError_t err = hipSuccess;
+    if (dw != nullptr) err = launch_ff_tiled(*dw, kFfStore, true, bf16, false, compute_units, stream);
+    if (err == hipSuccess && dx != nullptr) err = launch_ff_tiled(*dx, kFfStore, false, bf16, false, compute_units, stream);
+    return err;
 }
 
 // One gradient through registers; p becomes what was launched, for the joining pass.
@@ -397,19 +408,21 @@ hipError_t launch_ff_gradients(const FfParams* dw, const FfParams* dx, bool bf16
                                int compute_units, hipStream_t stream) {
     const bool w_tiled = dw != nullptr && ff_tiled_supported(*dw, kFfStore, true, true, false);
     const bool x_tiled = dx != nullptr && ff_tiled_supported(*dx, kFfStore, false, true, false);
-    if (w_tiled && x_tiled) return launch_pair(*dw, *dx, bf16, partial, partial_bytes, compute_units, stream);
+    hipError_t err = hipSuccess;
+    if (w_tiled || x_tiled) {
+        err = launch_pair(w_tiled ? dw : nullptr, x_tiled ? dx : nullptr, bf16, partial, partial_bytes, compute_units, stream);
+        if (err != hipSuccess || ((dw == nullptr || w_tiled) && (dx == nullptr || x_tiled))) return err;
+    }
+    // (what launch_pair left in `partial` is joined by now)
     FfParams w{}, x{};
     w.splits = x.splits = 1;
-    hipError_t err = hipSuccess;
-    if (dw != nullptr) {
+    if (dw != nullptr && !w_tiled) {
         w = prepared(*dw, true);
-        err = w_tiled ? launch_ff_tiled(*dw, kFfStore, true, bf16, false, compute_units, stream)
-                      : launch_staged_gradient(w, true, bf16, partial, partial_bytes, compute_units, stream);
+        err = launch_staged_gradient(w, true, bf16, partial, partial_bytes, compute_units, stream);
     }
-    if (err == hipSuccess && dx != nullptr) {
+    if (err == hipSuccess && dx != nullptr && !x_tiled) {
         x = prepared(*dx, false);
-        err = x_tiled ? launch_ff_tiled(*dx, kFfStore, false, bf16, false, compute_units, stream)
-                      : launch_staged_gradient(x, false, bf16, partial, partial_bytes, compute_units, stream);
+        err = launch_staged_gradient(x, false, bf16, partial, partial_bytes, compute_units, stream);
     }
     return err != hipSuccess ? err : launch_join(w, x, bf16, stream);
 }

@@ -318,6 +318,16 @@ def test_backward_parts(gated, activation):
     assert fn(dout, x, w, activation=activation, need_dx=False, need_dw=False, need_dbias=False) == (None, None, None)
 
 
+@pytest.mark.parametrize("m,n,k", [(154, 5120, 1288), (8200, 200, 136), (300, 2571, 137), (2200, 2056, 648), (40, 16, 2056)])
+def test_one_gradient_of_split_sums(m, n, k):
+    x, w, dout = values(1, m, k), values(2, n, k, std=k ** -0.5), values(3, m, n, std=0.3)
+    for activation in ("none", "gelu"):
+        got = sh.linear_act_backward(dout, x, w, activation=activation, need_dw=False)
+        check_backward(dout, x, w, None, activation, got, False)
+        got = sh.linear_act_backward(dout, x, w, activation=activation, need_dx=False, need_dbias=True)
+        check_backward(dout, x, w, None, activation, got, False)
+
+
 # the bias gradient without the weights': one share of the rows and many, whole and ragged groups of 8 columns, odd strides
 @pytest.mark.parametrize("m,n,pad", [(1, 3, 0), (127, 520, 0), (128, 512, 8), (5000, 1283, 0), (4097, 640, 3), (300, 10007, 1)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
