@@ -16,7 +16,7 @@ hipError_t ff_pair_f16(const FfParams& w, const FfParams& x, int w_tile, int x_t
 hipError_t ff_pair_bf16(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream);
 hipError_t ff_staged_f16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
 hipError_t ff_staged_bf16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
-hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool staged, bool one_per_cu, hipStream_t stream);
+hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool staged, FfDeepId id, hipStream_t stream);
 
 namespace {
 
@@ -74,16 +74,31 @@ float list_time(int64_t a, float a_time, int64_t b, float b_time, int64_t cus) {
     return end;
 }
 
-// The same for the 32 x 32 tiles whose waves share the depth (feed_forward_deep.hip): 0.095 us a 64-deep block
-// where every CU has at most one tile, else 0.33 us per two tiles of a CU (0.25 where the caches hold w), and 2.2 us
-// for the start and end of every two more (gated [8192, 64] -> 2 x 5120, 160 rounds of them: 420 us, on 256 x 320 tiles 58).
-float deep_time(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool& one_per_cu) {
+// The same for the tiles whose waves share the depth (feed_forward_deep.hip), by 64-deep blocks: 32 x 32 with eight
+// waves where every CU has at most one, else with four and two tiles a CU, or 64 x 64 with four. Measured in bf16, us
+// (the best tile with barriers behind): [248, 8192] x [2048, 8192] 26 on 32 x 32, 31 on 64 x 64 (47); gated the same,
+// 256 tiles of 64 x 64, 48 and 33 (48); [462, 5120] x [1280, 5120] 26 and 23 (32); [2048, 1280] x [1280, 1280] 37 and
+// 34 (19); gated [8192, 64] -> 2 x 5120, 160 rounds of 32 x 32, 420 (58). Staged rows: [617, 3411] x [1280, 3411] 49 and
+// 43 (55), [136, 5458] x [2048, 5458] 36 and 61.
+FfDeepId deep_choice(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool staged, float& time) {
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
-    const int64_t tiles = ((p.rows + 31) / 32) * ((cols + 31) / 32);
-    const float blocks = (float)((p.depth + 63) / 64), rounds = (float)tiles / (float)(2 * cus);
-    one_per_cu = tiles <= cus;
-    if (one_per_cu) return 3.0f + blocks * 0.095f;
-    return 3.0f + blocks * (0.33f * rounds > 0.19f ? 0.33f * rounds : 0.19f) + (rounds > 1.0f ? 2.2f * (rounds - 1.0f) : 0.0f);
+    const int64_t small = ((p.rows + 31) / 32) * ((cols + 31) / 32), large = ((p.rows + 63) / 64) * ((cols + 63) / 64);
+    const float blocks = (float)((p.depth + 63) / 64), rounds = (float)small / (float)(2 * cus);
+    FfDeepId id = kFfDeep32x4;
+    if (small <= cus) {
+        id = kFfDeep32x8;
+        time = staged ? 5.0f + 0.19f * blocks : 3.0f + 0.095f * blocks;
+    } else if (rounds <= 1.0f) {
+        time = 3.0f + (staged ? 0.6f : 0.19f) * blocks;
+    } else {
+        time = 3.0f + (staged ? 0.6f : 0.24f) * rounds * blocks + 2.2f * (rounds - 1.0f);
+    }
+    const float large_time = (float)((large + cus - 1) / cus) * (7.0f + (staged ? 0.65f : 0.19f) * blocks);
+    if (large_time < time) {
+        id = kFfDeep64x4;
+        time = large_time;
+    }
+    return id;
 }
 
 int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus, float& best_time) {
@@ -129,20 +144,12 @@ bool staged_large(const FfParams& p, int64_t cols, int compute_units) {
     return ((p.rows + 127) / 128) * ((cols + 127) / 128) >= (compute_units > 0 ? compute_units : 256);
 }
 
-// Rows through registers, on 64 x 64 tiles and on 32 x 32 ones whose waves share the depth, microseconds: a stage of the
-// first waits for its reads (0.85, more with over 256 tiles), the second have a block per wave under way. Measured in
-// bf16 [40, 5127] x [1280, 5127] 72 and 20, [600, 645] x [645, 645] 14.2 and 10.3, gated [1000, 323] -> 2 x 1280 12 and 33.
+// Rows through registers on 64 x 64 tiles, microseconds: a stage waits for its reads (0.85; more with over 256 tiles).
+// [40, 5127] x [1280, 5127] 72 (32 x 32, shared depth: 20), [600, 645] x [645, 645] 14.2 (10.3), gated [1000, 323] -> 2 x
+// 1280 12 (33).
 float staged_time(const FfParams& p, int64_t cols) {
     const int64_t tiles = ((p.rows + 63) / 64) * ((cols + 63) / 64);
     return 4.5f + (float)((p.depth + 63) / 64) * (tiles > 256 ? 0.85f + 0.0012f * (float)(tiles - 256) : 0.85f);
-}
-
-float staged_deep_time(const FfParams& p, int64_t cols, int compute_units, bool& one_per_cu) {
-    const int64_t cus = compute_units > 0 ? compute_units : 256, tiles = ((p.rows + 31) / 32) * ((cols + 31) / 32);
-    const float blocks = (float)((p.depth + 63) / 64), rounds = (float)tiles / (float)(2 * cus);
-    one_per_cu = tiles <= cus;
-    if (one_per_cu) return 5.0f + 0.19f * blocks;
-    return rounds > 1.0f ? 3.0f + 0.6f * rounds * blocks + 2.2f * (rounds - 1.0f) : 3.0f + 0.6f * blocks;
 }
 
 // ---- dw and dx in one launch. A side of it: a product on a tile, its depth in so many shares.
@@ -283,9 +290,9 @@ hipError_t launch_ff_staged(const FfParams& params, FfEpilogue epilogue, bool bf
     const FfParams p = prepared(params, false);
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
     const bool large = staged_large(p, cols, compute_units);
-    bool one_per_cu;
-    if (!large && staged_deep_time(p, cols, compute_units, one_per_cu) < staged_time(p, cols))
-        return ff_deep(p, epilogue, bf16, j_fp8, true, one_per_cu, stream);
+    float deep_time;
+    const FfDeepId deep = deep_choice(p, epilogue, compute_units > 0 ? compute_units : 256, true, deep_time);
+    if (!large && deep_time < staged_time(p, cols)) return ff_deep(p, epilogue, bf16, j_fp8, true, deep, stream);
     return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, large, stream);
 }
 
@@ -295,9 +302,11 @@ hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_t
     const int64_t cus = compute_units > 0 ? compute_units : 256;
     float time = 0.0f;
     const int tile = choose_tile(p, epilogue, j_fp8, cus, time);
-    bool one_per_cu;
-    if (epilogue != kFfStore && deep_time(p, epilogue, cus, one_per_cu) < time)
-        return ff_deep(p, epilogue, bf16, j_fp8, false, one_per_cu, stream);
+    if (epilogue != kFfStore) {
+        float deep_time;
+        const FfDeepId deep = deep_choice(p, epilogue, cus, false, deep_time);
+        if (deep_time < time) return ff_deep(p, epilogue, bf16, j_fp8, false, deep, stream);
+    }
     if (epilogue == kFfLinear || epilogue == kFfGated)
         return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, tile, stream);
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);

@@ -62,6 +62,9 @@ hipError_t launch_ff_general(const FfParams& p, FfEpilogue epilogue, bool i_tran
 // Tiles of the tiled kernel, rows x columns of sums.
 enum FfTileId : int { kFf256x320, kFf256x256, kFf128x256, kFf128x192, kFf128x128, kFf64x128, kFf64x64, kFfTiles };
 
+// Tiles whose waves share the depth (feed_forward_deep.hip), side x waves.
+enum FfDeepId : int { kFfDeep32x8, kFfDeep32x4, kFfDeep64x4 };
+
 // The tiled kernel: operands whose rows 16-byte accesses divide.
 bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);
 hipError_t launch_ff_tiled(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,

@@ -212,7 +212,7 @@ def test_backward_every_activation(activation, dtype):
 # few rows: one token to 16 rows (depths below a block, of one step and of several steps of 2048), then tens of
 # rows with much depth, with at most one 32 x 32 tile of sums per CU and with more; ragged edges
 FEW_ROWS = [(1, 1283, 2120), (2, 1280, 320), (16, 40, 4112), (5, 2056, 80), (9, 20, 16), (17, 72, 1304), (64, 643, 1296),
-            (150, 650, 528), (33, 3001, 336), (63, 16, 9000)]
+            (150, 650, 528), (33, 3001, 336), (63, 16, 9000), (460, 1283, 5120), (250, 1030, 8208)]
 
 
 @pytest.mark.parametrize("m,n,k", FEW_ROWS)
@@ -223,6 +223,8 @@ def test_few_rows(m, n, k, dtype):
     check_forward(x, w.double(), bias, "gelu", sh.gated_linear(x, w, bias=bias, gate_first=True), True, True)
     got = sh.linear_act(x, w[:n], bias=bias[:n].clone(), residual=residual, activation="silu")
     check_forward(x, w[:n].double(), bias[:n], "silu", got, False, residual=residual)
+    dout = values(6, m, n, std=0.3, dtype=dtype)
+    check_backward(dout, x, w, bias, "gelu", sh.gated_linear_backward(dout, x, w, bias=bias), True)
     codes, scale, w64 = e4m3(5, 2 * n, k)
     if k % 16 == 0:
         check_forward(x, w64, bias, "silu", sh.gated_linear(x, codes, bias=bias, w_scale=scale, activation="silu"), True)
@@ -381,7 +383,7 @@ def test_row_strides(m, n, k, pad):
 # rows that no 16-byte access divides, on 64 x 64 and on 128 x 128 tiles: the last chunk of a row of 8 elements or more is
 # its last 16 bytes; E4M3 rows of 16 codes or more
 @pytest.mark.parametrize("m,n,k", [(1, 1283, 321), (16, 1291, 2123), (7, 37, 4109), (5, 2056, 81), (19, 72, 1303), (63, 643, 1297),
-                                   (150, 651, 525), (33, 1501, 337), (40, 16, 9001), (40, 9, 8), (77, 100, 9), (130, 331, 71), (301, 257, 645), (2200, 1091, 133),
+                                   (150, 651, 525), (33, 1501, 337), (40, 16, 9001), (620, 1283, 3411), (620, 641, 3411), (40, 9, 8), (77, 100, 9), (130, 331, 71), (301, 257, 645), (2200, 1091, 133),
                                    (4100, 1543, 68)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_odd_rows(m, n, k, dtype):
