@@ -308,8 +308,8 @@ sdxl_status sdxl_ff_sublayer(const sdxl_ff_sublayer_desc* d, const void* x, cons
     if (x == nullptr || ln_gamma == nullptr || ln_beta == nullptr || y == nullptr ||
         (d->inner > 0 && (w_in == nullptr || w_out == nullptr)))
         return fail("sdxl_ff_sublayer", SDXL_STATUS_INVALID_ARGUMENT, "null tensor pointer");
-    if (d->inner > 0 && ((d->w_in_dtype == SDXL_DTYPE_E4M3 && w_in_scale == nullptr) ||
-                         (d->w_out_dtype == SDXL_DTYPE_E4M3 && w_out_scale == nullptr)))
+    if ((d->inner > 0 && d->w_in_dtype == SDXL_DTYPE_E4M3 && w_in_scale == nullptr) ||
+        (d->w_out_dtype == SDXL_DTYPE_E4M3 && w_out_scale == nullptr))
         return sdxl_hip_fail(SDXL_STATUS_INVALID_ARGUMENT, "FP8 weight has invalid scaling metadata");
     if (!aligned(x, 4) || !aligned(ln_gamma, 4) || !aligned(ln_beta, 4) || !aligned(y, 2) || !aligned(b_in, 2) ||
         !aligned(b_out, 2) || !aligned(w_in_scale, 4) || !aligned(w_out_scale, 4) ||

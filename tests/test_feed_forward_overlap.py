@@ -1,0 +1,26 @@
+"""Host-only: calls of the feed-forward C ABI that would write what they read, or that fail in a later step, are
+refused before the first launch (a launch fails here without a GPU, with another status)."""
+import ctypes
+
+import pytest
+
+import sdxl_hip as sh
+
+pytest.importorskip("torch")
+MIB = 1 << 20  # pointers a MiB apart, never followed
+SUBLAYER = ("x", "gamma", "beta", "w_in", "s_in", "b_in", "w_out", "s_out", "b_out", "y", "ws")
+
+
+def sublayer(rows=4, width=64, inner=256, w_in_dtype=sh.F16, w_out_dtype=sh.F16, **given):
+    d = sh.FfSublayerDesc(rows=rows, width=width, inner=inner, w_in_dtype=w_in_dtype, w_out_dtype=w_out_dtype, activation=2)
+    at = {name: MIB * (i + 1) for i, name in enumerate(SUBLAYER)} | given
+    size = sh.load().sdxl_ff_sublayer_workspace_bytes(ctypes.byref(d))
+    status = sh.load().sdxl_ff_sublayer(ctypes.byref(d), *(at[n] or None for n in SUBLAYER), size, None)
+    return status, sh.load().sdxl_last_error().decode()
+
+
+@pytest.mark.parametrize("inner", [0, 256])
+def test_sublayer_scales_are_checked_first(inner):
+    """sdxl_linear_act needs the scales of E4M3 weights without columns too: not after the LayerNorm is launched."""
+    status, error = sublayer(inner=inner, w_out_dtype=sh.E4M3, s_out=0)
+    assert status == sh.INVALID_ARGUMENT and "scaling metadata" in error
