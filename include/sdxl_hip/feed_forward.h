@@ -115,7 +115,8 @@ size_t sdxl_ff_sublayer_workspace_bytes(const sdxl_ff_sublayer_desc* desc);
 /* The feed-forward half of the transformer block, fp16, after sdxl_attn_sublayer and
  * sdxl_cross_attn_sublayer: y = x + gated(LN(x), w_in, b_in) . w_out^T + b_out, for x [rows, width];
  * w_in [2 inner, width] and b_in [2 inner] (value | gate), w_out [width, inner], b_out [width],
- * w_in_scale / w_out_scale for E4M3 weights. b_in and b_out are optional (NULL). y may equal x. */
+ * w_in_scale / w_out_scale for E4M3 weights. b_in and b_out are optional (NULL). y may equal x.
+ * A refused call launches nothing. */
 sdxl_status sdxl_ff_sublayer(const sdxl_ff_sublayer_desc* desc, const void* x, const void* ln_gamma,
                              const void* ln_beta, const void* w_in, const float* w_in_scale, const void* b_in,
                              const void* w_out, const float* w_out_scale, const void* b_out, void* y,

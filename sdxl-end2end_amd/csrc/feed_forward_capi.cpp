@@ -318,6 +318,8 @@ sdxl_status sdxl_ff_sublayer(const sdxl_ff_sublayer_desc* d, const void* x, cons
         return fail("sdxl_ff_sublayer", SDXL_STATUS_UNSUPPORTED, "misaligned tensor");
     if (workspace == nullptr || workspace_bytes < sublayer_workspace(d) || !aligned(workspace, 256))
         return fail("sdxl_ff_sublayer", SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");
+    if (one_of(y, {ln_gamma, ln_beta, w_in, w_in_scale, b_in, w_out, w_out_scale, b_out, workspace}))
+        return fail("sdxl_ff_sublayer", SDXL_STATUS_INVALID_ARGUMENT, "y overlaps an input");
     char* normed = static_cast<char*>(workspace);
     char* gated = normed + round256((size_t)d->rows * (size_t)d->width * 2);
     st = sdxl_layer_norm(d->rows, d->width, x, 0, ln_gamma, ln_beta, d->ln_eps, normed, 0, stream);

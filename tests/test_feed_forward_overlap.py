@@ -24,3 +24,12 @@ def test_sublayer_scales_are_checked_first(inner):
     """sdxl_linear_act needs the scales of E4M3 weights without columns too: not after the LayerNorm is launched."""
     status, error = sublayer(inner=inner, w_out_dtype=sh.E4M3, s_out=0)
     assert status == sh.INVALID_ARGUMENT and "scaling metadata" in error
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_sublayer_output_in_place_of_a_parameter_is_refused(fp8):
+    dtype = sh.E4M3 if fp8 else sh.F16
+    for name in ("gamma", "beta", "w_in", "b_in", "w_out", "b_out", "ws") + (("s_in", "s_out") if fp8 else ()):
+        at = MIB * (SUBLAYER.index(name) + 1)
+        status, error = sublayer(w_in_dtype=dtype, w_out_dtype=dtype, y=at)
+        assert status == sh.INVALID_ARGUMENT and "overlaps" in error, name
