@@ -176,9 +176,13 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     const size_t need = inputs ? backward_workspace(c) : 0;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");
-    for (const void* out : {want_dx ? dx : nullptr, want_dw ? dw : nullptr, want_db ? dbias : nullptr})
-        if (inputs && one_of(out, {dout, x, w, bias}))
+    const void* const grads[3] = {want_dx ? dx : nullptr, want_dw ? dw : nullptr, want_db ? dbias : nullptr};
+    for (int i = 0; i < 3; ++i) {
+        if (inputs && one_of(grads[i], {dout, x, w, bias}))
             return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "a gradient overlaps an input");
+        if (one_of(grads[i], {grads[(i + 1) % 3], need > 0 ? workspace : nullptr}))
+            return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "a gradient overlaps another one or the workspace");
+    }
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
 
     const void* dz = dout;

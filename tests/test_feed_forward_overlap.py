@@ -33,3 +33,25 @@ def test_sublayer_output_in_place_of_a_parameter_is_refused(fp8):
         at = MIB * (SUBLAYER.index(name) + 1)
         status, error = sublayer(w_in_dtype=dtype, w_out_dtype=dtype, y=at)
         assert status == sh.INVALID_ARGUMENT and "overlaps" in error, name
+
+
+BACKWARD = ("dout", "x", "w", "bias", "dx", "dw", "db", "ws")
+
+
+def backward(gated, m=8, n=8, k=64, **given):
+    d = sh.FfDesc(m=m, n=n, k=k, activation=2)
+    at = {name: MIB * (i + 1) for i, name in enumerate(BACKWARD)} | given
+    name = "sdxl_gated_linear_backward" if gated else "sdxl_linear_act_backward"
+    size = getattr(sh.load(), name + "_workspace_bytes")(ctypes.byref(d))
+    status = getattr(sh.load(), name)(ctypes.byref(d), *(at[n] or None for n in BACKWARD), size, None)
+    return status, sh.load().sdxl_last_error().decode()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_gradients_in_one_place_are_refused(gated):
+    dx, dw, db, ws = (MIB * (BACKWARD.index(name) + 1) for name in ("dx", "dw", "db", "ws"))
+    for given in (dict(dw=dx), dict(db=dx), dict(db=dw), dict(dx=ws), dict(dw=ws), dict(db=ws)):
+        status, error = backward(gated, **given)
+        assert status == sh.INVALID_ARGUMENT and "overlaps" in error, given
+    status, error = backward(gated, m=0, dw=db, x=0, dout=0)  # zeros are written too
+    assert status == sh.INVALID_ARGUMENT and "overlaps" in error
