@@ -22,8 +22,9 @@
  *
  * All calls are stream-ordered, allocate nothing, never synchronise and may be captured
  * into a HIP graph; the stream's device must be the current one. Outputs and workspace
- * must not overlap the inputs, except where a call says otherwise. Errors as in
- * attention.h (sdxl_last_error()).
+ * must not overlap the inputs or each other, except where a call says otherwise: refused
+ * wherever the strides are equal or one of the two is contiguous, else by their first and
+ * last rows (column slices of one tensor do not overlap). Errors as in attention.h (sdxl_last_error()).
  */
 #ifndef SDXL_HIP_FEED_FORWARD_H
 #define SDXL_HIP_FEED_FORWARD_H

@@ -23,10 +23,44 @@ sdxl_status fail(const char* name, sdxl_status status, const char* what) {
     return sdxl_hip_fail(status, std::string(name) + ": " + what);
 }
 
-// Outputs in place of an input that other workgroups still read: only the exact overlap is seen here.
-bool one_of(const void* out, std::initializer_list<const void*> inputs) {
-    for (const void* in : inputs)
-        if (out != nullptr && out == in) return true;
+// What a tensor occupies: rows of `row` bytes, `stride` bytes apart.
+struct Area {
+    const void* p;
+    int64_t rows, row, stride;
+};
+
+Area matrix(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t elem = 2) {
+    return {p, rows, cols * elem, ld * elem};
+}
+Area vector(const void* p, int64_t n, int64_t elem = 2) { return {p, 1, n * elem, n * elem}; }
+
+using i128 = __int128;  // (offsets of two 63-bit areas)
+
+i128 floor_div(i128 a, i128 b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
+
+// Whether two areas share a byte. Slices of one wide tensor lie between each other's rows and share none: seen where
+// the strides are equal or one of the areas is a single run of bytes. Of others, which lie between each other with
+// different strides, only the first and last rows are looked at.
+bool overlap(Area a, Area b) {
+    if (a.p == nullptr || b.p == nullptr || a.rows <= 0 || b.rows <= 0 || a.row <= 0 || b.row <= 0) return false;
+    const i128 d = (i128)(uintptr_t)b.p - (i128)(uintptr_t)a.p;  // b's begin from a's
+    for (Area* t : {&a, &b})
+        if (t->rows == 1 || t->stride == t->row) *t = {t->p, 1, t->rows * t->row, 0};
+    if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) {
+        const auto row = [](const Area& t, int64_t r) { return Area{(const char*)t.p + r * t.stride, 1, t.row, 0}; };
+        return overlap(row(a, 0), b) || overlap(row(a, a.rows - 1), b) || overlap(row(b, 0), a) || overlap(row(b, b.rows - 1), a);
+    }
+    if (a.rows == 1 && b.rows == 1) return d - a.row < 0 && d + b.row > 0;
+    // a's row i meets b's row j where (i - j) stride lies in (d - a.row, d + b.row): the least such i - j
+    const i128 stride = a.rows > 1 ? a.stride : b.stride;
+    i128 t = floor_div(d - a.row, stride) + 1;
+    if (t < -(i128)(b.rows - 1)) t = -(i128)(b.rows - 1);
+    return t <= a.rows - 1 && t * stride < d + b.row;
+}
+
+bool overlaps_one(Area out, std::initializer_list<Area> inputs) {
+    for (const Area& in : inputs)
+        if (overlap(out, in)) return true;
     return false;
 }
 
@@ -126,7 +160,11 @@ sdxl_status forward(const sdxl_ff_desc* d, bool gated, const char* name, const v
     if (!aligned(x, 2) || !aligned(w, c.w_fp8 ? 1 : 2) || !aligned(w_scale, 4) || !aligned(bias, 2) ||
         !aligned(residual, 2) || !aligned(out, 2))
         return fail(name, SDXL_STATUS_UNSUPPORTED, "tensor not aligned to its elements");
-    if (one_of(out, {x, w, bias, w_scale}) || (out == residual && c.ldr != c.ldo))
+    const Area to = matrix(out, c.m, c.n, c.ldo);
+    const bool in_place = out == residual && c.ldr == c.ldo;
+    if (overlaps_one(to, {matrix(x, c.m, c.k, c.ldx), matrix(w, c.features, c.k, c.ldw, c.w_fp8 ? 1 : 2),
+                          vector(bias, c.features), vector(w_scale, c.features, 4),
+                          matrix(in_place ? nullptr : residual, c.m, c.n, c.ldr)}))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "out overlaps an input");
     FfParams p = projection(c, x, w, w_scale, bias);
     p.residual = residual;
@@ -176,13 +214,20 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
     const size_t need = inputs ? backward_workspace(c) : 0;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");
-    const void* const grads[3] = {want_dx ? dx : nullptr, want_dw ? dw : nullptr, want_db ? dbias : nullptr};
+    const Area grads[3] = {matrix(want_dx ? dx : nullptr, c.m, c.k, c.lddx),
+                           matrix(want_dw ? dw : nullptr, c.features, c.k, c.lddw),
+                           vector(want_db ? dbias : nullptr, c.features)};
+    const Area read[4] = {matrix(dout, c.m, c.n, c.ldo), matrix(x, c.m, c.k, c.ldx), matrix(w, c.features, c.k, c.ldw),
+                          vector(bias, c.features)};
+    const Area work = vector(need > 0 ? workspace : nullptr, (int64_t)need, 1);
     for (int i = 0; i < 3; ++i) {
-        if (inputs && one_of(grads[i], {dout, x, w, bias}))
+        if (inputs && overlaps_one(grads[i], {read[0], read[1], read[2], read[3]}))
             return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "a gradient overlaps an input");
-        if (one_of(grads[i], {grads[(i + 1) % 3], need > 0 ? workspace : nullptr}))
+        if (overlaps_one(grads[i], {grads[(i + 1) % 3], work}))
             return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "a gradient overlaps another one or the workspace");
     }
+    if (inputs && overlaps_one(work, {read[0], read[1], read[2], read[3]}))
+        return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "the workspace overlaps an input");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
 
     const void* dz = dout;
@@ -322,8 +367,17 @@ sdxl_status sdxl_ff_sublayer(const sdxl_ff_sublayer_desc* d, const void* x, cons
         return fail("sdxl_ff_sublayer", SDXL_STATUS_UNSUPPORTED, "misaligned tensor");
     if (workspace == nullptr || workspace_bytes < sublayer_workspace(d) || !aligned(workspace, 256))
         return fail("sdxl_ff_sublayer", SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");
-    if (one_of(y, {ln_gamma, ln_beta, w_in, w_in_scale, b_in, w_out, w_out_scale, b_out, workspace}))
-        return fail("sdxl_ff_sublayer", SDXL_STATUS_INVALID_ARGUMENT, "y overlaps an input");
+    const int64_t in_elem = d->w_in_dtype == SDXL_DTYPE_E4M3 ? 1 : 2, out_elem = d->w_out_dtype == SDXL_DTYPE_E4M3 ? 1 : 2;
+    const Area to = matrix(y, d->rows, d->width, d->width), work = vector(workspace, (int64_t)sublayer_workspace(d), 1);
+    for (const Area& area : {to, work})
+        if (overlaps_one(area, {vector(ln_gamma, d->width), vector(ln_beta, d->width),
+                                matrix(w_in, 2 * d->inner, d->width, d->width, in_elem), vector(w_in_scale, 2 * d->inner, 4),
+                                vector(b_in, 2 * d->inner), matrix(w_out, d->width, d->inner, d->inner, out_elem),
+                                vector(w_out_scale, d->width, 4), vector(b_out, d->width)}))
+            return fail("sdxl_ff_sublayer", SDXL_STATUS_INVALID_ARGUMENT, "y or the workspace overlaps an input");
+    const Area from = matrix(x, d->rows, d->width, d->width);
+    if ((x != y && overlap(to, from)) || overlap(work, from) || overlap(work, to))
+        return fail("sdxl_ff_sublayer", SDXL_STATUS_INVALID_ARGUMENT, "one of x, y and the workspace overlaps another");
     char* normed = static_cast<char*>(workspace);
     char* gated = normed + round256((size_t)d->rows * (size_t)d->width * 2);
     st = sdxl_layer_norm(d->rows, d->width, x, 0, ln_gamma, ln_beta, d->ln_eps, normed, 0, stream);
