@@ -97,11 +97,12 @@ public:
 
     // hidden += gated(LN(hidden), in_weight, in_bias) . out_weight^T + out_bias in place: the
     // feed-forward half of the reference's transformer block (src/cuda/unet.cpp:133-147). hidden
-    // fp16 [..., W]; in_weight [2I, W] and out_weight [W, I] fp16 or packed E4M3; biases optional.
+    // fp16 [..., W]; in_weight [2I, W] and out_weight [W, I] fp16 or packed E4M3; biases optional;
+    // gate_first: in_weight holds the gate's rows first.
     void feed_forward_sublayer(Tensor& hidden, const Tensor& norm_weight, const Tensor& norm_bias,
                                const Tensor& in_weight, const Tensor* in_bias, const Tensor& out_weight,
                                const Tensor* out_bias, Activation activation = Activation::Gelu,
-                               float epsilon = 1.0e-5F) const;
+                               float epsilon = 1.0e-5F, bool gate_first = false) const;
 
 private:
     const Runtime* runtime_ = nullptr;

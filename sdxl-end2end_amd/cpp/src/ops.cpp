@@ -395,10 +395,10 @@ Tensor Ops::linear_activation(const Tensor& input, const Tensor& weight, const T
 
 void Ops::feed_forward_sublayer(Tensor& hidden, const Tensor& norm_weight, const Tensor& norm_bias,
                                 const Tensor& in_weight, const Tensor* in_bias, const Tensor& out_weight,
-                                const Tensor* out_bias, Activation activation, float epsilon) const {
+                                const Tensor* out_bias, Activation activation, float epsilon, bool gate_first) const {
     if (hidden.type() != ScalarType::Float16 || hidden.rank() < 2)
         throw HipError("feed-forward sublayer requires fp16 hidden [..., W]");
-    const sdxl_ff_desc in = feed_forward_desc(hidden, in_weight, in_bias, true, activation, false);
+    const sdxl_ff_desc in = feed_forward_desc(hidden, in_weight, in_bias, true, activation, gate_first);
     const std::size_t W = hidden.shape().back(), inner = in_weight.size(0) / 2;
     if (out_weight.rank() != 2 || out_weight.size(0) != W || out_weight.size(1) != inner ||
         (out_weight.type() != ScalarType::Float16 && out_weight.type() != ScalarType::Float8E4M3) ||
@@ -414,6 +414,7 @@ void Ops::feed_forward_sublayer(Tensor& hidden, const Tensor& norm_weight, const
     d.w_in_dtype = in.w_dtype;
     d.w_out_dtype = out_weight.type() == ScalarType::Float8E4M3 ? SDXL_DTYPE_E4M3 : SDXL_DTYPE_F16;
     d.activation = in.activation;
+    d.gate_first = in.gate_first;
     d.ln_eps = epsilon;
     const float *in_scales = weight_scales(in_weight), *out_scales = weight_scales(out_weight);
     const std::size_t ws_bytes = sdxl_ff_sublayer_workspace_bytes(&d);

@@ -426,6 +426,36 @@ void feed_forward_cases() {
     std::cout << "feed-forward cases passed\n";
 }
 
+// The sublayer with the gate's rows first gives what its steps give so, and what it gives with the rows the other way
+// round.
+void feed_forward_gate_first_cases() {
+    Runtime runtime;
+    Ops ops(runtime);
+    const std::size_t W = 64, I = 96;
+    const auto hh = filled({2, 33, W}, [](std::size_t i) { return std::sin(static_cast<float>(i) * 0.61F); });
+    const auto ones = Tensor::from_host_f32(runtime, filled({W}, [](std::size_t) { return 1.0F; }));
+    const auto zeros = Tensor::from_host_f32(runtime, filled({W}, [](std::size_t) { return 0.0F; }));
+    const auto row = [&](std::size_t r, std::size_t c) { return std::sin(static_cast<float>(r * W + c) * 0.19F) * 0.2F; };
+    const auto w_in = Tensor::from_host_f32(runtime, filled({2 * I, W}, [&](std::size_t i) { return row(i / W, i % W); }));
+    const auto w_swapped = Tensor::from_host_f32(runtime, filled({2 * I, W}, [&](std::size_t i) { return row((i / W + I) % (2 * I), i % W); }));
+    const auto w_out = Tensor::from_host_f32(runtime, filled({W, I}, [](std::size_t i) { return std::cos(static_cast<float>(i) * 0.23F) * 0.2F; }));
+    Tensor hidden = Tensor::from_host_f32(runtime, hh), other = Tensor::from_host_f32(runtime, hh), values = Tensor::from_host_f32(runtime, hh);
+    const auto steps = ops.linear_activation(ops.gated_linear(ops.layer_norm(hidden, ones, zeros), w_in, nullptr, Activation::Gelu, true),
+                                             w_out, nullptr, Activation::None, &hidden).to_host_f32(runtime);
+    ops.feed_forward_sublayer(hidden, ones, zeros, w_in, nullptr, w_out, nullptr, Activation::Gelu, 1.0e-5F, true);
+    ops.feed_forward_sublayer(other, ones, zeros, w_swapped, nullptr, w_out, nullptr);
+    ops.feed_forward_sublayer(values, ones, zeros, w_in, nullptr, w_out, nullptr);
+    const auto got = hidden.to_host_f32(runtime), swapped = other.to_host_f32(runtime), value_first = values.to_host_f32(runtime);
+    bool same = true;
+    for (std::size_t i = 0; i < got.values.size(); ++i) {
+        require_close(got.values[i], steps.values[i], 0.0F, "gate first against its steps");
+        require_close(got.values[i], swapped.values[i], 0.0F, "gate first against swapped rows");
+        same = same && got.values[i] == value_first.values[i];
+    }
+    require(!same, "gate_first changes the result");
+    std::cout << "feed-forward gate-first cases passed\n";
+}
+
 void device_cases() {
     Runtime runtime;
     Ops ops(runtime);
@@ -529,6 +559,7 @@ void device_cases() {
     sublayer_cases();
     out_projection_cases();
     feed_forward_cases();
+    feed_forward_gate_first_cases();
 }
 
 }  // namespace
