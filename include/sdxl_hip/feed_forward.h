@@ -97,6 +97,16 @@ sdxl_status sdxl_gated_linear_backward(const sdxl_ff_desc* desc, const void* dou
                                        const void* bias, void* dx, void* dw, void* dbias, void* workspace,
                                        size_t workspace_bytes, void* stream);
 
+/* The kernels that a call of this descriptor runs on the current device (without one: on 256 CUs), on tensors
+ * aligned to 16 bytes: those of sdxl_linear_act or sdxl_gated_linear (gated 1), or with gradients (1: dx, 2: dw,
+ * 4: dbias, added up) those of its backward. "tile 256x320" is the tiled kernel's tile, "deep 32x32/8" a tile whose
+ * eight waves share the depth, "rows/4" the kernel of few rows with four waves a workgroup, "staged" what takes rows
+ * that 16-byte accesses do not divide, "general" the rest; "; " stands between launches, " + " between products of one
+ * launch, "in 2 shares" where a depth is split and joined. Writes at most size bytes with the terminating zero to text
+ * (may be NULL) and returns the length without it; 0 where the call would be refused or launch nothing. Launches
+ * nothing itself. */
+size_t sdxl_ff_kernels(const sdxl_ff_desc* desc, int32_t gated, int32_t gradients, char* text, size_t size);
+
 typedef struct sdxl_ff_sublayer_desc {
     int64_t rows;  /* batch * seq */
     int64_t width; /* even, at most 2048 */

@@ -140,8 +140,8 @@ FfParams prepared(const FfParams& params, bool i_transposed) {
 
 // 128 x 128 tiles where every CU gets one, else 64 x 64: [8192, 2561] x [640, 2561], 320 of the large tiles, 62 us (small: 84);
 // [2632, 2567] x [640, 2567], 105, 66 (45); gated [2632, 2567] -> 2 x 640, 210, 68 (64).
-bool staged_large(const FfParams& p, int64_t cols, int compute_units) {
-    return ((p.rows + 127) / 128) * ((cols + 127) / 128) >= (compute_units > 0 ? compute_units : 256);
+bool staged_large(const FfParams& p, int64_t cols, int64_t cus) {
+    return ((p.rows + 127) / 128) * ((cols + 127) / 128) >= cus;
 }
 
 // Rows through registers on 64 x 64 tiles, microseconds: a stage waits for its reads (0.85; more with over 256 tiles).
@@ -277,6 +277,8 @@ bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpos
     return ((p.rows + 63) / 64) * ((p.cols + 31) / 32) <= (1 << 23);
 }
 
+namespace {
+
 bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8) {
     if (!ff_staged_supported(p, epilogue, i_transposed, j_transposed, j_fp8)) return false;
     // rows in whole 16-byte chunks: the depth, or the columns of an operand that is read by columns
@@ -285,31 +287,40 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
     return i_row % 8 == 0 && (j_transposed ? p.cols % 8 == 0 : p.depth % (j_fp8 ? 16 : 8) == 0);
 }
 
-hipError_t launch_ff_staged(const FfParams& params, FfEpilogue epilogue, bool bf16, bool j_fp8, int compute_units,
-                            hipStream_t stream) {
-    const FfParams p = prepared(params, false);
+int64_t units(int compute_units) { return compute_units > 0 ? compute_units : 256; }
+
+}  // namespace
+
+FfChoice choose_ff(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int compute_units) {
+    if (!ff_staged_supported(p, epilogue, false, false, j_fp8)) return {FfKernel::kGeneral, 0, false};
+    const bool staged = !ff_tiled_supported(p, epilogue, false, false, j_fp8);
+    if (ff_rows_supported(p, epilogue, j_fp8)) return {FfKernel::kRows, ff_rows_waves(p, epilogue == kFfGated), staged};
+    const int64_t cus = units(compute_units);
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
-    const bool large = staged_large(p, cols, compute_units);
-    float deep_time;
-    const FfDeepId deep = deep_choice(p, epilogue, compute_units > 0 ? compute_units : 256, true, deep_time);
-    if (!large && deep_time < staged_time(p, cols)) return ff_deep(p, epilogue, bf16, j_fp8, true, deep, stream);
-    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, large, stream);
+    float deep_time, time = 0.0f;
+    const FfDeepId deep = deep_choice(p, epilogue, cus, staged, deep_time);
+    if (staged) {
+        const bool large = staged_large(p, cols, cus);
+        if (!large && deep_time < staged_time(p, cols)) return {FfKernel::kDeep, deep, true};
+        return {FfKernel::kStaged, large ? 128 : 64, true};
+    }
+    const int tile = choose_tile(p, epilogue, j_fp8, cus, time);
+    if (deep_time < time) return {FfKernel::kDeep, deep, false};
+    return {FfKernel::kTile, tile, false};
 }
 
-hipError_t launch_ff_tiled(const FfParams& params, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
-                           int compute_units, hipStream_t stream) {
-    const FfParams p = prepared(params, i_transposed);
-    const int64_t cus = compute_units > 0 ? compute_units : 256;
-    float time = 0.0f;
-    const int tile = choose_tile(p, epilogue, j_fp8, cus, time);
-    if (epilogue != kFfStore) {
-        float deep_time;
-        const FfDeepId deep = deep_choice(p, epilogue, cus, false, deep_time);
-        if (deep_time < time) return ff_deep(p, epilogue, bf16, j_fp8, false, deep, stream);
+hipError_t launch_ff(const FfChoice& choice, const FfParams& params, FfEpilogue epilogue, bool bf16, bool j_fp8, hipStream_t stream) {
+    const FfParams p = prepared(params, false);
+    switch (choice.kernel) {
+    case FfKernel::kGeneral: return launch_ff_general(params, epilogue, false, false, bf16, j_fp8, stream);
+    case FfKernel::kRows: return launch_ff_rows(params, epilogue, choice.variant, choice.staged, bf16, j_fp8, stream);
+    case FfKernel::kDeep: return ff_deep(p, epilogue, bf16, j_fp8, choice.staged, (FfDeepId)choice.variant, stream);
+    case FfKernel::kStaged: return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, choice.variant == 128, stream);
+    case FfKernel::kTile: break;
     }
     if (epilogue == kFfLinear || epilogue == kFfGated)
-        return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, tile, stream);
-    return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, i_transposed, tile, stream);
+        return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, choice.variant, stream);
+    return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, false, choice.variant, stream);
 }
 
 size_t ff_partial_bytes(int64_t m, int64_t features, int64_t k) {
@@ -328,12 +339,9 @@ hipError_t launch_join(const FfParams& w, const FfParams& x, bool bf16, hipStrea
     return hipGetLastError();
 }
 
-// Both gradients on the tiled kernel, or one (the other's pointer null).
-hipError_t launch_pair(const FfParams* dw, const FfParams* dx, bool bf16, float* partial, size_t partial_bytes,
-                       int compute_units, hipStream_t stream) {
+// dw and dx on the tiled kernel, or one of them (the other's pointer null).
+void choose_pair(const FfParams* dw, const FfParams* dx, size_t partial_bytes, int64_t cus, FfGradients& plan) {
     FfParams w{}, x{};  // (no rows: no tasks)
-    w.splits = x.splits = 1;
-    const int64_t cus = compute_units > 0 ? compute_units : 256;
     // apart, or together on the best pair of tiles that take a CU each, of whole depths or of shares of them.
     // Measured on an MI355X, dw and dx of x [m, k], w [f, k]: m 2048, k 1280, f 10240 apart 142 us, together 117;
     // m 8192 apart 459, together 368; m 1111, k 640, f 5120 together 42 (105 tasks for 256 CUs), with dx's depth in 2
@@ -341,16 +349,14 @@ hipError_t launch_pair(const FfParams* dw, const FfParams* dx, bool bf16, float*
     float best = 0.0f, apart;
     if (dw != nullptr) {
         w = prepared(*dw, true);
-        choose_tile(w, kFfStore, false, cus, apart);
+        plan.w.choice = {FfKernel::kTile, choose_tile(w, kFfStore, false, cus, apart), false};
         best += apart;
     }
     if (dx != nullptr) {
         x = prepared(*dx, false);
-        choose_tile(x, kFfStore, false, cus, apart);
+        plan.x.choice = {FfKernel::kTile, choose_tile(x, kFfStore, false, cus, apart), false};
         best += apart;
     }
-    int best_w = -1, best_x = -1, w_splits = 1, x_splits = 1;
-    bool w_first = true;
     PairSide sides[2][kPairTiles][kSplitSteps];
     for (int side = 0; side < 2; ++side)
         for (int t = 0; t < kPairTiles; ++t)
@@ -370,30 +376,17 @@ hipError_t launch_pair(const FfParams* dw, const FfParams* dx, bool bf16, float*
                                                 : list_time(b.tasks, b.time, a.tasks, a.time, cus));
         if (time < best) {
             best = time;
-            best_w = kPairTile[tw];
-            best_x = kPairTile[tx];
-            w_splits = 1 << sw;
-            x_splits = 1 << sx;
-            w_first = first;
+            plan.one_launch = true;
+            plan.w_first = first;
+            if (dw != nullptr) plan.w = {true, {FfKernel::kTile, kPairTile[tw], false}, 1 << sw};
+            if (dx != nullptr) plan.x = {true, {FfKernel::kTile, kPairTile[tx], false}, 1 << sx};
         }
     }
-    if (best_w >= 0) {
-        if (dw != nullptr) set_splits(w, w_splits, partial);
-        if (dx != nullptr) set_splits(x, x_splits, partial + (size_t)pair_side(w, best_w, w_splits).partial / 4);
-        const hipError_t err = (bf16 ? ff_pair_bf16 : ff_pair_f16)(w, x, best_w, best_x, w_first, stream);
-        return err != hipSuccess ? err : launch_join(w, x, bf16, stream);
-    }
-    hipError_t err = hipSuccess;
-    if (dw != nullptr) err = launch_ff_tiled(*dw, kFfStore, true, bf16, false, compute_units, stream);
-    if (err == hipSuccess && dx != nullptr) err = launch_ff_tiled(*dx, kFfStore, false, bf16, false, compute_units, stream);
-    return err;
 }
 
-// One gradient through registers; p becomes what was launched, for the joining pass.
-hipError_t launch_staged_gradient(FfParams& p, bool i_transposed, bool bf16, float*& partial, size_t& partial_bytes,
-                                  int compute_units, hipStream_t stream) {
-    const int64_t cus = compute_units > 0 ? compute_units : 256;
-    const bool large = staged_large(p, p.cols, compute_units);
+// One gradient through registers.
+FfGradient choose_staged_gradient(const FfParams& p, size_t& partial_bytes, int64_t cus) {
+    const bool large = staged_large(p, p.cols, cus);
     // few tiles: shares of at least 16 stages until every CU has one (gradients of one row, w [10240, 1283]: 212 us, 76 so)
     int splits = 1;
     if (!large) {
@@ -402,50 +395,20 @@ hipError_t launch_staged_gradient(FfParams& p, bool i_transposed, bool bf16, flo
                pair_side(p, kFf64x64, 2 * splits).partial <= (int64_t)partial_bytes)
             splits *= 2;
     }
-    if (splits > 1) {
-        const size_t bytes = (size_t)pair_side(p, kFf64x64, splits).partial;
-        set_splits(p, splits, partial);
-        partial += bytes / 4;
-        partial_bytes -= bytes;
-    }
-    return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, kFfStore, i_transposed, false, large, stream);
+    if (splits > 1) partial_bytes -= (size_t)pair_side(p, kFf64x64, splits).partial;
+    return {true, {FfKernel::kStaged, large ? 128 : 64, true}, splits};
 }
 
-}  // namespace
-
-hipError_t launch_ff_gradients(const FfParams* dw, const FfParams* dx, bool bf16, float* partial, size_t partial_bytes,
-                               int compute_units, hipStream_t stream) {
-    const bool w_tiled = dw != nullptr && ff_tiled_supported(*dw, kFfStore, true, true, false);
-    const bool x_tiled = dx != nullptr && ff_tiled_supported(*dx, kFfStore, false, true, false);
-    hipError_t err = hipSuccess;
-    if (w_tiled || x_tiled) {
-        err = launch_pair(w_tiled ? dw : nullptr, x_tiled ? dx : nullptr, bf16, partial, partial_bytes, compute_units, stream);
-        if (err != hipSuccess || ((dw == nullptr || w_tiled) && (dx == nullptr || x_tiled))) return err;
-    }
-    // (what launch_pair left in `partial` is joined by now)
-    FfParams w{}, x{};
-    w.splits = x.splits = 1;
-    if (dw != nullptr && !w_tiled) {
-        w = prepared(*dw, true);
-        err = launch_staged_gradient(w, true, bf16, partial, partial_bytes, compute_units, stream);
-    }
-    if (err == hipSuccess && dx != nullptr && !x_tiled) {
-        x = prepared(*dx, false);
-        err = launch_staged_gradient(x, false, bf16, partial, partial_bytes, compute_units, stream);
-    }
-    return err != hipSuccess ? err : launch_join(w, x, bf16, stream);
+// The depth in shares whose sums begin at `partial`, which moves behind them.
+void take_shares(FfParams& p, const FfGradient& g, float*& partial) {
+    if (g.splits == 1) return;
+    set_splits(p, g.splits, partial);
+    partial += (size_t)pair_side(p, kFf64x64, g.splits).partial / 4;
 }
 
-hipError_t launch_ff_row_sums(const FfParams& params, bool bf16, float* partial, size_t partial_bytes, int compute_units,
-                              hipStream_t stream) {
+hipError_t launch_row_sums(const FfParams& params, int shares, bool bf16, float* partial, hipStream_t stream) {
     FfParams p = params;
-    const int64_t blocks = (p.rows + 511) / 512;
-    // shares of at least 64 rows until there are four workgroups a CU
-    int64_t shares = 1;
-    while (shares < kSumsMaxShares && blocks * shares < 4 * (int64_t)(compute_units > 0 ? compute_units : 256) &&
-           p.depth >= 128 * shares && 8 * shares * (size_t)p.rows <= partial_bytes)
-        shares *= 2;
-    const int64_t span = (p.depth + shares - 1) / shares;
+    const int64_t blocks = (p.rows + 511) / 512, span = (p.depth + shares - 1) / shares;
     p.partial = partial;
     const dim3 grid((unsigned)blocks, (unsigned)shares);
     if (bf16) hipLaunchKernelGGL(ff_row_sums_kernel<__bf16>, grid, dim3(256), 0, stream, p, span);
@@ -457,6 +420,71 @@ hipError_t launch_ff_row_sums(const FfParams& params, bool bf16, float* partial,
     p.cols = p.ld_partial = 0;
     p.splits = (int32_t)shares;
     return launch_join(p, none, bf16, stream);
+}
+
+}  // namespace
+
+FfGradients choose_ff_gradients(const FfParams* dw, const FfParams* dx, const FfParams* sums, size_t partial_bytes,
+                                int compute_units) {
+    const int64_t cus = units(compute_units);
+    FfGradients plan{};
+    plan.w = {dw != nullptr, {}, 1};
+    plan.x = {dx != nullptr, {}, 1};
+    const bool w_staged = dw != nullptr && ff_staged_supported(*dw, kFfStore, true, true, false);
+    const bool x_staged = dx != nullptr && ff_staged_supported(*dx, kFfStore, false, true, false);
+    const bool w_tiled = w_staged && ff_tiled_supported(*dw, kFfStore, true, true, false);
+    const bool x_tiled = x_staged && ff_tiled_supported(*dx, kFfStore, false, true, false);
+    // (each launch's shares are joined before the next one sums its own: they have one place)
+    if (w_tiled || x_tiled) choose_pair(w_tiled ? dw : nullptr, x_tiled ? dx : nullptr, partial_bytes, cus, plan);
+    size_t left = partial_bytes;
+    if (w_staged && !w_tiled) plan.w = choose_staged_gradient(prepared(*dw, true), left, cus);
+    if (x_staged && !x_tiled) plan.x = choose_staged_gradient(prepared(*dx, false), left, cus);
+    if (sums != nullptr) {
+        // shares of at least 64 rows until there are four workgroups a CU
+        const int64_t blocks = (sums->rows + 511) / 512;
+        plan.sum_shares = 1;
+        while (plan.sum_shares < kSumsMaxShares && blocks * plan.sum_shares < 4 * cus && sums->depth >= 128 * plan.sum_shares &&
+               8 * plan.sum_shares * (size_t)sums->rows <= partial_bytes)
+            plan.sum_shares *= 2;
+    }
+    return plan;
+}
+
+hipError_t launch_ff_gradients(const FfGradients& plan, const FfParams* dw, const FfParams* dx, const FfParams* sums,
+                               bool bf16, float* partial, hipStream_t stream) {
+    const auto on = [](const FfGradient& g, FfKernel kernel) { return g.wanted && g.choice.kernel == kernel; };
+    hipError_t err = hipSuccess;
+    for (FfKernel kernel : {FfKernel::kTile, FfKernel::kStaged}) {
+        FfParams w{}, x{};  // (no rows: no tasks)
+        w.splits = x.splits = 1;
+        float* at = partial;
+        const bool with_w = on(plan.w, kernel), with_x = on(plan.x, kernel);
+        if (with_w) {
+            w = prepared(*dw, true);
+            take_shares(w, plan.w, at);
+        }
+        if (with_x) {
+            x = prepared(*dx, false);
+            take_shares(x, plan.x, at);
+        }
+        if (kernel == FfKernel::kTile && plan.one_launch) {
+            err = (bf16 ? ff_pair_bf16 : ff_pair_f16)(w, x, with_w ? plan.w.choice.variant : kPairTile[0],
+                                                     with_x ? plan.x.choice.variant : kPairTile[0], plan.w_first, stream);
+        } else {
+            const auto one = [&](const FfParams& p, const FfGradient& g, bool i_transposed) {
+                if (kernel == FfKernel::kTile) return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, kFfStore, i_transposed, g.choice.variant, stream);
+                return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, kFfStore, i_transposed, false, g.choice.variant == 128, stream);
+            };
+            if (with_w) err = one(w, plan.w, true);
+            if (err == hipSuccess && with_x) err = one(x, plan.x, false);
+        }
+        if (err == hipSuccess) err = launch_join(w, x, bf16, stream);
+        if (err != hipSuccess) return err;
+    }
+    if (sums != nullptr) err = launch_row_sums(*sums, plan.sum_shares, bf16, partial, stream);
+    if (err == hipSuccess && on(plan.w, FfKernel::kGeneral)) err = launch_ff_general(*dw, kFfStore, true, true, bf16, false, stream);
+    if (err == hipSuccess && on(plan.x, FfKernel::kGeneral)) err = launch_ff_general(*dx, kFfStore, false, true, bf16, false, stream);
+    return err;
 }
 
 }  // namespace sdxl_hip

@@ -117,17 +117,8 @@ sdxl_status resolve(const sdxl_ff_desc* d, bool gated, bool backward, const char
 // A projection, or dz.
 sdxl_status product(const FfParams& p, sdxl_hip::FfEpilogue epilogue, const Call& c, bool w_fp8, hipStream_t stream,
                     const char* name) {
-    const int cus = sdxl_hip_compute_units();
-    hipError_t err;
-    if (sdxl_hip::ff_rows_supported(p, epilogue, w_fp8))
-        err = sdxl_hip::launch_ff_rows(p, epilogue, c.bf16, w_fp8, stream);
-    else if (sdxl_hip::ff_tiled_supported(p, epilogue, false, false, w_fp8))
-        err = sdxl_hip::launch_ff_tiled(p, epilogue, false, c.bf16, w_fp8, cus, stream);
-    else if (sdxl_hip::ff_staged_supported(p, epilogue, false, false, w_fp8))
-        err = sdxl_hip::launch_ff_staged(p, epilogue, c.bf16, w_fp8, cus, stream);
-    else
-        err = sdxl_hip::launch_ff_general(p, epilogue, false, false, c.bf16, w_fp8, stream);
-    return launch_status(err, name);
+    const sdxl_hip::FfChoice choice = sdxl_hip::choose_ff(p, epilogue, w_fp8, sdxl_hip_compute_units());
+    return launch_status(sdxl_hip::launch_ff(choice, p, epilogue, c.bf16, w_fp8, stream), name);
 }
 
 // The projections and their epilogue's inputs, shared by both directions.
@@ -193,6 +184,64 @@ size_t workspace_of(const sdxl_ff_desc* d, bool gated, const char* name) {
     return resolve(d, gated, true, name, c) == SDXL_STATUS_OK ? backward_workspace(c) : 0;
 }
 
+// The products of a backward call and the kernels that they run on.
+struct Backward {
+    FfParams z, w, x;
+    bool with_z, with_w, with_x, sums_alone;  // sums_alone: dbias without dw
+    sdxl_hip::FfEpilogue z_epilogue;
+    sdxl_hip::FfChoice z_choice;
+    sdxl_hip::FfGradients gradients;
+    float* partial;
+};
+
+Backward backward_plan(const Call& c, const void* dout, const void* x, const void* w, const void* bias, void* dx, void* dw,
+                       void* dbias, void* workspace) {
+    Backward b{};
+    const int cus = sdxl_hip_compute_units();
+    b.with_z = c.m > 0 && c.n > 0 && needs_dz(c);
+    b.with_x = dx != nullptr;
+    b.with_w = dw != nullptr;
+    b.sums_alone = dbias != nullptr && dw == nullptr;
+    const void* dz = dout;
+    int64_t lddz = c.ldo;
+    if (b.with_z) {
+        b.z = projection(c, x, w, nullptr, bias);
+        b.z.dout = dout;
+        b.z.ld_dout = c.ldo;
+        b.z.out = workspace;
+        b.z.ld_out = b.z.out_cols_padded = dz_stride(c);
+        b.z_epilogue = c.gated ? sdxl_hip::kFfGatedDz : sdxl_hip::kFfLinearDz;
+        b.z_choice = sdxl_hip::choose_ff(b.z, b.z_epilogue, false, cus);
+        dz = workspace;
+        lddz = dz_stride(c);
+    }
+    b.w.ip = dz;
+    b.w.jp = x;
+    b.w.ld_i = lddz;
+    b.w.ld_j = c.ldx;
+    b.w.rows = c.features;
+    b.w.cols = c.k;
+    b.w.depth = c.m;
+    b.w.out = dw;
+    b.w.ld_out = c.lddw;
+    b.w.row_sums = dbias;
+    b.x.ip = dz;
+    b.x.jp = w;
+    b.x.ld_i = lddz;
+    b.x.ld_j = c.ldw;
+    b.x.rows = c.m;
+    b.x.cols = c.k;
+    b.x.depth = c.features;
+    b.x.out = dx;
+    b.x.ld_out = c.lddx;
+    if (b.with_z) b.w.i_row = b.x.i_row = lddz;
+    b.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(dz_bytes(c)));
+    b.gradients = sdxl_hip::choose_ff_gradients(b.with_w ? &b.w : nullptr, b.with_x ? &b.x : nullptr,
+                                                b.sums_alone ? &b.w : nullptr,
+                                                sdxl_hip::ff_partial_bytes(c.m, c.features, c.k), cus);
+    return b;
+}
+
 sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const void* dout, const void* x,
                      const void* w, const void* bias, void* dx, void* dw, void* dbias, void* workspace,
                      size_t workspace_bytes, void* stream_ptr) {
@@ -230,57 +279,60 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "the workspace overlaps an input");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
 
-    const void* dz = dout;
-    int64_t lddz = c.ldo;
-    if (dz_needed) {
-        FfParams p = projection(c, x, w, nullptr, bias);
-        p.dout = dout;
-        p.ld_dout = c.ldo;
-        p.out = workspace;
-        p.ld_out = p.out_cols_padded = dz_stride(c);
-        st = product(p, gated ? sdxl_hip::kFfGatedDz : sdxl_hip::kFfLinearDz, c, false, stream, name);
-        if (st != SDXL_STATUS_OK) return st;
-        dz = workspace;
-        lddz = dz_stride(c);
-    }
-    FfParams pw{}, px{};
-    pw.ip = dz;
-    pw.jp = x;
-    pw.ld_i = lddz;
-    pw.ld_j = c.ldx;
-    pw.rows = c.features;
-    pw.cols = c.k;
-    pw.depth = c.m;
-    pw.out = dw;
-    pw.ld_out = c.lddw;
-    pw.row_sums = want_db ? dbias : nullptr;
-    px.ip = dz;
-    px.jp = w;
-    px.ld_i = lddz;
-    px.ld_j = c.ldw;
-    px.rows = c.m;
-    px.cols = c.k;
-    px.depth = c.features;
-    px.out = dx;
-    px.ld_out = c.lddx;
-    if (dz_needed) pw.i_row = px.i_row = lddz;
-    float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(dz_bytes(c)));
-    const size_t partial_bytes = sdxl_hip::ff_partial_bytes(c.m, c.features, c.k);
-    // the gradients that the tiled kernels take, then the others
-    const bool w_fast = want_dw && sdxl_hip::ff_staged_supported(pw, sdxl_hip::kFfStore, true, true, false);
-    const bool x_fast = want_dx && sdxl_hip::ff_staged_supported(px, sdxl_hip::kFfStore, false, true, false);
-    if (w_fast || x_fast) {
-        st = launch_status(sdxl_hip::launch_ff_gradients(w_fast ? &pw : nullptr, x_fast ? &px : nullptr, c.bf16, partial,
-                                                         partial_bytes, sdxl_hip_compute_units(), stream), name);
+    const Backward b = backward_plan(c, dout, x, w, bias, want_dx ? dx : nullptr, want_dw ? dw : nullptr,
+                                     want_db ? dbias : nullptr, workspace);
+    if (b.with_z) {
+        st = launch_status(sdxl_hip::launch_ff(b.z_choice, b.z, b.z_epilogue, c.bf16, false, stream), name);
         if (st != SDXL_STATUS_OK) return st;
     }
-    if (want_db && !want_dw)
-        st = launch_status(sdxl_hip::launch_ff_row_sums(pw, c.bf16, partial, partial_bytes, sdxl_hip_compute_units(), stream), name);
-    else if (want_dw && !w_fast)
-        st = launch_status(sdxl_hip::launch_ff_general(pw, sdxl_hip::kFfStore, true, true, c.bf16, false, stream), name);
-    if (st == SDXL_STATUS_OK && want_dx && !x_fast)
-        st = launch_status(sdxl_hip::launch_ff_general(px, sdxl_hip::kFfStore, false, true, c.bf16, false, stream), name);
-    return st;
+    return launch_status(sdxl_hip::launch_ff_gradients(b.gradients, b.with_w ? &b.w : nullptr, b.with_x ? &b.x : nullptr,
+                                                       b.sums_alone ? &b.w : nullptr, c.bf16, b.partial, stream), name);
+}
+
+std::string kernel_text(const sdxl_hip::FfChoice& c) {
+    using sdxl_hip::FfKernel;
+    static const char* const tiles[sdxl_hip::kFfTiles] = {"256x320", "256x256", "128x256", "128x192", "128x128", "64x128", "64x64"};
+    static const char* const deep[] = {"32x32/8", "32x32/4", "64x64/4"};
+    const std::string through = c.staged ? " staged" : "";
+    switch (c.kernel) {
+    case FfKernel::kGeneral: break;
+    case FfKernel::kRows: return "rows/" + std::to_string(c.variant) + through;
+    case FfKernel::kDeep: return std::string("deep ") + deep[c.variant] + through;
+    case FfKernel::kTile: return std::string("tile ") + tiles[c.variant];
+    case FfKernel::kStaged: return c.variant == 128 ? "staged 128x128" : "staged 64x64";
+    }
+    return "general";
+}
+
+std::string shares_text(int shares) { return shares > 1 ? " in " + std::to_string(shares) + " shares" : ""; }
+
+std::string kernels_text(const Call& c, int32_t gradients) {
+    const auto at = reinterpret_cast<void*>(uintptr_t{256});  // aligned to everything, never followed
+    if (gradients == 0) {
+        FfParams p = projection(c, at, at, nullptr, nullptr);
+        p.ld_res = c.ldr;
+        p.out = at;
+        p.ld_out = c.ldo;
+        return kernel_text(sdxl_hip::choose_ff(p, c.gated ? sdxl_hip::kFfGated : sdxl_hip::kFfLinear, c.w_fp8, sdxl_hip_compute_units()));
+    }
+    const auto wanted = [&](int32_t bit, bool any) { return (gradients & bit) != 0 && any ? at : nullptr; };
+    const Backward b = backward_plan(c, at, at, at, nullptr, wanted(1, c.m > 0 && c.k > 0), wanted(2, c.n > 0 && c.k > 0),
+                                     wanted(4, c.n > 0), at);
+    if (!b.with_x && !b.with_w && !b.sums_alone) return "";
+    const sdxl_hip::FfGradients& g = b.gradients;
+    std::string text = b.with_z ? "dz " + kernel_text(b.z_choice) : "";
+    const auto add = [&](const std::string& what, const char* joint) { text += (text.empty() ? "" : joint) + what; };
+    const std::string dw = "dw " + kernel_text(g.w.choice) + shares_text(g.w.splits);
+    const std::string dx = "dx " + kernel_text(g.x.choice) + shares_text(g.x.splits);
+    const bool together = g.one_launch && b.with_w && b.with_x && g.w.choice.kernel == g.x.choice.kernel;
+    if (together) {
+        add((g.w_first ? dw + " + " + dx : dx + " + " + dw), "; ");
+    } else {
+        if (b.with_w) add(dw, "; ");
+        if (b.with_x) add(dx, "; ");
+    }
+    if (b.sums_alone) add("dbias" + shares_text(g.sum_shares), "; ");
+    return text;
 }
 
 sdxl_status sublayer_shape(const sdxl_ff_sublayer_desc* d) {
@@ -340,6 +392,21 @@ sdxl_status sdxl_gated_linear_backward(const sdxl_ff_desc* d, const void* dout, 
                                        size_t workspace_bytes, void* stream) {
     return backward(d, true, "sdxl_gated_linear_backward", dout, x, w, bias, dx, dw, dbias, workspace,
                     workspace_bytes, stream);
+}
+
+size_t sdxl_ff_kernels(const sdxl_ff_desc* d, int32_t gated, int32_t gradients, char* text, size_t size) {
+    const char* name = "sdxl_ff_kernels";
+    if (text != nullptr && size > 0) text[0] = '\0';
+    Call c;
+    if (gradients < 0 || gradients > 7 || (gated != 0 && gated != 1)) {
+        fail(name, SDXL_STATUS_INVALID_ARGUMENT, "gated must be 0 or 1, gradients 0 to 7");
+        return 0;
+    }
+    if (resolve(d, gated == 1, gradients != 0, name, c) != SDXL_STATUS_OK) return 0;
+    if (gradients == 0 && (c.m == 0 || c.n == 0)) return 0;
+    const std::string kernels = kernels_text(c, gradients);
+    if (text != nullptr && size > 0) text[kernels.copy(text, size - 1)] = '\0';
+    return kernels.size();
 }
 
 size_t sdxl_ff_sublayer_workspace_bytes(const sdxl_ff_sublayer_desc* d) {

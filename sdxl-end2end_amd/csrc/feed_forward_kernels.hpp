@@ -65,29 +65,46 @@ enum FfTileId : int { kFf256x320, kFf256x256, kFf128x256, kFf128x192, kFf128x128
 // Tiles whose waves share the depth (feed_forward_deep.hip), side x waves.
 enum FfDeepId : int { kFfDeep32x8, kFfDeep32x4, kFfDeep64x4 };
 
-// The tiled kernel: operands whose rows 16-byte accesses divide.
-bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);
-hipError_t launch_ff_tiled(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool bf16, bool j_fp8,
-                           int compute_units, hipStream_t stream);
+// The kernel that a product runs on, and which of its variants: an FfTileId (tile), an FfDeepId (deep), the waves of a
+// workgroup (rows), the tile's side (staged).
+enum class FfKernel : int { kGeneral, kRows, kDeep, kTile, kStaged };
+struct FfChoice {
+    FfKernel kernel;
+    int variant;
+    bool staged;  // rows and deep: operands through registers
+};
 
-// Projections and dz through registers: rows of any alignment.
-bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);
-hipError_t launch_ff_staged(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, int compute_units,
-                            hipStream_t stream);
+// Projections and dz, by sizes, strides and alignment.
+FfChoice choose_ff(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int compute_units);
+hipError_t launch_ff(const FfChoice& choice, const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, hipStream_t stream);
 
-// dw (I transposed) and dx (nullable, each; both writing) of operands that ff_staged_supported takes: in one launch where
-// both are tiled and that is faster, with the depth split where tiles are few, as far as `partial` (256-byte aligned)
-// holds the shares' sums: ff_partial_bytes is enough for any split that is taken.
+// The gradients of a call: dw (I transposed), dx, and a bias gradient without dw. Both may run in one launch; either may
+// have its depth split, as far as the workspace's partial sums reach (ff_partial_bytes is enough for any split that is
+// taken).
+struct FfGradient {
+    bool wanted;
+    FfChoice choice;
+    int splits;
+};
+struct FfGradients {
+    FfGradient w, x;
+    bool one_launch, w_first;
+    int sum_shares;  // 0: no bias gradient alone
+};
 size_t ff_partial_bytes(int64_t m, int64_t features, int64_t k);
-hipError_t launch_ff_gradients(const FfParams* dw, const FfParams* dx, bool bf16, float* partial, size_t partial_bytes,
-                               int compute_units, hipStream_t stream);
+// dw and dx: null where not wanted; sums: dw's parameters for a bias gradient alone, else null.
+FfGradients choose_ff_gradients(const FfParams* dw, const FfParams* dx, const FfParams* sums, size_t partial_bytes,
+                                int compute_units);
+hipError_t launch_ff_gradients(const FfGradients& plan, const FfParams* dw, const FfParams* dx, const FfParams* sums,
+                               bool bf16, float* partial, hipStream_t stream);
 
-// Row sums of I = dz by columns (row_sums) without a product.
-hipError_t launch_ff_row_sums(const FfParams& p, bool bf16, float* partial, size_t partial_bytes, int compute_units,
-                              hipStream_t stream);
-
-// Projections of at most 16 rows whose rows 16-byte accesses divide.
+// Few rows (feed_forward_rows.hip): waves of a workgroup.
 bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8);
-hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, hipStream_t stream);
+int ff_rows_waves(const FfParams& p, bool gated);
+hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, int waves, bool staged, bool bf16, bool j_fp8,
+                          hipStream_t stream);
+
+// Whether a product's rows have the 16 bytes that all kernels but the general one need.
+bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8);
 
 }  // namespace sdxl_hip

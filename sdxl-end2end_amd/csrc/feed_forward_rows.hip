@@ -191,12 +191,13 @@ hipError_t launch(const FfParams& p, bool gated, hipStream_t stream) {
 }
 
 template <typename T, bool kJFp8, bool kStaged>
-hipError_t launch_rows(const FfParams& p, bool gated, hipStream_t stream) {
-    // waves of a workgroup: 2048 in all where there are blocks for them
-    const int64_t groups = gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16, blocks = (p.depth + 63) / 64;
-    if (groups * 8 < 2048 && blocks > 8) return launch<T, kJFp8, 16, kStaged>(p, gated, stream);
-    if (groups * 4 < 2048 && blocks > 4) return launch<T, kJFp8, 8, kStaged>(p, gated, stream);
-    return launch<T, kJFp8, 4, kStaged>(p, gated, stream);
+hipError_t launch_rows(const FfParams& p, bool gated, int waves, hipStream_t stream) {
+    switch (waves) {
+    case 16: return launch<T, kJFp8, 16, kStaged>(p, gated, stream);
+    case 8: return launch<T, kJFp8, 8, kStaged>(p, gated, stream);
+    case 4: return launch<T, kJFp8, 4, kStaged>(p, gated, stream);
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
@@ -208,11 +209,18 @@ bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8) {
            w_rows * p.ld_j * (j_fp8 ? 1 : 2) < (int64_t{1} << 31) && ff_staged_supported(p, epilogue, false, false, j_fp8);
 }
 
-hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, hipStream_t stream) {
-    const bool gated = epilogue == kFfGated, staged = !ff_tiled_supported(p, epilogue, false, false, j_fp8);
+// 2048 waves in all where there are blocks for them
+int ff_rows_waves(const FfParams& p, bool gated) {
+    const int64_t groups = gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16, blocks = (p.depth + 63) / 64;
+    return groups * 8 < 2048 && blocks > 8 ? 16 : groups * 4 < 2048 && blocks > 4 ? 8 : 4;
+}
+
+hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, int waves, bool staged, bool bf16, bool j_fp8,
+                          hipStream_t stream) {
+    const bool gated = epilogue == kFfGated;
     auto by_type = [&]<typename T>() {
-        if (staged) return j_fp8 ? launch_rows<T, true, true>(p, gated, stream) : launch_rows<T, false, true>(p, gated, stream);
-        return j_fp8 ? launch_rows<T, true, false>(p, gated, stream) : launch_rows<T, false, false>(p, gated, stream);
+        if (staged) return j_fp8 ? launch_rows<T, true, true>(p, gated, waves, stream) : launch_rows<T, false, true>(p, gated, waves, stream);
+        return j_fp8 ? launch_rows<T, true, false>(p, gated, waves, stream) : launch_rows<T, false, false>(p, gated, waves, stream);
     };
     return bf16 ? by_type.template operator()<__bf16>() : by_type.template operator()<_Float16>();
 }

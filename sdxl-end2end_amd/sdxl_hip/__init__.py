@@ -54,6 +54,7 @@ FEED_FORWARD_SYMBOLS = (
     "sdxl_gated_linear_backward_workspace_bytes",
     "sdxl_linear_act_backward",
     "sdxl_gated_linear_backward",
+    "sdxl_ff_kernels",
     "sdxl_ff_sublayer_workspace_bytes",
     "sdxl_ff_sublayer",
 )
@@ -210,6 +211,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(FfDesc), vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.sdxl_ff_kernels.restype = ctypes.c_size_t
+    lib.sdxl_ff_kernels.argtypes = [ctypes.POINTER(FfDesc), ctypes.c_int32, ctypes.c_int32, ctypes.c_char_p, ctypes.c_size_t]
     lib.sdxl_ff_sublayer_workspace_bytes.restype = ctypes.c_size_t
     lib.sdxl_ff_sublayer_workspace_bytes.argtypes = [ctypes.POINTER(FfSublayerDesc)]
     lib.sdxl_ff_sublayer.restype = ctypes.c_int
@@ -680,6 +683,15 @@ def ff_backward_workspace_bytes(M: int, N: int, K: int, gated: bool, activation:
     lib = load()
     return int((lib.sdxl_gated_linear_backward_workspace_bytes if gated else
                 lib.sdxl_linear_act_backward_workspace_bytes)(ctypes.byref(desc)))
+
+
+def ff_kernels(desc: FfDesc, gated: bool, gradients=()) -> str:
+    """The kernels that a call of this descriptor runs (sdxl_ff_kernels); gradients: of "dx", "dw", "dbias" (none: the
+    forward call)."""
+    bits = sum({"dx": 1, "dw": 2, "dbias": 4}[g] for g in gradients)
+    text = ctypes.create_string_buffer(256)
+    load().sdxl_ff_kernels(ctypes.byref(desc), 1 if gated else 0, bits, text, len(text))
+    return text.value.decode()
 
 
 def ff_sublayer(x, ln_gamma, ln_beta, w_in, w_in_scale, b_in, w_out, w_out_scale, b_out, activation: str = "gelu",
