@@ -347,7 +347,6 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
             for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
     float sums[kMI] = {};  // row sums of the I operand (dbias)
 
-    // at most kFlying of the wave's transfers are still on their way, and no wave reads LDS any more
     // at most kFlying stages' transfers of the wave are still on their way, and no wave reads LDS any more
     auto land = [&]<int kFlying>() __attribute__((always_inline)) {
         if (kFlying == 0 || kMore == 0 || wave < kMore) wait_vmem<kFlying * kXfers>();
@@ -755,7 +754,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     }
 }
 
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false, bool kStaged = false>
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
 __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) void ff_tile_kernel(FfParams p) {
     __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
     ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi>(p, blockIdx.x, smem);
@@ -791,7 +790,7 @@ void ff_blocks(FfParams& p, bool gated) {
     p.group_i = p.i_blocks < 8 ? p.i_blocks : 8;
 }
 
-template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi, bool kSplit = false, bool kStaged = false>
+template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
 hipError_t ff_launch(FfParams p, hipStream_t stream) {
     ff_blocks<Tile>(p, kEpi == kFfGated || kEpi == kFfGatedDz);
     hipLaunchKernelGGL((ff_tile_kernel<T, kIT, kJT, kJFp8, Tile, kEpi>), dim3((unsigned)((int64_t)p.i_blocks * p.j_blocks)),
