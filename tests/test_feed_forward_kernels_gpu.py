@@ -163,3 +163,18 @@ def test_gradients_of_integers(kernel, dtype):
             assert (got is not None) == (what in wanted or (what == "dbias" and with_sums))
             if got is not None:
                 exact(got, want[what](), what)
+
+
+@pytest.mark.parametrize("dtype,step", [(F16, 2.0 ** -24), (F16, 2.0 ** -20), (BF16, 2.0 ** -133)])
+@pytest.mark.parametrize("form,kernel,size", cases(linear=sizes.LINEAR))
+def test_subnormal_values_count(form, kernel, size, dtype, step):
+    """Small gradients and activations, whole multiples of the type's smallest step, are not flushed on the way."""
+    m, n, k = size
+    x, w, dout = integers(1, m, k, dtype=dtype), integers(2, n, k, dtype=dtype), integers(3, m, n, dtype=dtype)
+    small = lambda t: (t.double() * step).to(dtype)
+    exact(sh.linear_act(small(x), w), x.double() @ w.double().t() * step, "x")
+    exact(sh.linear_act(x, small(w)), x.double() @ w.double().t() * step, "w")
+    dx, dw, db = sh.linear_act_backward(small(dout), x, w, need_dbias=True)
+    for what, got, want in (("dx", dx, dout.double() @ w.double()), ("dw", dw, dout.double().t() @ x.double()), ("db", db, dout.double().sum(0))):
+        exact(got, want * step, what)
+    exact(sh.linear_act_backward(small(dout), x, w, need_dx=False, need_dw=False, need_dbias=True)[2], dout.double().sum(0) * step, "db alone")
