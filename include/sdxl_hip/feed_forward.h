@@ -13,12 +13,17 @@
  * w has that type or holds FP8 E4M3 codes with per-row fp32 scales (forward only).
  * Products are summed in fp32 and every output is rounded once; the backward calls round
  * dz (below) to the tensors' type in between, since it is an operand of the 16-bit matrix
- * cores. Any m, n, k >= 0 and any row strides of at least a row; tensors need only their
+ * cores: the gradients made of it are about 1.4 times as far from exact as one rounding
+ * leaves them. In fp16 dz also has the type's range: beyond 65504 it is infinite, below
+ * 2^-25 zero. dbias, its column sum, leaves that range with it unless terms cancel, and
+ * what is lost below is at most 2^-25 of every term; scale the loss as for any fp16
+ * gradient. Any m, n, k >= 0 and any row strides of at least a row; tensors need only their
  * element's alignment. Rows that 16-byte accesses divide (pointers and row strides
  * multiples of 16 bytes, k a multiple of 8 and with E4M3 weights of 16) run the fast
  * kernels; other rows of 16 bytes or more take about twice as long, shorter ones and
  * strides above 2^20 elements the general kernel (the sums' order differs).
- * An infinite pre-activation takes the activation's limit; NaN stays NaN.
+ * An infinite pre-activation takes the activation's limit; NaN stays NaN (and relu's slope
+ * at NaN is 1).
  *
  * All calls are stream-ordered, allocate nothing, never synchronise and may be captured
  * into a HIP graph; the stream's device must be the current one. Outputs and workspace
@@ -78,14 +83,16 @@ sdxl_status sdxl_gated_linear(const sdxl_ff_desc* desc, const void* x, const voi
                               const void* bias, void* out, void* stream);
 
 /* Workspace of the backward calls (dz, and up to 32 MiB of partial sums where a product of few
- * tiles splits its sum), 256-byte aligned; 0 for a descriptor that the call refuses. */
+ * tiles splits its sum), 256-byte aligned, the same whichever gradients are asked for, so that
+ * each is summed alike; 0 for a descriptor that the call refuses. */
 size_t sdxl_linear_act_backward_workspace_bytes(const sdxl_ff_desc* desc);
 size_t sdxl_gated_linear_backward_workspace_bytes(const sdxl_ff_desc* desc);
 
 /* Gradients of sdxl_linear_act for dout [m, n]: with z = x . w^T + bias (formed again here),
  * dz = dout * act'(z): dx = dz . w [m, k], dw = dz^T . x [n, k], dbias = column sums of dz [n].
  * The residual's gradient is dout itself. dx, dw and dbias are each optional (NULL: not
- * computed); bias as in the forward call (NULL if it had none). */
+ * computed); bias as in the forward call (NULL if it had none). There is no w_scale: a forward
+ * call with scales of 16-bit weights has its gradients through the scaled weights. */
 sdxl_status sdxl_linear_act_backward(const sdxl_ff_desc* desc, const void* dout, const void* x, const void* w,
                                      const void* bias, void* dx, void* dw, void* dbias, void* workspace,
                                      size_t workspace_bytes, void* stream);
