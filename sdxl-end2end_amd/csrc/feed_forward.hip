@@ -34,6 +34,8 @@ bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0;
 //   128 x 128  dx [2048, 1280] deep 10240 69 (256 x 256: 207, 128 x 256: 116)
 //    64 x 128  dw [640, 2560] deep 8192 51 (128 x 128: 56, 128 x 256: 95)
 //    64 x  64  [154, 5120] deep 1280 10 (128 x 128: 15, 256 x 256: 32)
+// The constants have no terms for bytes, caches or power and one end for every epilogue: they rank tiles, and miss the
+// times of whole chips by up to a fifth (gated [8192, 2048] -> 2 x 5456 316 for 340, [8192, 2560] -> 640 31 for 36).
 struct TileCost {
     int rows, cols;
     float alone, pair, ends;

@@ -1,5 +1,4 @@
-// Internal launch interface of the feed-forward kernels (feed_forward.hip,
-// feed_forward_general.hip).
+// Internal launch interface of the feed-forward kernels (feed_forward*.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
