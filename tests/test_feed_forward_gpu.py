@@ -234,6 +234,8 @@ def test_few_rows(m, n, k, dtype):
 
 # rows and columns of sums that each tile of the tiled kernel takes at a depth of 328 (six stages, the last one
 # ragged), largest tile last, every edge ragged
+# (as measured costs choose, some of these meet on one tile and 64 x 64 has none: every tile, by name, is in
+# test_feed_forward_kernels_gpu.py)
 TILES = [(200, 4104), (4100, 520), (4100, 744), (4100, 1032), (4100, 1496), (4100, 2056), (4100, 4104)]
 
 
@@ -275,6 +277,7 @@ def test_every_tile_backward(rows, cols, dtype):
 
 # dw and dx in one launch, either one's tasks first, on every pair of their tiles that the sizes of a call lead to
 # (rows, columns, features)
+# (five of the nine pairs; all of them, by name, are in test_feed_forward_kernels_gpu.py)
 @pytest.mark.parametrize("m,n,k", [(2056, 1283, 328), (328, 2056, 1288), (2400, 200, 1800), (200, 2400, 1800), (4100, 648, 2056),
                                    (648, 4100, 2056), (1111, 640, 640), (4104, 2056, 264), (70, 6001, 136)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
