@@ -1,4 +1,5 @@
-"""Python harness binding of the sdxl_hip C ABI (include/sdxl_hip/attention.h, sublayer.h, feed_forward.h).
+"""Python harness binding of the sdxl_hip C ABI (include/sdxl_hip/attention.h, sublayer.h, feed_forward.h,
+group_norm.h).
 
 This is a thin ctypes layer used by the test suite, the smoke check and bench.py.
 Device memory and streams come from PyTorch (plumbing only); every computation
@@ -57,6 +58,14 @@ FEED_FORWARD_SYMBOLS = (
     "sdxl_ff_kernels",
     "sdxl_ff_sublayer_workspace_bytes",
     "sdxl_ff_sublayer",
+)
+# of group_norm.h
+GROUP_NORM_SYMBOLS = (
+    "sdxl_group_norm_workspace_bytes",
+    "sdxl_group_norm_backward_workspace_bytes",
+    "sdxl_group_norm",
+    "sdxl_group_norm_backward",
+    "sdxl_group_norm_i8",
 )
 
 
@@ -121,6 +130,15 @@ class FfSublayerDesc(ctypes.Structure):
                 ("gate_first", ctypes.c_int32), ("ln_eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
+class GroupNormDesc(ctypes.Structure):
+    """Mirror of struct sdxl_group_norm_desc."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "pixels", "channels", "groups", "x_row_stride", "y_row_stride",
+                                              "dy_row_stride")] + \
+               [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
+
+
 # The descriptors as packed bytes (native alignment, as the structures above) and prototypes that
 # take them: on the call path one struct.pack costs a third of filling a ctypes structure.
 _ATTN_DESC = struct.Struct("9q4if4x")
@@ -129,6 +147,8 @@ _SUBLAYER_DESC = struct.Struct("3q2if2i4x")
 _CROSS_SUBLAYER_DESC = struct.Struct("4q2ifi")
 _FF_DESC = struct.Struct("9q5i4x")
 _FF_SUBLAYER_DESC = struct.Struct("3q4ifi")
+_GROUP_NORM_DESC = struct.Struct("7q2ifi")
+assert _GROUP_NORM_DESC.size == ctypes.sizeof(GroupNormDesc)
 assert _FF_DESC.size == ctypes.sizeof(FfDesc) and _FF_SUBLAYER_DESC.size == ctypes.sizeof(FfSublayerDesc)
 assert _ATTN_DESC.size == ctypes.sizeof(AttnDesc) and _LINEAR_DESC.size == ctypes.sizeof(LinearDesc)
 assert _SUBLAYER_DESC.size == ctypes.sizeof(SublayerDesc) and _CROSS_SUBLAYER_DESC.size == ctypes.sizeof(CrossSublayerDesc)
@@ -218,14 +238,27 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.sdxl_ff_sublayer.restype = ctypes.c_int
     lib.sdxl_ff_sublayer.argtypes = [ctypes.POINTER(FfSublayerDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                      ctypes.c_size_t, vp]
+    for name in ("sdxl_group_norm", "sdxl_group_norm_backward"):
+        fn = getattr(lib, name + "_workspace_bytes")
+        fn.restype = ctypes.c_size_t
+        fn.argtypes = [ctypes.POINTER(GroupNormDesc)]
+    lib.sdxl_group_norm.restype = ctypes.c_int
+    lib.sdxl_group_norm.argtypes = [ctypes.POINTER(GroupNormDesc), vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.sdxl_group_norm_i8.restype = ctypes.c_int
+    lib.sdxl_group_norm_i8.argtypes = [ctypes.POINTER(GroupNormDesc), vp, vp, vp, vp, i64, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.sdxl_group_norm_backward.restype = ctypes.c_int
+    lib.sdxl_group_norm_backward.argtypes = [ctypes.POINTER(GroupNormDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                             ctypes.c_size_t, vp]
     for name in ("sdxl_attn_fwd", "sdxl_linear", "sdxl_attn_sublayer", "sdxl_cross_attn_sublayer", "sdxl_linear_act",
-                 "sdxl_gated_linear", "sdxl_linear_act_backward", "sdxl_gated_linear_backward", "sdxl_ff_sublayer"):
+                 "sdxl_gated_linear", "sdxl_linear_act_backward", "sdxl_gated_linear_backward", "sdxl_ff_sublayer",
+                 "sdxl_group_norm", "sdxl_group_norm_i8", "sdxl_group_norm_backward"):
         fn = lib[name]  # a function object of its own, with its own prototype
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_char_p] + getattr(lib, name).argtypes[1:]
         setattr(lib, "packed_" + name, fn)
     for name in ("sdxl_linear_act_backward_workspace_bytes", "sdxl_gated_linear_backward_workspace_bytes",
-                 "sdxl_ff_sublayer_workspace_bytes"):
+                 "sdxl_ff_sublayer_workspace_bytes", "sdxl_group_norm_workspace_bytes",
+                 "sdxl_group_norm_backward_workspace_bytes"):
         fn = lib[name]
         fn.restype = ctypes.c_size_t
         fn.argtypes = [ctypes.c_char_p]
@@ -281,6 +314,7 @@ class _Torch:
         self.codes = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
         self.half_codes = {torch.float16: F16, torch.bfloat16: BF16}
         self.f16, self.f32, self.int32, self.uint8 = torch.float16, torch.float32, torch.int32, torch.uint8
+        self.int8 = torch.int8
         self.device = torch.cuda.device
         self.current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         self.empty, self.empty_like = torch.empty, torch.empty_like
@@ -539,7 +573,7 @@ def cross_attn_sublayer(x, ln_gamma, ln_beta, w_q, w_q_scale, kv, w_out, b_out, 
 def _ff_call(fn, index, t, *args) -> None:
     """fn(*args, stream) on the tensors' device, which is made current where it is not."""
     if index < 0:
-        raise SdxlError(INVALID_ARGUMENT, "feed-forward: tensors must be on a GPU")
+        raise SdxlError(INVALID_ARGUMENT, "sdxl: tensors must be on a GPU")
     if index == t.current_device():
         status = fn(*args, t.raw_stream(index))
     else:
@@ -731,6 +765,144 @@ def ff_sublayer(x, ln_gamma, ln_beta, w_in, w_in_scale, b_in, w_out, w_out_scale
              _ptr(w_in), _ptr(w_in_scale), _ptr(b_in), _ptr(w_out), _ptr(w_out_scale), _ptr(b_out), out.data_ptr(),
              workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return out
+
+
+# ---------------------------------------------------------------- group norm
+# (include/sdxl_hip/group_norm.h; reference src/cuda/unet.cpp:151-181)
+
+def _gn_stride(name, what, t, channels) -> int:
+    """The row stride of a channels-last tensor [batch, .., channels] that is not contiguous, after its checks."""
+    shape, stride = t.shape, t.stride()
+    if t.numel() == 0:
+        return 0
+    if channels > 1 and stride[-1] != 1:
+        raise SdxlError(INVALID_SHAPE, f"{name}: {what} must have unit channel stride")
+    row, rows, first = 0, 1, True
+    for size, step in zip(shape[-2::-1], stride[-2::-1]):
+        if size == 1:
+            continue
+        if first:
+            if step % rows != 0 or step < channels:
+                raise SdxlError(INVALID_SHAPE, f"{name}: row stride smaller than the row")
+            row, first = step, False
+        elif step != row * rows:
+            raise SdxlError(INVALID_SHAPE, f"{name}: {what} must have one stride from pixel to pixel")
+        rows *= size
+    return row
+
+
+def _gn_common(name, x, gamma, beta, groups, activation):
+    """(torch lookups, batch, pixels, channels, row stride, type code, activation code, device index)"""
+    t = _Torch.loaded or _Torch()
+    code = t.codes.get(x.dtype)
+    if code is None:
+        raise SdxlError(INVALID_SHAPE, f"{name}: tensors must be fp16, bf16 or fp32")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: activation must be one of {', '.join(ACTIVATIONS)}")
+    shape = x.shape
+    if len(shape) < 3:
+        raise SdxlError(INVALID_SHAPE, f"{name}: x must be [batch, .., channels]")
+    batch, channels = shape[0], shape[-1]
+    pixels = shape[1]
+    for size in shape[2:-1]:
+        pixels *= size
+    if groups <= 0 or channels % groups != 0:
+        raise SdxlError(INVALID_SHAPE, f"{name}: channels must be a multiple of groups")
+    index = x.get_device()
+    _ff_like(name, "gamma", gamma, (channels,), x.dtype, index)
+    _ff_like(name, "beta", beta, (channels,), x.dtype, index)
+    return t, batch, pixels, channels, 0 if x.is_contiguous() else _gn_stride(name, "x", x, channels), code, act, index
+
+
+def _gn_workspace(name, t, size, workspace, x, index):
+    if workspace is None:
+        return t.empty((size,), dtype=t.uint8, device=x.device)
+    if workspace.get_device() != index or not workspace.is_contiguous():
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: workspace must be contiguous and on x's device")
+    return workspace
+
+
+def _gn_stats(name, t, stats, with_stats, batch, groups, x, index):
+    if stats is not None:
+        if stats.shape != (batch, groups, 2) or stats.dtype != t.f32 or not stats.is_contiguous() or stats.get_device() != index:
+            raise SdxlError(INVALID_SHAPE, f"{name}: stats must be contiguous fp32 [{batch}, {groups}, 2] on x's device")
+        return stats
+    return t.empty((batch, groups, 2), dtype=t.f32, device=x.device) if with_stats else None
+
+
+def group_norm(x, gamma, beta, groups: int, activation: str = "none", eps: float = 1e-5, out=None,
+               with_stats: bool = False, workspace=None):
+    """act((x - mean) * rstd * gamma + beta), the statistics by image and group (sdxl_group_norm): x [batch, ..,
+    channels] fp16, bf16 or fp32 (channels last; pixel rows may be strided), gamma and beta [channels] of its type.
+    Returns y (out, which may be x, if given), with with_stats (y, stats): mean and rstd as fp32 [batch, groups, 2],
+    for group_norm_backward. workspace: contiguous, of group_norm_workspace_bytes, else one is allocated."""
+    name = "sdxl_group_norm"
+    t, batch, pixels, channels, ldx, code, act, index = _gn_common(name, x, gamma, beta, groups, activation)
+    ldy = 0
+    if out is None:
+        out = x.new_empty(x.shape)
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index:
+            raise SdxlError(INVALID_SHAPE, f"{name}: out must be like x")
+        ldy = 0 if out.is_contiguous() else _gn_stride(name, "out", out, channels)
+    stats = _gn_stats(name, t, None, with_stats, batch, groups, x, index)
+    desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, ldy, 0, code, act, _f32(eps), 0)
+    lib = load()
+    workspace = _gn_workspace(name, t, lib.packed_sdxl_group_norm_workspace_bytes(desc), workspace, x, index)
+    _ff_call(lib.packed_sdxl_group_norm, index, t, desc, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), out.data_ptr(),
+             stats.data_ptr() if stats is not None else None, workspace.data_ptr(),
+             workspace.numel() * workspace.element_size())
+    return (out, stats) if with_stats else out
+
+
+def group_norm_backward(dout, x, gamma, beta, groups: int, stats, activation: str = "none", need_dx: bool = True,
+                        need_dgamma: bool = True, need_dbeta: bool = True, workspace=None):
+    """Gradients (dx like x but contiguous, dgamma [channels], dbeta [channels]) of group_norm for dout like x, with the
+    stats of its forward call. What is not needed is None. workspace: contiguous, of group_norm_workspace_bytes(..,
+    backward=True), else one is allocated."""
+    name = "sdxl_group_norm_backward"
+    t, batch, pixels, channels, ldx, code, act, index = _gn_common(name, x, gamma, beta, groups, activation)
+    if dout.shape != x.shape or dout.dtype != x.dtype or dout.get_device() != index:
+        raise SdxlError(INVALID_SHAPE, f"{name}: dout must be like x")
+    lddy = 0 if dout.is_contiguous() else _gn_stride(name, "dout", dout, channels)
+    _gn_stats(name, t, stats, False, batch, groups, x, index)
+    desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, 0, lddy, code, act, 0.0, 0)
+    lib = load()
+    workspace = _gn_workspace(name, t, lib.packed_sdxl_group_norm_backward_workspace_bytes(desc), workspace, x, index)
+    dx = x.new_empty(x.shape) if need_dx else None
+    dgamma = x.new_empty((channels,)) if need_dgamma else None
+    dbeta = x.new_empty((channels,)) if need_dbeta else None
+    _ff_call(lib.packed_sdxl_group_norm_backward, index, t, desc, dout.data_ptr(), x.data_ptr(), gamma.data_ptr(),
+             beta.data_ptr(), stats.data_ptr(), _ptr(dx), _ptr(dgamma), _ptr(dbeta), workspace.data_ptr(),
+             workspace.numel() * workspace.element_size())
+    return dx, dgamma, dbeta
+
+
+def group_norm_i8(x, gamma, beta, groups: int, activation: str = "none", eps: float = 1e-5, with_stats: bool = False,
+                  workspace=None):
+    """group_norm of fp16 or bf16 x whose pixels are quantised by row (sdxl_group_norm_i8): returns (codes int8 like x,
+    scales fp32 [rows]) for linear_i8, with with_stats the stats too."""
+    name = "sdxl_group_norm_i8"
+    t, batch, pixels, channels, ldx, code, act, index = _gn_common(name, x, gamma, beta, groups, activation)
+    q = t.empty(x.shape, dtype=t.int8, device=x.device)
+    scale = t.empty((batch * pixels,), dtype=t.f32, device=x.device)
+    stats = _gn_stats(name, t, None, with_stats, batch, groups, x, index)
+    desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, 0, 0, code, act, _f32(eps), 0)
+    lib = load()
+    workspace = _gn_workspace(name, t, lib.packed_sdxl_group_norm_workspace_bytes(desc), workspace, x, index)
+    _ff_call(lib.packed_sdxl_group_norm_i8, index, t, desc, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), q.data_ptr(), 0,
+             scale.data_ptr(), stats.data_ptr() if stats is not None else None, workspace.data_ptr(),
+             workspace.numel() * workspace.element_size())
+    return (q, scale, stats) if with_stats else (q, scale)
+
+
+def group_norm_workspace_bytes(batch: int, pixels: int, channels: int, groups: int, dtype: int = F16,
+                               backward: bool = False) -> int:
+    """Workspace of group_norm and group_norm_i8, or of group_norm_backward."""
+    desc = GroupNormDesc(batch=batch, pixels=pixels, channels=channels, groups=groups, dtype=dtype)
+    lib = load()
+    return int((lib.sdxl_group_norm_backward_workspace_bytes if backward else lib.sdxl_group_norm_workspace_bytes)(ctypes.byref(desc)))
 
 
 def linear_flops(m: int, n: int, k: int) -> float:

@@ -1,0 +1,373 @@
+"""Group norm and its gradients against plain 64-bit forms on the same inputs.
+
+Tolerances are bounds, element by element, from 64-bit quantities. With u = 2^-24 and s the largest distance of a
+group's values from their mean: sums of at most L + 16 terms in fp32, taken about a value of the group, are off by
+(L + 16) u of their magnitudes, so a mean is off by (L + 16) u 2s + u |mean| and a variance by 4 (L + 16) u s^2 (L: the
+pixels, 1024 at most: no thread adds more of them in a row). Activations are evaluated to 2e-5 of their value for 16-bit
+tensors, for fp32 ones to 8 u (1 + |z| + |z|^3 / 10) (the argument of an exponential is rounded: exp2, the reciprocal and
+erfc add some units in the last place); slopes are at most 1.13, second derivatives 1.2. Every output is rounded once.
+"""
+import math
+
+import pytest
+
+import sdxl_hip as sh
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+HALF = {F16: 2.0 ** -11, BF16: 2.0 ** -8, F32: 2.0 ** -24}
+TINY = {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}
+U = 2.0 ** -24
+ACTS = ("none", "relu", "gelu", "gelu_tanh", "quick_gelu", "silu")
+TYPES = (F16, BF16, F32)
+
+
+def values(seed, *shape, std=1.0, mean=0.0, dtype=F16):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=gen) * std + mean).to(dtype).to(DEV)
+
+
+def act64(name, z):
+    if name == "none":
+        return z
+    if name == "relu":
+        return torch.relu(z)
+    if name == "gelu":
+        return z * torch.special.ndtr(z)
+    if name == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    return z * torch.sigmoid(z * (1.702 if name == "quick_gelu" else 1.0))
+
+
+def slope64(name, z):
+    z = z.detach().requires_grad_(True)
+    return torch.autograd.grad(act64(name, z).sum(), z)[0]
+
+
+def within(got, want, bound, what):
+    bad = ~((got.double() - want).abs() <= bound)
+    assert not bad.any(), (what, int(bad.sum()), (got.double() - want).abs()[bad].max().item(), bound.expand_as(want)[bad].min().item())
+
+
+def act_error(dtype, z):
+    """Of an activation's value, relative."""
+    return 2e-5 if dtype != F32 else 8 * U * (1 + z.abs() + z.abs() ** 3 / 10)
+
+
+def terms(pixels):
+    return min(pixels, 1024) + 16
+
+
+def parts(x, groups):
+    """x by groups in 64 bits, its mean and variance, the bounds of their errors in fp32"""
+    B, C = x.shape[0], x.shape[-1]
+    v = x.double().reshape(B, -1, groups, C // groups)
+    mean = v.mean(dim=(1, 3), keepdim=True)
+    var = (v - mean).square().mean(dim=(1, 3), keepdim=True)
+    s = (v - mean).abs().amax(dim=(1, 3), keepdim=True)
+    L = terms(v.shape[1])
+    return v, mean, var, L * U * 2 * s + U * mean.abs(), 4 * L * U * s * s
+
+
+def normal_form(x, gamma, beta, groups, eps):
+    """n, z and the bounds of their errors, with rstd and its own"""
+    v, mean, var, em, ev = parts(x, groups)
+    rstd = (var + eps).rsqrt()
+    er = 0.5 * ev / (var + eps) * 1.5 + 4 * U  # relative (ev is a small part of var + eps in every case here)
+    n = (v - mean) * rstd
+    en = rstd * (em + 2 * U * (v - mean).abs()) + n.abs() * er
+    g, b = (t.double().view(1, 1, groups, -1) for t in (gamma, beta))
+    z = n * g + b
+    ez = en * g.abs() + 4 * U * ((n * g).abs() + b.abs())
+    return n, en, z, ez, rstd, er
+
+
+def check_forward(x, gamma, beta, groups, activation, eps, got, stats=None):
+    n, en, z, ez, rstd, er = normal_form(x, gamma, beta, groups, eps)
+    want = act64(activation, z)
+    err = 1.13 * ez + act_error(x.dtype, z) * want.abs()
+    h, tiny = HALF[x.dtype], TINY[x.dtype]
+    within(got, want.reshape(x.shape), (err + h * (want.abs() + err) + tiny).reshape(x.shape), ("y", x.shape, groups, activation))
+    if stats is not None:
+        _, mean, _, em, _ = parts(x, groups)
+        B = x.shape[0]
+        within(stats[:, :, 0], mean.view(B, groups), em.view(B, groups) + 1e-30, ("mean", x.shape))
+        within(stats[:, :, 1], rstd.view(B, groups), (rstd * er).view(B, groups), ("rstd", x.shape))
+
+
+def stats64(x, groups, eps):
+    _, mean, var, _, _ = parts(x, groups)
+    return torch.stack((mean.flatten(1), (var + eps).rsqrt().flatten(1)), dim=2).float().contiguous()
+
+
+def check_backward(dy, x, gamma, beta, groups, activation, stats, grads):
+    B, C = x.shape[0], x.shape[-1]
+    v = x.double().reshape(B, -1, groups, C // groups)
+    P = v.shape[1]
+    mean, rstd = (stats[:, :, i].double().view(B, 1, groups, 1) for i in (0, 1))
+    g, b = (t.double().view(1, 1, groups, -1) for t in (gamma, beta))
+    n = (v - mean) * rstd
+    z = n * g + b
+    en = 3 * U * n.abs()
+    ez = 5 * U * ((n * g).abs() + b.abs())
+    d = dy.double().reshape(v.shape)
+    dz = d * slope64(activation, z)
+    edz = torch.zeros_like(dz) if activation == "none" else d.abs() * (1.2 * ez + act_error(x.dtype, z))
+    if activation == "relu":
+        edz = edz + d.abs() * (z.abs() <= ez)
+    edz = edz + 2 * U * dz.abs()
+    L = terms(P) + B
+    h, tiny = HALF[x.dtype], TINY[x.dtype]
+    dgamma, dbeta = (dz * n).sum(dim=(0, 1)).reshape(C), dz.sum(dim=(0, 1)).reshape(C)
+    mass_b = dz.abs().sum(dim=(0, 1)).reshape(C)
+    mass_g = (dz * n).abs().sum(dim=(0, 1)).reshape(C)
+    err_b = edz.sum(dim=(0, 1)).reshape(C) + L * U * mass_b
+    # (the sum runs over x - mean and takes rstd at its end)
+    err_g = (edz * n.abs() + dz.abs() * en).sum(dim=(0, 1)).reshape(C) + (L + 4) * U * mass_g
+    dx, got_g, got_b = grads
+    if got_b is not None:
+        within(got_b, dbeta, err_b + h * (dbeta.abs() + err_b) + tiny, ("dbeta", x.shape, activation))
+    if got_g is not None:
+        within(got_g, dgamma, err_g + h * (dgamma.abs() + err_g) + tiny, ("dgamma", x.shape, activation))
+    if dx is not None:
+        gd = dz * g
+        m = P * (C // groups)
+        A, Bs = gd.sum(dim=(1, 3), keepdim=True) / m, (gd * n).sum(dim=(1, 3), keepdim=True) / m
+        LG = L + 16  # (channels are added by teams)
+        eA = (edz * g.abs()).sum(dim=(1, 3), keepdim=True) / m + LG * U * gd.abs().sum(dim=(1, 3), keepdim=True) / m
+        eB = ((edz * n.abs() + dz.abs() * en) * g.abs()).sum(dim=(1, 3), keepdim=True) / m + \
+            LG * U * (gd * n).abs().sum(dim=(1, 3), keepdim=True) / m
+        want = rstd * (gd - A - n * Bs)
+        err = rstd * (edz * g.abs() + eA + n.abs() * eB + en * Bs.abs() + 6 * U * (gd.abs() + A.abs() + (n * Bs).abs()))
+        within(dx, want.reshape(x.shape), (err + h * (want.abs() + err) + tiny).reshape(x.shape), ("dx", x.shape, activation))
+
+
+# (batch, pixels, channels, groups): one value; a row of one pixel; rows of less than 16 bytes, of an odd number of
+# channels and with ends inside a vector; groups of 1, 3, 4, 10, 20, 30 and 40 channels; a group of every channel; many
+# channels; pixels that no chunk divides; many images; more chunks than one
+SIZES = [(1, 1, 1, 1), (2, 1, 64, 8), (1, 5, 3, 3), (3, 17, 7, 1), (2, 9, 12, 4), (2, 33, 27, 9), (1, 64, 32, 32),
+         (2, 50, 96, 32), (3, 41, 128, 32), (2, 100, 320, 32), (2, 63, 640, 32), (1, 300, 960, 32), (2, 256, 1280, 32),
+         (1, 77, 2560, 32), (1, 31, 1000, 1), (2, 7, 8192, 32), (1, 3, 20000, 4), (1, 3, 9001, 1), (700, 4, 64, 2),
+         (1, 5000, 320, 32), (2, 3001, 40, 4), (1, 20011, 128, 32), (1, 2500, 1288, 8), (1, 999, 514, 2)]
+
+
+def case(i):
+    return TYPES[i % 3], ACTS[(i // 3 + i) % 6], (1e-5, 1e-6)[i % 2]
+
+
+@pytest.mark.parametrize("turn", range(3))
+@pytest.mark.parametrize("i", range(len(SIZES)))
+def test_forward(i, turn):
+    B, P, C, G = SIZES[i]
+    dtype, activation, eps = case(i + 7 * turn)
+    x = values(i, B, P, C, std=1.5, mean=0.3, dtype=dtype)
+    gamma, beta = values(i + 50, C, std=0.3, mean=1.0, dtype=dtype), values(i + 90, C, std=0.5, dtype=dtype)
+    got, stats = sh.group_norm(x, gamma, beta, G, activation=activation, eps=eps, with_stats=True)
+    check_forward(x, gamma, beta, G, activation, eps, got, stats)
+    assert torch.equal(got, sh.group_norm(x, gamma, beta, G, activation=activation, eps=eps))
+
+
+@pytest.mark.parametrize("turn", range(3))
+@pytest.mark.parametrize("i", range(len(SIZES)))
+def test_backward(i, turn):
+    B, P, C, G = SIZES[i]
+    dtype, activation, eps = case(i + 5 * turn)
+    x = values(i, B, P, C, std=1.5, mean=-0.2, dtype=dtype)
+    gamma, beta = values(i + 50, C, std=0.3, mean=1.0, dtype=dtype), values(i + 90, C, std=0.5, dtype=dtype)
+    dy = values(i + 130, B, P, C, std=0.5, dtype=dtype)
+    stats = stats64(x, G, eps)
+    grads = sh.group_norm_backward(dy, x, gamma, beta, G, stats, activation=activation)
+    check_backward(dy, x, gamma, beta, G, activation, stats, grads)
+    for a, b in zip(grads, sh.group_norm_backward(dy, x, gamma, beta, G, stats, activation=activation)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("activation", ACTS)
+def test_every_activation(dtype, activation):
+    x = values(3, 2, 200, 320, std=3.0, dtype=dtype)
+    gamma, beta = values(4, 320, std=1.0, mean=1.0, dtype=dtype), values(5, 320, std=2.0, dtype=dtype)
+    dy = values(6, 2, 200, 320, dtype=dtype)
+    got, stats = sh.group_norm(x, gamma, beta, 32, activation=activation, with_stats=True)
+    check_forward(x, gamma, beta, 32, activation, 1e-5, got, stats)
+    check_backward(dy, x, gamma, beta, 32, activation, stats,
+                   sh.group_norm_backward(dy, x, gamma, beta, 32, stats, activation=activation))
+
+
+@pytest.mark.parametrize("dtype,activation", [(F16, "none"), (BF16, "silu"), (F32, "gelu"), (F32, "silu")])
+def test_gradients_against_differences(dtype, activation):
+    """Central differences of the plain form in 64 bits, along random directions: the gradients are the function's."""
+    B, P, C, G = 2, 37, 40, 4
+    x = values(1, B, P, C, dtype=dtype)
+    gamma, beta = values(2, C, std=0.3, mean=1.0, dtype=dtype), values(3, C, std=0.3, dtype=dtype)
+    dy = values(4, B, P, C, dtype=dtype)
+    _, stats = sh.group_norm(x, gamma, beta, G, activation=activation, with_stats=True)
+    grads = sh.group_norm_backward(dy, x, gamma, beta, G, stats, activation=activation)
+
+    def loss(x, gamma, beta):
+        _, _, z, _, _, _ = normal_form(x, gamma, beta, G, 1e-5)
+        return (act64(activation, z).reshape(dy.shape) * dy.double()).sum()
+
+    args = [x.double(), gamma.double(), beta.double()]
+    for which in range(3):
+        direction = values(10 + which, *args[which].shape, dtype=F32).double()
+        step = 1e-5
+        ends = []
+        for sign in (1, -1):
+            moved = list(args)
+            moved[which] = args[which] + sign * step * direction
+            ends.append(loss(*moved))
+        slope = (ends[0] - ends[1]) / (2 * step)
+        along = (grads[which].double() * direction).sum()
+        # every gradient's element is off by its rounding (and little more); the differences by about 1e-8
+        bound = (2 * HALF[dtype] + 1e-5) * (grads[which].double() * direction).abs().sum() + 1e-6
+        assert (along - slope).abs() <= bound, (which, along.item(), slope.item(), bound.item())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad,offset,C", [(8, 0, 320), (3, 1, 320), (64, 8, 96), (5, 2, 45), (1, 3, 128)])
+def test_strided_rows_and_any_alignment(dtype, pad, offset, C):
+    """Column slices of wider rows, from an element that 16 bytes do not divide; what lies beside them stays."""
+    B, P, G = 2, 150, 1 if C == 45 else 32
+    wide = values(1, B, P, C + pad + offset, dtype=dtype)
+    dwide = values(2, B, P, C + pad + offset, dtype=dtype)
+    x, dy = wide[:, :, offset:offset + C], dwide[:, :, offset:offset + C]
+    gamma, beta = values(3, C + 1, mean=1.0, dtype=dtype)[1:], values(4, C + 1, dtype=dtype)[1:]
+    out_wide = torch.full((B, P, C + pad + offset), 7.0, dtype=dtype, device=DEV)
+    out = out_wide[:, :, offset:offset + C]
+    got, stats = sh.group_norm(x, gamma, beta, G, activation="silu", out=out, with_stats=True)
+    check_forward(x, gamma, beta, G, "silu", 1e-5, got, stats)
+    keep = torch.ones(C + pad + offset, dtype=torch.bool, device=DEV)
+    keep[offset:offset + C] = False
+    assert (out_wide[:, :, keep] == 7.0).all()
+    assert torch.equal(got, sh.group_norm(x.contiguous(), gamma.clone(), beta.clone(), G, activation="silu"))
+    grads = sh.group_norm_backward(dy, x, gamma, beta, G, stats, activation="silu")
+    check_backward(dy, x, gamma, beta, G, "silu", stats, grads)
+
+
+def test_images_of_four_dimensions_and_in_place():
+    x = values(1, 2, 9, 11, 64)
+    gamma, beta = values(2, 64, mean=1.0), values(3, 64)
+    want = sh.group_norm(x, gamma, beta, 8, activation="silu")
+    assert want.shape == x.shape and torch.equal(want.view(2, 99, 64), sh.group_norm(x.view(2, 99, 64), gamma, beta, 8, activation="silu"))
+    # torch's channels-last images are such tensors
+    image = x.permute(0, 3, 1, 2)
+    assert image.is_contiguous(memory_format=torch.channels_last)
+    assert torch.equal(want, sh.group_norm(image.permute(0, 2, 3, 1), gamma, beta, 8, activation="silu"))
+    got = sh.group_norm(x, gamma, beta, 8, activation="silu", out=x)
+    assert got.data_ptr() == x.data_ptr() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("P", [50, 4000])
+def test_mean_far_from_zero(P):
+    """A variance of 1 about a mean of 1000: sums of squares about zero would lose it in fp32."""
+    x = values(1, 2, P, 320, dtype=F32) + 1000.0
+    gamma, beta = values(2, 320, mean=1.0, dtype=F32), values(3, 320, dtype=F32)
+    got, stats = sh.group_norm(x, gamma, beta, 32, with_stats=True)
+    check_forward(x, gamma, beta, 32, "none", 1e-5, got, stats)
+    # channels far from each other: the groups' own spread is large, and every channel keeps its digits
+    x = x + 100.0 * torch.arange(320, device=DEV)
+    got, stats = sh.group_norm(x, gamma, beta, 32, with_stats=True)
+    check_forward(x, gamma, beta, 32, "none", 1e-5, got, stats)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("P", [1, 300])
+def test_constant_groups(dtype, P):
+    """No variance: rstd is 1 / sqrt(eps), the output act(beta)."""
+    x = torch.full((2, P, 64), 3.0, dtype=dtype, device=DEV)
+    gamma, beta = values(2, 64, mean=1.0, dtype=dtype), values(3, 64, dtype=dtype)
+    got, stats = sh.group_norm(x, gamma, beta, 8, with_stats=True)
+    assert torch.equal(got, beta.expand(2, P, 64))
+    assert (stats[:, :, 0] == 3.0).all() and ((stats[:, :, 1] - 1e-5 ** -0.5).abs() <= 1e-4).all()
+    dy = values(4, 2, P, 64, dtype=dtype)
+    grads = sh.group_norm_backward(dy, x, gamma, beta, 8, stats)
+    check_backward(dy, x, gamma, beta, 8, "none", stats, grads)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype,P", [(F16, 60), (BF16, 2000), (F32, 60)])
+def test_what_is_not_finite_stays_in_its_group(value, dtype, P):
+    x = values(1, 2, P, 64, dtype=dtype)
+    gamma, beta = values(2, 64, mean=1.0, dtype=dtype), values(3, 64, dtype=dtype)
+    clean = sh.group_norm(x, gamma, beta, 8, activation="silu")
+    x[1, P // 2, 20] = value  # image 1, group 2
+    got, stats = sh.group_norm(x, gamma, beta, 8, activation="silu", with_stats=True)
+    hit = torch.zeros(2, P, 64, dtype=torch.bool, device=DEV)
+    hit[1, :, 16:24] = True
+    assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit])
+    assert stats[1, 2].isnan().any() and not torch.cat((stats[0], stats[1, :2], stats[1, 3:])).isnan().any()
+    dy = values(4, 2, P, 64, dtype=dtype)
+    dx, dgamma, dbeta = sh.group_norm_backward(dy, x, gamma, beta, 8, stats, activation="silu")
+    assert dx[hit].isnan().all() and not dx[~hit].isnan().any()
+    assert dgamma[16:24].isnan().all() and not dgamma[:16].isnan().any() and not dgamma[24:].isnan().any()
+
+
+def test_gradients_one_by_one():
+    x = values(1, 2, 700, 96)
+    gamma, beta, dy = values(2, 96, mean=1.0), values(3, 96), values(4, 2, 700, 96)
+    stats = stats64(x, 32, 1e-5)
+    whole = sh.group_norm_backward(dy, x, gamma, beta, 32, stats, activation="silu")
+    for wanted in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (False, False, False)):
+        got = sh.group_norm_backward(dy, x, gamma, beta, 32, stats, activation="silu", need_dx=wanted[0],
+                                     need_dgamma=wanted[1], need_dbeta=wanted[2])
+        for g, w, want in zip(got, wanted, whole):
+            assert (g is None) if not w else torch.equal(g, want)
+
+
+def test_no_pixels():
+    gamma, beta = values(1, 64), values(2, 64)
+    for shape in ((0, 5, 64), (2, 0, 64)):
+        x = torch.empty(*shape, dtype=F16, device=DEV)
+        assert sh.group_norm(x, gamma, beta, 8).shape == x.shape
+        stats = torch.empty(shape[0], 8, 2, device=DEV)
+        dx, dgamma, dbeta = sh.group_norm_backward(x, x, gamma, beta, 8, stats)
+        assert dx.shape == x.shape and (dgamma == 0).all() and (dbeta == 0).all()
+
+
+@pytest.mark.parametrize("P", [30, 5000])
+def test_captured_and_replayed_on_another_stream(P):
+    """Forward and backward as one graph on a side stream, replayed with eager calls between, inputs changed in place."""
+    x, dy = values(1, 2, P, 320), values(2, 2, P, 320)
+    gamma, beta = values(3, 320, mean=1.0), values(4, 320)
+
+    def both():
+        y, stats = sh.group_norm(x, gamma, beta, 32, activation="silu", with_stats=True)
+        return (y, stats) + sh.group_norm_backward(dy, x, gamma, beta, 32, stats, activation="silu")
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        both()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        outs = both()
+    for turn in range(4):
+        x.copy_(values(10 + turn, 2, P, 320))
+        dy.copy_(values(20 + turn, 2, P, 320))
+        graph.replay()
+        want = both()
+        torch.cuda.synchronize()
+        for got, expected in zip(outs, want):
+            assert torch.equal(got, expected), turn
+
+
+def test_two_calls_at_once():
+    """Calls in flight on two streams, each with a workspace of its own."""
+    xs = [values(i, 2, 3000, 320) for i in range(2)]
+    gamma, beta = values(3, 320, mean=1.0), values(4, 320)
+    want = [sh.group_norm(x, gamma, beta, 32) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(8):
+        for i, (x, s) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(sh.group_norm(x, gamma, beta, 32))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        for o in outs:
+            assert torch.equal(o, w)
