@@ -294,7 +294,7 @@ int64_t units(int compute_units) { return compute_units > 0 ? compute_units : 25
 }  // namespace
 
 FfChoice choose_ff(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int compute_units) {
-    if (!ff_staged_supported(p, epilogue, false, false, j_fp8)) return {FfKernel::kGeneral, 0, false};
+    if (p.i8 != 0 || !ff_staged_supported(p, epilogue, false, false, j_fp8)) return {FfKernel::kGeneral, 0, false};
     const bool staged = !ff_tiled_supported(p, epilogue, false, false, j_fp8);
     if (ff_rows_supported(p, epilogue, j_fp8)) return {FfKernel::kRows, ff_rows_waves(p, epilogue == kFfGated), staged};
     const int64_t cus = units(compute_units);

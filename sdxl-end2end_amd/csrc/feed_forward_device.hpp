@@ -56,6 +56,13 @@ struct FfType<__bf16> {
     }
 };
 
+// 8-bit integers, 16 consecutive bytes of depth a lane: 32 x 32 x 32, exact 32-bit sums
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ i32x16 mfma32_i8(i16x8 a, i16x8 b, i32x16 c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+
 // 16 bytes at any element's address
 template <int kAlign>
 struct __attribute__((packed, aligned(kAlign))) Unaligned {

@@ -44,6 +44,10 @@ struct FfParams {
     int32_t splits, share_stages;
     int64_t ld_partial;  // cols, up to a multiple of 8
     float* partial;
+    // both operands hold 8-bit integers (forward epilogues): ld_i, ld_j and depth in bytes, i_scale the fp32 scale of every
+    // I row, j_scale that of every J row
+    int32_t i8;
+    const float* i_scale;
 };
 
 // The joining pass of a product whose depth was split.

@@ -1,5 +1,5 @@
 """Python harness binding of the sdxl_hip C ABI (include/sdxl_hip/attention.h, sublayer.h, feed_forward.h,
-group_norm.h).
+group_norm.h, int8.h).
 
 This is a thin ctypes layer used by the test suite, the smoke check and bench.py.
 Device memory and streams come from PyTorch (plumbing only); every computation
@@ -18,7 +18,7 @@ LIB_PATH = os.environ.get("SDXL_HIP_LIB") or os.path.join(PKG_ROOT, "lib", "libs
 # sdxl_status
 OK, INVALID_ARGUMENT, INVALID_SHAPE, UNSUPPORTED, LAUNCH_FAILED, DEVICE_ERROR = range(6)
 # sdxl_dtype
-F16, BF16, F32, E4M3 = 0, 1, 2, 3
+F16, BF16, F32, E4M3, I8 = 0, 1, 2, 3, 4
 # sdxl_activation
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "quick_gelu": 4, "silu": 5}
 # sdxl_attn_backend (values of the reference's AttentionBackend, runtime.hpp:53-58)
@@ -66,6 +66,15 @@ GROUP_NORM_SYMBOLS = (
     "sdxl_group_norm",
     "sdxl_group_norm_backward",
     "sdxl_group_norm_i8",
+)
+# of int8.h
+INT8_SYMBOLS = (
+    "sdxl_quantize_i8_rows",
+    "sdxl_layer_norm_i8",
+    "sdxl_linear_i8_workspace_bytes",
+    "sdxl_gated_linear_i8_workspace_bytes",
+    "sdxl_linear_i8",
+    "sdxl_gated_linear_i8",
 )
 
 
@@ -139,6 +148,14 @@ class GroupNormDesc(ctypes.Structure):
                 ("reserved", ctypes.c_int32)]
 
 
+class I8Desc(ctypes.Structure):
+    """Mirror of struct sdxl_i8_desc."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("m", "n", "k", "x_row_stride", "w_row_stride", "out_row_stride",
+                                              "residual_row_stride")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "x_dtype", "activation", "gate_first", "reserved")]
+
+
 # The descriptors as packed bytes (native alignment, as the structures above) and prototypes that
 # take them: on the call path one struct.pack costs a third of filling a ctypes structure.
 _ATTN_DESC = struct.Struct("9q4if4x")
@@ -148,6 +165,8 @@ _CROSS_SUBLAYER_DESC = struct.Struct("4q2ifi")
 _FF_DESC = struct.Struct("9q5i4x")
 _FF_SUBLAYER_DESC = struct.Struct("3q4ifi")
 _GROUP_NORM_DESC = struct.Struct("7q2ifi")
+_I8_DESC = struct.Struct("7q5i4x")
+assert _I8_DESC.size == ctypes.sizeof(I8Desc)
 assert _GROUP_NORM_DESC.size == ctypes.sizeof(GroupNormDesc)
 assert _FF_DESC.size == ctypes.sizeof(FfDesc) and _FF_SUBLAYER_DESC.size == ctypes.sizeof(FfSublayerDesc)
 assert _ATTN_DESC.size == ctypes.sizeof(AttnDesc) and _LINEAR_DESC.size == ctypes.sizeof(LinearDesc)
@@ -249,16 +268,28 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.sdxl_group_norm_backward.restype = ctypes.c_int
     lib.sdxl_group_norm_backward.argtypes = [ctypes.POINTER(GroupNormDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                              ctypes.c_size_t, vp]
+    lib.sdxl_quantize_i8_rows.restype = ctypes.c_int
+    lib.sdxl_quantize_i8_rows.argtypes = [i64, i64, ctypes.c_int32, vp, i64, vp, i64, vp, vp]
+    lib.sdxl_layer_norm_i8.restype = ctypes.c_int
+    lib.sdxl_layer_norm_i8.argtypes = [i64, i64, ctypes.c_int32, vp, i64, vp, vp, ctypes.c_float, vp, i64, vp, vp]
+    for name in ("sdxl_linear_i8", "sdxl_gated_linear_i8"):
+        fn = getattr(lib, name + "_workspace_bytes")
+        fn.restype = ctypes.c_size_t
+        fn.argtypes = [ctypes.POINTER(I8Desc)]
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(I8Desc)] + [vp] * (6 if "gated" in name else 7) + [vp, ctypes.c_size_t, vp]
     for name in ("sdxl_attn_fwd", "sdxl_linear", "sdxl_attn_sublayer", "sdxl_cross_attn_sublayer", "sdxl_linear_act",
                  "sdxl_gated_linear", "sdxl_linear_act_backward", "sdxl_gated_linear_backward", "sdxl_ff_sublayer",
-                 "sdxl_group_norm", "sdxl_group_norm_i8", "sdxl_group_norm_backward"):
+                 "sdxl_group_norm", "sdxl_group_norm_i8", "sdxl_group_norm_backward", "sdxl_linear_i8", "sdxl_gated_linear_i8"):
         fn = lib[name]  # a function object of its own, with its own prototype
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_char_p] + getattr(lib, name).argtypes[1:]
         setattr(lib, "packed_" + name, fn)
     for name in ("sdxl_linear_act_backward_workspace_bytes", "sdxl_gated_linear_backward_workspace_bytes",
                  "sdxl_ff_sublayer_workspace_bytes", "sdxl_group_norm_workspace_bytes",
-                 "sdxl_group_norm_backward_workspace_bytes"):
+                 "sdxl_group_norm_backward_workspace_bytes", "sdxl_linear_i8_workspace_bytes",
+                 "sdxl_gated_linear_i8_workspace_bytes"):
         fn = lib[name]
         fn.restype = ctypes.c_size_t
         fn.argtypes = [ctypes.c_char_p]
@@ -903,6 +934,133 @@ def group_norm_workspace_bytes(batch: int, pixels: int, channels: int, groups: i
     desc = GroupNormDesc(batch=batch, pixels=pixels, channels=channels, groups=groups, dtype=dtype)
     lib = load()
     return int((lib.sdxl_group_norm_backward_workspace_bytes if backward else lib.sdxl_group_norm_workspace_bytes)(ctypes.byref(desc)))
+
+
+# ---------------------------------------------------------------- 8-bit integer linears
+# (include/sdxl_hip/int8.h; the places of src/cuda/unet.cpp:98-149)
+
+def _i8_rows(name, x, gamma, beta, eps):
+    """(codes, scales) of x's rows, or of their LayerNorm"""
+    t = _Torch.loaded or _Torch()
+    code = t.half_codes.get(x.dtype)
+    if code is None:
+        raise SdxlError(INVALID_SHAPE, f"{name}: tensors must be fp16 or bf16")
+    if x.dim() < 1:
+        raise SdxlError(INVALID_SHAPE, f"{name}: x must be [.., columns]")
+    index, cols = x.get_device(), x.shape[-1]
+    rows = 1
+    for size in x.shape[:-1]:
+        rows *= size
+    if gamma is not None:
+        _ff_like(name, "gamma", gamma, (cols,), x.dtype, index)
+        _ff_like(name, "beta", beta, (cols,), x.dtype, index)
+    ldx = 0 if x.is_contiguous() else _gn_stride(name, "x", x, cols)
+    q = t.empty(x.shape, dtype=t.int8, device=x.device)
+    scale = t.empty((rows,), dtype=t.f32, device=x.device)
+    lib = load()
+    if gamma is not None:
+        _ff_call(lib.sdxl_layer_norm_i8, index, t, rows, cols, code, x.data_ptr(), ldx, gamma.data_ptr(), beta.data_ptr(),
+                 eps, q.data_ptr(), 0, scale.data_ptr())
+    else:
+        _ff_call(lib.sdxl_quantize_i8_rows, index, t, rows, cols, code, x.data_ptr(), ldx, q.data_ptr(), 0, scale.data_ptr())
+    return q, scale
+
+
+def quantize_i8_rows(x):
+    """8-bit integers with a scale by row (sdxl_quantize_i8_rows): x [.., K] fp16 or bf16 (tokens, or a weight by output
+    channel; rows may be strided). Returns (codes int8 like x, scales fp32 [rows])."""
+    return _i8_rows("sdxl_quantize_i8_rows", x, None, None, 0.0)
+
+
+def layer_norm_i8(x, gamma, beta, eps: float = 1e-5):
+    """LayerNorm over the last dim, quantised by row (sdxl_layer_norm_i8): returns (codes int8 like x, scales fp32 [rows])
+    for linear_i8."""
+    return _i8_rows("sdxl_layer_norm_i8", x, gamma, beta, _f32(eps))
+
+
+def _linear_i8(name, gated, x, w, w_scale, x_scale, bias, residual, activation, gate_first, dtype, out, workspace):
+    t = _Torch.loaded or _Torch()
+    if w.dtype != t.int8:
+        raise SdxlError(INVALID_SHAPE, f"{name}: weights must be int8")
+    tokens = x.dtype != t.int8
+    given = x.dtype if tokens else dtype
+    if given is None:  # codes: what the other tensors are
+        for other in (out, bias, residual):
+            given = given or (other.dtype if other is not None else None)
+    code = t.half_codes.get(given)
+    if code is None or (dtype is not None and dtype != given):
+        raise SdxlError(INVALID_SHAPE, f"{name}: tensors must be fp16 or bf16 (8-bit x: give dtype), and of one type")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: activation must be one of {', '.join(ACTIVATIONS)}")
+    x_shape, w_shape = x.shape, w.shape
+    if len(x_shape) != 2 or len(w_shape) != 2 or w_shape[1] != x_shape[1] or (gated and w_shape[0] % 2 != 0):
+        raise SdxlError(INVALID_SHAPE, f"{name}: x must be [M, K] and w [{'2N' if gated else 'N'}, K]")
+    M, K = x_shape
+    features = w_shape[0]
+    N = features // 2 if gated else features
+    index = x.get_device()
+    if w.get_device() != index:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: w must be on x's device")
+    _ff_like(name, "w_scale", w_scale, (features,), t.f32, index)
+    if tokens != (x_scale is None):
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: x_scale goes with 8-bit x")
+    if x_scale is not None:
+        _ff_like(name, "x_scale", x_scale, (M,), t.f32, index)
+    if bias is not None:
+        _ff_like(name, "bias", bias, (features,), given, index)
+    ldr = ldo = 0
+    if residual is not None:
+        _ff_like(name, "residual", residual, (M, N), given, index)
+        ldr = 0 if residual.is_contiguous() else _ff_stride(name, "residual", residual)
+    if out is None:
+        out = t.empty((M, N), dtype=given, device=x.device)
+    else:
+        _ff_like(name, "out", out, (M, N), given, index)
+        ldo = 0 if out.is_contiguous() else _ff_stride(name, "out", out)
+    desc = _I8_DESC.pack(M, N, K, 0 if x.is_contiguous() else _ff_stride(name, "x", x),
+                         0 if w.is_contiguous() else _ff_stride(name, "w", w), ldo, ldr, code, code if tokens else I8, act,
+                         1 if gate_first else 0, 0)
+    lib = load()
+    if tokens:
+        size = (lib.packed_sdxl_gated_linear_i8_workspace_bytes if gated else lib.packed_sdxl_linear_i8_workspace_bytes)(desc)
+        workspace = _gn_workspace(name, t, size, workspace, x, index)
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    else:
+        ws_ptr, ws_bytes = None, 0
+    scale_ptr = x_scale.data_ptr() if x_scale is not None else None
+    bias_ptr = bias.data_ptr() if bias is not None else None
+    if gated:
+        _ff_call(lib.packed_sdxl_gated_linear_i8, index, t, desc, x.data_ptr(), scale_ptr, w.data_ptr(), w_scale.data_ptr(),
+                 bias_ptr, out.data_ptr(), ws_ptr, ws_bytes)
+    else:
+        _ff_call(lib.packed_sdxl_linear_i8, index, t, desc, x.data_ptr(), scale_ptr, w.data_ptr(), w_scale.data_ptr(), bias_ptr,
+                 residual.data_ptr() if residual is not None else None, out.data_ptr(), ws_ptr, ws_bytes)
+    return out
+
+
+def linear_i8(x, w, w_scale, x_scale=None, bias=None, residual=None, activation: str = "none", dtype=None, out=None,
+              workspace=None):
+    """act((x . w^T) * x_scale * w_scale + bias) + residual (sdxl_linear_i8): w [N, K] int8 with w_scale [N] fp32; x [M, K]
+    int8 with x_scale [M] fp32 (dtype: of the output where bias, residual and out do not say it), or fp16 / bf16 tokens,
+    which are quantised by row; bias [N], residual [M, N] (may be out). Rows may be strided. workspace: contiguous, of
+    linear_i8_workspace_bytes, for tokens, else one is allocated. Returns [M, N]."""
+    return _linear_i8("sdxl_linear_i8", False, x, w, w_scale, x_scale, bias, residual, activation, False, dtype, out, workspace)
+
+
+def gated_linear_i8(x, w, w_scale, x_scale=None, bias=None, activation: str = "gelu", gate_first: bool = False, dtype=None,
+                    out=None, workspace=None):
+    """value * act(gate) with [value | gate] = (x . w^T) * x_scale * w_scale + bias (sdxl_gated_linear_i8): w [2N, K] int8
+    with w_scale [2N], bias [2N]; gate_first: [gate | value]. Other arguments as linear_i8. Returns [M, N]."""
+    return _linear_i8("sdxl_gated_linear_i8", True, x, w, w_scale, x_scale, bias, None, activation, gate_first, dtype, out,
+                      workspace)
+
+
+def linear_i8_workspace_bytes(M: int, N: int, K: int, gated: bool = False, dtype: int = F16) -> int:
+    """Workspace of linear_i8 / gated_linear_i8 with 16-bit tokens."""
+    desc = I8Desc(m=M, n=N, k=K, dtype=dtype, x_dtype=dtype)
+    lib = load()
+    return int((lib.sdxl_gated_linear_i8_workspace_bytes if gated else lib.sdxl_linear_i8_workspace_bytes)(ctypes.byref(desc)))
 
 
 def linear_flops(m: int, n: int, k: int) -> float:
