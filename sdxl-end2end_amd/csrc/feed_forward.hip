@@ -16,6 +16,10 @@ hipError_t ff_pair_f16(const FfParams& w, const FfParams& x, int w_tile, int x_t
 hipError_t ff_pair_bf16(const FfParams& w, const FfParams& x, int w_tile, int x_tile, bool w_first, hipStream_t stream);
 hipError_t ff_staged_f16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
 hipError_t ff_staged_bf16(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream);
+hipError_t ff_i8_forward_f16(const FfParams& p, FfEpilogue epilogue, int tile, hipStream_t stream);
+hipError_t ff_i8_forward_bf16(const FfParams& p, FfEpilogue epilogue, int tile, hipStream_t stream);
+hipError_t ff_i8_staged_f16(const FfParams& p, FfEpilogue epilogue, bool large, hipStream_t stream);
+hipError_t ff_i8_staged_bf16(const FfParams& p, FfEpilogue epilogue, bool large, hipStream_t stream);
 hipError_t ff_deep(const FfParams& p, FfEpilogue epilogue, bool bf16, bool j_fp8, bool staged, FfDeepId id, hipStream_t stream);
 
 namespace {
@@ -85,7 +89,7 @@ float list_time(int64_t a, float a_time, int64_t b, float b_time, int64_t cus) {
 FfDeepId deep_choice(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool staged, float& time) {
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
     const int64_t small = ((p.rows + 31) / 32) * ((cols + 31) / 32), large = ((p.rows + 63) / 64) * ((cols + 63) / 64);
-    const float blocks = (float)((p.depth + 63) / 64), rounds = (float)small / (float)(2 * cus);
+    const float blocks = (float)ff_stages(p), rounds = (float)small / (float)(2 * cus);
     FfDeepId id = kFfDeep32x4;
     if (small <= cus) {
         id = kFfDeep32x8;
@@ -105,7 +109,7 @@ FfDeepId deep_choice(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool s
 
 int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus, float& best_time) {
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
-    const float stages = (float)((p.depth + 63) / 64);
+    const float stages = (float)ff_stages(p);
     int best = 0;
     for (int t = 0; t < kFfTiles; ++t) {
         if (j_fp8 && t == kFf128x128) continue;  // its waves share a stage's depth, E4M3 codes come in pairs of steps
@@ -151,7 +155,7 @@ bool staged_large(const FfParams& p, int64_t cols, int64_t cus) {
 // 1280 12 (33).
 float staged_time(const FfParams& p, int64_t cols) {
     const int64_t tiles = ((p.rows + 63) / 64) * ((cols + 63) / 64);
-    return 4.5f + (float)((p.depth + 63) / 64) * (tiles > 256 ? 0.85f + 0.0012f * (float)(tiles - 256) : 0.85f);
+    return 4.5f + (float)ff_stages(p) * (tiles > 256 ? 0.85f + 0.0012f * (float)(tiles - 256) : 0.85f);
 }
 
 // ---- dw and dx in one launch. A side of it: a product on a tile, its depth in so many shares.
@@ -272,7 +276,8 @@ __global__ __launch_bounds__(256) void ff_row_sums_kernel(FfParams p, int64_t sp
 bool ff_staged_supported(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool j_fp8) {
     if (p.depth <= 0 || (epilogue == kFfStore && !j_transposed)) return false;
     // rows of 16 bytes or more: a row's last chunk is read as its last 16 bytes
-    if ((i_transposed ? p.rows : p.depth) < 8 || (j_transposed ? p.cols : p.depth) < (j_fp8 ? 16 : 8)) return false;
+    if (p.i8 != 0) j_fp8 = true;  // (both operands in bytes)
+    if ((i_transposed ? p.rows : p.depth) < (p.i8 != 0 ? 16 : 8) || (j_transposed ? p.cols : p.depth) < (j_fp8 ? 16 : 8)) return false;
     // a window (at most 320 rows) stays below 2^31 bytes, the threads of a launch below 2^32
     if (p.ld_i > (1 << 20) || p.ld_j > (1 << 20) || p.ld_out > (1 << 20) || p.ld_dout > (1 << 20) || p.ld_res > (1 << 20))
         return false;
@@ -285,6 +290,7 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
     if (!ff_staged_supported(p, epilogue, i_transposed, j_transposed, j_fp8)) return false;
     // rows in whole 16-byte chunks: the depth, or the columns of an operand that is read by columns
     const int64_t i_row = p.i_row != 0 ? p.i_row : i_transposed ? p.rows : p.depth;
+    if (p.i8 != 0) return aligned(p.ip, 16) && aligned(p.jp, 16) && p.ld_i % 16 == 0 && p.ld_j % 16 == 0 && p.depth % 16 == 0;
     if (!aligned(p.ip, 16) || !aligned(p.jp, 16) || p.ld_i % 8 != 0 || p.ld_j % (j_fp8 ? 16 : 8) != 0) return false;
     return i_row % 8 == 0 && (j_transposed ? p.cols % 8 == 0 : p.depth % (j_fp8 ? 16 : 8) == 0);
 }
@@ -294,7 +300,7 @@ int64_t units(int compute_units) { return compute_units > 0 ? compute_units : 25
 }  // namespace
 
 FfChoice choose_ff(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int compute_units) {
-    if (p.i8 != 0 || !ff_staged_supported(p, epilogue, false, false, j_fp8)) return {FfKernel::kGeneral, 0, false};
+    if (!ff_staged_supported(p, epilogue, false, false, j_fp8)) return {FfKernel::kGeneral, 0, false};
     const bool staged = !ff_tiled_supported(p, epilogue, false, false, j_fp8);
     if (ff_rows_supported(p, epilogue, j_fp8)) return {FfKernel::kRows, ff_rows_waves(p, epilogue == kFfGated), staged};
     const int64_t cus = units(compute_units);
@@ -317,9 +323,12 @@ hipError_t launch_ff(const FfChoice& choice, const FfParams& params, FfEpilogue 
     case FfKernel::kGeneral: return launch_ff_general(params, epilogue, false, false, bf16, j_fp8, stream);
     case FfKernel::kRows: return launch_ff_rows(params, epilogue, choice.variant, choice.staged, bf16, j_fp8, stream);
     case FfKernel::kDeep: return ff_deep(p, epilogue, bf16, j_fp8, choice.staged, (FfDeepId)choice.variant, stream);
-    case FfKernel::kStaged: return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, choice.variant == 128, stream);
+    case FfKernel::kStaged:
+        if (p.i8 != 0) return (bf16 ? ff_i8_staged_bf16 : ff_i8_staged_f16)(p, epilogue, choice.variant == 128, stream);
+        return (bf16 ? ff_staged_bf16 : ff_staged_f16)(p, epilogue, false, j_fp8, choice.variant == 128, stream);
     case FfKernel::kTile: break;
     }
+    if (p.i8 != 0) return (bf16 ? ff_i8_forward_bf16 : ff_i8_forward_f16)(p, epilogue, choice.variant, stream);
     if (epilogue == kFfLinear || epilogue == kFfGated)
         return (bf16 ? ff_forward_bf16 : ff_forward_f16)(p, epilogue, j_fp8, choice.variant, stream);
     return (bf16 ? ff_backward_bf16 : ff_backward_f16)(p, epilogue, false, choice.variant, stream);

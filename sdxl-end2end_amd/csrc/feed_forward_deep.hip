@@ -24,11 +24,15 @@ namespace sdxl_hip {
 namespace {
 
 typedef __attribute__((address_space(3))) i16x8 lds_op;
-typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
 template <typename T, bool kJFp8, int kSide, int kWaves, FfEpilogue kEpi, bool kStaged>
 __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     using F = FfType<T>;
+    using Out = typename F::Out;
+    using Acc = typename F::Acc;
+    using Acc4 = typename F::Acc4;
+    typedef __attribute__((address_space(3))) Acc4 lds_acc4;
+    constexpr int kElem = F::kElem, kDepth = 128 / kElem, kChunk = 16 / kElem;  // elements of a block, of 16 bytes
     constexpr bool kGated = kEpi == kFfGated || kEpi == kFfGatedDz, kDz = kEpi == kFfLinearDz || kEpi == kFfGatedDz;
     constexpr int kT = kSide / 32, kRing = 2, kCols = kGated ? kSide / 2 : kSide;
     constexpr int kIBytes = kSide * 128, kBlock = kIBytes + kSide * (kJFp8 ? 64 : 128), kXfers = kBlock / 1024, kIXfers = kIBytes / 1024;
@@ -38,7 +42,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t value_row = p.gate_first ? p.cols : 0, gate_row = p.gate_first ? 0 : p.cols;
-    const int64_t ldi_b = p.ld_i * 2, ldj_b = p.ld_j * (kJFp8 ? 1 : 2);
+    const int64_t ldi_b = p.ld_i * kElem, ldj_b = p.ld_j * (kJFp8 ? 1 : kElem);
     // tasks by XCD, rows fastest: an XCD's workgroups share their J rows in its L2
     int64_t i0, j0;
     {
@@ -50,7 +54,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
         j0 = (int64_t)(task / p.i_blocks) * kCols;
     }
     const int64_t i_rows = min(p.rows - i0, (int64_t)kSide), j_rows = min(p.cols - j0, (int64_t)kCols);
-    const int blocks = (int)((p.depth + 63) / 64);
+    const int blocks = (int)((p.depth + kDepth - 1) / kDepth);
     const int mine = (blocks - wave + kWaves - 1) / kWaves;  // blocks of the wave
 
     // the lane's part of a transfer: 8 rows (by the parity of its number) or, of E4M3 rows, 16
@@ -64,14 +68,14 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
         return (kGated ? 16 * (n >> 2) + 8 * (n & 1) : 8 * n) + row8;
     };
     auto request = [&](int it, int slot) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)(it * kWaves + wave) * 64, left = p.depth - at, i_left = p.i_row - at;
+        const int64_t at = (int64_t)(it * kWaves + wave) * kDepth, left = p.depth - at, i_left = p.i_row - at;
         const uint32_t buf = lds0 + slot * kBlock;
-        const u32x4 ir = window_rsrc({(const char*)p.ip + i0 * ldi_b + at * 2, (uint32_t)((i_rows - 1) * ldi_b + i_left * 2)});
+        const u32x4 ir = window_rsrc({(const char*)p.ip + i0 * ldi_b + at * kElem, (uint32_t)((i_rows - 1) * ldi_b + i_left * kElem)});
 #pragma unroll
         for (int n = 0; n < kIXfers; ++n)
-            window_to_lds(ir, 8 * chunk8[n & 1] < i_left ? (uint32_t)((8 * n + row8) * ldi_b) + 16 * chunk8[n & 1] : kOutside, buf + n * 1024);
-        const char* base = (const char*)p.jp + at * (kJFp8 ? 1 : 2);
-        const uint32_t size = (uint32_t)((j_rows - 1) * ldj_b + left * (kJFp8 ? 1 : 2));
+            window_to_lds(ir, kChunk * chunk8[n & 1] < i_left ? (uint32_t)((8 * n + row8) * ldi_b) + 16 * chunk8[n & 1] : kOutside, buf + n * 1024);
+        const char* base = (const char*)p.jp + at * (kJFp8 ? 1 : kElem);
+        const uint32_t size = (uint32_t)((j_rows - 1) * ldj_b + left * (kJFp8 ? 1 : kElem));
         const u32x4 jv = window_rsrc({base + (kGated ? value_row + j0 : j0) * ldj_b, size});
         const u32x4 jg = window_rsrc({base + (kGated ? gate_row + j0 : j0) * ldj_b, size});
 #pragma unroll
@@ -79,7 +83,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
             const bool gate = gate_of(n);
             uint32_t off;
             if constexpr (kJFp8) off = 16 * chunk16 < left ? (uint32_t)(j_row(n) * ldj_b) + 16 * chunk16 : kOutside;
-            else off = 8 * chunk8[n & 1] < left ? (uint32_t)(j_row(n) * ldj_b) + 16 * chunk8[n & 1] : kOutside;
+            else off = kChunk * chunk8[n & 1] < left ? (uint32_t)(j_row(n) * ldj_b) + 16 * chunk8[n & 1] : kOutside;
             window_to_lds(gate ? jg : jv, off, buf + kIBytes + n * 1024);
         }
     };
@@ -87,13 +91,13 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     int row_off[4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) row_off[ks] = col * 128 + (((4 * (ks >> 1) + 2 * hf + (ks & 1)) ^ swz(col)) << 4);
-    f32x16 acc[kT][kT];  // [J][I]
+    Acc acc[kT][kT];  // [J][I]
 #pragma unroll
     for (int t = 0; t < kT; ++t)
 #pragma unroll
         for (int m = 0; m < kT; ++m)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[t][m][r] = 0.0f;
+            for (int r = 0; r < 16; ++r) acc[t][m][r] = 0;
     auto multiply = [&](int slot) __attribute__((always_inline)) {
         const char* buf = smem + (wave * kRing + slot) * kBlock;
         u32x4 codes[kT];
@@ -122,25 +126,25 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
         // through registers, two blocks ahead, and one place in LDS
         u32x4 held[2][kXfers];
         auto part = [&](int it, int n, const char*& at) __attribute__((always_inline)) {
-            const int64_t k0 = (int64_t)(it * kWaves + wave) * 64;
-            const int left = (int)min(p.depth - k0, (int64_t)64);
+            const int64_t k0 = (int64_t)(it * kWaves + wave) * kDepth;
+            const int left = (int)min(p.depth - k0, (int64_t)kDepth);
             if (n < kIXfers) {
-                at = (const char*)p.ip + (i0 + 8 * n + row8) * ldi_b + k0 * 2 + 16 * chunk8[n & 1];
-                return 8 * n + row8 < i_rows ? left - 8 * chunk8[n & 1] : 0;
+                at = (const char*)p.ip + (i0 + 8 * n + row8) * ldi_b + k0 * kElem + 16 * chunk8[n & 1];
+                return 8 * n + row8 < i_rows ? left - kChunk * chunk8[n & 1] : 0;
             }
             n -= kIXfers;
             const bool gate = gate_of(n);
             const int row = j_row(n);
             const int chunk = kJFp8 ? chunk16 : chunk8[n & 1];
-            at = (const char*)p.jp + ((kGated ? (gate ? gate_row : value_row) : 0) + j0 + row) * ldj_b + k0 * (kJFp8 ? 1 : 2) + 16 * chunk;
-            return row < j_rows ? left - (kJFp8 ? 16 : 8) * chunk : 0;
+            at = (const char*)p.jp + ((kGated ? (gate ? gate_row : value_row) : 0) + j0 + row) * ldj_b + k0 * (kJFp8 ? 1 : kElem) + 16 * chunk;
+            return row < j_rows ? left - (kJFp8 ? 16 : kChunk) * chunk : 0;
         };
         auto fetch = [&](int it, u32x4 (&to)[kXfers]) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < kXfers; ++n) {
                 const char* at;
                 const int valid = it < mine ? part(it, n, at) : 0;
-                to[n] = kJFp8 && n >= kIXfers ? fetch_chunk<16>(at, valid) : fetch_chunk<8>(at, valid);
+                to[n] = kJFp8 && n >= kIXfers ? fetch_chunk<16>(at, valid) : fetch_chunk<kChunk>(at, valid);
             }
         };
         auto turn = [&](int it, u32x4 (&from)[kXfers]) __attribute__((always_inline)) {
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
             for (int n = 0; n < kXfers; ++n) {
                 const char* at;
                 const int valid = part(it, n, at);
-                *(lds_u32x4*)(buf + n * 1024) = kJFp8 && n >= kIXfers ? settle_chunk<16>(from[n], valid) : settle_chunk<8>(from[n], valid);
+                *(lds_u32x4*)(buf + n * 1024) = kJFp8 && n >= kIXfers ? settle_chunk<16>(from[n], valid) : settle_chunk<kChunk>(from[n], valid);
             }
             fetch(it + 2, from);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -181,23 +185,25 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     constexpr int kGroups = kT * kT * 4;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-        const f32x16& v = acc[g / 4 / kT][g / 4 % kT];
-        *(lds_f32x4*)(smem + ((wave * kGroups + g) * 64 + lane) * 16) =
-            f32x4{v[4 * (g & 3)], v[4 * (g & 3) + 1], v[4 * (g & 3) + 2], v[4 * (g & 3) + 3]};
+        const Acc& v = acc[g / 4 / kT][g / 4 % kT];
+        *(lds_acc4*)(smem + ((wave * kGroups + g) * 64 + lane) * 16) =
+            Acc4{v[4 * (g & 3)], v[4 * (g & 3) + 1], v[4 * (g & 3) + 2], v[4 * (g & 3) + 3]};
     }
     __syncthreads();
 
     const FfAct act = ff_act(p.activation);
     const FfFamily fam = ff_family(p.activation);
     auto sum_of = [&](int g) {
-        f32x4 s{};
+        Acc4 s{};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) s += *(const lds_f32x4*)(smem + ((w * kGroups + g) * 64 + lane) * 16);
+        for (int w = 0; w < kWaves; ++w) s += *(const lds_acc4*)(smem + ((w * kGroups + g) * 64 + lane) * 16);
         return s;
     };
+    float row_scale = 1.0f;  // 8-bit integers: of the lane's row
     auto z_of = [&](float sum, int64_t j) {
+        if constexpr (F::kI8) sum *= row_scale;
         if (p.j_scale != nullptr) sum *= p.j_scale[j];
-        if (p.bias != nullptr) sum += (float)((const T*)p.bias)[j];
+        if (p.bias != nullptr) sum += (float)((const Out*)p.bias)[j];
         return sum;
     };
     // groups of 4 columns by waves (gated: a tile's first two, with the gates of its last two)
@@ -205,27 +211,28 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
     for (int own = wave; own < kT * kT * kOwn; own += kWaves) {
         const int tile = own / kOwn, u = own % kOwn;
         const int64_t i = i0 + 32 * (tile % kT) + col, c = j0 + (kGated ? 16 : 32) * (tile / kT) + 8 * u + 4 * hf;
-        const f32x4 a = sum_of(4 * tile + u);
-        f32x4 b{};
+        const Acc4 a = sum_of(4 * tile + u);
+        Acc4 b{};
         if constexpr (kGated) b = sum_of(4 * tile + u + 2);
         if (i >= p.rows) continue;
+        if constexpr (F::kI8) row_scale = p.i_scale[i];
         if constexpr (kDz) {
-            const T* dout = (const T*)p.dout + i * p.ld_dout;
-            T* out = (T*)p.out + i * p.ld_out;
+            const Out* dout = (const Out*)p.dout + i * p.ld_dout;
+            Out* out = (Out*)p.out + i * p.ld_out;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if (c + q >= p.cols) continue;
                 const float d = (float)dout[c + q];
                 float value;
                 if constexpr (kGated) {
-                    const float s = ff_slope_of(act, fam, z_of(b[q], gate_row + c + q), value);
-                    out[value_row + c + q] = (T)(d * value);
-                    out[gate_row + c + q] = (T)(d * z_of(a[q], value_row + c + q) * s);
+                    const float s = ff_slope_of(act, fam, z_of((float)b[q], gate_row + c + q), value);
+                    out[value_row + c + q] = (Out)(d * value);
+                    out[gate_row + c + q] = (Out)(d * z_of((float)a[q], value_row + c + q) * s);
                 } else {
-                    out[c + q] = (T)(ff_slope_of(act, fam, z_of(a[q], c + q), value) * d);
+                    out[c + q] = (Out)(ff_slope_of(act, fam, z_of((float)a[q], c + q), value) * d);
                 }
                 if (c + q == p.cols - 1)  // up to the padded row
-                    for (int64_t z = kGated ? 2 * p.cols : p.cols; z < p.out_cols_padded; ++z) out[z] = (T)0.0f;
+                    for (int64_t z = kGated ? 2 * p.cols : p.cols; z < p.out_cols_padded; ++z) out[z] = (Out)0.0f;
             }
         } else {
             float v[4];
@@ -233,16 +240,16 @@ __global__ __launch_bounds__(64 * kWaves) void ff_deep_kernel(FfParams p) {
             for (int q = 0; q < 4; ++q) {
                 v[q] = 0.0f;
                 if (c + q >= p.cols) continue;
-                if constexpr (kGated) v[q] = z_of(a[q], value_row + c + q) * ff_value_of(act, fam, z_of(b[q], gate_row + c + q));
-                else v[q] = ff_value_of(act, fam, z_of(a[q], c + q)) + (p.residual != nullptr ? (float)((const T*)p.residual)[i * p.ld_res + c + q] : 0.0f);
+                if constexpr (kGated) v[q] = z_of((float)a[q], value_row + c + q) * ff_value_of(act, fam, z_of((float)b[q], gate_row + c + q));
+                else v[q] = ff_value_of(act, fam, z_of((float)a[q], c + q)) + (p.residual != nullptr ? (float)((const Out*)p.residual)[i * p.ld_res + c + q] : 0.0f);
             }
-            T* out = (T*)p.out + i * p.ld_out + c;
+            Out* out = (Out*)p.out + i * p.ld_out + c;
             if (p.vec && c < p.cols) {
                 *(u32x2*)out = u32x2{F::pack(v[0], v[1]), F::pack(v[2], v[3])};
             } else {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (c + q < p.cols) out[q] = (T)v[q];
+                    if (c + q < p.cols) out[q] = (Out)v[q];
             }
         }
     }
@@ -258,7 +265,7 @@ hipError_t launch(FfParams p, FfEpilogue epilogue, hipStream_t stream) {
         hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kSide, kWaves, kFfGated, kStaged>), grid, block, 0, stream, p);
     } else if (epilogue == kFfLinear) {
         hipLaunchKernelGGL((ff_deep_kernel<T, kJFp8, kSide, kWaves, kFfLinear, kStaged>), grid, block, 0, stream, p);
-    } else if constexpr (!kJFp8) {
+    } else if constexpr (!kJFp8 && !FfType<T>::kI8) {
         if (epilogue == kFfGatedDz) hipLaunchKernelGGL((ff_deep_kernel<T, false, kSide, kWaves, kFfGatedDz, kStaged>), grid, block, 0, stream, p);
         else hipLaunchKernelGGL((ff_deep_kernel<T, false, kSide, kWaves, kFfLinearDz, kStaged>), grid, block, 0, stream, p);
     }
@@ -267,6 +274,14 @@ hipError_t launch(FfParams p, FfEpilogue epilogue, hipStream_t stream) {
 
 template <typename T, bool kStaged>
 hipError_t launch_type(const FfParams& p, FfEpilogue epilogue, bool j_fp8, FfDeepId id, hipStream_t stream) {
+    if (p.i8 != 0) {
+        switch (id) {
+        case kFfDeep32x8: return launch<I8<T>, false, 32, 8, kStaged>(p, epilogue, stream);
+        case kFfDeep32x4: return launch<I8<T>, false, 32, 4, kStaged>(p, epilogue, stream);
+        case kFfDeep64x4: return launch<I8<T>, false, 64, 4, kStaged>(p, epilogue, stream);
+        }
+        return hipErrorInvalidValue;
+    }
     switch (id) {
     case kFfDeep32x8: return j_fp8 ? launch<T, true, 32, 8, kStaged>(p, epilogue, stream) : launch<T, false, 32, 8, kStaged>(p, epilogue, stream);
     case kFfDeep32x4: return j_fp8 ? launch<T, true, 32, 4, kStaged>(p, epilogue, stream) : launch<T, false, 32, 4, kStaged>(p, epilogue, stream);

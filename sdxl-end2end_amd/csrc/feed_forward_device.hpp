@@ -15,10 +15,23 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// What a product's operands hold and what its sums are, beside T, the type of bias, residual, dout and out.
+// kElem: bytes of an operand's element.
+struct FfHalfSums {
+    typedef f32x16 Acc;
+    typedef f32x4 Acc4;
+    static constexpr int kElem = 2;
+    static constexpr bool kI8 = false;
+};
+
 template <typename T>
 struct FfType;
 template <>
-struct FfType<_Float16> {
+struct FfType<_Float16> : FfHalfSums {
+    typedef _Float16 Out;
     static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) { return mfma32(a, b, c); }
     // two values rounded to nearest even
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -35,7 +48,8 @@ struct FfType<_Float16> {
     static __device__ __forceinline__ uint2 decode(uint32_t codes) { return e4m3x4_to_f16(codes); }
 };
 template <>
-struct FfType<__bf16> {
+struct FfType<__bf16> : FfHalfSums {
+    typedef __bf16 Out;
     static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
@@ -57,11 +71,22 @@ struct FfType<__bf16> {
 };
 
 // 8-bit integers, 16 consecutive bytes of depth a lane: 32 x 32 x 32, exact 32-bit sums
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ i32x16 mfma32_i8(i16x8 a, i16x8 b, i32x16 c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
+
+// Both operands of 8-bit integers, the rest of type T. A 16-byte chunk has twice the elements of a 16-bit type's and its
+// matrix instruction twice the depth, so that the kernels' layouts, counted in bytes, stay the same.
+template <typename T>
+struct I8;
+template <typename T>
+struct FfType<I8<T>> : FfType<T> {
+    typedef i32x16 Acc;
+    typedef i32x4 Acc4;
+    static constexpr int kElem = 1;
+    static constexpr bool kI8 = true;
+    static __device__ __forceinline__ i32x16 mfma(i16x8 a, i16x8 b, i32x16 c) { return mfma32_i8(a, b, c); }
+};
 
 // 16 bytes at any element's address
 template <int kAlign>

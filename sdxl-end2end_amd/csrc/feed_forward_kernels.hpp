@@ -58,6 +58,9 @@ struct FfJoin {
     int32_t rows, cols, ld, splits, vec, blocks;
 };
 
+// The depth in the kernels' stages of 128 bytes.
+inline int64_t ff_stages(const FfParams& p) { return p.i8 != 0 ? (p.depth + 127) / 128 : (p.depth + 63) / 64; }
+
 // The general kernel: any size, stride and alignment.
 hipError_t launch_ff_general(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool bf16,
                              bool j_fp8, hipStream_t stream);

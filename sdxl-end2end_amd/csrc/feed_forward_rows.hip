@@ -23,11 +23,11 @@
 namespace sdxl_hip {
 namespace {
 
-typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-
-template <typename T>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (__is_same(T, _Float16))
+template <typename T, typename Acc4>
+__device__ __forceinline__ Acc4 mfma16(u32x4 a, u32x4 b, Acc4 c) {
+    if constexpr (FfType<T>::kI8)
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+    else if constexpr (__is_same(T, _Float16))
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -36,18 +36,22 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 template <typename T, bool kJFp8, int kWaves, bool kGated, bool kStaged>
 __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
     using F = FfType<T>;
+    using Out = typename F::Out;
+    using Acc4 = typename F::Acc4;
+    typedef __attribute__((address_space(3))) Acc4 lds_acc4;
     constexpr int kBlocks = 32 / kWaves;  // of a wave at a time
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // [kBlocks][kWaves] of kBlockBytes; then the sums
-    constexpr int kBlockBytes = kJFp8 ? 1024 : 2048, kElem = kJFp8 ? 1 : 2;
+    constexpr int kBlockBytes = kJFp8 ? 1024 : 2048, kElem = kJFp8 ? 1 : F::kElem;  // w's
+    constexpr int kXElem = F::kElem, kDepth = 128 / kXElem, kChunk = 16 / kXElem;     // elements of a block, of 16 bytes of x
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     constexpr int kCols = kGated ? 8 : 16;
     const int64_t c0 = (int64_t)blockIdx.x * kCols;
     const int64_t value_row = p.gate_first ? p.cols : 0, gate_row = p.gate_first ? 0 : p.cols;
-    const int depth = (int)p.depth, blocks = (depth + 63) / 64;
+    const int depth = (int)p.depth, blocks = (depth + kDepth - 1) / kDepth;
     const u32x4 w_rsrc = window_rsrc({(const char*)p.jp, (uint32_t)((((kGated ? 2 : 1) * p.cols - 1) * p.ld_j + p.depth) * kElem)});
-    const u32x4 x_win = window_rsrc({(const char*)p.ip, (uint32_t)(((p.rows - 1) * p.ld_i + p.depth) * 2)});
+    const u32x4 x_win = window_rsrc({(const char*)p.ip, (uint32_t)(((p.rows - 1) * p.ld_i + p.depth) * kXElem)});
     const auto x_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p.ip, 0, (int)x_win[2], 0x00020000);
 
     // the lane's row in a transfer (rows past the last one: outside), its chunk of 16 bytes
@@ -59,34 +63,34 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
     const int row = kJFp8 ? lane >> 2 : lane >> 3;
     const uint32_t w_at[2] = {w_offset(row), kJFp8 ? 0u : w_offset(8 + row)};
     const int chunk_at[2] = {kJFp8 ? (lane & 3) ^ ((row >> 2) & 3) : (lane & 7) ^ swz(row), (lane & 7) ^ swz(8 + row)};
-    const uint32_t x_at = r16 < p.rows ? (uint32_t)(r16 * p.ld_i * 2) : kOutside;
+    const uint32_t x_at = r16 < p.rows ? (uint32_t)(r16 * p.ld_i * kXElem) : kOutside;
 
     const uint32_t lds0 = lds_addr(smem);
     u32x4 x[kBlocks][2];
-    f32x4 acc{};
+    Acc4 acc{};
     for (int first = 0; first < blocks; first += 32) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of the blocks' place are done
         if constexpr (kStaged) {
             // through registers: all reads first
-            constexpr int kAll = kJFp8 ? 16 : 8, kH = kJFp8 ? 1 : 2;
+            constexpr int kAll = kJFp8 ? 16 : kChunk, kH = kJFp8 ? 1 : 2;
             u32x4 held[kBlocks][kH];
-            auto x_valid = [&](int block, int q) { return r16 < p.rows ? depth - (64 * block + 32 * q + 8 * g) : 0; };
-            auto w_valid = [&](int block, int h) { return w_at[h] != kOutside ? depth - 64 * block - kAll * chunk_at[h] : 0; };
+            auto x_valid = [&](int block, int q) { return r16 < p.rows ? depth - (kDepth * block + kChunk * (4 * q + g)) : 0; };
+            auto w_valid = [&](int block, int h) { return w_at[h] != kOutside ? depth - kDepth * block - kAll * chunk_at[h] : 0; };
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const int block = first + b * kWaves + wave;
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
-                    x[b][q] = fetch_chunk<8>((const char*)p.ip + (r16 * p.ld_i + 64 * block + 32 * q + 8 * g) * 2, x_valid(block, q));
+                    x[b][q] = fetch_chunk<kChunk>((const char*)p.ip + (r16 * p.ld_i + kDepth * block + kChunk * (4 * q + g)) * kXElem, x_valid(block, q));
 #pragma unroll
                 for (int h = 0; h < kH; ++h)
-                    held[b][h] = fetch_chunk<kAll>((const char*)p.jp + w_at[h] + (int64_t)(64 * block + kAll * chunk_at[h]) * kElem, w_valid(block, h));
+                    held[b][h] = fetch_chunk<kAll>((const char*)p.jp + w_at[h] + (int64_t)(kDepth * block + kAll * chunk_at[h]) * kElem, w_valid(block, h));
             }
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const int block = first + b * kWaves + wave;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) x[b][q] = settle_chunk<8>(x[b][q], x_valid(block, q));
+                for (int q = 0; q < 2; ++q) x[b][q] = settle_chunk<kChunk>(x[b][q], x_valid(block, q));
                 if (block < blocks) {  // (LDS holds no others)
 #pragma unroll
                     for (int h = 0; h < kH; ++h)
@@ -101,8 +105,8 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
                 if (block < blocks) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        const int k = 64 * block + 32 * q + 8 * g;
-                        x[b][q] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, k < depth && x_at != kOutside ? x_at + 2 * k : kOutside, 0, 0);
+                        const int k = kDepth * block + kChunk * (4 * q + g);
+                        x[b][q] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, k < depth && x_at != kOutside ? x_at + kXElem * k : kOutside, 0, 0);
                     }
                 }
             }
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
                 if (block < blocks) {
 #pragma unroll
                     for (int h = 0; h < (kJFp8 ? 1 : 2); ++h) {
-                        const int k = 64 * block + (kJFp8 ? 16 : 8) * chunk_at[h];
+                        const int k = kDepth * block + (kJFp8 ? 16 : kChunk) * chunk_at[h];
                         window_to_lds(w_rsrc, k < depth && w_at[h] != kOutside ? w_at[h] + kElem * k : kOutside,
                                       lds0 + (b * kWaves + wave) * kBlockBytes + 1024 * h);
                     }
@@ -142,39 +146,41 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
         }
     }
     __syncthreads();  // the sums take the blocks' place
-    *(lds_f32x4*)(smem + (wave * 64 + lane) * 16) = acc;
+    *(lds_acc4*)(smem + (wave * 64 + lane) * 16) = acc;
     __syncthreads();
 
     // acc[e] of lane l: column (w row) 4 (l / 16) + e, row l % 16
     const FfAct act = ff_act(p.activation);
     const FfFamily fam = ff_family(p.activation);
     auto sum_of = [&](int from) {
-        f32x4 s{};
-        for (int v = 0; v < kWaves; ++v) s += *(const lds_f32x4*)(smem + (v * 64 + from) * 16);
+        Acc4 s{};
+        for (int v = 0; v < kWaves; ++v) s += *(const lds_acc4*)(smem + (v * 64 + from) * 16);
         return s;
     };
+    const float row_scale = F::kI8 && r16 < p.rows ? p.i_scale[r16] : 1.0f;
     auto z_of = [&](float sum, int64_t row) {
+        if constexpr (F::kI8) sum *= row_scale;
         if (p.j_scale != nullptr) sum *= p.j_scale[row];
-        if (p.bias != nullptr) sum += (float)((const T*)p.bias)[row];
+        if (p.bias != nullptr) sum += (float)((const Out*)p.bias)[row];
         return sum;
     };
     if (threadIdx.x < (kGated ? 32 : 64)) {
         const int64_t i = r16;
         if (i >= p.rows) return;
-        const f32x4 a = sum_of(lane);
-        f32x4 b{};
+        const Acc4 a = sum_of(lane);
+        Acc4 b{};
         if constexpr (kGated) b = sum_of(lane + 32);
-        T* out = (T*)p.out + i * p.ld_out;
+        Out* out = (Out*)p.out + i * p.ld_out;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int64_t n = c0 + 4 * g + e;
             if (n >= p.cols) continue;
             if constexpr (kGated) {
-                out[n] = (T)(z_of(a[e], value_row + n) * ff_value_of(act, fam, z_of(b[e], gate_row + n)));
+                out[n] = (Out)(z_of((float)a[e], value_row + n) * ff_value_of(act, fam, z_of((float)b[e], gate_row + n)));
             } else {
-                float v = ff_value_of(act, fam, z_of(a[e], n));
-                if (p.residual != nullptr) v += (float)((const T*)p.residual)[i * p.ld_res + n];
-                out[n] = (T)v;
+                float v = ff_value_of(act, fam, z_of((float)a[e], n));
+                if (p.residual != nullptr) v += (float)((const Out*)p.residual)[i * p.ld_res + n];
+                out[n] = (Out)v;
             }
         }
     }
@@ -183,7 +189,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
 template <typename T, bool kJFp8, int kWaves, bool kStaged>
 hipError_t launch(const FfParams& p, bool gated, hipStream_t stream) {
     const dim3 grid((unsigned)(gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16)), block(64 * kWaves);
-    const int64_t blocks = (p.depth + 63) / 64, held = blocks < 32 ? (blocks + kWaves - 1) / kWaves * kWaves : 32;
+    const int64_t blocks = (p.depth + 128 / FfType<T>::kElem - 1) / (128 / FfType<T>::kElem), held = blocks < 32 ? (blocks + kWaves - 1) / kWaves * kWaves : 32;
     const size_t lds = (size_t)held * (kJFp8 ? 1024 : 2048);  // (the sums take 1 KiB a wave)
     if (gated) hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, true, kStaged>), grid, block, lds, stream, p);
     else hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, false, kStaged>), grid, block, lds, stream, p);
@@ -206,12 +212,12 @@ bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8) {
     // one window (below 2^31 bytes) holds w, one x
     const int64_t w_rows = epilogue == kFfGated ? 2 * p.cols : p.cols;
     return (epilogue == kFfLinear || epilogue == kFfGated) && p.rows <= 16 &&
-           w_rows * p.ld_j * (j_fp8 ? 1 : 2) < (int64_t{1} << 31) && ff_staged_supported(p, epilogue, false, false, j_fp8);
+           w_rows * p.ld_j * (j_fp8 || p.i8 != 0 ? 1 : 2) < (int64_t{1} << 31) && ff_staged_supported(p, epilogue, false, false, j_fp8);
 }
 
 // 2048 waves in all where there are blocks for them
 int ff_rows_waves(const FfParams& p, bool gated) {
-    const int64_t groups = gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16, blocks = (p.depth + 63) / 64;
+    const int64_t groups = gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16, blocks = ff_stages(p);
     return groups * 8 < 2048 && blocks > 8 ? 16 : groups * 4 < 2048 && blocks > 4 ? 8 : 4;
 }
 
@@ -219,6 +225,7 @@ hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, int waves, boo
                           hipStream_t stream) {
     const bool gated = epilogue == kFfGated;
     auto by_type = [&]<typename T>() {
+        if (p.i8 != 0) return staged ? launch_rows<I8<T>, false, true>(p, gated, waves, stream) : launch_rows<I8<T>, false, false>(p, gated, waves, stream);
         if (staged) return j_fp8 ? launch_rows<T, true, true>(p, gated, waves, stream) : launch_rows<T, false, true>(p, gated, waves, stream);
         return j_fp8 ? launch_rows<T, true, false>(p, gated, waves, stream) : launch_rows<T, false, false>(p, gated, waves, stream);
     };

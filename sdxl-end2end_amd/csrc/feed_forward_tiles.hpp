@@ -53,7 +53,6 @@ namespace sdxl_hip {
 namespace {
 
 typedef __attribute__((address_space(3))) i16x8 lds_op;
-typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 typedef __attribute__((address_space(3))) float lds_float;
 
 __device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
@@ -91,6 +90,11 @@ template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue 
 __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* smem) {
     constexpr int kWI = Tile::kWI, kWJ = Tile::kWJ, kWK = Tile::kWK, kMI = Tile::kMI, kMJ = Tile::kMJ, kRing = Tile::kRing;
     using F = FfType<T>;
+    using Out = typename F::Out;
+    using Acc = typename F::Acc;
+    using Acc4 = typename F::Acc4;
+    typedef __attribute__((address_space(3))) Acc4 lds_acc4;
+    constexpr int kElem = F::kElem, kDepth = 128 / kElem, kChunk = 16 / kElem;  // elements of a stage, of 16 bytes
     constexpr bool kGated = kEpi == kFfGated || kEpi == kFfGatedDz;
     constexpr int kWaves = Tile::kWaves, kBI = Tile::kBI, kBJ = Tile::kBJ;
     constexpr int kCols = kGated ? kBJ / 2 : kBJ;  // columns of C per tile
@@ -108,20 +112,21 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     static_assert(kWK == 1 || (kWK == 2 && !kJFp8), "depth shares");
     static_assert(!kGated || (!kIT && !kJT), "gated products are projections");
     static_assert(!kJFp8 || !kJT, "E4M3: by rows");
+    static_assert(!F::kI8 || (!kIT && !kJT && !kJFp8 && !kSplit && (kEpi == kFfLinear || kEpi == kFfGated)), "8-bit integers: projections");
     static_assert(Tile::smem_bytes(kJFp8) <= 160 * 1024, "LDS of one CU");
 
     const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave % kWI, wj = wave / kWI % kWJ, wk = kWK > 1 ? wave / (kWI * kWJ) : 0;
     const int64_t value_row = p.gate_first ? p.cols : 0, gate_row = p.gate_first ? 0 : p.cols;
-    const int64_t ldi_b = p.ld_i * 2, ldj_b = p.ld_j * (kJFp8 ? 1 : 2);
+    const int64_t ldi_b = p.ld_i * kElem, ldj_b = p.ld_j * (kJFp8 ? 1 : kElem);
     // the workgroup's share of the depth: from depth0 on
     static_assert(!kSplit || kEpi == kFfStore, "shares are joined before an epilogue");
     const int n_tiles = p.i_blocks * p.j_blocks, share = kSplit ? task_id / n_tiles : 0, id = kSplit ? task_id % n_tiles : task_id;
-    const int64_t depth0 = kSplit ? (int64_t)share * p.share_stages * 64 : 0;
-    const int64_t depth = kSplit ? min64(p.depth - depth0, (int64_t)p.share_stages * 64) : p.depth;
+    const int64_t depth0 = kSplit ? (int64_t)share * p.share_stages * kDepth : 0;
+    const int64_t depth = kSplit ? min64(p.depth - depth0, (int64_t)p.share_stages * kDepth) : p.depth;
     const int64_t i_row = kIT ? p.i_row : p.i_row - depth0;  // (by columns the row runs along C)
-    const int n_stages = (int)((depth + 63) / 64);
+    const int n_stages = (int)((depth + kDepth - 1) / kDepth);
 
     // ---- task: each XCD takes one contiguous range of them, in groups of
     // group_i row blocks (rows fastest, then columns), so that its workgroups
@@ -150,27 +155,27 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         iw.base = (const char*)p.ip + i0 * 2 + depth0 * ldi_b;
         i_lane = (uint32_t)(row8 * ldi_b) + chunk8 * 16;
     } else {
-        iw.base = (const char*)p.ip + i0 * ldi_b + depth0 * 2;
+        iw.base = (const char*)p.ip + i0 * ldi_b + depth0 * kElem;
         i_lane = (uint32_t)(row8 * ldi_b) + chunk8 * 16;
     }
     const int64_t j_first = kGated ? j0 + ((kJFp8 ? wave & 1 : wave & 2) ? gate_row : value_row) : j0;
     if constexpr (kJT) jw.base = (const char*)p.jp + j0 * 2 + depth0 * ldj_b;
-    else jw.base = (const char*)p.jp + j_first * ldj_b + depth0 * (kJFp8 ? 1 : 2);
+    else jw.base = (const char*)p.jp + j_first * ldj_b + depth0 * (kJFp8 ? 1 : kElem);
     j_lane = kJFp8 ? (uint32_t)(row16 * ldj_b) + chunk16 * 16 : (uint32_t)(row8 * ldj_b) + chunk8 * 16;
     const int64_t i_rows = min64(p.rows - i0, kBI), j_rows = min64(p.cols - j0, kGated ? kCols : kBJ);
     // window of stage st: everything from its first byte to the last valid one
     // (past the last stage: nothing, its transfers write zeros that nobody reads)
     auto i_window = [&](int st) __attribute__((always_inline)) {
-        const int64_t left = depth - (int64_t)st * 64;
+        const int64_t left = depth - (int64_t)st * kDepth;
         const char* base = iw.base + (kIT ? (int64_t)st * 64 * ldi_b : (int64_t)st * 128);
         const int64_t size = kIT ? (min64(left, 64) - 1) * ldi_b + min64(i_row - i0, kBI) * 2
-                                 : (i_rows - 1) * ldi_b + (i_row - (int64_t)st * 64) * 2;
+                                 : (i_rows - 1) * ldi_b + (i_row - (int64_t)st * kDepth) * kElem;
         return window_rsrc({base, left > 0 ? (uint32_t)size : 0u});
     };
     auto j_window = [&](int st) __attribute__((always_inline)) {
-        const int64_t left = depth - (int64_t)st * 64;
+        const int64_t left = depth - (int64_t)st * kDepth;
         const char* base = jw.base + (kJT ? (int64_t)st * 64 * ldj_b : (int64_t)st * (kJFp8 ? 64 : 128));
-        const int64_t size = kJT ? (min64(left, 64) - 1) * ldj_b + j_rows * 2 : (j_rows - 1) * ldj_b + left * (kJFp8 ? 1 : 2);
+        const int64_t size = kJT ? (min64(left, 64) - 1) * ldj_b + j_rows * 2 : (j_rows - 1) * ldj_b + left * (kJFp8 ? 1 : kElem);
         return window_rsrc({base, left > 0 ? (uint32_t)size : 0u});
     };
     const uint32_t lds0 = lds_addr(smem);
@@ -181,8 +186,8 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     u32x4 held[kStaged ? kXfers : 1];
     // part x of stage st: its address, and how many of the chunk's elements its row has (none: 0 or less)
     auto part = [&](int st, int x, const char*& from) __attribute__((always_inline)) {
-        const int64_t d_left = depth - (int64_t)st * 64;
-        const int left = (int)min64(d_left, 64);
+        const int64_t d_left = depth - (int64_t)st * kDepth;
+        const int left = (int)min64(d_left, kDepth);
         int64_t off;
         int valid;
         if (x < kIX) {
@@ -192,7 +197,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                 valid = 8 * (n & 7) + row8 < left ? (int)min64(i_row - i0, kBI) - 64 * (n >> 3) - 8 * chunk8 : 0;
             } else {
                 off = (int64_t)st * 128 + (int64_t)(8 * n) * ldi_b + i_lane;
-                valid = 8 * n + row8 < i_rows ? (int)min64(i_row - (int64_t)st * 64, 64) - 8 * chunk8 : 0;
+                valid = 8 * n + row8 < i_rows ? (int)min64(i_row - (int64_t)st * kDepth, kDepth) - kChunk * chunk8 : 0;
             }
             from = iw.base + off;
         } else {
@@ -203,16 +208,16 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
             } else {
                 const int first = kJFp8 ? 16 * (kGated ? n >> 1 : n) : kGated ? 16 * (n >> 2) + 8 * (n & 1) : 8 * n;
                 off = (int64_t)st * (kJFp8 ? 64 : 128) + (int64_t)first * ldj_b + j_lane;
-                valid = first + (kJFp8 ? row16 : row8) < j_rows ? left - (kJFp8 ? 16 * chunk16 : 8 * chunk8) : 0;
+                valid = first + (kJFp8 ? row16 : row8) < j_rows ? left - (kJFp8 ? 16 * chunk16 : kChunk * chunk8) : 0;
             }
             from = jw.base + off;
         }
         return valid;
     };
     const bool inner_tile = i_rows == kBI && j_rows == (kGated ? kCols : kBJ) && (!kIT || i_row - i0 >= kBI);
-    auto whole = [&](int st) __attribute__((always_inline)) { return inner_tile && depth - (int64_t)st * 64 >= 64; };
+    auto whole = [&](int st) __attribute__((always_inline)) { return inner_tile && depth - (int64_t)st * kDepth >= kDepth; };
     auto read16 = [&](int x, const char* from) __attribute__((always_inline)) {
-        return kJFp8 && x >= kIX ? ((const Unaligned<1>*)from)->v : ((const Unaligned<2>*)from)->v;
+        return kJFp8 && x >= kIX ? ((const Unaligned<1>*)from)->v : ((const Unaligned<kElem>*)from)->v;
     };
     auto fetch = [&](int st) __attribute__((always_inline)) {
         const char* from;
@@ -226,7 +231,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
 #pragma unroll
             for (int x = 0; x < kXfers; ++x) {
                 const int valid = part(st, x, from);
-                held[x] = kJFp8 && x >= kIX ? fetch_chunk<16>(from, valid) : fetch_chunk<8>(from, valid);
+                held[x] = kJFp8 && x >= kIX ? fetch_chunk<16>(from, valid) : fetch_chunk<kChunk>(from, valid);
             }
         }
     };
@@ -237,7 +242,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
             for (int x = 0; x < kXfers; ++x) {
                 const char* from;
                 const int valid = part(st, x, from);
-                held[x] = kJFp8 && x >= kIX ? settle_chunk<16>(held[x], valid) : settle_chunk<8>(held[x], valid);
+                held[x] = kJFp8 && x >= kIX ? settle_chunk<16>(held[x], valid) : settle_chunk<kChunk>(held[x], valid);
             }
         }
 #pragma unroll
@@ -248,7 +253,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     auto issue = [&](int st, int buffer, int x, u32x4 irsrc, u32x4 jrsrc) __attribute__((always_inline)) {
         const uint32_t buf = lds0 + buffer * kStage;
         // depth of the stage, by I's rows and by J's
-        const int i_left = (int)min64(i_row - (int64_t)st * 64, 64), left = (int)min64(depth - (int64_t)st * 64, 64);
+        const int i_left = (int)min64(i_row - (int64_t)st * kDepth, kDepth), left = (int)min64(depth - (int64_t)st * kDepth, kDepth);
         if (x < kIX) {
             const int n = x * kWaves + wave;
             if (kIXfers % kWaves != 0 && n >= kIXfers) return;
@@ -257,7 +262,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                 off = (uint32_t)((8 * (n & 7)) * ldi_b) + (n >> 3) * 128 + i_lane;
             } else {
                 off = (uint32_t)(8 * n * ldi_b) + i_lane;
-                if (8 * chunk8 >= i_left) off = kOutside;
+                if (kChunk * chunk8 >= i_left) off = kOutside;
             }
             window_to_lds(irsrc, off, buf + n * 1024);
         } else {
@@ -271,7 +276,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                 if (16 * chunk16 >= left) off = kOutside;
             } else {
                 off = (uint32_t)((kGated ? 16 * (n >> 2) + 8 * (n & 1) : 8 * n) * ldj_b) + j_lane;
-                if (8 * chunk8 >= left) off = kOutside;
+                if (kChunk * chunk8 >= left) off = kOutside;
             }
             window_to_lds(jrsrc, off, buf + kIBytes + n * 1024);
         }
@@ -338,13 +343,13 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         }
     };
 
-    f32x16 acc[kMJ][kMI];
+    Acc acc[kMJ][kMI];
 #pragma unroll
     for (int j = 0; j < kMJ; ++j)
 #pragma unroll
         for (int i = 0; i < kMI; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
+            for (int r = 0; r < 16; ++r) acc[j][i][r] = 0;
     float sums[kMI] = {};  // row sums of the I operand (dbias)
 
     // at most kFlying stages' transfers of the wave are still on their way, and no wave reads LDS any more
@@ -516,8 +521,11 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     // dz: zeros behind the last column, up to the padded row
     auto zero_pad = [&](uint32_t row, int64_t first) __attribute__((always_inline)) {
         if (j0 + kCols >= p.cols && wj == 0 && hf == 0 && (int64_t)row < i_rows)
-            for (int64_t z = first; z < p.out_cols_padded; ++z) ((T*)p.out)[(i0 + row) * p.ld_out + z] = (T)0.0f;
+            for (int64_t z = first; z < p.out_cols_padded; ++z) ((Out*)p.out)[(i0 + row) * p.ld_out + z] = (Out)0.0f;
     };
+    // (rows past the end: 0)
+    const auto row_scales = __builtin_amdgcn_make_buffer_rsrc((void*)((uintptr_t)p.i_scale + (uintptr_t)(i0 * 4)), 0,
+                                                              F::kI8 ? (int)(i_rows * 4) : 0, 0x00020000);
     const auto dout = rows_window(p.dout, p.ld_dout, j0), residual = rows_window(p.residual, p.ld_res, j0);
     const auto out = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? value_row : 0) + j0);
     const auto out_g = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? gate_row : 0) + j0);
@@ -575,7 +583,15 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         }
     };
     // one 32 x 32 tile of sums: the lane's row of C's tile, first column c0, what read_tile gave
-    auto finish = [&]<FfFamily kFam>(const f32x16& z, uint32_t row, int c0, const u32x4 (&in)[kSets]) __attribute__((always_inline)) {
+    auto finish = [&]<FfFamily kFam>(const Acc& tile_sums, uint32_t row, int c0, const u32x4 (&in)[kSets]) __attribute__((always_inline)) {
+        f32x16 z;
+        if constexpr (F::kI8) {  // with the row's scale
+            const float row_scale = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(row_scales, row * 4, 0, 0));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = (float)tile_sums[r] * row_scale;
+        } else {
+            z = tile_sums;
+        }
         if constexpr (kGated) {
             float va[2][4], vb[2][4], d[2][4];
             if constexpr (kEpi == kFfGatedDz) values16(in[0], d);
@@ -623,13 +639,13 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         }
     };
     // a share's sums, 4 columns a lane
-    auto store_share = [&](const f32x16& z, uint32_t row, int c0) __attribute__((always_inline)) {
+    auto store_share = [&](const Acc& z, uint32_t row, int c0) __attribute__((always_inline)) {
         const uint64_t b = (uint64_t)(uintptr_t)p.partial + (uint64_t)(((share * p.rows + i0) * p.ld_partial + j0) * 4);
         const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)b, 0, (int)((i_rows * p.ld_partial - j0) * 4), 0x00020000);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int c = c0 + 8 * u + 4 * hf;
-            const f32x4 v{z[4 * u], z[4 * u + 1], z[4 * u + 2], z[4 * u + 3]};
+            const Acc4 v{z[4 * u], z[4 * u + 1], z[4 * u + 2], z[4 * u + 3]};
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, c < cols ? (uint32_t)(row * p.ld_partial + c) * 4 : kOutside, 0, 0);
         }
     };
@@ -664,7 +680,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
 #pragma unroll
             for (int r = 0; r < (kTiles + kWK - 1) / kWK; ++r) {
                 land.template operator()<0>();  // the stage buffers, or the last round's sums, are free
-                f32x16 own{};
+                Acc own{};
 #pragma unroll
                 for (int o = 0; o < kWK; ++o) {
                     const int q = r * kWK + o;
@@ -674,7 +690,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            *(lds_f32x4*)(slot(o, wk) + e * 1024) = f32x4{acc[q / kMI][q % kMI][4 * e], acc[q / kMI][q % kMI][4 * e + 1],
+                            *(lds_acc4*)(slot(o, wk) + e * 1024) = Acc4{acc[q / kMI][q % kMI][4 * e], acc[q / kMI][q % kMI][4 * e + 1],
                                                                          acc[q / kMI][q % kMI][4 * e + 2], acc[q / kMI][q % kMI][4 * e + 3]};
                     }
                 }
@@ -682,14 +698,14 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                 __builtin_amdgcn_s_barrier();
                 const int q = r * kWK + wk;
                 if (q < kTiles) {
-                    f32x16 sum{};
+                    Acc sum{};
 #pragma unroll
                     for (int from = 0; from < kWK; ++from) {
-                        f32x16 part = own;
+                        Acc part = own;
                         if (from != wk) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const f32x4 v = *(const lds_f32x4*)(slot(wk, from) + e * 1024);
+                                const Acc4 v = *(const lds_acc4*)(slot(wk, from) + e * 1024);
 #pragma unroll
                                 for (int x = 0; x < 4; ++x) part[4 * e + x] = v[x];
                             }
@@ -744,7 +760,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     const float v = sums[s] + __shfl_xor(sums[s], 32);
                     if (hf == 0 && i < p.rows) {
                         if (kSplit && p.splits > 1) p.partial[(p.splits * p.ld_partial + share) * p.rows + i] = v;
-                        else ((T*)p.row_sums)[i] = (T)v;
+                        else ((Out*)p.row_sums)[i] = (Out)v;
                     }
                 }
             }
@@ -875,6 +891,26 @@ hipError_t ff_forward(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int ti
     return hipErrorInvalidValue;
 }
 
+// Projections of 8-bit integers, on tiles and through registers (below).
+template <typename T>
+hipError_t ff_i8_forward(const FfParams& p, FfEpilogue epilogue, int tile, hipStream_t stream) {
+    const bool gated = epilogue == kFfGated;
+    auto by_tile = [&]<typename Tile>() {
+        return gated ? ff_launch<I8<T>, false, false, false, Tile, kFfGated>(p, stream)
+                     : ff_launch<I8<T>, false, false, false, Tile, kFfLinear>(p, stream);
+    };
+    switch (tile) {
+    case kFf256x320: return by_tile.template operator()<FfTile256x320>();
+    case kFf256x256: return by_tile.template operator()<FfTile256x256>();
+    case kFf128x256: return by_tile.template operator()<FfTile128x256>();
+    case kFf128x192: return by_tile.template operator()<FfTile128x192>();
+    case kFf128x128: return by_tile.template operator()<FfTile128x128>();
+    case kFf64x128: return by_tile.template operator()<FfTile64x128>();
+    case kFf64x64: return by_tile.template operator()<FfTile64x64>();
+    }
+    return hipErrorInvalidValue;
+}
+
 template <typename T>
 hipError_t ff_backward(const FfParams& p, FfEpilogue epilogue, bool i_transposed, int tile, hipStream_t stream) {
     switch (tile) {
@@ -915,6 +951,16 @@ template <typename T>
 hipError_t ff_staged(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_fp8, bool large, hipStream_t stream) {
     return large ? ff_staged_tile<T, FfStaged128x128>(p, epilogue, i_transposed, j_fp8, stream)
                  : ff_staged_tile<T, FfStaged64x64>(p, epilogue, i_transposed, j_fp8, stream);
+}
+
+template <typename T>
+hipError_t ff_i8_staged(const FfParams& p, FfEpilogue epilogue, bool large, hipStream_t stream) {
+    const bool gated = epilogue == kFfGated;
+    auto by_tile = [&]<typename Tile>() {
+        return gated ? ff_launch_staged<I8<T>, false, false, false, Tile, kFfGated>(p, stream)
+                     : ff_launch_staged<I8<T>, false, false, false, Tile, kFfLinear>(p, stream);
+    };
+    return large ? by_tile.template operator()<FfStaged128x128>() : by_tile.template operator()<FfStaged64x64>();
 }
 
 }  // namespace
