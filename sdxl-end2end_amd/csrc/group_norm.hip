@@ -1,25 +1,656 @@
-// Which kernels a group norm call runs on (include/sdxl_hip/group_norm.h).
+// Group norm and its gradients (include/sdxl_hip/group_norm.h), for gfx950
+// (MI355X, CDNA4).
+//
+// Bound by the tensor's bytes. Two launches a direction: the first one reads x
+// (and dy) and leaves sums by chunk of pixels, the second one reads them again,
+// out of the Infinity Cache where they fit it, and writes y (dx). A thread keeps
+// to 16 bytes of channels (8 of a 16-bit type, 4 fp32 values) and goes down the
+// pixels, so that a channel's constants and sums stay in registers and groups of
+// any width (10, 20, 30 channels) cost nothing. A row's last 16 bytes may overlap
+// the ones before them (any channel count from a vector up); what is there twice
+// counts once.
+//
+// A workgroup owns a slab of whole groups, 512 bytes of every row or a little
+// more, and a chunk of pixels: with full rows instead it would take as many
+// chunks as workgroups, whose parts every workgroup of the second pass has to
+// merge ([2, 4096, 960] fp16: 66 us, of which 256 chunks' parts were most).
+//
+// Statistics: a thread sums x - p and (x - p)^2 with p its own first value of the
+// channel, which gives its mean and sum of squares about it; these are merged in
+// the same way about one of the means, M = sum M_i + n_i d_i^2 - (sum n_i d_i)^2 /
+// n with d_i = mean_i - mean_0, first the workgroup's threads in LDS, then the
+// chunks. The value that sums are taken about is one of the n that they are made
+// of, so that its distance from the mean is at most sqrt(M) and the subtraction
+// costs M at most a relative n 2^-24, whatever the mean.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "group_norm_device.hpp"
+#include "int8_device.hpp"
 
 namespace sdxl_hip {
+namespace {
 
-GnPlan gn_plan(const GnParams& p, GnType, bool) { return {false, 1, p.pixels}; }
+constexpr int kMaxThreads = 1024;
 
-hipError_t launch_gn_forward(const GnPlan&, const GnParams& p, GnType type, hipStream_t stream) {
-    const hipError_t err = launch_gn_stats_general(p, type, stream);
-    return err != hipSuccess ? err : launch_gn_apply_general(p, type, stream);
+// The workgroup's slab: its first group, groups, first channel and channels.
+struct GnSlab {
+    int g0, groups, c0, channels;
+};
+__device__ __forceinline__ GnSlab slab_of(const GnParams& p, int slab) {
+    const int g0 = slab * p.slab_groups;
+    return {g0, p.slab_groups, g0 * p.group_channels, p.slab_groups * p.group_channels};
 }
 
-hipError_t launch_gn_backward(const GnPlan&, const GnParams& p, GnType type, hipStream_t stream) {
-    hipError_t err = hipSuccess;
-    if (p.batch > 0 && p.pixels > 0) {
-        err = launch_gn_sums_general(p, type, stream);
-        if (err == hipSuccess && p.y != nullptr) err = launch_gn_dx_general(p, type, stream);
+// The thread's place: row r of the rows at a time, first channel c0 of its vector in the slab, of which the first `skip`
+// are the vector's before.
+struct GnPlace {
+    int r, c0, skip;
+};
+template <int kV>
+__device__ __forceinline__ GnPlace place_of(const GnParams& p, const GnSlab& slab) {
+    const int r = (int)threadIdx.x / p.vecs, v = (int)threadIdx.x % p.vecs;
+    const int c0 = min(v * kV, slab.channels - kV);
+    return {r, c0, v * kV - c0};
+}
+
+__device__ __forceinline__ float team_sum(float v, int team) {
+    for (int d = 1; d < team; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// pixels that row r of `rows` has of `count`
+__device__ __forceinline__ int share_of(int count, int r, int rows) { return (count - r + rows - 1) / rows; }
+
+// Visits f(values...) for the thread's n pixels, kBatch loads of every tensor on their way at a time.
+template <int kBatch, typename Fn>
+__device__ __forceinline__ void over_pixels(int n, const char* x, int64_t step_x, Fn&& f) {
+    int i = 0;
+    for (; i + kBatch <= n; i += kBatch) {
+        u32x4 d[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) d[b] = ((const Unaligned<2>*)(x + b * step_x))->v;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) f(d[b]);
+        x += kBatch * step_x;
     }
-    if (err == hipSuccess && (p.dgamma != nullptr || p.dbeta != nullptr)) err = launch_gn_parameters_general(p, type, stream);
-    return err;
+    for (; i < n; ++i) {
+        f(((const Unaligned<2>*)x)->v);
+        x += step_x;
+    }
+}
+
+// The mean and centred sum of parts {mean, centred sum} of n values each, as sums about one of the means.
+struct GnMerge {
+    float about, first = 0.0f, second = 0.0f;
+    __device__ __forceinline__ void add(float2 part, float n) {
+        const float d = part.x - about;
+        first = __builtin_fmaf(d, n, first);
+        second += __builtin_fmaf(d * d, n, part.y);
+    }
+    // of all `values` values, over the team
+    __device__ __forceinline__ float2 finish(float values, int team) {
+        const float f = team_sum(first, team) / values, s = team_sum(second, team);
+        // (negative by rounding where there is no spread; NaN stays)
+        const float m = __builtin_fmaf(-f * values, f, s);
+        return float2{about + f, m < 0.0f ? 0.0f : m};
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
+    using V = GnVec<T>;
+    constexpr int kV = V::kV;
+    extern __shared__ __attribute__((aligned(16))) float2 parts[];  // [rows][channels] {mean, sum of squares about it}
+    const int task = (int)blockIdx.x / p.slabs, image = task / p.chunks, chunk = task % p.chunks;
+    const GnSlab slab = slab_of(p, (int)blockIdx.x % p.slabs);
+    const int64_t first = (int64_t)chunk * p.chunk_pixels;
+    const int count = (int)(p.pixels - first < p.chunk_pixels ? p.pixels - first : p.chunk_pixels);
+    const GnPlace at = place_of<kV>(p, slab);
+    const int rows = min(p.rows_at_once, count);
+    if (at.r < rows) {
+        const int64_t step = p.ld_x * p.rows_at_once * (int64_t)sizeof(T);
+        const char* x = (const char*)p.x + ((image * p.pixels + first + at.r) * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
+        const int n = share_of(count, at.r, p.rows_at_once);
+        float pivot[kV], s[kV] = {}, q[kV] = {};
+        V::unpack(V::load(x), pivot);
+        over_pixels<8>(n - 1, x + step, step, [&](u32x4 d) __attribute__((always_inline)) {
+            float v[kV];
+            V::unpack(d, v);
+#pragma unroll
+            for (int e = 0; e < kV; ++e) {
+                const float t = v[e] - pivot[e];
+                s[e] += t;
+                q[e] = __builtin_fmaf(t, t, q[e]);
+            }
+        });
+        const float over = 1.0f / (float)n;
+        float2* to = parts + at.r * slab.channels + at.c0;
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+            const float m = s[e] * over, c = __builtin_fmaf(-s[e], m, q[e]);
+            if (e >= at.skip) to[e] = float2{pivot[e] + m, c < 0.0f ? 0.0f : c};
+        }
+    }
+    __syncthreads();
+    const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
+    const float over_channels = 1.0f / (float)p.group_channels;
+    for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
+        const float2* from = parts + g * p.group_channels;
+        const int all = rows * p.group_channels;
+        GnMerge merge{from[0].x};
+#pragma unroll 4
+        for (int e = lane; e < all; e += p.team) {
+            const int r = (int)(((float)e + 0.5f) * over_channels), c = e - r * p.group_channels;  // (e < 2^13: exact)
+            merge.add(from[r * slab.channels + c], (float)share_of(count, r, p.rows_at_once));
+        }
+        const float2 m = merge.finish((float)count * (float)p.group_channels, p.team);
+        if (lane == 0) ((float2*)p.partial)[(int64_t)task * p.groups + slab.g0 + g] = m;
+    }
+}
+
+// mean and rstd of `groups` groups of an image from g0 on, from its chunks (in one order, whoever merges)
+constexpr int kMergeTeam = 16;
+__device__ __forceinline__ void merge_stats(const GnParams& p, int image, int g0, int groups, bool keep, float2* stats) {
+    const int teams = (int)blockDim.x / kMergeTeam, lane = (int)threadIdx.x % kMergeTeam;
+    const float values = (float)p.pixels * (float)p.group_channels;
+    const float whole = (float)p.chunk_pixels * (float)p.group_channels;
+    const float last = (float)(p.pixels - (p.chunks - 1) * p.chunk_pixels) * (float)p.group_channels;
+    for (int g = (int)threadIdx.x / kMergeTeam; g < groups; g += teams) {
+        const float2* from = (const float2*)p.partial + (int64_t)image * p.chunks * p.groups + g0 + g;
+        GnMerge merge{from[0].x};
+#pragma unroll 4
+        for (int k = lane; k < p.chunks; k += kMergeTeam) merge.add(from[(int64_t)k * p.groups], k == p.chunks - 1 ? last : whole);
+        const float2 m = merge.finish(values, kMergeTeam);
+        if (lane == 0) {
+            const float2 s{m.x, 1.0f / __builtin_sqrtf(m.y / values + p.eps)};
+            stats[g] = s;
+            if (keep) ((float2*)p.stats_out)[(int64_t)image * p.groups + g0 + g] = s;
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T>
+__device__ __forceinline__ void load_channels(const void* from, int c0, float (&v)[GnVec<T>::kV]) {
+    GnVec<T>::unpack(GnVec<T>::load((const char*)from + c0 * (int64_t)sizeof(T)), v);
+}
+
+// y. The chunks go from the end: what the first pass read last is what the caches hold.
+template <typename T, FfFamily kFam>
+__global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
+    using V = GnVec<T>;
+    constexpr int kV = V::kV;
+    extern __shared__ __attribute__((aligned(16))) float2 stats[];
+    const int block = (int)gridDim.x - 1 - (int)blockIdx.x;
+    const int task = block / p.slabs, image = task / p.apply_chunks, chunk = task % p.apply_chunks;
+    const GnSlab slab = slab_of(p, block % p.slabs);
+    merge_stats(p, image, slab.g0, slab.groups, p.stats_out != nullptr && chunk == 0, stats);
+    const int64_t first = (int64_t)chunk * p.apply_pixels;
+    const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
+    const GnPlace at = place_of<kV>(p, slab);
+    if (at.r >= min(p.rows_at_once, count)) return;
+    const FfAct act = ff_act(p.activation);
+    float mean[kV], a[kV], beta[kV];
+    load_channels<T>(p.gamma, slab.c0 + at.c0, a);
+    load_channels<T>(p.beta, slab.c0 + at.c0, beta);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+        const float2 s = stats[(at.c0 + e) / p.group_channels];
+        mean[e] = s.x;
+        a[e] *= s.y;
+    }
+    const int64_t row = image * p.pixels + first + at.r;
+    const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    char* y = (char*)p.y + (row * p.ld_y + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    const int64_t step_y = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
+    over_pixels<4>(share_of(count, at.r, p.rows_at_once), x, p.ld_x * p.rows_at_once * (int64_t)sizeof(T), [&](u32x4 d) __attribute__((always_inline)) {
+        float v[kV];
+        V::unpack(d, v);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) v[e] = gn_value<T, kFam>(act, __builtin_fmaf(v[e] - mean[e], a[e], beta[e]));
+        V::store(y, V::pack(v));
+        y += step_y;
+    });
+}
+
+// Codes by row. The row's lanes keep their channels' constants: z = x a + b, with b = beta - mean a rounded to 2^-24 of
+// mean a (a 16-bit x itself has 2^-12 of it at best).
+template <typename T, FfFamily kFam, int kWaves, int kVecs>
+__global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
+    extern __shared__ __attribute__((aligned(16))) float2 stats[];
+    __shared__ float part[4];
+    const int task = (int)gridDim.x - 1 - (int)blockIdx.x;
+    const int image = task / p.apply_chunks, chunk = task % p.apply_chunks;
+    merge_stats(p, image, 0, p.groups, p.stats_out != nullptr && chunk == 0, stats);
+    const I8Row<kWaves, kVecs> row(p.channels);
+    const FfAct act = ff_act(p.activation);
+    float a[kVecs][8], b[kVecs][8];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+        if (row.has(i)) {
+            load_channels<T>(p.gamma, row.column(i), a[i]);
+            load_channels<T>(p.beta, row.column(i), b[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 s = stats[(row.column(i) + e) / p.group_channels];
+                a[i][e] *= s.y;
+                b[i][e] = __builtin_fmaf(-s.x, a[i][e], b[i][e]);
+            }
+        }
+    }
+    const int64_t first = (int64_t)chunk * p.apply_pixels;
+    const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
+    for (int r = (int)threadIdx.x / (64 * kWaves); r < count; r += 4 / kWaves) {
+        const int64_t at = image * p.pixels + first + r;
+        const char* x = (const char*)p.x + at * p.ld_x * 2;
+        u32x4 d[kVecs];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+            d[i] = row.has(i) ? GnVec<T>::load(x + row.column(i) * 2) : u32x4{};
+        float v[kVecs][8];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            GnVec<T>::unpack(d[i], v[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = ff_value<kFam>(act, __builtin_fmaf(v[i][e], a[i][e], b[i][e]));
+        }
+        const float scale = row.quantise(v, part, p.q + at * p.ld_q, 0);
+        if (row.lane == 0) p.q_scale[at] = scale;
+    }
+}
+
+// The thread's constants of the gradients: z = (x - mean) a + beta.
+template <typename T>
+struct GnBackward {
+    static constexpr int kV = GnVec<T>::kV;
+    float mean[kV], rstd[kV], a[kV], beta[kV];
+    __device__ __forceinline__ void load(const GnParams& p, int image, int c0) {
+        load_channels<T>(p.gamma, c0, a);
+        load_channels<T>(p.beta, c0, beta);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+            const float2 s = ((const float2*)p.stats)[(int64_t)image * p.groups + (c0 + e) / p.group_channels];
+            mean[e] = s.x;
+            rstd[e] = s.y;
+            a[e] *= s.y;
+        }
+    }
+};
+
+// The sums of dz and of dz n by channel, and of both by group with gamma.
+template <typename T, FfFamily kFam>
+__global__ __launch_bounds__(kMaxThreads) void gn_sums_kernel(GnParams p) {
+    using V = GnVec<T>;
+    constexpr int kV = V::kV;
+    extern __shared__ __attribute__((aligned(16))) float2 parts[];  // [rows][channels]
+    const int task = (int)blockIdx.x / p.slabs, image = task / p.chunks, chunk = task % p.chunks;
+    const GnSlab slab = slab_of(p, (int)blockIdx.x % p.slabs);
+    const int64_t first = (int64_t)chunk * p.chunk_pixels;
+    const int count = (int)(p.pixels - first < p.chunk_pixels ? p.pixels - first : p.chunk_pixels);
+    const GnPlace at = place_of<kV>(p, slab);
+    const int rows = min(p.rows_at_once, count);
+    if (at.r < rows) {
+        const FfAct act = ff_act(p.activation);
+        GnBackward<T> b;
+        b.load(p, image, slab.c0 + at.c0);
+        const int64_t row = image * p.pixels + first + at.r;
+        const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
+        const char* dy = (const char*)p.dy + (row * p.ld_dy + slab.c0 + at.c0) * (int64_t)sizeof(T);
+        const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_dy = p.ld_dy * p.rows_at_once * (int64_t)sizeof(T);
+        float s1[kV] = {}, s2[kV] = {};
+        auto add = [&](u32x4 dx, u32x4 dd) __attribute__((always_inline)) {
+            float v[kV], d[kV];
+            V::unpack(dx, v);
+            V::unpack(dd, d);
+#pragma unroll
+            for (int e = 0; e < kV; ++e) {
+                const float t = v[e] - b.mean[e];
+                const float dz = kFam == kFamLinear && p.activation == SDXL_ACT_NONE ? d[e] : d[e] * gn_slope<T, kFam>(act, __builtin_fmaf(t, b.a[e], b.beta[e]));
+                s1[e] += dz;
+                s2[e] = __builtin_fmaf(dz, t, s2[e]);
+            }
+        };
+        const int n = share_of(count, at.r, p.rows_at_once);
+        constexpr int kBatch = 4;
+        int i = 0;
+        for (; i + kBatch <= n; i += kBatch) {
+            u32x4 dx[kBatch], dd[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                dx[k] = V::load(x + k * step_x);
+                dd[k] = V::load(dy + k * step_dy);
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) add(dx[k], dd[k]);
+            x += kBatch * step_x;
+            dy += kBatch * step_dy;
+        }
+        for (; i < n; ++i) {
+            add(V::load(x), V::load(dy));
+            x += step_x;
+            dy += step_dy;
+        }
+        float2* to = parts + at.r * slab.channels + at.c0;
+#pragma unroll
+        for (int e = 0; e < kV; ++e)
+            if (e >= at.skip) to[e] = float2{s1[e], s2[e] * b.rstd[e]};
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < slab.channels; c += blockDim.x) {
+        float2 sum = parts[c];
+        for (int r = 1; r < rows; ++r) {
+            sum.x += parts[r * slab.channels + c].x;
+            sum.y += parts[r * slab.channels + c].y;
+        }
+        ((float2*)p.channel_sums)[(int64_t)task * p.channels + slab.c0 + c] = sum;
+        const float gamma = (float)((const T*)p.gamma)[slab.c0 + c];
+        parts[c] = float2{sum.x * gamma, sum.y * gamma};  // (this thread's column alone)
+    }
+    __syncthreads();
+    const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
+    for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
+        float a = 0.0f, b = 0.0f;
+        for (int c = lane; c < p.group_channels; c += p.team) {
+            a += parts[g * p.group_channels + c].x;
+            b += parts[g * p.group_channels + c].y;
+        }
+        a = team_sum(a, p.team);
+        b = team_sum(b, p.team);
+        if (lane == 0) ((float2*)p.partial)[(int64_t)task * p.groups + slab.g0 + g] = float2{a, b};
+    }
+}
+
+constexpr int kParamChannels = 32;  // of a workgroup that adds up dgamma and dbeta
+
+// dx, and in workgroups of their own, the last ones, dgamma and dbeta.
+template <typename T, FfFamily kFam>
+__global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
+    using V = GnVec<T>;
+    constexpr int kV = V::kV;
+    extern __shared__ __attribute__((aligned(16))) float2 means[];
+    const int tasks = p.y != nullptr ? p.batch * p.apply_chunks * p.slabs : 0;
+    if ((int)blockIdx.x >= tasks) {
+        const int c = ((int)blockIdx.x - tasks) * kParamChannels + (int)threadIdx.x % kParamChannels;
+        const int lanes = (int)blockDim.x / kParamChannels, lane = (int)threadIdx.x / kParamChannels, parts = p.batch * p.chunks;
+        float2 sum{0.0f, 0.0f};
+        if (c < p.channels)
+            for (int k = lane; k < parts; k += lanes) {
+                const float2 a = ((const float2*)p.channel_sums)[(int64_t)k * p.channels + c];
+                sum.x += a.x;
+                sum.y += a.y;
+            }
+        means[threadIdx.x] = sum;
+        __syncthreads();
+        if (lane == 0 && c < p.channels) {
+            for (int k = 1; k < lanes; ++k) {
+                sum.x += means[k * kParamChannels + threadIdx.x].x;
+                sum.y += means[k * kParamChannels + threadIdx.x].y;
+            }
+            if (p.dbeta != nullptr) ((T*)p.dbeta)[c] = (T)sum.x;
+            if (p.dgamma != nullptr) ((T*)p.dgamma)[c] = (T)sum.y;
+        }
+        return;
+    }
+    const int block = tasks - 1 - (int)blockIdx.x;
+    const int task = block / p.slabs, image = task / p.apply_chunks, chunk = task % p.apply_chunks;
+    const GnSlab slab = slab_of(p, block % p.slabs);
+    {
+        const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
+        const float over = 1.0f / ((float)p.pixels * (float)p.group_channels);
+        for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
+            const float2* from = (const float2*)p.partial + (int64_t)image * p.chunks * p.groups + slab.g0 + g;
+            float a = 0.0f, b = 0.0f;
+#pragma unroll 4
+            for (int k = lane; k < p.chunks; k += p.team) {
+                a += from[(int64_t)k * p.groups].x;
+                b += from[(int64_t)k * p.groups].y;
+            }
+            a = team_sum(a, p.team);
+            b = team_sum(b, p.team);
+            if (lane == 0) means[g] = float2{a * over, b * over};
+        }
+        __syncthreads();
+    }
+    const int64_t first = (int64_t)chunk * p.apply_pixels;
+    const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
+    const GnPlace at = place_of<kV>(p, slab);
+    if (at.r >= min(p.rows_at_once, count)) return;
+    const FfAct act = ff_act(p.activation);
+    GnBackward<T> b;
+    b.load(p, image, slab.c0 + at.c0);
+    float a1[kV], a2[kV];  // dx = a dz - a1 - (x - mean) a2
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+        const float2 m = means[(at.c0 + e) / p.group_channels];
+        a1[e] = b.rstd[e] * m.x;
+        a2[e] = b.rstd[e] * b.rstd[e] * m.y;
+    }
+    const int64_t row = image * p.pixels + first + at.r;
+    const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    const char* dy = (const char*)p.dy + (row * p.ld_dy + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    char* dx = (char*)p.y + (row * p.ld_y + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_dy = p.ld_dy * p.rows_at_once * (int64_t)sizeof(T);
+    const int64_t step_dx = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
+    auto one = [&](u32x4 xd, u32x4 dd) __attribute__((always_inline)) {
+        float v[kV], d[kV];
+        V::unpack(xd, v);
+        V::unpack(dd, d);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+            const float t = v[e] - b.mean[e];
+            const float dz = kFam == kFamLinear && p.activation == SDXL_ACT_NONE ? d[e] : d[e] * gn_slope<T, kFam>(act, __builtin_fmaf(t, b.a[e], b.beta[e]));
+            v[e] = __builtin_fmaf(-t, a2[e], __builtin_fmaf(dz, b.a[e], -a1[e]));
+        }
+        V::store(dx, V::pack(v));
+        dx += step_dx;
+    };
+    const int n = share_of(count, at.r, p.rows_at_once);
+    constexpr int kBatch = 4;
+    int i = 0;
+    for (; i + kBatch <= n; i += kBatch) {
+        u32x4 xd[kBatch], dd[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            xd[k] = V::load(x + k * step_x);
+            dd[k] = V::load(dy + k * step_dy);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) one(xd[k], dd[k]);
+        x += kBatch * step_x;
+        dy += kBatch * step_dy;
+    }
+    for (; i < n; ++i) {
+        one(V::load(x), V::load(dy));
+        x += step_x;
+        dy += step_dy;
+    }
+}
+
+// ---- launches
+
+int elem_of(GnType type) { return type == kGnF32 ? 4 : 2; }
+
+// Groups of a slab: the smallest divisor of the groups that makes kSlabBytes of a row, else all.
+constexpr int64_t kSlabBytes = 512;
+int slab_groups_of(const GnParams& p, GnType type) {
+    const int64_t bytes = (int64_t)p.group_channels * elem_of(type);
+    for (int d = (int)((kSlabBytes + bytes - 1) / bytes); d < p.groups; ++d)
+        if (p.groups % d == 0) return d;
+    return p.groups;
+}
+int64_t vecs_of(const GnParams& p, GnType type, int slab_groups) {
+    return ((int64_t)p.group_channels * slab_groups * elem_of(type) + 15) / 16;
+}
+
+// Threads of a workgroup: of 4 to 16 waves the most whose lanes have work, the most of equals.
+int threads_of(int vecs, int most) {
+    int best = 0, best_used = -1;
+    for (int t = 256; t <= most; t += 64) {
+        const int used = t / vecs * vecs * 1024 / t;
+        if (t >= vecs && used >= best_used) {
+            best = t;
+            best_used = used;
+        }
+    }
+    return best;
+}
+
+int team_of(int groups, int threads) {
+    int team = 1;
+    while (team < 64 && 2 * team * groups <= threads) team *= 2;
+    return team;
+}
+
+// Workgroups of the two passes, and the rounds that one has at least where there are that many.
+constexpr int kStatsThreads = 1024, kApplyThreads = 512;
+constexpr int kFirstTasks = 512, kSecondTasks = 1024;
+constexpr int kFirstRounds = 4, kSecondRounds = 4;
+
+// `columns` (images by slabs) in chunks of whole rounds of `rows` pixels: `tasks` chunks in all or a little fewer, of at
+// least `least` rounds; more where a chunk would have over 1024 (what a thread adds up).
+int64_t chunk_of(int64_t columns, int64_t pixels, int rows, int tasks, int least) {
+    const int64_t each = tasks / columns < 1 ? 1 : tasks / columns;
+    const int64_t rounds = (pixels + rows - 1) / rows, chunk = (rounds + each - 1) / each;
+    return (chunk < least ? least : chunk < 1024 ? chunk : 1024) * rows;
+}
+
+template <typename T, typename Fn>
+hipError_t by_family(int32_t activation, Fn&& f) {
+    switch (activation) {
+    case SDXL_ACT_NONE:
+    case SDXL_ACT_RELU: return f.template operator()<T, kFamLinear>();
+    case SDXL_ACT_GELU: return f.template operator()<T, kFamErf>();
+    case SDXL_ACT_GELU_TANH: return f.template operator()<T, kFamTanh>();
+    default: return f.template operator()<T, kFamSigmoid>();
+    }
+}
+
+template <typename Fn>
+hipError_t by_type(GnType type, int32_t activation, Fn&& f) {
+    return type == kGnF16 ? by_family<_Float16>(activation, f) : type == kGnBf16 ? by_family<__bf16>(activation, f) : by_family<float>(activation, f);
+}
+
+// Fills in what the kernels of `threads` threads need.
+void lay_out(GnParams& p, GnType type, int threads) {
+    p.slab_groups = slab_groups_of(p, type);
+    p.slabs = p.groups / p.slab_groups;
+    p.vecs = (int32_t)vecs_of(p, type, p.slab_groups);
+    p.rows_at_once = threads / p.vecs;
+    p.team = team_of(p.slab_groups, threads);
+}
+
+void cut_second(GnParams& p, int64_t columns, int rows) {
+    p.apply_pixels = chunk_of(columns, p.pixels, rows, kSecondTasks, kSecondRounds);
+    p.apply_chunks = (int32_t)((p.pixels + p.apply_pixels - 1) / p.apply_pixels);
+}
+
+// Codes: a wave a row up to 5 vectors a lane, else four.
+constexpr int kRowVecs = 5;
+
+template <typename T, FfFamily kFam, int kWaves>
+hipError_t launch_rows_of(const GnParams& p, hipStream_t stream) {
+    const dim3 grid((unsigned)(p.batch * p.apply_chunks)), block(256);
+    const size_t lds = (size_t)p.groups * 8;
+    switch ((p.vecs + 64 * kWaves - 1) / (64 * kWaves)) {
+    case 1: hipLaunchKernelGGL((gn_rows_kernel<T, kFam, kWaves, 1>), grid, block, lds, stream, p); break;
+    case 2: hipLaunchKernelGGL((gn_rows_kernel<T, kFam, kWaves, 2>), grid, block, lds, stream, p); break;
+    case 3: hipLaunchKernelGGL((gn_rows_kernel<T, kFam, kWaves, 3>), grid, block, lds, stream, p); break;
+    case 4: hipLaunchKernelGGL((gn_rows_kernel<T, kFam, kWaves, 4>), grid, block, lds, stream, p); break;
+    case 5: hipLaunchKernelGGL((gn_rows_kernel<T, kFam, kWaves, 5>), grid, block, lds, stream, p); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_rows(const GnParams& params, GnType type, hipStream_t stream) {
+    GnParams p = params;
+    p.vecs = (p.channels + 7) / 8;
+    const bool wave = p.vecs <= 64 * kRowVecs;
+    p.team = team_of(p.groups, 256);
+    cut_second(p, p.batch, wave ? 4 : 1);
+    auto launch = [&]<typename T, FfFamily kFam>() {
+        return wave ? launch_rows_of<T, kFam, 1>(p, stream) : launch_rows_of<T, kFam, 4>(p, stream);
+    };
+    return type == kGnF16 ? by_family<_Float16>(p.activation, launch) : by_family<__bf16>(p.activation, launch);
+}
+
+}  // namespace
+
+GnPlan gn_plan(const GnParams& p, GnType type, bool) {
+    if (p.batch == 0 || p.pixels == 0 || p.channels == 0) return {false, 1, p.pixels};
+    const int slab_groups = slab_groups_of(p, type);
+    const int64_t vecs = vecs_of(p, type, slab_groups), columns = (int64_t)p.batch * (p.groups / slab_groups);
+    const bool fast = p.channels >= 16 / elem_of(type) && vecs <= kApplyThreads && columns <= (1 << 18) && p.groups <= 4096 &&
+                      p.pixels < (1 << 28) && p.ld_x <= (1 << 20) && p.ld_y <= (1 << 20) && p.ld_dy <= (1 << 20);
+    if (!fast) return {false, 1, p.pixels};
+    const int threads = threads_of((int)vecs, kStatsThreads);
+    const int64_t chunk = chunk_of(columns, p.pixels, threads / (int)vecs, kFirstTasks, kFirstRounds);
+    return {true, (int32_t)((p.pixels + chunk - 1) / chunk), chunk};
+}
+
+hipError_t launch_gn_forward(const GnPlan& plan, const GnParams& params, GnType type, hipStream_t stream) {
+    GnParams p = params;
+    if (!plan.fast || (p.q != nullptr && p.channels > 4 * 64 * 8 * kRowVecs)) {
+        p.chunks = 1;
+        const hipError_t err = launch_gn_stats_general(p, type, stream);
+        return err != hipSuccess ? err : launch_gn_apply_general(p, type, stream);
+    }
+    const int vecs = (int)vecs_of(p, type, slab_groups_of(p, type));
+    {
+        const int threads = threads_of(vecs, kStatsThreads);
+        lay_out(p, type, threads);
+        const dim3 grid((unsigned)(p.batch * p.chunks * p.slabs));
+        const size_t lds = (size_t)p.rows_at_once * p.slab_groups * p.group_channels * 8;
+        if (type == kGnF16) hipLaunchKernelGGL(gn_stats_kernel<_Float16>, grid, dim3(threads), lds, stream, p);
+        else if (type == kGnBf16) hipLaunchKernelGGL(gn_stats_kernel<__bf16>, grid, dim3(threads), lds, stream, p);
+        else hipLaunchKernelGGL(gn_stats_kernel<float>, grid, dim3(threads), lds, stream, p);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+    }
+    const int threads = threads_of(vecs, kApplyThreads);
+    lay_out(p, type, threads);
+    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once);
+    if (p.q != nullptr) return launch_rows(p, type, stream);
+    return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
+        hipLaunchKernelGGL((gn_apply_kernel<T, kFam>), dim3((unsigned)(p.batch * p.apply_chunks * p.slabs)), dim3(threads),
+                           (size_t)p.slab_groups * 8, stream, p);
+        return hipGetLastError();
+    });
+}
+
+hipError_t launch_gn_backward(const GnPlan& plan, const GnParams& params, GnType type, hipStream_t stream) {
+    GnParams p = params;
+    const bool parameters = p.dgamma != nullptr || p.dbeta != nullptr;
+    if (!plan.fast) {
+        hipError_t err = hipSuccess;
+        if (p.batch > 0 && p.pixels > 0) {
+            err = launch_gn_sums_general(p, type, stream);
+            if (err == hipSuccess && p.y != nullptr) err = launch_gn_dx_general(p, type, stream);
+        }
+        return err == hipSuccess && parameters ? launch_gn_parameters_general(p, type, stream) : err;
+    }
+    const int vecs = (int)vecs_of(p, type, slab_groups_of(p, type));
+    {
+        const int threads = threads_of(vecs, kStatsThreads);
+        lay_out(p, type, threads);
+        const size_t lds = (size_t)p.rows_at_once * p.slab_groups * p.group_channels * 8;
+        const hipError_t err = by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
+            hipLaunchKernelGGL((gn_sums_kernel<T, kFam>), dim3((unsigned)(p.batch * p.chunks * p.slabs)), dim3(threads), lds, stream, p);
+            return hipGetLastError();
+        });
+        if (err != hipSuccess) return err;
+    }
+    const int threads = threads_of(vecs, kApplyThreads);
+    lay_out(p, type, threads);
+    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once);
+    const int64_t grid = (p.y != nullptr ? (int64_t)p.batch * p.apply_chunks * p.slabs : 0) + (parameters ? (p.channels + kParamChannels - 1) / kParamChannels : 0);
+    const size_t lds = (size_t)(p.slab_groups > threads ? p.slab_groups : threads) * 8;
+    return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
+        hipLaunchKernelGGL((gn_dx_kernel<T, kFam>), dim3((unsigned)grid), dim3(threads), lds, stream, p);
+        return hipGetLastError();
+    });
 }
 
 }  // namespace sdxl_hip

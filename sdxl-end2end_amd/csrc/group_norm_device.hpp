@@ -1,5 +1,5 @@
 // Device helpers shared by the group norm kernels: the activation by element
-// type, and a row quantised to 8-bit integers.
+// type, 16 bytes of a row as fp32 values.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -35,16 +35,33 @@ __device__ __forceinline__ float gn_slope(const FfAct& a, float z) {
     }
 }
 
-// What one step of a row's codes stands for, and the code of a value: the rule of sdxl_quantize_i8_rows. amax is over
-// the row's finite values; a row with a NaN has a NaN for its scale.
-__device__ __forceinline__ float i8_scale(float amax, bool has_nan) {
-    const float s = amax > 0.0f ? __builtin_fmaxf(amax / 127.0f, 1e-12f) : 1.0f;
-    return has_nan ? __builtin_nanf("") : s;
-}
-// (scale NaN: 0)
-__device__ __forceinline__ int i8_code(float v, float scale) {
-    return (int)__builtin_rintf(__builtin_amdgcn_fmed3f(v / scale, -127.0f, 127.0f));
-}
+// 16 bytes of a row as fp32 values
+template <typename T>
+struct GnVec {
+    static constexpr int kV = 16 / (int)sizeof(T);
+    static __device__ __forceinline__ u32x4 load(const char* at) { return ((const Unaligned<sizeof(T)>*)at)->v; }
+    static __device__ __forceinline__ void store(char* at, u32x4 d) { ((Unaligned<sizeof(T)>*)at)->v = d; }
+    static __device__ __forceinline__ void unpack(u32x4 d, float (&v)[kV]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 4) {
+                v[e] = __uint_as_float(d[e]);
+            } else {
+                v[2 * e] = FfType<T>::lo(d[e]);
+                v[2 * e + 1] = FfType<T>::hi(d[e]);
+            }
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&v)[kV]) {
+        u32x4 d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 4) d[e] = __float_as_uint(v[e]);
+            else d[e] = FfType<T>::pack(v[2 * e], v[2 * e + 1]);
+        }
+        return d;
+    }
+};
 
 }  // namespace
 }  // namespace sdxl_hip

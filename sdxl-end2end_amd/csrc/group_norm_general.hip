@@ -1,11 +1,12 @@
 // The general group norm kernels (include/sdxl_hip/group_norm.h): any batch,
 // pixels, channels, groups, strides and alignment, element by element, sums in
-// 64 bits. The fast kernels (group_norm.hip) take rows of 16 bytes to 16 KiB.
+// 64 bits. The fast kernels (group_norm.hip) take rows of 16 bytes and more.
 // One workgroup sums a group of an image, one thread an element of the second
 // pass; what bounds them is the element loads ([2, 4096, 960] fp16 is 31 MB).
 #include <hip/hip_runtime.h>
 
 #include "group_norm_device.hpp"
+#include "int8_device.hpp"
 
 namespace sdxl_hip {
 namespace {

@@ -24,6 +24,11 @@ struct GnParams {
     int32_t batch, channels, groups, group_channels, chunks;
     int32_t activation;
     float eps;
+    // of the fast kernels, filled in by their launcher: slabs of whole groups, vectors of 16 bytes a slab's row, rows of the
+    // workgroup at a time, lanes that add a group's parts; chunks of the second pass
+    int32_t slabs, slab_groups, vecs, rows_at_once, team;
+    int32_t apply_chunks;
+    int64_t apply_pixels;
 };
 
 enum GnType : int { kGnF16, kGnBf16, kGnF32 };

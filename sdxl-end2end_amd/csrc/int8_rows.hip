@@ -4,7 +4,7 @@
 // says).
 #include <hip/hip_runtime.h>
 
-#include "group_norm_device.hpp"
+#include "int8_device.hpp"
 #include "int8_kernels.hpp"
 
 namespace sdxl_hip {
@@ -70,18 +70,94 @@ __global__ __launch_bounds__(kThreads) void i8_rows_general_kernel(I8RowsParams 
     }
 }
 
+// Rows in registers: a wave a row, or four.
+template <typename T, bool kNorm, int kWaves, int kVecs>
+__global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
+    using F = FfType<T>;
+    __shared__ float part[4];
+    const I8Row<kWaves, kVecs> row((int)p.cols);
+    constexpr int kRows = 4 / kWaves;  // of a workgroup at a time
+    for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / (64 * kWaves); r < p.rows; r += (int64_t)gridDim.x * kRows) {
+        const char* x = (const char*)p.x + r * p.ld_x * 2;
+        u32x4 d[kVecs];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            d[i] = u32x4{};
+            if (row.has(i)) d[i] = ((const Unaligned<2>*)(x + row.column(i) * 2))->v;
+        }
+        float v[kVecs][8];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][2 * e] = F::lo(d[i][e]), v[i][2 * e + 1] = F::hi(d[i][e]);
+        if constexpr (kNorm) {
+            auto add = [](float a, float b) { return a + b; };
+            float sum = 0.0f, centred = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int skip = row.has(i) ? row.skip(i) : 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += e >= skip ? v[i][e] : 0.0f;
+            }
+            const float mean = row.reduce(sum, part, add) / (float)p.cols;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int skip = row.has(i) ? row.skip(i) : 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float t = e >= skip ? v[i][e] - mean : 0.0f;
+                    centred = __builtin_fmaf(t, t, centred);
+                }
+            }
+            const float rstd = 1.0f / __builtin_sqrtf(row.reduce(centred, part, add) / (float)p.cols + p.eps);
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                if (row.has(i)) {
+                    const u32x4 g = ((const Unaligned<2>*)((const char*)p.gamma + row.column(i) * 2))->v;
+                    const u32x4 b = ((const Unaligned<2>*)((const char*)p.beta + row.column(i) * 2))->v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[i][2 * e] = __builtin_fmaf((v[i][2 * e] - mean) * rstd, F::lo(g[e]), F::lo(b[e]));
+                        v[i][2 * e + 1] = __builtin_fmaf((v[i][2 * e + 1] - mean) * rstd, F::hi(g[e]), F::hi(b[e]));
+                    }
+                }
+            }
+        }
+        const float scale = row.quantise(v, part, p.q + r * p.ld_q, (int)p.q_cols);
+        if (row.lane == 0) p.q_scale[r] = scale;
+    }
+}
+
+template <typename T, bool kNorm, int kWaves>
+hipError_t launch_vecs(const I8RowsParams& p, hipStream_t stream) {
+    const int64_t blocks = (p.rows * kWaves + 3) / 4;
+    const dim3 grid((unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid)), block(kThreads);
+    switch ((p.cols + 512 * kWaves - 1) / (512 * kWaves)) {
+    case 1: hipLaunchKernelGGL((i8_rows_kernel<T, kNorm, kWaves, 1>), grid, block, 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((i8_rows_kernel<T, kNorm, kWaves, 2>), grid, block, 0, stream, p); break;
+    case 3: hipLaunchKernelGGL((i8_rows_kernel<T, kNorm, kWaves, 3>), grid, block, 0, stream, p); break;
+    case 4: hipLaunchKernelGGL((i8_rows_kernel<T, kNorm, kWaves, 4>), grid, block, 0, stream, p); break;
+    case 5: hipLaunchKernelGGL((i8_rows_kernel<T, kNorm, kWaves, 5>), grid, block, 0, stream, p); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+// A wave a row up to 5 vectors a lane, four up to 20; shorter rows than a vector and longer ones: the general kernel.
+template <typename T, bool kNorm>
+hipError_t launch_rows(const I8RowsParams& p, hipStream_t stream) {
+    if (p.cols < 8 || p.cols > 4 * 2560) {
+        hipLaunchKernelGGL((i8_rows_general_kernel<T, kNorm>), dim3((unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid)), dim3(kThreads), 0, stream, p);
+        return hipGetLastError();
+    }
+    return p.cols <= 2560 ? launch_vecs<T, kNorm, 1>(p, stream) : launch_vecs<T, kNorm, 4>(p, stream);
+}
+
 }  // namespace
 
 hipError_t launch_i8_rows(const I8RowsParams& p, bool bf16, hipStream_t stream) {
-    const dim3 grid((unsigned)(p.rows < kMaxGrid ? p.rows : kMaxGrid));
-    if (p.gamma != nullptr) {
-        if (bf16) hipLaunchKernelGGL((i8_rows_general_kernel<__bf16, true>), grid, dim3(kThreads), 0, stream, p);
-        else hipLaunchKernelGGL((i8_rows_general_kernel<_Float16, true>), grid, dim3(kThreads), 0, stream, p);
-    } else {
-        if (bf16) hipLaunchKernelGGL((i8_rows_general_kernel<__bf16, false>), grid, dim3(kThreads), 0, stream, p);
-        else hipLaunchKernelGGL((i8_rows_general_kernel<_Float16, false>), grid, dim3(kThreads), 0, stream, p);
-    }
-    return hipGetLastError();
+    if (p.gamma != nullptr) return bf16 ? launch_rows<__bf16, true>(p, stream) : launch_rows<_Float16, true>(p, stream);
+    return bf16 ? launch_rows<__bf16, false>(p, stream) : launch_rows<_Float16, false>(p, stream);
 }
 
 }  // namespace sdxl_hip
