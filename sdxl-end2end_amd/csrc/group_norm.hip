@@ -28,11 +28,12 @@
 
 #include "group_norm_device.hpp"
 #include "int8_device.hpp"
+#include "wave_reduce.hpp"
 
 namespace sdxl_hip {
 namespace {
 
-constexpr int kMaxThreads = 1024;
+constexpr int kMaxThreads = 512;
 
 // The workgroup's slab: its first group, groups, first channel and channels.
 struct GnSlab {
@@ -55,31 +56,53 @@ __device__ __forceinline__ GnPlace place_of(const GnParams& p, const GnSlab& sla
     return {r, c0, v * kV - c0};
 }
 
+// over a team of 16 lanes or of 64
 __device__ __forceinline__ float team_sum(float v, int team) {
-    for (int d = 1; d < team; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+    v = reduce16(v, Add{});
+    return team == 64 ? reduce_rows(v, Add{}) : v;
 }
 
 // pixels that row r of `rows` has of `count`
 __device__ __forceinline__ int share_of(int count, int r, int rows) { return (count - r + rows - 1) / rows; }
 
-// Visits f(values...) for the thread's n pixels, kBatch loads of every tensor on their way at a time.
-template <int kBatch, typename Fn>
-__device__ __forceinline__ void over_pixels(int n, const char* x, int64_t step_x, Fn&& f) {
-    int i = 0;
-    for (; i + kBatch <= n; i += kBatch) {
-        u32x4 d[kBatch];
+// kBatch pixels' vectors of one tensor or two (b), on their way together: without the scheduling barriers the compiler
+// takes them one by one to save registers. `left` pixels: those past them are not read.
+template <int kBatch, bool kTwo>
+struct GnBatch {
+    u32x4 a[kBatch], b[kTwo ? kBatch : 1];
+
+    __device__ __forceinline__ void load(int left, const char* from_a, int64_t step_a, const char* from_b, int64_t step_b) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) d[b] = ((const Unaligned<2>*)(x + b * step_x))->v;
+        for (int k = 0; k < kBatch; ++k) {
+            if (k < left) {
+                a[k] = ((const Unaligned<2>*)(from_a + k * step_a))->v;
+                if constexpr (kTwo) b[k] = ((const Unaligned<2>*)(from_b + k * step_b))->v;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // f(a's vector, b's) of each, from pixel `first` of the batch on
+    template <int kFirst = 0, typename Fn>
+    __device__ __forceinline__ void visit(int left, Fn&& f) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) f(d[b]);
-        x += kBatch * step_x;
+        for (int k = kFirst; k < kBatch; ++k) {
+            if (k < left) f(a[k], b[kTwo ? k : 0]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
-    for (; i < n; ++i) {
-        f(((const Unaligned<2>*)x)->v);
-        x += step_x;
+    // the batch that is loaded, after whose start f is called with what follows it, up to n pixels
+    template <int kFirst = 0, typename Fn>
+    __device__ __forceinline__ void visit_all(int n, const char* from_a, int64_t step_a, const char* from_b, int64_t step_b, Fn&& f) {
+        visit<kFirst>(n, f);
+        while (n > kBatch) {
+            n -= kBatch;
+            from_a += kBatch * step_a;
+            if constexpr (kTwo) from_b += kBatch * step_b;
+            load(n, from_a, step_a, from_b, step_b);
+            visit(n, f);
+        }
     }
-}
+};
 
 // The mean and centred sum of parts {mean, centred sum} of n values each, as sums about one of the means.
 struct GnMerge {
@@ -113,9 +136,11 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
         const int64_t step = p.ld_x * p.rows_at_once * (int64_t)sizeof(T);
         const char* x = (const char*)p.x + ((image * p.pixels + first + at.r) * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
         const int n = share_of(count, at.r, p.rows_at_once);
+        GnBatch<8, false> batch;
+        batch.load(n, x, step, nullptr, 0);
         float pivot[kV], s[kV] = {}, q[kV] = {};
-        V::unpack(V::load(x), pivot);
-        over_pixels<8>(n - 1, x + step, step, [&](u32x4 d) __attribute__((always_inline)) {
+        V::unpack(batch.a[0], pivot);
+        batch.visit_all<1>(n, x, step, nullptr, 0, [&](u32x4 d, u32x4) __attribute__((always_inline)) {
             float v[kV];
             V::unpack(d, v);
 #pragma unroll
@@ -186,11 +211,17 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
     const int block = (int)gridDim.x - 1 - (int)blockIdx.x;
     const int task = block / p.slabs, image = task / p.apply_chunks, chunk = task % p.apply_chunks;
     const GnSlab slab = slab_of(p, block % p.slabs);
-    merge_stats(p, image, slab.g0, slab.groups, p.stats_out != nullptr && chunk == 0, stats);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
     const GnPlace at = place_of<kV>(p, slab);
-    if (at.r >= min(p.rows_at_once, count)) return;
+    const int n = at.r < p.rows_at_once ? share_of(count, at.r, p.rows_at_once) : 0;
+    const int64_t row = image * p.pixels + first + at.r;
+    const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_y = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
+    GnBatch<4, false> batch;
+    batch.load(n, x, step_x, nullptr, 0);
+    merge_stats(p, image, slab.g0, slab.groups, p.stats_out != nullptr && chunk == 0, stats);
+    if (n <= 0) return;
     const FfAct act = ff_act(p.activation);
     float mean[kV], a[kV], beta[kV];
     load_channels<T>(p.gamma, slab.c0 + at.c0, a);
@@ -201,11 +232,8 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
         mean[e] = s.x;
         a[e] *= s.y;
     }
-    const int64_t row = image * p.pixels + first + at.r;
-    const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
     char* y = (char*)p.y + (row * p.ld_y + slab.c0 + at.c0) * (int64_t)sizeof(T);
-    const int64_t step_y = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
-    over_pixels<4>(share_of(count, at.r, p.rows_at_once), x, p.ld_x * p.rows_at_once * (int64_t)sizeof(T), [&](u32x4 d) __attribute__((always_inline)) {
+    batch.visit_all(n, x, step_x, nullptr, 0, [&](u32x4 d, u32x4) __attribute__((always_inline)) {
         float v[kV];
         V::unpack(d, v);
 #pragma unroll
@@ -223,8 +251,18 @@ __global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
     __shared__ float part[4];
     const int task = (int)gridDim.x - 1 - (int)blockIdx.x;
     const int image = task / p.apply_chunks, chunk = task % p.apply_chunks;
-    merge_stats(p, image, 0, p.groups, p.stats_out != nullptr && chunk == 0, stats);
     const I8Row<kWaves, kVecs> row(p.channels);
+    const int64_t first = (int64_t)chunk * p.apply_pixels;
+    const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
+    u32x4 d[kVecs];
+    auto fetch = [&](int r) __attribute__((always_inline)) {
+        const char* x = (const char*)p.x + (image * p.pixels + first + r) * p.ld_x * 2;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) d[i] = r < count && row.has(i) ? GnVec<T>::load(x + row.column(i) * 2) : u32x4{};
+    };
+    int r = (int)threadIdx.x / (64 * kWaves);
+    fetch(r);
+    merge_stats(p, image, 0, p.groups, p.stats_out != nullptr && chunk == 0, stats);
     const FfAct act = ff_act(p.activation);
     float a[kVecs][8], b[kVecs][8];
 #pragma unroll
@@ -240,15 +278,7 @@ __global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
             }
         }
     }
-    const int64_t first = (int64_t)chunk * p.apply_pixels;
-    const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
-    for (int r = (int)threadIdx.x / (64 * kWaves); r < count; r += 4 / kWaves) {
-        const int64_t at = image * p.pixels + first + r;
-        const char* x = (const char*)p.x + at * p.ld_x * 2;
-        u32x4 d[kVecs];
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i)
-            d[i] = row.has(i) ? GnVec<T>::load(x + row.column(i) * 2) : u32x4{};
+    for (; r < count; r += 4 / kWaves) {
         float v[kVecs][8];
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
@@ -256,6 +286,8 @@ __global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = ff_value<kFam>(act, __builtin_fmaf(v[i][e], a[i][e], b[i][e]));
         }
+        fetch(r + 4 / kWaves);
+        const int64_t at = image * p.pixels + first + r;
         const float scale = row.quantise(v, part, p.q + at * p.ld_q, 0);
         if (row.lane == 0) p.q_scale[at] = scale;
     }
@@ -292,13 +324,16 @@ __global__ __launch_bounds__(kMaxThreads) void gn_sums_kernel(GnParams p) {
     const GnPlace at = place_of<kV>(p, slab);
     const int rows = min(p.rows_at_once, count);
     if (at.r < rows) {
-        const FfAct act = ff_act(p.activation);
-        GnBackward<T> b;
-        b.load(p, image, slab.c0 + at.c0);
         const int64_t row = image * p.pixels + first + at.r;
         const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
         const char* dy = (const char*)p.dy + (row * p.ld_dy + slab.c0 + at.c0) * (int64_t)sizeof(T);
         const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_dy = p.ld_dy * p.rows_at_once * (int64_t)sizeof(T);
+        const int n = share_of(count, at.r, p.rows_at_once);
+        GnBatch<4, true> batch;
+        batch.load(n, x, step_x, dy, step_dy);
+        const FfAct act = ff_act(p.activation);
+        GnBackward<T> b;
+        b.load(p, image, slab.c0 + at.c0);
         float s1[kV] = {}, s2[kV] = {};
         auto add = [&](u32x4 dx, u32x4 dd) __attribute__((always_inline)) {
             float v[kV], d[kV];
@@ -312,26 +347,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_sums_kernel(GnParams p) {
                 s2[e] = __builtin_fmaf(dz, t, s2[e]);
             }
         };
-        const int n = share_of(count, at.r, p.rows_at_once);
-        constexpr int kBatch = 4;
-        int i = 0;
-        for (; i + kBatch <= n; i += kBatch) {
-            u32x4 dx[kBatch], dd[kBatch];
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                dx[k] = V::load(x + k * step_x);
-                dd[k] = V::load(dy + k * step_dy);
-            }
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) add(dx[k], dd[k]);
-            x += kBatch * step_x;
-            dy += kBatch * step_dy;
-        }
-        for (; i < n; ++i) {
-            add(V::load(x), V::load(dy));
-            x += step_x;
-            dy += step_dy;
-        }
+        batch.visit_all(n, x, step_x, dy, step_dy, add);
         float2* to = parts + at.r * slab.channels + at.c0;
 #pragma unroll
         for (int e = 0; e < kV; ++e)
@@ -396,27 +412,33 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     const int block = tasks - 1 - (int)blockIdx.x;
     const int task = block / p.slabs, image = task / p.apply_chunks, chunk = task % p.apply_chunks;
     const GnSlab slab = slab_of(p, block % p.slabs);
-    {
-        const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
-        const float over = 1.0f / ((float)p.pixels * (float)p.group_channels);
-        for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
-            const float2* from = (const float2*)p.partial + (int64_t)image * p.chunks * p.groups + slab.g0 + g;
-            float a = 0.0f, b = 0.0f;
-#pragma unroll 4
-            for (int k = lane; k < p.chunks; k += p.team) {
-                a += from[(int64_t)k * p.groups].x;
-                b += from[(int64_t)k * p.groups].y;
-            }
-            a = team_sum(a, p.team);
-            b = team_sum(b, p.team);
-            if (lane == 0) means[g] = float2{a * over, b * over};
-        }
-        __syncthreads();
-    }
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
     const GnPlace at = place_of<kV>(p, slab);
-    if (at.r >= min(p.rows_at_once, count)) return;
+    const int n = at.r < p.rows_at_once ? share_of(count, at.r, p.rows_at_once) : 0;
+    const int64_t row = image * p.pixels + first + at.r;
+    const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    const char* dy = (const char*)p.dy + (row * p.ld_dy + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_dy = p.ld_dy * p.rows_at_once * (int64_t)sizeof(T);
+    const int64_t step_dx = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
+    GnBatch<4, true> batch;
+    batch.load(n, x, step_x, dy, step_dy);
+    const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
+    const float over = 1.0f / ((float)p.pixels * (float)p.group_channels);
+    for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
+        const float2* from = (const float2*)p.partial + (int64_t)image * p.chunks * p.groups + slab.g0 + g;
+        float a = 0.0f, b = 0.0f;
+#pragma unroll 4
+        for (int k = lane; k < p.chunks; k += p.team) {
+            a += from[(int64_t)k * p.groups].x;
+            b += from[(int64_t)k * p.groups].y;
+        }
+        a = team_sum(a, p.team);
+        b = team_sum(b, p.team);
+        if (lane == 0) means[g] = float2{a * over, b * over};
+    }
+    __syncthreads();
+    if (n <= 0) return;
     const FfAct act = ff_act(p.activation);
     GnBackward<T> b;
     b.load(p, image, slab.c0 + at.c0);
@@ -427,13 +449,8 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
         a1[e] = b.rstd[e] * m.x;
         a2[e] = b.rstd[e] * b.rstd[e] * m.y;
     }
-    const int64_t row = image * p.pixels + first + at.r;
-    const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
-    const char* dy = (const char*)p.dy + (row * p.ld_dy + slab.c0 + at.c0) * (int64_t)sizeof(T);
     char* dx = (char*)p.y + (row * p.ld_y + slab.c0 + at.c0) * (int64_t)sizeof(T);
-    const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_dy = p.ld_dy * p.rows_at_once * (int64_t)sizeof(T);
-    const int64_t step_dx = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
-    auto one = [&](u32x4 xd, u32x4 dd) __attribute__((always_inline)) {
+    batch.visit_all(n, x, step_x, dy, step_dy, [&](u32x4 xd, u32x4 dd) __attribute__((always_inline)) {
         float v[kV], d[kV];
         V::unpack(xd, v);
         V::unpack(dd, d);
@@ -445,27 +462,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
         }
         V::store(dx, V::pack(v));
         dx += step_dx;
-    };
-    const int n = share_of(count, at.r, p.rows_at_once);
-    constexpr int kBatch = 4;
-    int i = 0;
-    for (; i + kBatch <= n; i += kBatch) {
-        u32x4 xd[kBatch], dd[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            xd[k] = V::load(x + k * step_x);
-            dd[k] = V::load(dy + k * step_dy);
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) one(xd[k], dd[k]);
-        x += kBatch * step_x;
-        dy += kBatch * step_dy;
-    }
-    for (; i < n; ++i) {
-        one(V::load(x), V::load(dy));
-        x += step_x;
-        dy += step_dy;
-    }
+    });
 }
 
 // ---- launches
@@ -484,10 +481,10 @@ int64_t vecs_of(const GnParams& p, GnType type, int slab_groups) {
     return ((int64_t)p.group_channels * slab_groups * elem_of(type) + 15) / 16;
 }
 
-// Threads of a workgroup: of 4 to 16 waves the most whose lanes have work, the most of equals.
-int threads_of(int vecs, int most) {
+// Threads of a workgroup: of 4 to 8 waves the most whose lanes have work, the most of equals.
+int threads_of(int vecs) {
     int best = 0, best_used = -1;
-    for (int t = 256; t <= most; t += 64) {
+    for (int t = 256; t <= kMaxThreads; t += 64) {
         const int used = t / vecs * vecs * 1024 / t;
         if (t >= vecs && used >= best_used) {
             best = t;
@@ -497,23 +494,18 @@ int threads_of(int vecs, int most) {
     return best;
 }
 
-int team_of(int groups, int threads) {
-    int team = 1;
-    while (team < 64 && 2 * team * groups <= threads) team *= 2;
-    return team;
-}
+int team_of(int groups, int threads) { return 64 * groups <= threads ? 64 : 16; }
 
-// Workgroups of the two passes, and the rounds that one has at least where there are that many.
-constexpr int kStatsThreads = 1024, kApplyThreads = 512;
-constexpr int kFirstTasks = 512, kSecondTasks = 1024;
-constexpr int kFirstRounds = 4, kSecondRounds = 4;
+// Workgroups of the two passes (codes: of the second), and the rounds that a chunk has a multiple of.
+constexpr int kFirstTasks = 512, kSecondTasks = 1024, kRowTasks = 2048;
+constexpr int kBatchRounds = 4;
 
-// `columns` (images by slabs) in chunks of whole rounds of `rows` pixels: `tasks` chunks in all or a little fewer, of at
-// least `least` rounds; more where a chunk would have over 1024 (what a thread adds up).
-int64_t chunk_of(int64_t columns, int64_t pixels, int rows, int tasks, int least) {
+// `columns` (images by slabs) in chunks of whole rounds of `rows` pixels: `tasks` chunks in all or a little fewer, of
+// whole batches of rounds; more where a chunk would have over 1024 (what a thread adds up).
+int64_t chunk_of(int64_t columns, int64_t pixels, int rows, int tasks, int batch) {
     const int64_t each = tasks / columns < 1 ? 1 : tasks / columns;
-    const int64_t rounds = (pixels + rows - 1) / rows, chunk = (rounds + each - 1) / each;
-    return (chunk < least ? least : chunk < 1024 ? chunk : 1024) * rows;
+    const int64_t rounds = (pixels + rows - 1) / rows, chunk = ((rounds + each - 1) / each + batch - 1) / batch * batch;
+    return (chunk < 1024 ? chunk : 1024) * rows;
 }
 
 template <typename T, typename Fn>
@@ -541,8 +533,8 @@ void lay_out(GnParams& p, GnType type, int threads) {
     p.team = team_of(p.slab_groups, threads);
 }
 
-void cut_second(GnParams& p, int64_t columns, int rows) {
-    p.apply_pixels = chunk_of(columns, p.pixels, rows, kSecondTasks, kSecondRounds);
+void cut_second(GnParams& p, int64_t columns, int rows, int tasks, int batch) {
+    p.apply_pixels = chunk_of(columns, p.pixels, rows, tasks, batch);
     p.apply_chunks = (int32_t)((p.pixels + p.apply_pixels - 1) / p.apply_pixels);
 }
 
@@ -569,7 +561,7 @@ hipError_t launch_rows(const GnParams& params, GnType type, hipStream_t stream) 
     p.vecs = (p.channels + 7) / 8;
     const bool wave = p.vecs <= 64 * kRowVecs;
     p.team = team_of(p.groups, 256);
-    cut_second(p, p.batch, wave ? 4 : 1);
+    cut_second(p, p.batch, wave ? 4 : 1, kRowTasks, 1);
     auto launch = [&]<typename T, FfFamily kFam>() {
         return wave ? launch_rows_of<T, kFam, 1>(p, stream) : launch_rows_of<T, kFam, 4>(p, stream);
     };
@@ -582,11 +574,11 @@ GnPlan gn_plan(const GnParams& p, GnType type, bool) {
     if (p.batch == 0 || p.pixels == 0 || p.channels == 0) return {false, 1, p.pixels};
     const int slab_groups = slab_groups_of(p, type);
     const int64_t vecs = vecs_of(p, type, slab_groups), columns = (int64_t)p.batch * (p.groups / slab_groups);
-    const bool fast = p.channels >= 16 / elem_of(type) && vecs <= kApplyThreads && columns <= (1 << 18) && p.groups <= 4096 &&
+    const bool fast = p.channels >= 16 / elem_of(type) && vecs <= kMaxThreads && columns <= (1 << 18) && p.groups <= 4096 &&
                       p.pixels < (1 << 28) && p.ld_x <= (1 << 20) && p.ld_y <= (1 << 20) && p.ld_dy <= (1 << 20);
     if (!fast) return {false, 1, p.pixels};
-    const int threads = threads_of((int)vecs, kStatsThreads);
-    const int64_t chunk = chunk_of(columns, p.pixels, threads / (int)vecs, kFirstTasks, kFirstRounds);
+    const int threads = threads_of((int)vecs);
+    const int64_t chunk = chunk_of(columns, p.pixels, threads / (int)vecs, kFirstTasks, kBatchRounds);
     return {true, (int32_t)((p.pixels + chunk - 1) / chunk), chunk};
 }
 
@@ -599,7 +591,7 @@ hipError_t launch_gn_forward(const GnPlan& plan, const GnParams& params, GnType 
     }
     const int vecs = (int)vecs_of(p, type, slab_groups_of(p, type));
     {
-        const int threads = threads_of(vecs, kStatsThreads);
+        const int threads = threads_of(vecs);
         lay_out(p, type, threads);
         const dim3 grid((unsigned)(p.batch * p.chunks * p.slabs));
         const size_t lds = (size_t)p.rows_at_once * p.slab_groups * p.group_channels * 8;
@@ -609,9 +601,9 @@ hipError_t launch_gn_forward(const GnPlan& plan, const GnParams& params, GnType 
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
-    const int threads = threads_of(vecs, kApplyThreads);
+    const int threads = threads_of(vecs);
     lay_out(p, type, threads);
-    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once);
+    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once, kSecondTasks, kBatchRounds);
     if (p.q != nullptr) return launch_rows(p, type, stream);
     return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
         hipLaunchKernelGGL((gn_apply_kernel<T, kFam>), dim3((unsigned)(p.batch * p.apply_chunks * p.slabs)), dim3(threads),
@@ -633,7 +625,7 @@ hipError_t launch_gn_backward(const GnPlan& plan, const GnParams& params, GnType
     }
     const int vecs = (int)vecs_of(p, type, slab_groups_of(p, type));
     {
-        const int threads = threads_of(vecs, kStatsThreads);
+        const int threads = threads_of(vecs);
         lay_out(p, type, threads);
         const size_t lds = (size_t)p.rows_at_once * p.slab_groups * p.group_channels * 8;
         const hipError_t err = by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
@@ -642,9 +634,9 @@ hipError_t launch_gn_backward(const GnPlan& plan, const GnParams& params, GnType
         });
         if (err != hipSuccess) return err;
     }
-    const int threads = threads_of(vecs, kApplyThreads);
+    const int threads = threads_of(vecs);
     lay_out(p, type, threads);
-    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once);
+    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once, kSecondTasks, kBatchRounds);
     const int64_t grid = (p.y != nullptr ? (int64_t)p.batch * p.apply_chunks * p.slabs : 0) + (parameters ? (p.channels + kParamChannels - 1) / kParamChannels : 0);
     const size_t lds = (size_t)(p.slab_groups > threads ? p.slab_groups : threads) * 8;
     return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {

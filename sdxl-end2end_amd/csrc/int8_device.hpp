@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "feed_forward_device.hpp"
+#include "wave_reduce.hpp"
 
 namespace sdxl_hip {
 namespace {
@@ -41,8 +42,7 @@ struct I8Row {
     // over the row's lanes; part: a place for every wave
     template <typename Fn>
     static __device__ __forceinline__ float reduce(float v, float* part, Fn&& f) {
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) v = f(v, __shfl_xor(v, d));
+        v = reduce64(v, f);
         if constexpr (kWaves > 1) {
             static_assert(kWaves == 4, "a wave or four");
             __syncthreads();  // the part's last values are read
@@ -68,7 +68,7 @@ struct I8Row {
                 }
             }
         }
-        amax = reduce(nan ? __builtin_inff() : amax, part, [](float a, float b) { return __builtin_fmaxf(a, b); });
+        amax = reduce(nan ? __builtin_inff() : amax, part, Max{});
         const float scale = i8_scale(amax, amax == __builtin_inff());
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {

@@ -91,7 +91,6 @@ __global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i][2 * e] = F::lo(d[i][e]), v[i][2 * e + 1] = F::hi(d[i][e]);
         if constexpr (kNorm) {
-            auto add = [](float a, float b) { return a + b; };
             float sum = 0.0f, centred = 0.0f;
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
@@ -99,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum += e >= skip ? v[i][e] : 0.0f;
             }
-            const float mean = row.reduce(sum, part, add) / (float)p.cols;
+            const float mean = row.reduce(sum, part, Add{}) / (float)p.cols;
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
                 const int skip = row.has(i) ? row.skip(i) : 8;
@@ -109,7 +108,7 @@ __global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
                     centred = __builtin_fmaf(t, t, centred);
                 }
             }
-            const float rstd = 1.0f / __builtin_sqrtf(row.reduce(centred, part, add) / (float)p.cols + p.eps);
+            const float rstd = 1.0f / __builtin_sqrtf(row.reduce(centred, part, Add{}) / (float)p.cols + p.eps);
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
                 if (row.has(i)) {
