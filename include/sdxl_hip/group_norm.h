@@ -51,9 +51,10 @@ typedef struct sdxl_group_norm_desc {
     int32_t reserved;      /* must be 0 */
 } sdxl_group_norm_desc;
 
-/* Workspace of sdxl_group_norm and sdxl_group_norm_i8 (partial statistics), and of
- * sdxl_group_norm_backward, 256-byte aligned; 0 for a descriptor that the call refuses. */
+/* Workspaces of the calls below (parts of the sums), 256-byte aligned; 0 where a call needs none
+ * (sdxl_group_norm of small images) and for a descriptor that the call refuses. */
 size_t sdxl_group_norm_workspace_bytes(const sdxl_group_norm_desc* desc);
+size_t sdxl_group_norm_i8_workspace_bytes(const sdxl_group_norm_desc* desc);
 size_t sdxl_group_norm_backward_workspace_bytes(const sdxl_group_norm_desc* desc);
 
 /* y = act((x - mean) * rstd * gamma + beta), gamma and beta [channels]. stats (NULL: not

@@ -56,6 +56,9 @@ __device__ __forceinline__ GnPlace place_of(const GnParams& p, const GnSlab& sla
     return {r, c0, v * kV - c0};
 }
 
+// The group of channel c (below 2^22: the quotient is at least half a step from the next integer).
+__device__ __forceinline__ int group_of(const GnParams& p, int c) { return (int)(((float)c + 0.5f) * (1.0f / (float)p.group_channels)); }
+
 // over a team of 16 lanes or of 64
 __device__ __forceinline__ float team_sum(float v, int team) {
     v = reduce16(v, Add{});
@@ -65,8 +68,10 @@ __device__ __forceinline__ float team_sum(float v, int team) {
 // pixels that row r of `rows` has of `count`
 __device__ __forceinline__ int share_of(int count, int r, int rows) { return (count - r + rows - 1) / rows; }
 
-// kBatch pixels' vectors of one tensor or two (b), on their way together: without the scheduling barriers the compiler
-// takes them one by one to save registers. `left` pixels: those past them are not read.
+// kBatch pixels' vectors of one tensor or two (b), on their way together. Past the `left` pixels that there are the last one
+// is read again (none: the address itself, which has to be there): loads under conditions wait for each other, as they do
+// without the scheduling barriers, between which the compiler takes them one by one to save registers ([1, 262144, 256]
+// fp32, the first pass: 72 us so).
 template <int kBatch, bool kTwo>
 struct GnBatch {
     u32x4 a[kBatch], b[kTwo ? kBatch : 1];
@@ -74,9 +79,11 @@ struct GnBatch {
     __device__ __forceinline__ void load(int left, const char* from_a, int64_t step_a, const char* from_b, int64_t step_b) {
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-            if (k < left) {
-                a[k] = ((const Unaligned<2>*)(from_a + k * step_a))->v;
-                if constexpr (kTwo) b[k] = ((const Unaligned<2>*)(from_b + k * step_b))->v;
+            a[k] = ((const Unaligned<2>*)from_a)->v;
+            if (k + 1 < left) from_a += step_a;
+            if constexpr (kTwo) {
+                b[k] = ((const Unaligned<2>*)from_b)->v;
+                if (k + 1 < left) from_b += step_b;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -126,8 +133,9 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
     using V = GnVec<T>;
     constexpr int kV = V::kV;
     extern __shared__ __attribute__((aligned(16))) float2 parts[];  // [rows][channels] {mean, sum of squares about it}
-    const int task = (int)blockIdx.x / p.slabs, image = task / p.chunks, chunk = task % p.chunks;
-    const GnSlab slab = slab_of(p, (int)blockIdx.x % p.slabs);
+    const int column = (int)blockIdx.x % p.columns, chunk = (int)blockIdx.x / p.columns;
+    const int image = column / p.slabs, task = image * p.chunks + chunk;
+    const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.chunk_pixels;
     const int count = (int)(p.pixels - first < p.chunk_pixels ? p.pixels - first : p.chunk_pixels);
     const GnPlace at = place_of<kV>(p, slab);
@@ -202,6 +210,20 @@ __device__ __forceinline__ void load_channels(const void* from, int c0, float (&
     GnVec<T>::unpack(GnVec<T>::load((const char*)from + c0 * (int64_t)sizeof(T)), v);
 }
 
+// z of a channel's values, (x - mean) a + beta: a value that is the mean gives beta itself. (x a + (beta - mean a) is an
+// instruction less, and off by 2^-24 of mean a.)
+template <typename T>
+struct GnAffine {
+    static constexpr int kV = GnVec<T>::kV;
+    float mean[kV], a[kV], b[kV];
+    // gamma and beta are in a and b
+    __device__ __forceinline__ void set(int e, float2 stats) {
+        mean[e] = stats.x;
+        a[e] *= stats.y;
+    }
+    __device__ __forceinline__ float z(int e, float x) const { return __builtin_fmaf(x - mean[e], a[e], b[e]); }
+};
+
 // y. The chunks go from the end: what the first pass read last is what the caches hold.
 template <typename T, FfFamily kFam>
 __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
@@ -209,13 +231,13 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
     constexpr int kV = V::kV;
     extern __shared__ __attribute__((aligned(16))) float2 stats[];
     const int block = (int)gridDim.x - 1 - (int)blockIdx.x;
-    const int task = block / p.slabs, image = task / p.apply_chunks, chunk = task % p.apply_chunks;
-    const GnSlab slab = slab_of(p, block % p.slabs);
+    const int column = block % p.columns, chunk = block / p.columns, image = column / p.slabs;
+    const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
     const GnPlace at = place_of<kV>(p, slab);
-    const int n = at.r < p.rows_at_once ? share_of(count, at.r, p.rows_at_once) : 0;
-    const int64_t row = image * p.pixels + first + at.r;
+    const int n = at.r < p.rows_at_once && at.r < count ? share_of(count, at.r, p.rows_at_once) : 0;
+    const int64_t row = image * p.pixels + first + (n > 0 ? at.r : 0);
     const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
     const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_y = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
     GnBatch<4, false> batch;
@@ -223,21 +245,17 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
     merge_stats(p, image, slab.g0, slab.groups, p.stats_out != nullptr && chunk == 0, stats);
     if (n <= 0) return;
     const FfAct act = ff_act(p.activation);
-    float mean[kV], a[kV], beta[kV];
-    load_channels<T>(p.gamma, slab.c0 + at.c0, a);
-    load_channels<T>(p.beta, slab.c0 + at.c0, beta);
+    GnAffine<T> affine;
+    load_channels<T>(p.gamma, slab.c0 + at.c0, affine.a);
+    load_channels<T>(p.beta, slab.c0 + at.c0, affine.b);
 #pragma unroll
-    for (int e = 0; e < kV; ++e) {
-        const float2 s = stats[(at.c0 + e) / p.group_channels];
-        mean[e] = s.x;
-        a[e] *= s.y;
-    }
+    for (int e = 0; e < kV; ++e) affine.set(e, stats[group_of(p, at.c0 + e)]);
     char* y = (char*)p.y + (row * p.ld_y + slab.c0 + at.c0) * (int64_t)sizeof(T);
     batch.visit_all(n, x, step_x, nullptr, 0, [&](u32x4 d, u32x4) __attribute__((always_inline)) {
         float v[kV];
         V::unpack(d, v);
 #pragma unroll
-        for (int e = 0; e < kV; ++e) v[e] = gn_value<T, kFam>(act, __builtin_fmaf(v[e] - mean[e], a[e], beta[e]));
+        for (int e = 0; e < kV; ++e) v[e] = gn_value<T, kFam>(act, affine.z(e, v[e]));
         V::store(y, V::pack(v));
         y += step_y;
     });
@@ -272,7 +290,7 @@ __global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
             load_channels<T>(p.beta, row.column(i), b[i]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float2 s = stats[(row.column(i) + e) / p.group_channels];
+                const float2 s = stats[group_of(p, row.column(i) + e)];
                 a[i][e] *= s.y;
                 b[i][e] = __builtin_fmaf(-s.x, a[i][e], b[i][e]);
             }
@@ -303,7 +321,7 @@ struct GnBackward {
         load_channels<T>(p.beta, c0, beta);
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-            const float2 s = ((const float2*)p.stats)[(int64_t)image * p.groups + (c0 + e) / p.group_channels];
+            const float2 s = ((const float2*)p.stats)[(int64_t)image * p.groups + group_of(p, c0 + e)];
             mean[e] = s.x;
             rstd[e] = s.y;
             a[e] *= s.y;
@@ -317,8 +335,9 @@ __global__ __launch_bounds__(kMaxThreads) void gn_sums_kernel(GnParams p) {
     using V = GnVec<T>;
     constexpr int kV = V::kV;
     extern __shared__ __attribute__((aligned(16))) float2 parts[];  // [rows][channels]
-    const int task = (int)blockIdx.x / p.slabs, image = task / p.chunks, chunk = task % p.chunks;
-    const GnSlab slab = slab_of(p, (int)blockIdx.x % p.slabs);
+    const int column = (int)blockIdx.x % p.columns, chunk = (int)blockIdx.x / p.columns;
+    const int image = column / p.slabs, task = image * p.chunks + chunk;
+    const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.chunk_pixels;
     const int count = (int)(p.pixels - first < p.chunk_pixels ? p.pixels - first : p.chunk_pixels);
     const GnPlace at = place_of<kV>(p, slab);
@@ -386,7 +405,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     using V = GnVec<T>;
     constexpr int kV = V::kV;
     extern __shared__ __attribute__((aligned(16))) float2 means[];
-    const int tasks = p.y != nullptr ? p.batch * p.apply_chunks * p.slabs : 0;
+    const int tasks = p.y != nullptr ? p.apply_chunks * p.columns : 0;
     if ((int)blockIdx.x >= tasks) {
         const int c = ((int)blockIdx.x - tasks) * kParamChannels + (int)threadIdx.x % kParamChannels;
         const int lanes = (int)blockDim.x / kParamChannels, lane = (int)threadIdx.x / kParamChannels, parts = p.batch * p.chunks;
@@ -410,13 +429,13 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
         return;
     }
     const int block = tasks - 1 - (int)blockIdx.x;
-    const int task = block / p.slabs, image = task / p.apply_chunks, chunk = task % p.apply_chunks;
-    const GnSlab slab = slab_of(p, block % p.slabs);
+    const int column = block % p.columns, chunk = block / p.columns, image = column / p.slabs;
+    const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
     const GnPlace at = place_of<kV>(p, slab);
-    const int n = at.r < p.rows_at_once ? share_of(count, at.r, p.rows_at_once) : 0;
-    const int64_t row = image * p.pixels + first + at.r;
+    const int n = at.r < p.rows_at_once && at.r < count ? share_of(count, at.r, p.rows_at_once) : 0;
+    const int64_t row = image * p.pixels + first + (n > 0 ? at.r : 0);
     const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
     const char* dy = (const char*)p.dy + (row * p.ld_dy + slab.c0 + at.c0) * (int64_t)sizeof(T);
     const int64_t step_x = p.ld_x * p.rows_at_once * (int64_t)sizeof(T), step_dy = p.ld_dy * p.rows_at_once * (int64_t)sizeof(T);
@@ -445,7 +464,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     float a1[kV], a2[kV];  // dx = a dz - a1 - (x - mean) a2
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
-        const float2 m = means[(at.c0 + e) / p.group_channels];
+        const float2 m = means[group_of(p, at.c0 + e)];
         a1[e] = b.rstd[e] * m.x;
         a2[e] = b.rstd[e] * b.rstd[e] * m.y;
     }
@@ -465,16 +484,148 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     });
 }
 
+// ---- One launch, where a set of groups of an image fits a workgroup's registers.
+
+constexpr int kHeldVecs = 32;  // vectors of a set's row at most
+
+// Sums by group over the workgroup, of what its threads have of the two groups that a vector may lie in.
+struct GnHeld {
+    int vecs, rows, group_channels;
+    float2 *parts, *totals;  // [vecs][rows], [vecs]
+    int* group;              // [vecs]: a vector's first group
+
+    // a: of the vector's first group, b: of the next one; returns both groups' sums
+    __device__ __forceinline__ float2 sums(const GnPlace& at, int v, float2 mine) const {
+        if (at.r < rows) parts[v * rows + at.r] = mine;
+        __syncthreads();
+        const int lane = threadIdx.x & 63;
+        for (int w = (int)threadIdx.x >> 6; w < vecs; w += (int)blockDim.x >> 6) {
+            float2 t{0.0f, 0.0f};
+            for (int r = lane; r < rows; r += 64) {
+                t.x += parts[w * rows + r].x;
+                t.y += parts[w * rows + r].y;
+            }
+            t.x = reduce64(t.x, Add{});
+            t.y = reduce64(t.y, Add{});
+            if (lane == 0) totals[w] = t;
+        }
+        __syncthreads();
+        const int g = group[v];
+        float2 all{0.0f, 0.0f};
+        for (int w = 0; w < vecs; ++w) {
+            const int d = group[w] - g;
+            const float2 t = totals[w];
+            all.x += d == 0 ? t.x : d == -1 ? t.y : 0.0f;
+            all.y += d == 0 ? t.y : d == 1 ? t.x : 0.0f;
+        }
+        return all;
+    }
+};
+
+// LDS of the held kernels: parts, totals, groups.
+__device__ __forceinline__ GnHeld held_of(const GnParams& p, char* lds, const GnPlace& at) {
+    GnHeld h{p.vecs, p.rows_at_once, p.group_channels, (float2*)lds, nullptr, nullptr};
+    h.totals = h.parts + p.vecs * p.rows_at_once;
+    h.group = (int*)(h.totals + p.vecs);
+    if (at.r == 0) h.group[(int)threadIdx.x] = group_of(p, at.c0);  // (read behind the first barrier)
+    return h;
+}
+size_t held_lds(const GnParams& p) { return (size_t)p.vecs * (p.rows_at_once + 1) * 8 + (size_t)p.vecs * 4; }
+
+// The workgroup's image and set: neighbouring sets, which share cache lines, on one XCD.
+__device__ __forceinline__ int held_task() {
+    const int n = (int)gridDim.x, id = (int)blockIdx.x, xcd = id & 7, per = n >> 3, extra = n & 7;
+    return xcd * per + (xcd < extra ? xcd : extra) + (id >> 3);
+}
+
+// Two passes over the registers: the mean from sums about a value of the group, then the squares about the mean.
+template <typename T, FfFamily kFam, int kHold>
+__global__ __launch_bounds__(kMaxThreads) void gn_held_kernel(GnParams p) {
+    using V = GnVec<T>;
+    constexpr int kV = V::kV;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int task = held_task(), image = task / p.slabs;
+    const GnSlab slab = slab_of(p, task % p.slabs);
+    const GnPlace at = place_of<kV>(p, slab);
+    const int pixels = (int)p.pixels, n = at.r < p.rows_at_once && at.r < pixels ? share_of(pixels, at.r, p.rows_at_once) : 0;
+    const int64_t row = image * p.pixels + (n > 0 ? at.r : 0);
+    const char* x = (const char*)p.x + (row * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    GnBatch<kHold, false> batch;
+    batch.load(n, x, p.ld_x * p.rows_at_once * (int64_t)sizeof(T), nullptr, 0);
+    const int g = group_of(p, at.c0), next = (g + 1) * p.group_channels - at.c0;  // elements from `next` on: the next group's
+    const int g2 = min(g + 1, slab.groups - 1);
+    const T* pivots = (const T*)p.x + image * p.pixels * p.ld_x + slab.c0;
+    const float2 pivot{(float)pivots[g * p.group_channels], (float)pivots[g2 * p.group_channels]};
+    GnAffine<T> affine;
+    load_channels<T>(p.gamma, slab.c0 + at.c0, affine.a);
+    load_channels<T>(p.beta, slab.c0 + at.c0, affine.b);
+    const GnHeld held = held_of(p, lds, at);
+    const int v = (int)threadIdx.x % p.vecs;
+    auto split = [&](const float (&s)[kV]) __attribute__((always_inline)) {
+        float2 sum{0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+            const float t = e >= at.skip ? s[e] : 0.0f;
+            if (e < next) sum.x += t;
+            else sum.y += t;
+        }
+        return sum;
+    };
+    const float over = 1.0f / ((float)pixels * (float)p.group_channels);
+    float s[kV] = {};
+    batch.visit(n, [&](u32x4 d, u32x4) __attribute__((always_inline)) {
+        float u[kV];
+        V::unpack(d, u);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) s[e] += u[e] - (e < next ? pivot.x : pivot.y);
+    });
+    const float2 first = held.sums(at, v, split(s));
+    const float2 mean{__builtin_fmaf(first.x, over, pivot.x), __builtin_fmaf(first.y, over, pivot.y)};
+#pragma unroll
+    for (int e = 0; e < kV; ++e) s[e] = 0.0f;
+    batch.visit(n, [&](u32x4 d, u32x4) __attribute__((always_inline)) {
+        float u[kV];
+        V::unpack(d, u);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+            const float t = u[e] - (e < next ? mean.x : mean.y);
+            s[e] = __builtin_fmaf(t, t, s[e]);
+        }
+    });
+    const float2 second = held.sums(at, v, split(s));
+    const float2 stats{mean.x, 1.0f / __builtin_sqrtf(__builtin_fmaf(second.x, over, p.eps))};
+    const float2 stats2{mean.y, 1.0f / __builtin_sqrtf(__builtin_fmaf(second.y, over, p.eps))};
+    if (n <= 0) return;
+    if (p.stats_out != nullptr && at.r == 0) {  // the threads that have a group's first channel
+        float2* to = (float2*)p.stats_out + (int64_t)image * p.groups + slab.g0;
+        if (at.c0 == g * p.group_channels) to[g] = stats;
+        if (next < kV) to[g + 1] = stats2;
+    }
+    const FfAct act = ff_act(p.activation);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) affine.set(e, e < next ? stats : stats2);
+    char* y = (char*)p.y + (row * p.ld_y + slab.c0 + at.c0) * (int64_t)sizeof(T);
+    const int64_t step_y = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
+    batch.visit(n, [&](u32x4 d, u32x4) __attribute__((always_inline)) {
+        float u[kV];
+        V::unpack(d, u);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) u[e] = gn_value<T, kFam>(act, affine.z(e, u[e]));
+        V::store(y, V::pack(u));
+        y += step_y;
+    });
+}
+
 // ---- launches
 
 int elem_of(GnType type) { return type == kGnF32 ? 4 : 2; }
 
-// Groups of a slab: the smallest divisor of the groups that makes kSlabBytes of a row, else all.
-constexpr int64_t kSlabBytes = 512;
-int slab_groups_of(const GnParams& p, GnType type) {
+// Groups of a slab: the smallest divisor of the groups that makes `least` bytes of a row (and whole vectors), else all.
+constexpr int64_t kSlabBytes = 512, kHeldBytes = 64;
+int slab_groups_of(const GnParams& p, GnType type, int64_t least) {
     const int64_t bytes = (int64_t)p.group_channels * elem_of(type);
-    for (int d = (int)((kSlabBytes + bytes - 1) / bytes); d < p.groups; ++d)
-        if (p.groups % d == 0) return d;
+    for (int d = (int)((least + bytes - 1) / bytes); d < p.groups; ++d)
+        if (p.groups % d == 0 && (d * bytes % 16 == 0 || least == kSlabBytes)) return d;
     return p.groups;
 }
 int64_t vecs_of(const GnParams& p, GnType type, int slab_groups) {
@@ -497,7 +648,7 @@ int threads_of(int vecs) {
 int team_of(int groups, int threads) { return 64 * groups <= threads ? 64 : 16; }
 
 // Workgroups of the two passes (codes: of the second), and the rounds that a chunk has a multiple of.
-constexpr int kFirstTasks = 512, kSecondTasks = 1024, kRowTasks = 2048;
+constexpr int kFirstTasks = 512, kSecondTasks = 1024, kRowTasks = 512;
 constexpr int kBatchRounds = 4;
 
 // `columns` (images by slabs) in chunks of whole rounds of `rows` pixels: `tasks` chunks in all or a little fewer, of
@@ -525,12 +676,13 @@ hipError_t by_type(GnType type, int32_t activation, Fn&& f) {
 }
 
 // Fills in what the kernels of `threads` threads need.
-void lay_out(GnParams& p, GnType type, int threads) {
-    p.slab_groups = slab_groups_of(p, type);
+void lay_out(GnParams& p, GnType type, int slab_groups, int threads) {
+    p.slab_groups = slab_groups;
     p.slabs = p.groups / p.slab_groups;
     p.vecs = (int32_t)vecs_of(p, type, p.slab_groups);
     p.rows_at_once = threads / p.vecs;
     p.team = team_of(p.slab_groups, threads);
+    p.columns = p.batch * p.slabs;
 }
 
 void cut_second(GnParams& p, int64_t columns, int rows, int tasks, int batch) {
@@ -570,30 +722,81 @@ hipError_t launch_rows(const GnParams& params, GnType type, hipStream_t stream) 
 
 }  // namespace
 
-GnPlan gn_plan(const GnParams& p, GnType type, bool) {
-    if (p.batch == 0 || p.pixels == 0 || p.channels == 0) return {false, 1, p.pixels};
-    const int slab_groups = slab_groups_of(p, type);
-    const int64_t vecs = vecs_of(p, type, slab_groups), columns = (int64_t)p.batch * (p.groups / slab_groups);
-    const bool fast = p.channels >= 16 / elem_of(type) && vecs <= kMaxThreads && columns <= (1 << 18) && p.groups <= 4096 &&
-                      p.pixels < (1 << 28) && p.ld_x <= (1 << 20) && p.ld_y <= (1 << 20) && p.ld_dy <= (1 << 20);
-    if (!fast) return {false, 1, p.pixels};
-    const int threads = threads_of((int)vecs);
-    const int64_t chunk = chunk_of(columns, p.pixels, threads / (int)vecs, kFirstTasks, kBatchRounds);
-    return {true, (int32_t)((p.pixels + chunk - 1) / chunk), chunk};
+namespace {
+
+// The vectors that a thread of the held kernels has, 0 where they do not take the call: a set of groups that they can tell
+// apart (a vector lies in two at most) and hold.
+constexpr int kHolds[] = {1, 2, 4, 8, 16};
+int hold_of(const GnParams& p, GnType type, int most, int& slab_groups, int& threads) {
+    const int kV = 16 / elem_of(type);
+    slab_groups = slab_groups_of(p, type, kHeldBytes);
+    const int64_t vecs = vecs_of(p, type, slab_groups);
+    if (slab_groups > 1 && p.group_channels < kV && (p.group_channels * 2 != kV || slab_groups * p.group_channels % kV != 0)) return 0;
+    if (vecs > kHeldVecs || p.pixels > (1 << 16) || (int64_t)p.batch * (p.groups / slab_groups) > (1 << 20)) return 0;
+    threads = (int)(vecs * p.pixels < kMaxThreads ? (vecs * p.pixels + 63) / 64 * 64 : kMaxThreads);
+    const int rows = threads / (int)vecs, needed = (int)((p.pixels + rows - 1) / rows);
+    for (int hold : kHolds)
+        if (hold >= needed && hold <= most) return hold;
+    return 0;
 }
+
+bool fast_of(const GnParams& p, GnType type) {
+    const int slab_groups = slab_groups_of(p, type, kSlabBytes);
+    const int64_t vecs = vecs_of(p, type, slab_groups), columns = (int64_t)p.batch * (p.groups / slab_groups);
+    return p.batch > 0 && p.pixels > 0 && p.channels >= 16 / elem_of(type) && vecs <= kMaxThreads && columns <= (1 << 18) &&
+           p.groups <= 4096 && p.pixels < (1 << 28) && p.ld_x <= (1 << 20) && p.ld_y <= (1 << 20) && p.ld_dy <= (1 << 20);
+}
+
+}  // namespace
+
+GnPlan gn_plan(const GnParams& p, GnType type, GnCall call) {
+    if (!fast_of(p, type) || (call == kGnRows && p.channels > 4 * 64 * 8 * kRowVecs)) return {false, 0, 1, p.pixels};
+    int slab_groups, threads;
+    if (call == kGnForward) {
+        const int hold = hold_of(p, type, 16, slab_groups, threads);
+        if (hold > 0) return {true, hold, 0, 0};
+    }
+    slab_groups = slab_groups_of(p, type, kSlabBytes);
+    const int vecs = (int)vecs_of(p, type, slab_groups);
+    const int64_t chunk = chunk_of((int64_t)p.batch * (p.groups / slab_groups), p.pixels, threads_of(vecs) / vecs, kFirstTasks, kBatchRounds);
+    return {true, 0, (int32_t)((p.pixels + chunk - 1) / chunk), chunk};
+}
+
+namespace {
+
+template <typename T, FfFamily kFam>
+hipError_t launch_held(const GnParams& p, int hold, int threads, hipStream_t stream) {
+    const dim3 grid((unsigned)(p.batch * p.slabs)), block(threads);
+    const size_t lds = held_lds(p);
+    switch (hold) {
+    case 1: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 1>), grid, block, lds, stream, p); break;
+    case 2: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 2>), grid, block, lds, stream, p); break;
+    case 4: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 4>), grid, block, lds, stream, p); break;
+    case 8: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 8>), grid, block, lds, stream, p); break;
+    case 16: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 16>), grid, block, lds, stream, p); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_gn_forward(const GnPlan& plan, const GnParams& params, GnType type, hipStream_t stream) {
     GnParams p = params;
-    if (!plan.fast || (p.q != nullptr && p.channels > 4 * 64 * 8 * kRowVecs)) {
-        p.chunks = 1;
+    if (!plan.fast) {
         const hipError_t err = launch_gn_stats_general(p, type, stream);
         return err != hipSuccess ? err : launch_gn_apply_general(p, type, stream);
     }
-    const int vecs = (int)vecs_of(p, type, slab_groups_of(p, type));
+    if (plan.hold > 0) {
+        int slab_groups, threads;
+        hold_of(p, type, plan.hold, slab_groups, threads);
+        lay_out(p, type, slab_groups, threads);
+        return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() { return launch_held<T, kFam>(p, plan.hold, threads, stream); });
+    }
+    const int slab_groups = slab_groups_of(p, type, kSlabBytes), threads = threads_of((int)vecs_of(p, type, slab_groups));
+    lay_out(p, type, slab_groups, threads);
     {
-        const int threads = threads_of(vecs);
-        lay_out(p, type, threads);
-        const dim3 grid((unsigned)(p.batch * p.chunks * p.slabs));
+        const dim3 grid((unsigned)(p.columns * p.chunks));
         const size_t lds = (size_t)p.rows_at_once * p.slab_groups * p.group_channels * 8;
         if (type == kGnF16) hipLaunchKernelGGL(gn_stats_kernel<_Float16>, grid, dim3(threads), lds, stream, p);
         else if (type == kGnBf16) hipLaunchKernelGGL(gn_stats_kernel<__bf16>, grid, dim3(threads), lds, stream, p);
@@ -601,13 +804,10 @@ hipError_t launch_gn_forward(const GnPlan& plan, const GnParams& params, GnType 
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
-    const int threads = threads_of(vecs);
-    lay_out(p, type, threads);
-    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once, kSecondTasks, kBatchRounds);
     if (p.q != nullptr) return launch_rows(p, type, stream);
+    cut_second(p, p.columns, p.rows_at_once, kSecondTasks, kBatchRounds);
     return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
-        hipLaunchKernelGGL((gn_apply_kernel<T, kFam>), dim3((unsigned)(p.batch * p.apply_chunks * p.slabs)), dim3(threads),
-                           (size_t)p.slab_groups * 8, stream, p);
+        hipLaunchKernelGGL((gn_apply_kernel<T, kFam>), dim3((unsigned)(p.columns * p.apply_chunks)), dim3(threads), (size_t)p.slab_groups * 8, stream, p);
         return hipGetLastError();
     });
 }
@@ -623,21 +823,16 @@ hipError_t launch_gn_backward(const GnPlan& plan, const GnParams& params, GnType
         }
         return err == hipSuccess && parameters ? launch_gn_parameters_general(p, type, stream) : err;
     }
-    const int vecs = (int)vecs_of(p, type, slab_groups_of(p, type));
-    {
-        const int threads = threads_of(vecs);
-        lay_out(p, type, threads);
-        const size_t lds = (size_t)p.rows_at_once * p.slab_groups * p.group_channels * 8;
-        const hipError_t err = by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
-            hipLaunchKernelGGL((gn_sums_kernel<T, kFam>), dim3((unsigned)(p.batch * p.chunks * p.slabs)), dim3(threads), lds, stream, p);
-            return hipGetLastError();
-        });
-        if (err != hipSuccess) return err;
-    }
-    const int threads = threads_of(vecs);
-    lay_out(p, type, threads);
-    cut_second(p, (int64_t)p.batch * p.slabs, p.rows_at_once, kSecondTasks, kBatchRounds);
-    const int64_t grid = (p.y != nullptr ? (int64_t)p.batch * p.apply_chunks * p.slabs : 0) + (parameters ? (p.channels + kParamChannels - 1) / kParamChannels : 0);
+    const int slab_groups = slab_groups_of(p, type, kSlabBytes), threads = threads_of((int)vecs_of(p, type, slab_groups));
+    lay_out(p, type, slab_groups, threads);
+    const hipError_t err = by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
+        hipLaunchKernelGGL((gn_sums_kernel<T, kFam>), dim3((unsigned)(p.columns * p.chunks)), dim3(threads),
+                           (size_t)p.rows_at_once * p.slab_groups * p.group_channels * 8, stream, p);
+        return hipGetLastError();
+    });
+    if (err != hipSuccess) return err;
+    cut_second(p, p.columns, p.rows_at_once, kSecondTasks, kBatchRounds);
+    const int64_t grid = (p.y != nullptr ? (int64_t)p.columns * p.apply_chunks : 0) + (parameters ? (p.channels + kParamChannels - 1) / kParamChannels : 0);
     const size_t lds = (size_t)(p.slab_groups > threads ? p.slab_groups : threads) * 8;
     return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
         hipLaunchKernelGGL((gn_dx_kernel<T, kFam>), dim3((unsigned)grid), dim3(threads), lds, stream, p);

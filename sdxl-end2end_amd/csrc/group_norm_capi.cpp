@@ -85,10 +85,10 @@ size_t workspace_of(const Call& c, const GnPlan& plan, bool backward) {
     return group_bytes(c.p, plan) + (backward ? channel_bytes(c.p, plan) : 0);
 }
 
-size_t workspace_bytes_of(const sdxl_group_norm_desc* d, bool backward, const char* name) {
+size_t workspace_bytes_of(const sdxl_group_norm_desc* d, sdxl_hip::GnCall call, const char* name) {
     Call c;
     if (resolve(d, name, c) != SDXL_STATUS_OK || c.empty) return 0;
-    return workspace_of(c, gn_plan(c.p, c.type, backward), backward);
+    return workspace_of(c, gn_plan(c.p, c.type, call), call == sdxl_hip::kGnBackward);
 }
 
 void use_workspace(GnParams& p, const GnPlan& plan, void* workspace) {
@@ -122,14 +122,14 @@ sdxl_status forward(const sdxl_group_norm_desc* d, const char* name, const void*
     const uintptr_t e = (uintptr_t)c.elem;
     if (!aligned(x, e) || !aligned(gamma, e) || !aligned(beta, e) || !aligned(y, e) || !aligned(q_scale, 4) || !aligned(stats, 4))
         return fail(name, SDXL_STATUS_UNSUPPORTED, "tensor not aligned to its elements");
-    const GnPlan plan = gn_plan(p, c.type, false);
+    const GnPlan plan = gn_plan(p, c.type, codes ? sdxl_hip::kGnRows : sdxl_hip::kGnForward);
     const size_t need = workspace_of(c, plan, false);
-    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256))
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");
     const Area in = matrix(x, c.rows, p.channels, p.ld_x, c.elem), g = vector(gamma, p.channels, c.elem), b = vector(beta, p.channels, c.elem);
     const Area out[4] = {codes ? matrix(q, c.rows, p.channels, p.ld_q, 1) : matrix(y, c.rows, p.channels, p.ld_y, c.elem),
                          vector(codes ? q_scale : nullptr, c.rows, 4), vector(stats, 2 * (int64_t)p.batch * p.groups, 4),
-                         vector(workspace, (int64_t)need, 1)};
+                         vector(need > 0 ? workspace : nullptr, (int64_t)need, 1)};
     const bool in_place = !codes && x == y && p.ld_x == p.ld_y;
     for (int i = 0; i < 4; ++i) {
         if (overlaps_one(out[i], {g, b}) || (!(i == 0 && in_place) && overlap(out[i], in)))
@@ -153,11 +153,15 @@ sdxl_status forward(const sdxl_group_norm_desc* d, const char* name, const void*
 extern "C" {
 
 size_t sdxl_group_norm_workspace_bytes(const sdxl_group_norm_desc* d) {
-    return workspace_bytes_of(d, false, "sdxl_group_norm");
+    return workspace_bytes_of(d, sdxl_hip::kGnForward, "sdxl_group_norm");
+}
+
+size_t sdxl_group_norm_i8_workspace_bytes(const sdxl_group_norm_desc* d) {
+    return workspace_bytes_of(d, sdxl_hip::kGnRows, "sdxl_group_norm_i8");
 }
 
 size_t sdxl_group_norm_backward_workspace_bytes(const sdxl_group_norm_desc* d) {
-    return workspace_bytes_of(d, true, "sdxl_group_norm_backward");
+    return workspace_bytes_of(d, sdxl_hip::kGnBackward, "sdxl_group_norm_backward");
 }
 
 sdxl_status sdxl_group_norm(const sdxl_group_norm_desc* d, const void* x, const void* gamma, const void* beta, void* y,
@@ -190,7 +194,7 @@ sdxl_status sdxl_group_norm_backward(const sdxl_group_norm_desc* d, const void* 
     if (!aligned(dy, e) || !aligned(x, e) || !aligned(gamma, e) || !aligned(beta, e) || !aligned(dx, e) ||
         !aligned(dgamma, e) || !aligned(dbeta, e) || !aligned(stats, 4))
         return fail(name, SDXL_STATUS_UNSUPPORTED, "tensor not aligned to its elements");
-    const GnPlan plan = gn_plan(p, c.type, true);
+    const GnPlan plan = gn_plan(p, c.type, sdxl_hip::kGnBackward);
     const size_t need = c.empty ? 0 : workspace_of(c, plan, true);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");

@@ -27,6 +27,7 @@ struct GnParams {
     // of the fast kernels, filled in by their launcher: slabs of whole groups, vectors of 16 bytes a slab's row, rows of the
     // workgroup at a time, lanes that add a group's parts; chunks of the second pass
     int32_t slabs, slab_groups, vecs, rows_at_once, team;
+    int32_t columns;  // images by slabs
     int32_t apply_chunks;
     int64_t apply_pixels;
 };
@@ -41,12 +42,14 @@ hipError_t launch_gn_dx_general(const GnParams& p, GnType type, hipStream_t stre
 hipError_t launch_gn_parameters_general(const GnParams& p, GnType type, hipStream_t stream);
 
 // How a call is cut and which kernels it runs on, by sizes and strides alone (a call's sums have one order everywhere).
+enum GnCall : int { kGnForward, kGnRows, kGnBackward };
 struct GnPlan {
     bool fast;
+    int32_t hold;  // vectors that a thread of the one-launch kernel holds; 0: two passes
     int32_t chunks;
     int64_t chunk_pixels;
 };
-GnPlan gn_plan(const GnParams& p, GnType type, bool backward);
+GnPlan gn_plan(const GnParams& p, GnType type, GnCall call);
 
 // With p.chunks and p.chunk_pixels of the plan.
 hipError_t launch_gn_forward(const GnPlan& plan, const GnParams& p, GnType type, hipStream_t stream);

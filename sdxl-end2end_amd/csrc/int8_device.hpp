@@ -17,9 +17,15 @@ __device__ __forceinline__ float i8_scale(float amax, bool has_nan) {
     const float s = amax > 0.0f ? __builtin_fmaxf(amax / 127.0f, 1e-12f) : 1.0f;
     return has_nan ? __builtin_nanf("") : s;
 }
-// (scale NaN: 0)
+// (scale NaN: any code)
 __device__ __forceinline__ int i8_code(float v, float scale) {
     return (int)__builtin_rintf(__builtin_amdgcn_fmed3f(v / scale, -127.0f, 127.0f));
+}
+// The same of a v of at most 127 steps, in the low byte: the quotient from the scale's reciprocal, one residual step
+// from which leaves it correctly rounded (Markstein), then rounded to an integer (ties to even) by the addition.
+__device__ __forceinline__ uint32_t i8_code_bits(float v, float scale, float over) {
+    const float q = v * over;
+    return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, scale, v), over, q) + 12582912.0f);  // 3 * 2^22
 }
 
 struct __attribute__((packed, aligned(1))) Unaligned8 {
@@ -55,30 +61,39 @@ struct I8Row {
 
     // The codes of the values and their scale: codes to q, zeros from `cols` to q_cols; returns the scale.
     __device__ __forceinline__ float quantise(const float (&v)[kVecs][8], float* part, int8_t* q, int q_cols) const {
-        float amax = 0.0f;
-        bool nan = false;
+        constexpr uint32_t kInf = 0x7f800000u;
+        auto largest = [&](uint32_t most) __attribute__((always_inline)) {
+            uint32_t top = 0;  // magnitudes compare as their bits do, NaN above infinity
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            if (has(i)) {
+            for (int i = 0; i < kVecs; ++i) {
+                if (has(i)) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float m = __builtin_fabsf(v[i][e]);
-                    nan |= m != m;
-                    amax = __builtin_fmaxf(amax, m < __builtin_inff() ? m : 0.0f);
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t m = __float_as_uint(v[i][e]) & 0x7fffffffu;
+                        top = max(top, m <= most ? m : 0);
+                    }
                 }
             }
-        }
-        amax = reduce(nan ? __builtin_inff() : amax, part, Max{});
-        const float scale = i8_scale(amax, amax == __builtin_inff());
+            return __float_as_uint(reduce(__uint_as_float(top), part, [](float a, float b) __attribute__((always_inline)) {
+                return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+            }));
+        };
+        uint32_t top = largest(0xffffffffu);
+        const bool nan = top > kInf;
+        if (top >= kInf) top = largest(kInf - 1);  // (all of the row's lanes)
+        const float scale = i8_scale(__uint_as_float(top), nan), over = 1.0f / scale, limit = 127.0f * scale;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
             if (has(i)) {
                 uint32_t d[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    d[h] = 0;
+                    uint32_t c[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) d[h] |= (uint32_t)(i8_code(v[i][4 * h + e], scale) & 0xff) << (8 * e);
+                    for (int e = 0; e < 4; ++e) c[e] = i8_code_bits(__builtin_amdgcn_fmed3f(v[i][4 * h + e], -limit, limit), scale, over);
+                    // low bytes of two, then of all
+                    const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
+                    d[h] = lo | hi << 16;
                 }
                 ((Unaligned8*)(q + column(i)))->v = u32x2{d[0], d[1]};
             }

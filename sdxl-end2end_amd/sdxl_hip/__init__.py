@@ -62,6 +62,7 @@ FEED_FORWARD_SYMBOLS = (
 # of group_norm.h
 GROUP_NORM_SYMBOLS = (
     "sdxl_group_norm_workspace_bytes",
+    "sdxl_group_norm_i8_workspace_bytes",
     "sdxl_group_norm_backward_workspace_bytes",
     "sdxl_group_norm",
     "sdxl_group_norm_backward",
@@ -257,7 +258,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.sdxl_ff_sublayer.restype = ctypes.c_int
     lib.sdxl_ff_sublayer.argtypes = [ctypes.POINTER(FfSublayerDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                      ctypes.c_size_t, vp]
-    for name in ("sdxl_group_norm", "sdxl_group_norm_backward"):
+    for name in ("sdxl_group_norm", "sdxl_group_norm_i8", "sdxl_group_norm_backward"):
         fn = getattr(lib, name + "_workspace_bytes")
         fn.restype = ctypes.c_size_t
         fn.argtypes = [ctypes.POINTER(GroupNormDesc)]
@@ -288,7 +289,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         setattr(lib, "packed_" + name, fn)
     for name in ("sdxl_linear_act_backward_workspace_bytes", "sdxl_gated_linear_backward_workspace_bytes",
                  "sdxl_ff_sublayer_workspace_bytes", "sdxl_group_norm_workspace_bytes",
-                 "sdxl_group_norm_backward_workspace_bytes", "sdxl_linear_i8_workspace_bytes",
+                 "sdxl_group_norm_i8_workspace_bytes", "sdxl_group_norm_backward_workspace_bytes", "sdxl_linear_i8_workspace_bytes",
                  "sdxl_gated_linear_i8_workspace_bytes"):
         fn = lib[name]
         fn.restype = ctypes.c_size_t
@@ -846,12 +847,16 @@ def _gn_common(name, x, gamma, beta, groups, activation):
     return t, batch, pixels, channels, 0 if x.is_contiguous() else _gn_stride(name, "x", x, channels), code, act, index
 
 
-def _gn_workspace(name, t, size, workspace, x, index):
+def _workspace(name, t, size, workspace, x, index):
+    """(pointer, bytes, the tensor to keep) of a workspace that the caller gave, or of one of `size` bytes"""
     if workspace is None:
-        return t.empty((size,), dtype=t.uint8, device=x.device)
+        if size == 0:
+            return None, 0, None
+        workspace = t.empty((size,), dtype=t.uint8, device=x.device)
+        return workspace.data_ptr(), size, workspace
     if workspace.get_device() != index or not workspace.is_contiguous():
         raise SdxlError(INVALID_ARGUMENT, f"{name}: workspace must be contiguous and on x's device")
-    return workspace
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 def _gn_stats(name, t, stats, with_stats, batch, groups, x, index):
@@ -880,10 +885,9 @@ def group_norm(x, gamma, beta, groups: int, activation: str = "none", eps: float
     stats = _gn_stats(name, t, None, with_stats, batch, groups, x, index)
     desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, ldy, 0, code, act, _f32(eps), 0)
     lib = load()
-    workspace = _gn_workspace(name, t, lib.packed_sdxl_group_norm_workspace_bytes(desc), workspace, x, index)
+    ws, ws_bytes, workspace = _workspace(name, t, lib.packed_sdxl_group_norm_workspace_bytes(desc), workspace, x, index)
     _ff_call(lib.packed_sdxl_group_norm, index, t, desc, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), out.data_ptr(),
-             stats.data_ptr() if stats is not None else None, workspace.data_ptr(),
-             workspace.numel() * workspace.element_size())
+             stats.data_ptr() if stats is not None else None, ws, ws_bytes)
     return (out, stats) if with_stats else out
 
 
@@ -891,7 +895,7 @@ def group_norm_backward(dout, x, gamma, beta, groups: int, stats, activation: st
                         need_dgamma: bool = True, need_dbeta: bool = True, workspace=None):
     """Gradients (dx like x but contiguous, dgamma [channels], dbeta [channels]) of group_norm for dout like x, with the
     stats of its forward call. What is not needed is None. workspace: contiguous, of group_norm_workspace_bytes(..,
-    backward=True), else one is allocated."""
+    call="backward"), else one is allocated."""
     name = "sdxl_group_norm_backward"
     t, batch, pixels, channels, ldx, code, act, index = _gn_common(name, x, gamma, beta, groups, activation)
     if dout.shape != x.shape or dout.dtype != x.dtype or dout.get_device() != index:
@@ -900,13 +904,12 @@ def group_norm_backward(dout, x, gamma, beta, groups: int, stats, activation: st
     _gn_stats(name, t, stats, False, batch, groups, x, index)
     desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, 0, lddy, code, act, 0.0, 0)
     lib = load()
-    workspace = _gn_workspace(name, t, lib.packed_sdxl_group_norm_backward_workspace_bytes(desc), workspace, x, index)
+    ws, ws_bytes, workspace = _workspace(name, t, lib.packed_sdxl_group_norm_backward_workspace_bytes(desc), workspace, x, index)
     dx = x.new_empty(x.shape) if need_dx else None
     dgamma = x.new_empty((channels,)) if need_dgamma else None
     dbeta = x.new_empty((channels,)) if need_dbeta else None
     _ff_call(lib.packed_sdxl_group_norm_backward, index, t, desc, dout.data_ptr(), x.data_ptr(), gamma.data_ptr(),
-             beta.data_ptr(), stats.data_ptr(), _ptr(dx), _ptr(dgamma), _ptr(dbeta), workspace.data_ptr(),
-             workspace.numel() * workspace.element_size())
+             beta.data_ptr(), stats.data_ptr(), _ptr(dx), _ptr(dgamma), _ptr(dbeta), ws, ws_bytes)
     return dx, dgamma, dbeta
 
 
@@ -921,19 +924,20 @@ def group_norm_i8(x, gamma, beta, groups: int, activation: str = "none", eps: fl
     stats = _gn_stats(name, t, None, with_stats, batch, groups, x, index)
     desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, 0, 0, code, act, _f32(eps), 0)
     lib = load()
-    workspace = _gn_workspace(name, t, lib.packed_sdxl_group_norm_workspace_bytes(desc), workspace, x, index)
+    ws, ws_bytes, workspace = _workspace(name, t, lib.packed_sdxl_group_norm_i8_workspace_bytes(desc), workspace, x, index)
     _ff_call(lib.packed_sdxl_group_norm_i8, index, t, desc, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), q.data_ptr(), 0,
-             scale.data_ptr(), stats.data_ptr() if stats is not None else None, workspace.data_ptr(),
-             workspace.numel() * workspace.element_size())
+             scale.data_ptr(), stats.data_ptr() if stats is not None else None, ws, ws_bytes)
     return (q, scale, stats) if with_stats else (q, scale)
 
 
 def group_norm_workspace_bytes(batch: int, pixels: int, channels: int, groups: int, dtype: int = F16,
-                               backward: bool = False) -> int:
-    """Workspace of group_norm and group_norm_i8, or of group_norm_backward."""
+                               call: str = "forward") -> int:
+    """Workspace of group_norm ("forward"), group_norm_i8 ("i8") or group_norm_backward ("backward")."""
     desc = GroupNormDesc(batch=batch, pixels=pixels, channels=channels, groups=groups, dtype=dtype)
     lib = load()
-    return int((lib.sdxl_group_norm_backward_workspace_bytes if backward else lib.sdxl_group_norm_workspace_bytes)(ctypes.byref(desc)))
+    size = {"forward": lib.sdxl_group_norm_workspace_bytes, "i8": lib.sdxl_group_norm_i8_workspace_bytes,
+            "backward": lib.sdxl_group_norm_backward_workspace_bytes}[call]
+    return int(size(ctypes.byref(desc)))
 
 
 # ---------------------------------------------------------------- 8-bit integer linears
@@ -1022,12 +1026,8 @@ def _linear_i8(name, gated, x, w, w_scale, x_scale, bias, residual, activation, 
                          0 if w.is_contiguous() else _ff_stride(name, "w", w), ldo, ldr, code, code if tokens else I8, act,
                          1 if gate_first else 0, 0)
     lib = load()
-    if tokens:
-        size = (lib.packed_sdxl_gated_linear_i8_workspace_bytes if gated else lib.packed_sdxl_linear_i8_workspace_bytes)(desc)
-        workspace = _gn_workspace(name, t, size, workspace, x, index)
-        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    else:
-        ws_ptr, ws_bytes = None, 0
+    size = (lib.packed_sdxl_gated_linear_i8_workspace_bytes if gated else lib.packed_sdxl_linear_i8_workspace_bytes)(desc) if tokens else 0
+    ws_ptr, ws_bytes, workspace = _workspace(name, t, size, workspace, x, index)
     scale_ptr = x_scale.data_ptr() if x_scale is not None else None
     bias_ptr = bias.data_ptr() if bias is not None else None
     if gated:

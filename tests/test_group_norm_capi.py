@@ -13,7 +13,7 @@ torch = pytest.importorskip("torch")
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "sdxl_hip", "group_norm.h")
 P = 4096  # a pointer that is never followed: aligned to everything
-MIB = 1 << 20
+GIB = 1 << 30
 
 
 def test_header_declarations_are_exported():
@@ -25,7 +25,7 @@ def test_header_declarations_are_exported():
     assert re.findall(r"(?:int(?:32|64)_t|float) (\w+);", header) == [f[0] for f in sh.GroupNormDesc._fields_]
 
 
-def desc(batch=2, pixels=16, channels=64, groups=8, dtype=sh.F16, **kw):
+def desc(batch=2, pixels=1 << 17, channels=64, groups=8, dtype=sh.F16, **kw):
     return sh.GroupNormDesc(batch=batch, pixels=pixels, channels=channels, groups=groups, dtype=dtype, **kw)
 
 
@@ -34,9 +34,9 @@ ARGS = {"forward": ("x", "gamma", "beta", "y", "stats", "ws"), "i8": ("x", "gamm
 NAMES = {"forward": "sdxl_group_norm", "i8": "sdxl_group_norm_i8", "backward": "sdxl_group_norm_backward"}
 
 
-def call(kind, d, ws_bytes=MIB, **given):
-    """Every pointer a MiB from the next, but for those given."""
-    at = {name: MIB * (i + 1) for i, name in enumerate(ARGS[kind])} | {"ld_q": 0} | given
+def call(kind, d, ws_bytes=GIB, **given):
+    """Every pointer a GiB from the next, but for those given."""
+    at = {name: GIB * (i + 1) for i, name in enumerate(ARGS[kind])} | {"ld_q": 0} | given
     ref = ctypes.byref(d) if d is not None else None
     args = [at[n] if n == "ld_q" else at[n] or None for n in ARGS[kind]]
     return getattr(sh.load(), NAMES[kind])(ref, *args, ws_bytes, None)
@@ -56,7 +56,7 @@ def call(kind, d, ws_bytes=MIB, **given):
 def test_refused_descriptors(kind, bad, status):
     assert call(kind, desc(**bad)) == status
     assert sh.load().sdxl_last_error()
-    size = sh.load().sdxl_group_norm_backward_workspace_bytes if kind == "backward" else sh.load().sdxl_group_norm_workspace_bytes
+    size = getattr(sh.load(), NAMES[kind] + "_workspace_bytes")
     assert size(ctypes.byref(desc(**bad))) == 0
 
 
@@ -85,7 +85,7 @@ def test_refused_pointers(kind):
 
 @pytest.mark.parametrize("kind", ARGS)
 def test_overlaps_are_refused(kind):
-    at = {name: MIB * (i + 1) for i, name in enumerate(ARGS[kind])}
+    at = {name: GIB * (i + 1) for i, name in enumerate(ARGS[kind])}
     outputs = {"forward": ("y", "stats", "ws"), "i8": ("q", "q_scale", "stats", "ws"),
                "backward": ("dx", "dgamma", "dbeta", "ws")}[kind]
     inputs = [n for n in ARGS[kind] if n not in outputs and n != "ld_q"]
@@ -111,11 +111,13 @@ def test_empty_problems_launch_nothing(kind):
 
 def test_workspaces():
     for dtype in (sh.F16, sh.F32):
-        small = sh.group_norm_workspace_bytes(2, 16, 64, 8, dtype)
-        assert small % 256 == 0 and 0 < small <= 1 << 16
-        assert sh.group_norm_workspace_bytes(2, 16, 64, 8, dtype, backward=True) > small
+        assert sh.group_norm_workspace_bytes(2, 16, 64, 8, dtype) == 0  # one launch
+        small = sh.group_norm_workspace_bytes(2, 1 << 17, 64, 8, dtype)
+        assert small % 256 == 0 and 0 < small <= 1 << 18
+        assert sh.group_norm_workspace_bytes(2, 1 << 17, 64, 8, dtype, call="backward") > small
+    assert sh.group_norm_workspace_bytes(2, 16, 64, 8, call="i8") > 0
     # parts of the sums, not of the tensor: [1, 2^20, 128] fp32 is 512 MiB
-    assert sh.group_norm_workspace_bytes(1, 1 << 20, 128, 32, sh.F32, backward=True) < 8 << 20
+    assert sh.group_norm_workspace_bytes(1, 1 << 20, 128, 32, sh.F32, call="backward") < 8 << 20
 
 
 def test_python_refusals():

@@ -9,7 +9,7 @@ half a step more.
 import pytest
 
 import sdxl_hip as sh
-from test_group_norm_gpu import BF16, DEV, F16, HALF, TINY, U, act64, normal_form, values, within
+from test_group_norm_gpu import BF16, DEV, F16, HALF, TINY, U, act64, check_forward, normal_form, values, within
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -187,7 +187,9 @@ def test_group_norm_codes(B, P, C, G, dtype):
     assert q.shape == x.shape and s.shape == (B * P,)
     _, _, z, ez, _, _ = normal_form(x, gamma, beta, G, 1e-6)
     check_norm_codes(q, s, z, ez)
-    assert torch.equal(stats, sh.group_norm(x, gamma, beta, G, eps=1e-6, with_stats=True)[1])
+    y, y_stats = sh.group_norm(x, gamma, beta, G, eps=1e-6, with_stats=True)
+    check_forward(x, gamma, beta, G, "none", 1e-6, y, stats)
+    check_forward(x, gamma, beta, G, "none", 1e-6, y, y_stats)
     q, s = sh.group_norm_i8(x, gamma, beta, G, activation="silu", eps=1e-6)
     a = act64("silu", z)
     check_norm_codes(q, s, a, 1.13 * ez + ACT * a.abs())
