@@ -224,14 +224,15 @@ struct GnAffine {
     __device__ __forceinline__ float z(int e, float x) const { return __builtin_fmaf(x - mean[e], a[e], b[e]); }
 };
 
-// y. The chunks go from the end: what the first pass read last is what the caches hold.
+// y, by stores that pass the caches: kept there, it costs the reads of the next call's first pass the time to write it back
+// ([1, 262144, 256] fp32 156 us, 134 so; with a kernel behind that reads y, [2, 65536, 640] fp16 150 us either way, [2,
+// 16384, 640] 41 and 42).
 template <typename T, FfFamily kFam>
 __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
     using V = GnVec<T>;
     constexpr int kV = V::kV;
     extern __shared__ __attribute__((aligned(16))) float2 stats[];
-    const int block = (int)gridDim.x - 1 - (int)blockIdx.x;
-    const int column = block % p.columns, chunk = block / p.columns, image = column / p.slabs;
+    const int column = (int)blockIdx.x % p.columns, chunk = (int)blockIdx.x / p.columns, image = column / p.slabs;
     const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
         V::unpack(d, v);
 #pragma unroll
         for (int e = 0; e < kV; ++e) v[e] = gn_value<T, kFam>(act, affine.z(e, v[e]));
-        V::store(y, V::pack(v));
+        V::store_through(y, V::pack(v));
         y += step_y;
     });
 }
@@ -267,7 +268,7 @@ template <typename T, FfFamily kFam, int kWaves, int kVecs>
 __global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
     extern __shared__ __attribute__((aligned(16))) float2 stats[];
     __shared__ float part[4];
-    const int task = (int)gridDim.x - 1 - (int)blockIdx.x;
+    const int task = (int)blockIdx.x;
     const int image = task / p.apply_chunks, chunk = task % p.apply_chunks;
     const I8Row<kWaves, kVecs> row(p.channels);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
@@ -428,8 +429,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
         }
         return;
     }
-    const int block = tasks - 1 - (int)blockIdx.x;
-    const int column = block % p.columns, chunk = block / p.columns, image = column / p.slabs;
+    const int column = (int)blockIdx.x % p.columns, chunk = (int)blockIdx.x / p.columns, image = column / p.slabs;
     const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
@@ -479,22 +479,31 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
             const float dz = kFam == kFamLinear && p.activation == SDXL_ACT_NONE ? d[e] : d[e] * gn_slope<T, kFam>(act, __builtin_fmaf(t, b.a[e], b.beta[e]));
             v[e] = __builtin_fmaf(-t, a2[e], __builtin_fmaf(dz, b.a[e], -a1[e]));
         }
-        V::store(dx, V::pack(v));
+        V::store_through(dx, V::pack(v));
         dx += step_dx;
     });
 }
 
-// ---- One launch, where a set of groups of an image fits a workgroup's registers.
+// ---- One launch, where a set of groups of an image fits a workgroup's registers, eight vectors a thread: [2, 256, 1280] fp16
+// 6.1 us on the device (two passes 9.0), [2, 576, 1280] 8.2 (9.6); with twelve, [2, 1024, 1280], 9.4 (9.2). (The gradients so:
+// their sets are a workgroup's for all images, whose arithmetic is too much for it; [2, 256, 1280] 14.5, two passes 11.4.)
 
 constexpr int kHeldVecs = 32;  // vectors of a set's row at most
 
 // Sums by group over the workgroup, of what its threads have of the two groups that a vector may lie in.
 struct GnHeld {
-    int vecs, rows, group_channels;
+    int vecs, rows;
     float2 *parts, *totals;  // [vecs][rows], [vecs]
     int* group;              // [vecs]: a vector's first group
 
-    // a: of the vector's first group, b: of the next one; returns both groups' sums
+    __device__ __forceinline__ GnHeld(const GnParams& p, char* lds, const GnPlace& at) : vecs(p.vecs), rows(p.rows_at_once), parts((float2*)lds) {
+        totals = parts + vecs * rows;
+        group = (int*)(totals + vecs);
+        if (at.r == 0) group[(int)threadIdx.x] = group_of(p, at.c0);  // (read behind the first barrier)
+    }
+    static size_t bytes(const GnParams& p) { return (size_t)p.vecs * (p.rows_at_once + 1) * 8 + (size_t)p.vecs * 4; }
+
+    // x: of vector v's first group, y: of the next one; returns both groups' sums
     __device__ __forceinline__ float2 sums(const GnPlace& at, int v, float2 mine) const {
         if (at.r < rows) parts[v * rows + at.r] = mine;
         __syncthreads();
@@ -521,16 +530,6 @@ struct GnHeld {
         return all;
     }
 };
-
-// LDS of the held kernels: parts, totals, groups.
-__device__ __forceinline__ GnHeld held_of(const GnParams& p, char* lds, const GnPlace& at) {
-    GnHeld h{p.vecs, p.rows_at_once, p.group_channels, (float2*)lds, nullptr, nullptr};
-    h.totals = h.parts + p.vecs * p.rows_at_once;
-    h.group = (int*)(h.totals + p.vecs);
-    if (at.r == 0) h.group[(int)threadIdx.x] = group_of(p, at.c0);  // (read behind the first barrier)
-    return h;
-}
-size_t held_lds(const GnParams& p) { return (size_t)p.vecs * (p.rows_at_once + 1) * 8 + (size_t)p.vecs * 4; }
 
 // The workgroup's image and set: neighbouring sets, which share cache lines, on one XCD.
 __device__ __forceinline__ int held_task() {
@@ -559,7 +558,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_held_kernel(GnParams p) {
     GnAffine<T> affine;
     load_channels<T>(p.gamma, slab.c0 + at.c0, affine.a);
     load_channels<T>(p.beta, slab.c0 + at.c0, affine.b);
-    const GnHeld held = held_of(p, lds, at);
+    const GnHeld held(p, lds, at);
     const int v = (int)threadIdx.x % p.vecs;
     auto split = [&](const float (&s)[kV]) __attribute__((always_inline)) {
         float2 sum{0.0f, 0.0f};
@@ -647,8 +646,10 @@ int threads_of(int vecs) {
 
 int team_of(int groups, int threads) { return 64 * groups <= threads ? 64 : 16; }
 
-// Workgroups of the two passes (codes: of the second), and the rounds that a chunk has a multiple of.
-constexpr int kFirstTasks = 512, kSecondTasks = 1024, kRowTasks = 512;
+// Workgroups of the two passes (codes: of the second), and the rounds that a chunk has a multiple of. One workgroup a CU
+// reads fast enough and leaves few parts: [2, 131072, 256] bf16 backward 126 us with 512 and 512, 119 with 256 and 512 or
+// 768, 126 with 256 and 256, 152 with 128 and 512.
+constexpr int kFirstTasks = 256, kSecondTasks = 512, kRowTasks = 512;
 constexpr int kBatchRounds = 4;
 
 // `columns` (images by slabs) in chunks of whole rounds of `rows` pixels: `tasks` chunks in all or a little fewer, of
@@ -726,8 +727,8 @@ namespace {
 
 // The vectors that a thread of the held kernels has, 0 where they do not take the call: a set of groups that they can tell
 // apart (a vector lies in two at most) and hold.
-constexpr int kHolds[] = {1, 2, 4, 8, 16};
-int hold_of(const GnParams& p, GnType type, int most, int& slab_groups, int& threads) {
+constexpr int kHolds[] = {1, 2, 4, 8};
+int hold_of(const GnParams& p, GnType type, int& slab_groups, int& threads) {
     const int kV = 16 / elem_of(type);
     slab_groups = slab_groups_of(p, type, kHeldBytes);
     const int64_t vecs = vecs_of(p, type, slab_groups);
@@ -736,7 +737,7 @@ int hold_of(const GnParams& p, GnType type, int most, int& slab_groups, int& thr
     threads = (int)(vecs * p.pixels < kMaxThreads ? (vecs * p.pixels + 63) / 64 * 64 : kMaxThreads);
     const int rows = threads / (int)vecs, needed = (int)((p.pixels + rows - 1) / rows);
     for (int hold : kHolds)
-        if (hold >= needed && hold <= most) return hold;
+        if (hold >= needed) return hold;
     return 0;
 }
 
@@ -753,7 +754,7 @@ GnPlan gn_plan(const GnParams& p, GnType type, GnCall call) {
     if (!fast_of(p, type) || (call == kGnRows && p.channels > 4 * 64 * 8 * kRowVecs)) return {false, 0, 1, p.pixels};
     int slab_groups, threads;
     if (call == kGnForward) {
-        const int hold = hold_of(p, type, 16, slab_groups, threads);
+        const int hold = hold_of(p, type, slab_groups, threads);
         if (hold > 0) return {true, hold, 0, 0};
     }
     slab_groups = slab_groups_of(p, type, kSlabBytes);
@@ -764,19 +765,26 @@ GnPlan gn_plan(const GnParams& p, GnType type, GnCall call) {
 
 namespace {
 
-template <typename T, FfFamily kFam>
-hipError_t launch_held(const GnParams& p, int hold, int threads, hipStream_t stream) {
-    const dim3 grid((unsigned)(p.batch * p.slabs)), block(threads);
-    const size_t lds = held_lds(p);
-    switch (hold) {
-    case 1: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 1>), grid, block, lds, stream, p); break;
-    case 2: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 2>), grid, block, lds, stream, p); break;
-    case 4: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 4>), grid, block, lds, stream, p); break;
-    case 8: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 8>), grid, block, lds, stream, p); break;
-    case 16: hipLaunchKernelGGL((gn_held_kernel<T, kFam, 16>), grid, block, lds, stream, p); break;
-    default: return hipErrorInvalidValue;
-    }
+template <typename T, FfFamily kFam, int kHold>
+hipError_t launch_held_of(const GnParams& p, int threads, hipStream_t stream) {
+    hipLaunchKernelGGL((gn_held_kernel<T, kFam, kHold>), dim3((unsigned)(p.batch * p.slabs)), dim3(threads), GnHeld::bytes(p), stream, p);
     return hipGetLastError();
+}
+
+hipError_t launch_held(const GnParams& params, GnType type, int hold, hipStream_t stream) {
+    GnParams p = params;
+    int slab_groups, threads;
+    hold_of(p, type, slab_groups, threads);
+    lay_out(p, type, slab_groups, threads);
+    return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
+        switch (hold) {
+        case 1: return launch_held_of<T, kFam, 1>(p, threads, stream);
+        case 2: return launch_held_of<T, kFam, 2>(p, threads, stream);
+        case 4: return launch_held_of<T, kFam, 4>(p, threads, stream);
+        case 8: return launch_held_of<T, kFam, 8>(p, threads, stream);
+        }
+        return hipErrorInvalidValue;
+    });
 }
 
 }  // namespace
@@ -787,12 +795,7 @@ hipError_t launch_gn_forward(const GnPlan& plan, const GnParams& params, GnType 
         const hipError_t err = launch_gn_stats_general(p, type, stream);
         return err != hipSuccess ? err : launch_gn_apply_general(p, type, stream);
     }
-    if (plan.hold > 0) {
-        int slab_groups, threads;
-        hold_of(p, type, plan.hold, slab_groups, threads);
-        lay_out(p, type, slab_groups, threads);
-        return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() { return launch_held<T, kFam>(p, plan.hold, threads, stream); });
-    }
+    if (plan.hold > 0) return launch_held(p, type, plan.hold, stream);
     const int slab_groups = slab_groups_of(p, type, kSlabBytes), threads = threads_of((int)vecs_of(p, type, slab_groups));
     lay_out(p, type, slab_groups, threads);
     {

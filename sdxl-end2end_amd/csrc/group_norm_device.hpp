@@ -41,6 +41,11 @@ struct GnVec {
     static constexpr int kV = 16 / (int)sizeof(T);
     static __device__ __forceinline__ u32x4 load(const char* at) { return ((const Unaligned<sizeof(T)>*)at)->v; }
     static __device__ __forceinline__ void store(char* at, u32x4 d) { ((Unaligned<sizeof(T)>*)at)->v = d; }
+    // what nobody reads again before the caches are full of it
+    static __device__ __forceinline__ void store_through(char* at, u32x4 d) {
+        typedef u32x4 __attribute__((aligned(2))) u32x4_element;
+        __builtin_nontemporal_store(d, (u32x4_element*)at);
+    }
     static __device__ __forceinline__ void unpack(u32x4 d, float (&v)[kV]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
