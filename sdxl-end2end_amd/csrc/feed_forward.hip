@@ -49,6 +49,21 @@ constexpr TileCost kTiles[kFfTiles] = {{256, 320, 1.60f, 0.0f, 15.0f}, {256, 256
                                        {128, 128, 0.45f, 0.0f, 5.5f},
                                        {64, 128, 0.35f, 0.58f, 5.0f},  {64, 64, 0.30f, 0.46f, 4.5f}};
 
+// The same of 8-bit integers, by stages of 128, and a tile more: their stages take the same bytes and nearly the same time for
+// twice the products, so that starts and ends (a conversion and a scale more for every sum) weigh more. Measured in fp16 out:
+//   256 x 320  gated [2048, 1280] -> 2 x 5120 32 us (256 x 256: 45, 128 x 256: 42)
+//   256 x 256  gated [8192, 2048] -> 2 x 5456 195 (1.88 POP/s), [16384, 2048] x [2048, 2048] 76-80
+//   256 x 192  [8192, 5120] x [1280, 5120] 66 (256 x 256: 72, 128 x 192: 73)
+//   128 x 256  [2048, 1280] x [3840, 1280] 19 (256 x 256: 25)
+//    64 x 128  [4940, 640] x [640, 640] 9.2 (128 x 128: 10.4)
+//    64 x  64  [154, 1280] x [5120, 1280] 7.7 (32 x 32, shared depth: 10.1)
+// On a whole chip the matrix cores' power holds the long products back, the library's too (8192 cubed 1.97 POP/s).
+constexpr TileCost kI8Tiles[kFfI8Tiles] = {{256, 320, 1.65f, 0.0f, 16.5f}, {256, 256, 1.47f, 0.0f, 11.8f},
+                                           {128, 256, 0.69f, 0.0f, 10.2f}, {128, 192, 0.55f, 0.0f, 9.0f},
+                                           {128, 128, 0.44f, 0.0f, 8.3f},
+                                           {64, 128, 0.39f, 0.55f, 6.5f},  {64, 64, 0.33f, 0.49f, 4.4f},
+                                           {256, 192, 1.05f, 0.0f, 11.3f}};
+
 // Time of two kinds of tasks, a tasks of a_time each before b of b_time, on CUs that take the next task when
 // they are free: the CUs as groups that become free together.
 float list_time(int64_t a, float a_time, int64_t b, float b_time, int64_t cus) {
@@ -104,6 +119,7 @@ FfDeepId deep_choice(const FfParams& p, FfEpilogue epilogue, int64_t cus, bool s
         id = kFfDeep64x4;
         time = large_time;
     }
+    if (p.i8 != 0) time += 2.0f;
     return id;
 }
 
@@ -111,9 +127,9 @@ int choose_tile(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int64_t cus,
     const int64_t cols = epilogue == kFfGated || epilogue == kFfGatedDz ? 2 * p.cols : p.cols;
     const float stages = (float)ff_stages(p);
     int best = 0;
-    for (int t = 0; t < kFfTiles; ++t) {
+    for (int t = 0; t < (p.i8 != 0 ? (int)kFfI8Tiles : (int)kFfTiles); ++t) {
         if (j_fp8 && t == kFf128x128) continue;  // its waves share a stage's depth, E4M3 codes come in pairs of steps
-        const TileCost& c = kTiles[t];
+        const TileCost& c = p.i8 != 0 ? kI8Tiles[t] : kTiles[t];
         const int64_t tiles = ((p.rows + c.rows - 1) / c.rows) * ((cols + c.cols - 1) / c.cols);
         float time;
         if (c.pair == 0.0f) {

@@ -65,8 +65,8 @@ inline int64_t ff_stages(const FfParams& p) { return p.i8 != 0 ? (p.depth + 127)
 hipError_t launch_ff_general(const FfParams& p, FfEpilogue epilogue, bool i_transposed, bool j_transposed, bool bf16,
                              bool j_fp8, hipStream_t stream);
 
-// Tiles of the tiled kernel, rows x columns of sums.
-enum FfTileId : int { kFf256x320, kFf256x256, kFf128x256, kFf128x192, kFf128x128, kFf64x128, kFf64x64, kFfTiles };
+// Tiles of the tiled kernel, rows x columns of sums; the last for 8-bit integers alone.
+enum FfTileId : int { kFf256x320, kFf256x256, kFf128x256, kFf128x192, kFf128x128, kFf64x128, kFf64x64, kFfTiles, kFf256x192 = kFfTiles, kFfI8Tiles };
 
 // Tiles whose waves share the depth (feed_forward_deep.hip), side x waves.
 enum FfDeepId : int { kFfDeep32x8, kFfDeep32x4, kFfDeep64x4 };

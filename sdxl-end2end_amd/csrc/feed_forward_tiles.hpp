@@ -77,6 +77,8 @@ struct FfTile {
         const int stages = kRing * stage_bytes(j_fp8), exchange = kWI * kWJ * kWK * (kWK - 1) * 4096;
         return stages > exchange ? stages : exchange;
     }
+    // 8-bit integers: behind them the columns' scales and biases
+    static constexpr int constant_bytes(bool i8) { return i8 ? kBJ * 8 : 0; }
     // workgroups that one CU's LDS and registers (512 per lane and SIMD) hold
     static constexpr int waves_per_simd(bool j_fp8) {
         const int by_lds = kWaves / 4 * (160 * 1024 / smem_bytes(j_fp8));
@@ -343,6 +345,28 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         }
     };
 
+    // 8-bit integers: thread t's column constants and the lane's row scales, loaded ahead of the main loop and put down (read)
+    // behind it. Loaded tile by tile there, each round of them waited for the caches: gated [8192, 2048] -> 2 x 5456 228 us, 200 so.
+    constexpr int kConstants = F::kI8 ? (kCols + 64 * kWaves - 1) / (64 * kWaves) : 0;
+    float column[kConstants > 0 ? kConstants : 1][4], row_scale[F::kI8 ? kMI : 1];
+    if constexpr (F::kI8) {
+#pragma unroll
+        for (int n = 0; n < kConstants; ++n) {
+            const int64_t c = j0 + n * 64 * kWaves + threadIdx.x;
+            const bool there = c < p.cols && n * 64 * kWaves + (int)threadIdx.x < kCols;
+            const int64_t v = (kGated ? value_row : 0) + c, g = gate_row + c;
+            column[n][0] = there ? p.j_scale[v] : 0.0f;
+            column[n][1] = there && p.bias != nullptr ? (float)((const Out*)p.bias)[v] : 0.0f;
+            column[n][2] = kGated && there ? p.j_scale[g] : 0.0f;
+            column[n][3] = kGated && there && p.bias != nullptr ? (float)((const Out*)p.bias)[g] : 0.0f;
+        }
+#pragma unroll
+        for (int s = 0; s < kMI; ++s) {
+            const int64_t i = i0 + 32 * (kWI * s + wi) + col;
+            row_scale[s] = i < p.rows ? p.i_scale[i] : 0.0f;
+        }
+    }
+
     Acc acc[kMJ][kMI];
 #pragma unroll
     for (int j = 0; j < kMJ; ++j)
@@ -523,9 +547,20 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         if (j0 + kCols >= p.cols && wj == 0 && hf == 0 && (int64_t)row < i_rows)
             for (int64_t z = first; z < p.out_cols_padded; ++z) ((Out*)p.out)[(i0 + row) * p.ld_out + z] = (Out)0.0f;
     };
-    // (rows past the end: 0)
-    const auto row_scales = __builtin_amdgcn_make_buffer_rsrc((void*)((uintptr_t)p.i_scale + (uintptr_t)(i0 * 4)), 0,
-                                                              F::kI8 ? (int)(i_rows * 4) : 0, 0x00020000);
+    lds_float* const constant = (lds_float*)(smem + Tile::smem_bytes(kJFp8));  // [4][kCols]: scale, bias, the gate's
+    if constexpr (F::kI8) {
+#pragma unroll
+        for (int n = 0; n < kConstants; ++n) {
+            const int c = n * 64 * kWaves + threadIdx.x;
+            if (c < kCols) {
+#pragma unroll
+                for (int e = 0; e < (kGated ? 4 : 2); ++e) constant[e * kCols + c] = column[n][e];
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
     const auto dout = rows_window(p.dout, p.ld_dout, j0), residual = rows_window(p.residual, p.ld_res, j0);
     const auto out = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? value_row : 0) + j0);
     const auto out_g = rows_window(p.out, p.ld_out, (kEpi == kFfGatedDz ? gate_row : 0) + j0);
@@ -562,6 +597,25 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
     // the columns' constants of the tile from column c0 of C's tile on
     auto constants = [&](int c0) __attribute__((always_inline)) {
         if constexpr (kEpi == kFfStore) return;
+        if constexpr (F::kI8) {
+            auto from = [&](int e, int c, float (&v)[4]) __attribute__((always_inline)) {
+                typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+                const f32x4 d = *(const lds_f32x4*)(constant + e * kCols + c);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q] = d[q];
+            };
+#pragma unroll
+            for (int u = 0; u < kHalves; ++u) {
+                const int c = c0 + 8 * u + 4 * hf;
+                from(0, c, scale[u]);
+                from(1, c, bias[u]);
+                if constexpr (kGated) {
+                    from(2, c, scale_g[u]);
+                    from(3, c, bias_g[u]);
+                }
+            }
+            return;
+        }
         const int64_t first = kGated ? value_row : 0;
         const auto b = vector_window(p.bias, first + j0, 2), sc = vector_window(p.j_scale, first + j0, 4);
         const auto bg = vector_window(p.bias, gate_row + j0, 2), sg = vector_window(p.j_scale, gate_row + j0, 4);
@@ -583,12 +637,11 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
         }
     };
     // one 32 x 32 tile of sums: the lane's row of C's tile, first column c0, what read_tile gave
-    auto finish = [&]<FfFamily kFam>(const Acc& tile_sums, uint32_t row, int c0, const u32x4 (&in)[kSets]) __attribute__((always_inline)) {
+    auto finish = [&]<FfFamily kFam>(const Acc& tile_sums, uint32_t row, [[maybe_unused]] float of_row, int c0, const u32x4 (&in)[kSets]) __attribute__((always_inline)) {
         f32x16 z;
         if constexpr (F::kI8) {  // with the row's scale
-            const float row_scale = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(row_scales, row * 4, 0, 0));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = (float)tile_sums[r] * row_scale;
+            for (int r = 0; r < 16; ++r) z[r] = (float)tile_sums[r] * of_row;
         } else {
             z = tile_sums;
         }
@@ -661,11 +714,11 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     if constexpr (kShare) {
                         store_share(acc[t][s], row, c0);
                     } else if constexpr (kAhead) {
-                        finish.template operator()<kFam>(acc[t][s], row, c0, ahead[t][s]);
+                        finish.template operator()<kFam>(acc[t][s], row, row_scale[F::kI8 ? s : 0], c0, ahead[t][s]);
                     } else {
                         u32x4 in[kSets];
                         if constexpr (kReads) read_tile(row, c0, in);
-                        finish.template operator()<kFam>(acc[t][s], row, c0, in);
+                        finish.template operator()<kFam>(acc[t][s], row, row_scale[F::kI8 ? s : 0], c0, in);
                     }
                 }
             }
@@ -721,7 +774,7 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
                     } else {
                         u32x4 in[kSets];
                         if constexpr (kReads) read_tile(row, c0, in);
-                        finish.template operator()<kFam>(sum, row, c0, in);
+                        finish.template operator()<kFam>(sum, row, row_scale[F::kI8 ? q % kMI : 0], c0, in);
                     }
                 }
             }
@@ -772,14 +825,14 @@ __device__ __forceinline__ void ff_tile(const FfParams& p, int task_id, char* sm
 
 template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
 __global__ __launch_bounds__(64 * Tile::kWaves, Tile::waves_per_simd(kJFp8)) void ff_tile_kernel(FfParams p) {
-    __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
+    __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8) + Tile::constant_bytes(FfType<T>::kI8)];
     ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi>(p, blockIdx.x, smem);
 }
 
 // Rows that 16-byte accesses do not divide.
 template <typename T, bool kIT, bool kJT, bool kJFp8, typename Tile, FfEpilogue kEpi>
 __global__ __launch_bounds__(64 * Tile::kWaves, Tile::kMI * Tile::kMJ > 1 ? 2 : 4) void ff_staged_kernel(FfParams p) {
-    __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8)];
+    __shared__ __attribute__((aligned(1024))) char smem[Tile::smem_bytes(kJFp8) + Tile::constant_bytes(FfType<T>::kI8)];
     ff_tile<T, kIT, kJT, kJFp8, Tile, kEpi, kEpi == kFfStore, true>(p, blockIdx.x, smem);
 }
 
@@ -835,6 +888,7 @@ hipError_t ff_launch_pair(FfParams w, FfParams x, bool w_first, hipStream_t stre
 // The tiles that the launcher chooses from (feed_forward.hip), and their products by direction.
 typedef FfTile<4, 2, 1, 2, 5, 2, 2> FfTile256x320;
 typedef FfTile<4, 2, 1, 2, 4, 2, 2> FfTile256x256;
+typedef FfTile<4, 2, 1, 2, 3, 2, 2> FfTile256x192;  // 8-bit integers alone
 typedef FfTile<2, 4, 1, 2, 2, 3, 2> FfTile128x256;
 typedef FfTile<4, 2, 1, 1, 3, 3, 2> FfTile128x192;
 typedef FfTile<2, 2, 2, 2, 2, 4, 2> FfTile128x128;
@@ -902,6 +956,7 @@ hipError_t ff_i8_forward(const FfParams& p, FfEpilogue epilogue, int tile, hipSt
     switch (tile) {
     case kFf256x320: return by_tile.template operator()<FfTile256x320>();
     case kFf256x256: return by_tile.template operator()<FfTile256x256>();
+    case kFf256x192: return by_tile.template operator()<FfTile256x192>();
     case kFf128x256: return by_tile.template operator()<FfTile128x256>();
     case kFf128x192: return by_tile.template operator()<FfTile128x192>();
     case kFf128x128: return by_tile.template operator()<FfTile128x128>();
