@@ -67,7 +67,8 @@ typedef struct sdxl_i8_desc {
 } sdxl_i8_desc;
 
 /* Workspace of the calls below, 256-byte aligned: codes and scales of 16-bit tokens (0 for codes,
- * and for a descriptor that the call refuses). */
+ * for up to four tokens, whose product quantises them on the way, and for a descriptor that the call
+ * refuses). */
 size_t sdxl_linear_i8_workspace_bytes(const sdxl_i8_desc* desc);
 size_t sdxl_gated_linear_i8_workspace_bytes(const sdxl_i8_desc* desc);
 

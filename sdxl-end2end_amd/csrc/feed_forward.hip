@@ -306,7 +306,8 @@ bool ff_tiled_supported(const FfParams& p, FfEpilogue epilogue, bool i_transpose
     if (!ff_staged_supported(p, epilogue, i_transposed, j_transposed, j_fp8)) return false;
     // rows in whole 16-byte chunks: the depth, or the columns of an operand that is read by columns
     const int64_t i_row = p.i_row != 0 ? p.i_row : i_transposed ? p.rows : p.depth;
-    if (p.i8 != 0) return aligned(p.ip, 16) && aligned(p.jp, 16) && p.ld_i % 16 == 0 && p.ld_j % 16 == 0 && p.depth % 16 == 0;
+    if (p.i8 != 0)  // (tokens are quantised on the way)
+        return aligned(p.jp, 16) && p.ld_j % 16 == 0 && p.depth % 16 == 0 && (p.i8 == kFfI8Tokens || (aligned(p.ip, 16) && p.ld_i % 16 == 0));
     if (!aligned(p.ip, 16) || !aligned(p.jp, 16) || p.ld_i % 8 != 0 || p.ld_j % (j_fp8 ? 16 : 8) != 0) return false;
     return i_row % 8 == 0 && (j_transposed ? p.cols % 8 == 0 : p.depth % (j_fp8 ? 16 : 8) == 0);
 }

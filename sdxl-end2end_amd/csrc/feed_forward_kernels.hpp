@@ -45,10 +45,12 @@ struct FfParams {
     int64_t ld_partial;  // cols, up to a multiple of 8
     float* partial;
     // both operands hold 8-bit integers (forward epilogues): ld_i, ld_j and depth in bytes, i_scale the fp32 scale of every
-    // I row, j_scale that of every J row
+    // I row, j_scale that of every J row; or an FfI8: I holds 16-bit values, which the kernel of few rows quantises
     int32_t i8;
     const float* i_scale;
 };
+
+enum FfI8 : int32_t { kFfI8None = 0, kFfI8Codes = 1, kFfI8Tokens = 2 };
 
 // The joining pass of a product whose depth was split.
 struct FfJoin {
@@ -107,6 +109,8 @@ hipError_t launch_ff_gradients(const FfGradients& plan, const FfParams* dw, cons
 // Few rows (feed_forward_rows.hip): waves of a workgroup.
 bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8);
 int ff_rows_waves(const FfParams& p, bool gated);
+// Whether it takes 16-bit tokens of a product of 8-bit weights (i8: kFfI8Tokens).
+bool ff_rows_tokens(const FfParams& p, FfEpilogue epilogue);
 hipError_t launch_ff_rows(const FfParams& p, FfEpilogue epilogue, int waves, bool staged, bool bf16, bool j_fp8,
                           hipStream_t stream);
 

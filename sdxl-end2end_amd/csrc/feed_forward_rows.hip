@@ -15,13 +15,22 @@
 // 1280], a plain read of those bytes 5.7, this 5.7 on the device.) Rows that 16-byte
 // accesses do not divide come through registers, as many blocks at once: [16,
 // 5127] x [1280, 5127] 20 us, [1, 1283] x [5120, 1283] 6.7.
+//
+// 8-bit weights with up to four tokens in 16 bits (kTokens): every workgroup quantises the tokens
+// itself, into LDS, while its weights are on their way, instead of a launch before and a workspace:
+// gated [1, 1280] -> 2 x 5120 13.4 us a call so, 8.0 here.
 #include <hip/hip_runtime.h>
 
 #include "feed_forward_device.hpp"
+#include "int8_device.hpp"
 #include "feed_forward_kernels.hpp"
 
 namespace sdxl_hip {
 namespace {
+
+typedef __attribute__((address_space(3))) float lds_float;
+
+constexpr int kMaxTokens = 4, kMaxTokenDepth = 8192;
 
 template <typename T, typename Acc4>
 __device__ __forceinline__ Acc4 mfma16(u32x4 a, u32x4 b, Acc4 c) {
@@ -33,7 +42,7 @@ __device__ __forceinline__ Acc4 mfma16(u32x4 a, u32x4 b, Acc4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, bool kJFp8, int kWaves, bool kGated, bool kStaged>
+template <typename T, bool kJFp8, int kWaves, bool kGated, bool kStaged, bool kTokens = false>
 __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
     using F = FfType<T>;
     using Out = typename F::Out;
@@ -63,6 +72,57 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
     const int row = kJFp8 ? lane >> 2 : lane >> 3;
     const uint32_t w_at[2] = {w_offset(row), kJFp8 ? 0u : w_offset(8 + row)};
     const int chunk_at[2] = {kJFp8 ? (lane & 3) ^ ((row >> 2) & 3) : (lane & 7) ^ swz(row), (lane & 7) ^ swz(8 + row)};
+    // kTokens: rows of codes behind the blocks, as many bytes as the blocks' depth and 16 more, then the rows' scales
+    const int code_row = blocks * 128 + 16;
+    char* const codes = smem + (blocks < 32 ? (blocks + kWaves - 1) / kWaves * kWaves : 32) * kBlockBytes;
+    lds_float* const code_scale = (lds_float*)(codes + kMaxTokens * code_row);
+    auto quantise = [&]() __attribute__((always_inline)) {
+        constexpr uint32_t kInf = 0x7f800000u;
+        lds_float* const part = code_scale + kMaxTokens;
+        const int vecs = blocks * 16;  // of 8 values, zeros past the depth
+        for (int row = 0; row < (int)p.rows; ++row) {
+            const char* x = (const char*)p.ip + row * p.ld_i * 2;
+            auto values = [&](int v, float (&f)[8]) __attribute__((always_inline)) {
+                const int valid = depth - 8 * v;
+                const u32x4 d = settle_chunk<8>(fetch_chunk<8>(x + 16 * v, valid), valid);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[2 * e] = F::lo(d[e]), f[2 * e + 1] = F::hi(d[e]);
+            };
+            auto largest = [&](uint32_t most) __attribute__((always_inline)) {
+                uint32_t top = 0;
+                for (int v = (int)threadIdx.x; v < vecs; v += 64 * kWaves) {
+                    float f[8];
+                    values(v, f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t m = __float_as_uint(f[e]) & 0x7fffffffu;
+                        top = max(top, m <= most ? m : 0);
+                    }
+                }
+                auto larger = [](float a, float b) __attribute__((always_inline)) {
+                    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+                };
+                const float mine = reduce64(__uint_as_float(top), larger);
+                __syncthreads();  // the last values are read
+                if (lane == 0) part[wave] = mine;
+                __syncthreads();
+                float all = part[0];
+                for (int w = 1; w < kWaves; ++w) all = larger(all, part[w]);
+                return __float_as_uint(all);
+            };
+            uint32_t top = largest(0xffffffffu);
+            const bool nan = top > kInf;
+            if (top >= kInf) top = largest(kInf - 1);
+            const float scale = i8_scale(__uint_as_float(top), nan), over = 1.0f / scale, limit = 127.0f * scale;
+            for (int v = (int)threadIdx.x; v < vecs; v += 64 * kWaves) {
+                float f[8];
+                values(v, f);
+                *(lds_u32x2*)(codes + row * code_row + 8 * v) = i8_codes(f, scale, over, limit);
+            }
+            if (threadIdx.x == 0) code_scale[row] = scale;
+        }
+        __syncthreads();
+    };
     const uint32_t x_at = r16 < p.rows ? (uint32_t)(r16 * p.ld_i * kXElem) : kOutside;
 
     const uint32_t lds0 = lds_addr(smem);
@@ -80,7 +140,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
             for (int b = 0; b < kBlocks; ++b) {
                 const int block = first + b * kWaves + wave;
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+                for (int q = 0; q < (kTokens ? 0 : 2); ++q)
                     x[b][q] = fetch_chunk<kChunk>((const char*)p.ip + (r16 * p.ld_i + kDepth * block + kChunk * (4 * q + g)) * kXElem, x_valid(block, q));
 #pragma unroll
                 for (int h = 0; h < kH; ++h)
@@ -90,7 +150,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
             for (int b = 0; b < kBlocks; ++b) {
                 const int block = first + b * kWaves + wave;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) x[b][q] = settle_chunk<kChunk>(x[b][q], x_valid(block, q));
+                for (int q = 0; q < (kTokens ? 0 : 2); ++q) x[b][q] = settle_chunk<kChunk>(x[b][q], x_valid(block, q));
                 if (block < blocks) {  // (LDS holds no others)
 #pragma unroll
                     for (int h = 0; h < kH; ++h)
@@ -98,11 +158,12 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (kTokens && first == 0) quantise();
         } else {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const int block = first + b * kWaves + wave;
-                if (block < blocks) {
+                if (!kTokens && block < blocks) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const int k = kDepth * block + kChunk * (4 * q + g);
@@ -122,6 +183,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
                     }
                 }
             }
+            if (kTokens && first == 0) quantise();  // (its reads wait for the weights too)
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
 #pragma unroll
@@ -141,7 +203,11 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
                     for (int q = 0; q < 2; ++q) a[q] = *(const lds_u32x4*)(from + r16 * 128 + (((4 * q + g) ^ swz(r16)) << 4));
                 }
 #pragma unroll
-                for (int q = 0; q < 2; ++q) acc = mfma16<T>(a[q], x[b][q], acc);
+                for (int q = 0; q < 2; ++q) {
+                    if constexpr (kTokens)  // (columns past the rows: any)
+                        x[b][q] = *(const lds_u32x4*)(codes + (r16 < p.rows ? r16 : 0) * code_row + kDepth * (first + b * kWaves + wave) + kChunk * (4 * q + g));
+                    acc = mfma16<T>(a[q], x[b][q], acc);
+                }
             }
         }
     }
@@ -157,7 +223,7 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
         for (int v = 0; v < kWaves; ++v) s += *(const lds_acc4*)(smem + (v * 64 + from) * 16);
         return s;
     };
-    const float row_scale = F::kI8 && r16 < p.rows ? p.i_scale[r16] : 1.0f;
+    const float row_scale = kTokens ? code_scale[r16 < p.rows ? r16 : 0] : F::kI8 && r16 < p.rows ? p.i_scale[r16] : 1.0f;
     auto z_of = [&](float sum, int64_t row) {
         if constexpr (F::kI8) sum *= row_scale;
         if (p.j_scale != nullptr) sum *= p.j_scale[row];
@@ -188,6 +254,16 @@ __global__ __launch_bounds__(64 * kWaves) void ff_rows_kernel(FfParams p) {
 
 template <typename T, bool kJFp8, int kWaves, bool kStaged>
 hipError_t launch(const FfParams& p, bool gated, hipStream_t stream) {
+    if constexpr (FfType<T>::kI8) {
+        if (p.i8 == kFfI8Tokens) {
+            const int64_t blocks = ff_stages(p), held = blocks < 32 ? (blocks + kWaves - 1) / kWaves * kWaves : 32;
+            const size_t lds = (size_t)held * 2048 + kMaxTokens * ((size_t)blocks * 128 + 16) + (kMaxTokens + kWaves) * 4;
+            const dim3 grid((unsigned)(gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16)), block(64 * kWaves);
+            if (gated) hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, true, kStaged, true>), grid, block, lds, stream, p);
+            else hipLaunchKernelGGL((ff_rows_kernel<T, kJFp8, kWaves, false, kStaged, true>), grid, block, lds, stream, p);
+            return hipGetLastError();
+        }
+    }
     const dim3 grid((unsigned)(gated ? (p.cols + 7) / 8 : (p.cols + 15) / 16)), block(64 * kWaves);
     const int64_t blocks = (p.depth + 128 / FfType<T>::kElem - 1) / (128 / FfType<T>::kElem), held = blocks < 32 ? (blocks + kWaves - 1) / kWaves * kWaves : 32;
     const size_t lds = (size_t)held * (kJFp8 ? 1024 : 2048);  // (the sums take 1 KiB a wave)
@@ -213,6 +289,10 @@ bool ff_rows_supported(const FfParams& p, FfEpilogue epilogue, bool j_fp8) {
     const int64_t w_rows = epilogue == kFfGated ? 2 * p.cols : p.cols;
     return (epilogue == kFfLinear || epilogue == kFfGated) && p.rows <= 16 &&
            w_rows * p.ld_j * (j_fp8 || p.i8 != 0 ? 1 : 2) < (int64_t{1} << 31) && ff_staged_supported(p, epilogue, false, false, j_fp8);
+}
+
+bool ff_rows_tokens(const FfParams& p, FfEpilogue epilogue) {
+    return p.rows <= kMaxTokens && p.depth <= kMaxTokenDepth && p.ld_i < (1 << 20) && ff_rows_supported(p, epilogue, false);
 }
 
 // 2048 waves in all where there are blocks for them

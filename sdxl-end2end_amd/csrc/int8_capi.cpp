@@ -108,13 +108,32 @@ size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 // The workspace of 16-bit tokens: their codes, in rows that 16-byte accesses divide, then the scales.
 int64_t code_stride(const Call& c) { return (c.k + 15) / 16 * 16; }
 size_t code_bytes(const Call& c) { return round256((size_t)c.m * (size_t)code_stride(c)); }
-size_t workspace_of(const Call& c) {
-    return !c.tokens || c.m == 0 || c.n == 0 ? 0 : code_bytes(c) + round256((size_t)c.m * 4);
+// The product of the call, without its tensors; tokens: its x is theirs.
+FfParams product_of(const Call& c, const sdxl_i8_desc* d, bool tokens) {
+    FfParams p{};
+    p.i8 = tokens ? sdxl_hip::kFfI8Tokens : sdxl_hip::kFfI8Codes;
+    p.ld_i = c.tokens && !tokens ? code_stride(c) : c.ldx;
+    p.ld_j = c.ldw;
+    p.ld_res = c.ldr;
+    p.ld_out = c.ldo;
+    p.rows = c.m;
+    p.cols = c.n;
+    p.depth = c.k;
+    p.activation = d->activation;
+    p.gate_first = d->gate_first;
+    return p;
+}
+// Tokens that the product's kernel quantises itself.
+bool quantises(const Call& c, const sdxl_i8_desc* d, bool gated) {
+    return c.tokens && ff_rows_tokens(product_of(c, d, true), gated ? sdxl_hip::kFfGated : sdxl_hip::kFfLinear);
+}
+size_t workspace_of(const Call& c, const sdxl_i8_desc* d, bool gated) {
+    return !c.tokens || c.m == 0 || c.n == 0 || quantises(c, d, gated) ? 0 : code_bytes(c) + round256((size_t)c.m * 4);
 }
 
 size_t workspace_bytes_of(const sdxl_i8_desc* d, bool gated, const char* name) {
     Call c;
-    return resolve(d, gated, name, c) == SDXL_STATUS_OK ? workspace_of(c) : 0;
+    return resolve(d, gated, name, c) == SDXL_STATUS_OK ? workspace_of(c, d, gated) : 0;
 }
 
 sdxl_status product(const sdxl_i8_desc* d, bool gated, const char* name, const void* x, const float* x_scale,
@@ -131,7 +150,7 @@ sdxl_status product(const sdxl_i8_desc* d, bool gated, const char* name, const v
     if (!aligned(x, c.tokens ? 2 : 1) || !aligned(x_scale, 4) || !aligned(w_scale, 4) || !aligned(bias, 2) ||
         !aligned(residual, 2) || !aligned(out, 2))
         return fail(name, SDXL_STATUS_UNSUPPORTED, "tensor not aligned to its elements");
-    const size_t need = workspace_of(c);
+    const size_t need = workspace_of(c, d, gated);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "workspace missing, small or misaligned");
     const Area to = matrix(out, c.m, c.n, c.ldo), work = vector(need > 0 ? workspace : nullptr, (int64_t)need, 1);
@@ -144,7 +163,10 @@ sdxl_status product(const sdxl_i8_desc* d, bool gated, const char* name, const v
     if ((!in_place && overlap(to, res)) || overlap(work, res) || overlap(work, to))
         return fail(name, SDXL_STATUS_INVALID_ARGUMENT, "one of out, residual and the workspace overlaps another");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
-    if (c.tokens) {
+    FfParams p = product_of(c, d, quantises(c, d, gated));
+    p.ip = x;
+    p.i_scale = x_scale;
+    if (need > 0) {
         I8RowsParams q{};
         q.x = x;
         q.q = static_cast<int8_t*>(workspace);
@@ -155,28 +177,14 @@ sdxl_status product(const sdxl_i8_desc* d, bool gated, const char* name, const v
         q.ld_q = q.q_cols = code_stride(c);
         const hipError_t err = launch_i8_rows(q, c.bf16, stream);
         if (err != hipSuccess) return launched(err, name);
-        x = q.q;
-        x_scale = q.q_scale;
-        c.ldx = q.ld_q;
+        p.ip = q.q;
+        p.i_scale = q.q_scale;
     }
-    FfParams p{};
-    p.ip = x;
     p.jp = w;
-    p.ld_i = c.ldx;
-    p.ld_j = c.ldw;
-    p.i8 = 1;
-    p.i_scale = x_scale;
     p.j_scale = w_scale;
     p.bias = bias;
     p.residual = residual;
-    p.ld_res = c.ldr;
     p.out = out;
-    p.ld_out = c.ldo;
-    p.rows = c.m;
-    p.cols = c.n;
-    p.depth = c.k;
-    p.activation = d->activation;
-    p.gate_first = d->gate_first;
     const sdxl_hip::FfEpilogue epilogue = gated ? sdxl_hip::kFfGated : sdxl_hip::kFfLinear;
     const sdxl_hip::FfChoice choice = sdxl_hip::choose_ff(p, epilogue, false, sdxl_hip_compute_units());
     return launched(sdxl_hip::launch_ff(choice, p, epilogue, c.bf16, false, stream), name);

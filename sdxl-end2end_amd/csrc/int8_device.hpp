@@ -28,6 +28,19 @@ __device__ __forceinline__ uint32_t i8_code_bits(float v, float scale, float ove
     return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, scale, v), over, q) + 12582912.0f);  // 3 * 2^22
 }
 
+// Eight codes: the low bytes of two, then of all.
+__device__ __forceinline__ u32x2 i8_codes(const float (&v)[8], float scale, float over, float limit) {
+    u32x2 d;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t c[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = i8_code_bits(__builtin_amdgcn_fmed3f(v[4 * h + e], -limit, limit), scale, over);
+        d[h] = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u) | __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u) << 16;
+    }
+    return d;
+}
+
 struct __attribute__((packed, aligned(1))) Unaligned8 {
     u32x2 v;
 };
@@ -84,19 +97,7 @@ struct I8Row {
         const float scale = i8_scale(__uint_as_float(top), nan), over = 1.0f / scale, limit = 127.0f * scale;
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-            if (has(i)) {
-                uint32_t d[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t c[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c[e] = i8_code_bits(__builtin_amdgcn_fmed3f(v[i][4 * h + e], -limit, limit), scale, over);
-                    // low bytes of two, then of all
-                    const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
-                    d[h] = lo | hi << 16;
-                }
-                ((Unaligned8*)(q + column(i)))->v = u32x2{d[0], d[1]};
-            }
+            if (has(i)) ((Unaligned8*)(q + column(i)))->v = i8_codes(v[i], scale, over, limit);
         }
         if (cols + lane < q_cols) q[cols + lane] = 0;  // (fewer than 16)
         return scale;

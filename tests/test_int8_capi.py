@@ -104,6 +104,8 @@ def test_workspaces():
     assert sh.linear_i8_workspace_bytes(10, 64, 100) == 1280 + 256  # codes in rows of 112 bytes, scales
     assert sh.linear_i8_workspace_bytes(10, 64, 100, gated=True, dtype=sh.BF16) == 1280 + 256
     assert sh.load().sdxl_linear_i8_workspace_bytes(ctypes.byref(desc())) == 0  # codes are there already
+    assert sh.linear_i8_workspace_bytes(4, 64, 100) == 0  # quantised by the product
+    assert sh.linear_i8_workspace_bytes(4, 64, 8) > 0 and sh.linear_i8_workspace_bytes(4, 64, 9000) > 0  # not by the general kernel, not so deep
 
 
 def quantize(norm, rows=4, cols=64, dtype=sh.F16, ldx=0, ldq=0, eps=1e-5, **given):
