@@ -2,8 +2,9 @@
 // the reference's Ops (include/sdxl/cuda/ops.hpp:92-97) and the operators of
 // the UNet transformer block's attention sublayer (layer_norm, linear with
 // fp16 or FP8 E4M3 weights, FP8 weight packing) and of its feed-forward half
-// (gated projection, linear with an activation), implemented over the C ABI
-// (include/sdxl_hip/attention.h, sublayer.h, feed_forward.h).
+// (gated projection, linear with an activation), group norm and the 8-bit integer
+// linears, implemented over the C ABI (include/sdxl_hip/attention.h, sublayer.h,
+// feed_forward.h, group_norm.h, int8.h).
 #pragma once
 
 #include "sdxl_hip/runtime.hpp"
@@ -13,7 +14,7 @@
 
 namespace sdxl::hip {
 
-// Activations of the feed-forward operators (sdxl_activation in feed_forward.h).
+// Activations of the feed-forward operators and of group norm (sdxl_activation in feed_forward.h).
 enum class Activation { None, Relu, Gelu, GeluTanh, QuickGelu, Silu };
 
 class Ops final {
@@ -86,12 +87,14 @@ public:
     // value * act(gate) with [value | gate] = input . weight^T + bias (the reference's GEGLU
     // projection, unet.cpp:98-149, both halves and their product in one kernel): input [..., K]
     // fp16 or bf16, weight [2N, K] of its type or Float8E4M3 with attached scales, optional bias
-    // [2N]; gate_first: [gate | value]. Any sizes. Returns [..., N].
+    // [2N]; gate_first: [gate | value]. Any sizes. Returns [..., N]. Int8 weights (pack_int8) take
+    // the 8-bit integer product: the input is quantised by row, or Int8 codes with scales itself
+    // (group_norm_int8, layer_norm_int8, pack_int8; the output is of the bias's type, else fp16).
     [[nodiscard]] Tensor gated_linear(const Tensor& input, const Tensor& weight, const Tensor* bias = nullptr,
                                       Activation activation = Activation::Gelu, bool gate_first = false) const;
 
     // act(input . weight^T + bias) + residual in one kernel (the text encoder's MLP, the time
-    // embedding): weight [N, K] as above, optional bias [N] and residual [..., N]. Any sizes.
+    // embedding): input and weight [N, K] as above, optional bias [N] and residual [..., N]. Any sizes.
     [[nodiscard]] Tensor linear_activation(const Tensor& input, const Tensor& weight, const Tensor* bias,
                                            Activation activation, const Tensor* residual = nullptr) const;
 
@@ -103,6 +106,23 @@ public:
                                const Tensor& in_weight, const Tensor* in_bias, const Tensor& out_weight,
                                const Tensor* out_bias, Activation activation = Activation::Gelu,
                                float epsilon = 1.0e-5F, bool gate_first = false) const;
+
+    // act((input - mean) * rstd * weight + bias) with the statistics of an image's groups, channels
+    // last (the spatial transformer's and the residual blocks' norms, unet.cpp:151-181): input
+    // [B, ..., C] fp16, bf16 or fp32, weight and bias [C] of its type.
+    [[nodiscard]] Tensor group_norm(const Tensor& input, const Tensor& weight, const Tensor& bias, std::size_t groups,
+                                    Activation activation = Activation::None, float epsilon = 1.0e-5F) const;
+
+    // group_norm, and LayerNorm over the last dim, of fp16 or bf16 inputs whose rows come out as
+    // Int8 codes with a scale each, for the linears with Int8 weights.
+    [[nodiscard]] Tensor group_norm_int8(const Tensor& input, const Tensor& weight, const Tensor& bias, std::size_t groups,
+                                         Activation activation = Activation::None, float epsilon = 1.0e-5F) const;
+    [[nodiscard]] Tensor layer_norm_int8(const Tensor& input, const Tensor& weight, const Tensor& bias,
+                                         float epsilon = 1.0e-5F) const;
+
+    // Int8 codes with a scale by row of an fp16 or bf16 tensor [..., K]: a weight by output channel,
+    // or tokens.
+    [[nodiscard]] Tensor pack_int8(const Tensor& input) const;
 
 private:
     const Runtime* runtime_ = nullptr;

@@ -17,7 +17,8 @@ namespace sdxl::hip {
 
 // Float8E4M3: finite-only E4M3 codes (bias 7), used for linear weights with an
 // attached per-output-channel dequantisation scale (the reference's FP8 weights).
-enum class ScalarType : std::uint8_t { Float16, BFloat16, Float32, Int32, Float8E4M3 };
+// Int8: codes of weights or tokens with an attached scale by row.
+enum class ScalarType : std::uint8_t { Float16, BFloat16, Float32, Int32, Float8E4M3, Int8 };
 
 [[nodiscard]] std::size_t scalar_size(ScalarType type) noexcept;
 
@@ -56,8 +57,8 @@ public:
     [[nodiscard]] void* data() const noexcept { return data_.get(); }
     [[nodiscard]] const std::int32_t* int32_data() const;
 
-    // Dequantisation scales of an FP8 tensor (fp32, one per output channel or
-    // one for the tensor), as the reference's Tensor::attach_dequant_scale.
+    // Dequantisation scales of an FP8 or Int8 tensor (fp32, one per output channel or
+    // one for the tensor; Int8: one per row), as the reference's Tensor::attach_dequant_scale.
     void attach_dequant_scale(Tensor scale);
     [[nodiscard]] bool has_dequant_scale() const noexcept { return scale_ != nullptr; }
     [[nodiscard]] const float* dequant_scale_data() const;

@@ -6,6 +6,8 @@
 
 #include "sdxl_hip/attention.h"
 #include "sdxl_hip/feed_forward.h"
+#include "sdxl_hip/group_norm.h"
+#include "sdxl_hip/int8.h"
 #include "sdxl_hip/sublayer.h"
 
 #include <sstream>
@@ -351,6 +353,53 @@ sdxl_ff_desc feed_forward_desc(const Tensor& input, const Tensor& weight, const 
     return d;
 }
 
+// The 8-bit integer product (weight: Int8), which gated_linear and linear_activation share.
+Tensor int8_product(const Runtime& runtime, const Tensor& input, const Tensor& weight, const Tensor* bias, const Tensor* residual,
+                    bool gated, Activation activation, bool gate_first) {
+    const bool codes = input.type() == ScalarType::Int8;
+    const ScalarType type = !codes ? input.type() : bias != nullptr ? bias->type() : residual != nullptr ? residual->type() : ScalarType::Float16;
+    if ((type != ScalarType::Float16 && type != ScalarType::BFloat16) || input.rank() < 2 || weight.rank() != 2)
+        throw HipError("8-bit linear requires an fp16, bf16 or Int8 input and a rank-2 weight");
+    if (weight.size(1) != input.shape().back() || (gated && weight.size(0) % 2 != 0))
+        throw HipError("8-bit linear feature mismatch");
+    sdxl_i8_desc d{};
+    d.m = 1;
+    for (std::size_t i = 0; i + 1 < input.rank(); ++i) d.m *= static_cast<std::int64_t>(input.size(i));
+    d.n = static_cast<std::int64_t>(gated ? weight.size(0) / 2 : weight.size(0));
+    d.k = static_cast<std::int64_t>(weight.size(1));
+    d.dtype = dtype_code(type);
+    d.x_dtype = codes ? SDXL_DTYPE_I8 : d.dtype;
+    d.activation = activation_code(activation);
+    d.gate_first = gate_first ? 1 : 0;
+    if (!weight.has_dequant_scale() || weight.dequant_scale_count() != weight.size(0) ||
+        (codes && (!input.has_dequant_scale() || input.dequant_scale_count() != static_cast<std::size_t>(d.m))))
+        throw HipError("8-bit linear requires a scale for every row of 8-bit integers");
+    std::vector<std::size_t> shape = input.shape();
+    shape.back() = static_cast<std::size_t>(d.n);
+    if (bias != nullptr && (bias->type() != type || bias->rank() != 1 || bias->size(0) != weight.size(0)))
+        throw HipError("8-bit linear bias mismatch");
+    if (residual != nullptr && (residual->type() != type || residual->shape() != shape))
+        throw HipError("8-bit linear residual mismatch");
+    Tensor output = Tensor::allocate(runtime, shape, type);
+    const std::size_t ws_bytes = gated ? sdxl_gated_linear_i8_workspace_bytes(&d) : sdxl_linear_i8_workspace_bytes(&d);
+    Tensor workspace = Tensor::allocate(runtime, {ws_bytes}, ScalarType::Int8);  // raw bytes
+    std::ostringstream label;
+    label << "ops/" << (gated ? "gated_linear" : "linear_activation") << "/i8/m" << d.m << "_n" << d.n << "_k" << d.k;
+    const int scope = runtime.begin_profile(label.str());
+    const float* x_scale = codes ? input.dequant_scale_data() : nullptr;
+    const auto* w = static_cast<const std::int8_t*>(weight.data());
+    const void* b = bias != nullptr ? bias->data() : nullptr;
+    const sdxl_status st =
+        gated ? sdxl_gated_linear_i8(&d, input.data(), x_scale, w, weight.dequant_scale_data(), b, output.data(),
+                                     workspace.data(), ws_bytes, runtime.stream())
+              : sdxl_linear_i8(&d, input.data(), x_scale, w, weight.dequant_scale_data(), b,
+                               residual != nullptr ? residual->data() : nullptr, output.data(), workspace.data(), ws_bytes,
+                               runtime.stream());
+    runtime.end_profile(scope);
+    check(st);
+    return output;
+}
+
 std::string feed_forward_label(const char* name, const sdxl_ff_desc& d) {
     std::ostringstream label;
     label << "ops/" << name << '/'
@@ -363,6 +412,8 @@ std::string feed_forward_label(const char* name, const sdxl_ff_desc& d) {
 
 Tensor Ops::gated_linear(const Tensor& input, const Tensor& weight, const Tensor* bias, Activation activation,
                          bool gate_first) const {
+    if (weight.type() == ScalarType::Int8)
+        return int8_product(*runtime_, input, weight, bias, nullptr, true, activation, gate_first);
     const sdxl_ff_desc d = feed_forward_desc(input, weight, bias, true, activation, gate_first);
     const float* scales = weight_scales(weight);
     std::vector<std::size_t> shape = input.shape();
@@ -378,6 +429,8 @@ Tensor Ops::gated_linear(const Tensor& input, const Tensor& weight, const Tensor
 
 Tensor Ops::linear_activation(const Tensor& input, const Tensor& weight, const Tensor* bias, Activation activation,
                               const Tensor* residual) const {
+    if (weight.type() == ScalarType::Int8)
+        return int8_product(*runtime_, input, weight, bias, residual, false, activation, false);
     const sdxl_ff_desc d = feed_forward_desc(input, weight, bias, false, activation, false);
     const float* scales = weight_scales(weight);
     std::vector<std::size_t> shape = input.shape();
@@ -429,6 +482,99 @@ void Ops::feed_forward_sublayer(Tensor& hidden, const Tensor& norm_weight, const
         hidden.data(), workspace.data(), ws_bytes, runtime_->stream());
     runtime_->end_profile(scope);
     check(st);
+}
+
+namespace {
+
+sdxl_group_norm_desc group_norm_desc(const Tensor& input, const Tensor& weight, const Tensor& bias, std::size_t groups,
+                                     Activation activation, float epsilon) {
+    if ((input.type() != ScalarType::Float16 && input.type() != ScalarType::BFloat16 && input.type() != ScalarType::Float32) ||
+        input.rank() < 3 || weight.type() != input.type() || bias.type() != input.type() || weight.rank() != 1 ||
+        bias.rank() != 1 || weight.size(0) != input.shape().back() || bias.size(0) != input.shape().back())
+        throw HipError("group norm shape/type mismatch");
+    sdxl_group_norm_desc d{};
+    d.batch = static_cast<std::int64_t>(input.size(0));
+    d.pixels = 1;
+    for (std::size_t i = 1; i + 1 < input.rank(); ++i) d.pixels *= static_cast<std::int64_t>(input.size(i));
+    d.channels = static_cast<std::int64_t>(input.shape().back());
+    d.groups = static_cast<std::int64_t>(groups);
+    d.dtype = dtype_code(input.type());
+    d.activation = activation_code(activation);
+    d.eps = epsilon;
+    return d;
+}
+
+std::string group_norm_label(const char* name, const sdxl_group_norm_desc& d) {
+    std::ostringstream label;
+    label << "ops/" << name << "/b" << d.batch << "_p" << d.pixels << "_c" << d.channels << "_g" << d.groups;
+    return label.str();
+}
+
+// Codes like the input, with a scale by row attached.
+Tensor int8_like(const Runtime& runtime, const Tensor& input) {
+    std::size_t rows = 1;
+    for (std::size_t i = 0; i + 1 < input.rank(); ++i) rows *= input.size(i);
+    Tensor codes = Tensor::allocate(runtime, input.shape(), ScalarType::Int8);
+    codes.attach_dequant_scale(Tensor::allocate(runtime, {rows}, ScalarType::Float32));
+    return codes;
+}
+
+float* scales_of(const Tensor& codes) { return const_cast<float*>(codes.dequant_scale_data()); }
+
+}  // namespace
+
+Tensor Ops::group_norm(const Tensor& input, const Tensor& weight, const Tensor& bias, std::size_t groups,
+                       Activation activation, float epsilon) const {
+    const sdxl_group_norm_desc d = group_norm_desc(input, weight, bias, groups, activation, epsilon);
+    Tensor output = Tensor::allocate(*runtime_, input.shape(), input.type());
+    const std::size_t ws_bytes = sdxl_group_norm_workspace_bytes(&d);
+    Tensor workspace = Tensor::allocate(*runtime_, {ws_bytes}, ScalarType::Int8);  // raw bytes
+    const int scope = runtime_->begin_profile(group_norm_label("group_norm", d));
+    const sdxl_status st = sdxl_group_norm(&d, input.data(), weight.data(), bias.data(), output.data(), nullptr,
+                                           workspace.data(), ws_bytes, runtime_->stream());
+    runtime_->end_profile(scope);
+    check(st);
+    return output;
+}
+
+Tensor Ops::group_norm_int8(const Tensor& input, const Tensor& weight, const Tensor& bias, std::size_t groups,
+                            Activation activation, float epsilon) const {
+    const sdxl_group_norm_desc d = group_norm_desc(input, weight, bias, groups, activation, epsilon);
+    Tensor codes = int8_like(*runtime_, input);
+    const std::size_t ws_bytes = sdxl_group_norm_i8_workspace_bytes(&d);
+    Tensor workspace = Tensor::allocate(*runtime_, {ws_bytes}, ScalarType::Int8);  // raw bytes
+    const int scope = runtime_->begin_profile(group_norm_label("group_norm_i8", d));
+    const sdxl_status st = sdxl_group_norm_i8(&d, input.data(), weight.data(), bias.data(), static_cast<std::int8_t*>(codes.data()),
+                                              0, scales_of(codes), nullptr, workspace.data(), ws_bytes, runtime_->stream());
+    runtime_->end_profile(scope);
+    check(st);
+    return codes;
+}
+
+Tensor Ops::layer_norm_int8(const Tensor& input, const Tensor& weight, const Tensor& bias, float epsilon) const {
+    if ((input.type() != ScalarType::Float16 && input.type() != ScalarType::BFloat16) || input.rank() < 2 ||
+        weight.type() != input.type() || bias.type() != input.type() || weight.rank() != 1 || bias.rank() != 1 ||
+        weight.size(0) != input.shape().back() || bias.size(0) != input.shape().back())
+        throw HipError("CUDA layer norm shape/type mismatch");
+    Tensor codes = int8_like(*runtime_, input);
+    const int scope = runtime_->begin_profile("ops/layer_norm_i8/w" + std::to_string(input.shape().back()));
+    const sdxl_status st = sdxl_layer_norm_i8(static_cast<std::int64_t>(codes.dequant_scale_count()),
+                                              static_cast<std::int64_t>(input.shape().back()), dtype_code(input.type()),
+                                              input.data(), 0, weight.data(), bias.data(), epsilon,
+                                              static_cast<std::int8_t*>(codes.data()), 0, scales_of(codes), runtime_->stream());
+    runtime_->end_profile(scope);
+    check(st);
+    return codes;
+}
+
+Tensor Ops::pack_int8(const Tensor& input) const {
+    if ((input.type() != ScalarType::Float16 && input.type() != ScalarType::BFloat16) || input.rank() < 2)
+        throw HipError("8-bit packing requires an fp16 or bf16 tensor of rank 2 or more");
+    Tensor codes = int8_like(*runtime_, input);
+    check(sdxl_quantize_i8_rows(static_cast<std::int64_t>(codes.dequant_scale_count()),
+                                static_cast<std::int64_t>(input.shape().back()), dtype_code(input.type()), input.data(), 0,
+                                static_cast<std::int8_t*>(codes.data()), 0, scales_of(codes), runtime_->stream()));
+    return codes;
 }
 
 }  // namespace sdxl::hip

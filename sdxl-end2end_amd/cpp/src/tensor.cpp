@@ -16,7 +16,8 @@ std::size_t scalar_size(ScalarType type) noexcept {
     case ScalarType::BFloat16: return 2;
     case ScalarType::Float32:
     case ScalarType::Int32: return 4;
-    case ScalarType::Float8E4M3: return 1;
+    case ScalarType::Float8E4M3:
+    case ScalarType::Int8: return 1;
     }
     return 0;
 }
@@ -126,6 +127,7 @@ Tensor Tensor::from_host_f32(const Runtime& runtime, const FloatTensor& host, Sc
     }
     if (type == ScalarType::Int32) throw HipError("use from_host_i32 for int32 tensors");
     if (type == ScalarType::Float8E4M3) throw HipError("use Ops::pack_e4m3 for FP8 weights");
+    if (type == ScalarType::Int8) throw HipError("use Ops::pack_int8 for 8-bit integers");
     std::vector<std::uint16_t> bits(host.values.size());
     for (std::size_t i = 0; i < bits.size(); ++i)
         bits[i] = type == ScalarType::Float16 ? float_to_half(host.values[i]) : float_to_bf16(host.values[i]);
@@ -159,6 +161,13 @@ FloatTensor Tensor::to_host_f32(const Runtime& runtime) const {
         SDXL_HIP_CHECK(hipMemcpyAsync(codes.data(), data(), bytes(), hipMemcpyDeviceToHost, runtime.stream()));
         runtime.synchronize();
         for (std::size_t i = 0; i < codes.size(); ++i) host.values[i] = e4m3_to_float(codes[i]);
+        return host;
+    }
+    if (type_ == ScalarType::Int8) {
+        std::vector<std::int8_t> codes(elements());
+        SDXL_HIP_CHECK(hipMemcpyAsync(codes.data(), data(), bytes(), hipMemcpyDeviceToHost, runtime.stream()));
+        runtime.synchronize();
+        for (std::size_t i = 0; i < codes.size(); ++i) host.values[i] = static_cast<float>(codes[i]);
         return host;
     }
     if (type_ == ScalarType::Int32) {

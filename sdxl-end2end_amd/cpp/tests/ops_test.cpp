@@ -456,6 +456,76 @@ void feed_forward_gate_first_cases() {
     std::cout << "feed-forward gate-first cases passed\n";
 }
 
+// Group norm and the 8-bit integer linears against host double-precision forms.
+void group_norm_and_int8_cases() {
+    Runtime runtime;
+    Ops ops(runtime);
+    const std::size_t P = 20, C = 16, G = 4, N = 12;
+    const auto hx = filled({1, P, C}, [](std::size_t i) { return std::sin(static_cast<float>(i) * 0.37F) * 2.0F + static_cast<float>(i % 16) * 0.25F; });
+    const auto hw = filled({C}, [](std::size_t i) { return 0.5F + static_cast<float>(i) * 0.0625F; });
+    const auto hb = filled({C}, [](std::size_t i) { return static_cast<float>(i) * 0.125F - 1.0F; });
+    const auto x = Tensor::from_host_f32(runtime, hx), w = Tensor::from_host_f32(runtime, hw), b = Tensor::from_host_f32(runtime, hb);
+    const auto vx = x.to_host_f32(runtime);  // as rounded to fp16
+    std::vector<double> z(P * C);
+    for (std::size_t g = 0; g < G; ++g) {
+        const std::size_t c0 = g * C / G, c1 = c0 + C / G;
+        double mean = 0.0, var = 0.0;
+        for (std::size_t p = 0; p < P; ++p)
+            for (std::size_t c = c0; c < c1; ++c) mean += vx.values[p * C + c];
+        mean /= static_cast<double>(P * C / G);
+        for (std::size_t p = 0; p < P; ++p)
+            for (std::size_t c = c0; c < c1; ++c) var += (vx.values[p * C + c] - mean) * (vx.values[p * C + c] - mean);
+        var /= static_cast<double>(P * C / G);
+        for (std::size_t p = 0; p < P; ++p)
+            for (std::size_t c = c0; c < c1; ++c) z[p * C + c] = (vx.values[p * C + c] - mean) / std::sqrt(var + 1.0e-6) * hw.values[c] + hb.values[c];
+    }
+    const auto y = ops.group_norm(x, w, b, G, Activation::Silu, 1.0e-6F).to_host_f32(runtime);
+    for (std::size_t i = 0; i < P * C; ++i) {
+        const double want = z[i] / (1.0 + std::exp(-z[i]));
+        require_close(y.values[i], static_cast<float>(want), static_cast<float>(std::fabs(want)) * 0x1p-10F + 1.0e-4F, "group norm");
+    }
+    // codes: half a step of the row's largest value over 127
+    const Tensor codes = ops.group_norm_int8(x, w, b, G, Activation::None, 1.0e-6F);
+    const auto q = codes.to_host_f32(runtime);
+    std::vector<float> scale(P);
+    SDXL_HIP_CHECK(hipMemcpy(scale.data(), codes.dequant_scale_data(), P * 4, hipMemcpyDeviceToHost));
+    for (std::size_t i = 0; i < P * C; ++i)
+        require_close(q.values[i] * scale[i / C], static_cast<float>(z[i]), 0.501F * scale[i / C] + 1.0e-4F, "group norm codes");
+    // products of the codes, with the weights' own: exact integers, two scales, one rounding
+    const Tensor weight = ops.pack_int8(Tensor::from_host_f32(runtime, filled({N, C}, [](std::size_t i) { return std::cos(static_cast<float>(i) * 0.23F); })));
+    const auto qw = weight.to_host_f32(runtime);
+    std::vector<float> w_scale(N);
+    SDXL_HIP_CHECK(hipMemcpy(w_scale.data(), weight.dequant_scale_data(), N * 4, hipMemcpyDeviceToHost));
+    const auto hbias = filled({N}, [](std::size_t i) { return static_cast<float>(i) * 0.5F; });
+    const auto bias = Tensor::from_host_f32(runtime, hbias);
+    const auto out = ops.linear_activation(codes, weight, &bias, Activation::None).to_host_f32(runtime);
+    std::vector<double> all(P * N);
+    for (std::size_t p = 0; p < P; ++p)
+        for (std::size_t n = 0; n < N; ++n) {
+            double sum = 0.0;
+            for (std::size_t c = 0; c < C; ++c) sum += static_cast<double>(q.values[p * C + c]) * qw.values[n * C + c];
+            all[p * N + n] = sum * scale[p] * w_scale[n] + hbias.values[n];
+            require_close(out.values[p * N + n], static_cast<float>(all[p * N + n]), static_cast<float>(std::fabs(all[p * N + n])) * 0x1p-10F + 1.0e-5F, "8-bit linear");
+        }
+    const auto gated = ops.gated_linear(codes, weight, &bias, Activation::Silu).to_host_f32(runtime);
+    require(gated.shape.back() == N / 2, "8-bit gated shape");
+    for (std::size_t p = 0; p < P; ++p)
+        for (std::size_t n = 0; n < N / 2; ++n) {
+            const double g = all[p * N + N / 2 + n], want = all[p * N + n] * g / (1.0 + std::exp(-g));
+            require_close(gated.values[p * (N / 2) + n], static_cast<float>(want), static_cast<float>(std::fabs(want)) * 0x1p-9F + 1.0e-4F, "8-bit gated linear");
+        }
+    // tokens in fp16: the same as their codes
+    const auto steps = ops.linear_activation(ops.pack_int8(x), weight, &bias, Activation::Gelu).to_host_f32(runtime);
+    const auto tokens = ops.linear_activation(x, weight, &bias, Activation::Gelu).to_host_f32(runtime);
+    for (std::size_t i = 0; i < steps.values.size(); ++i) require_close(tokens.values[i], steps.values[i], 0.0F, "tokens against their codes");
+    (void)ops.layer_norm_int8(x, w, b);
+    require_throws([&] { (void)ops.group_norm(x, w, Tensor::from_host_f32(runtime, hbias), G); }, "group norm shape/type mismatch", "group norm bias");
+    require_throws([&] { (void)ops.group_norm(x, w, b, 5); }, "multiple of groups", "groups");
+    require_throws([&] { (void)ops.linear_activation(Tensor::allocate(runtime, {P, C}, ScalarType::Int8), weight, nullptr, Activation::None); },
+                   "scale for every row", "codes without scales");
+    std::cout << "group norm and 8-bit cases passed\n";
+}
+
 void device_cases() {
     Runtime runtime;
     Ops ops(runtime);
@@ -560,6 +630,7 @@ void device_cases() {
     out_projection_cases();
     feed_forward_cases();
     feed_forward_gate_first_cases();
+    group_norm_and_int8_cases();
 }
 
 }  // namespace

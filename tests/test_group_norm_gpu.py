@@ -8,6 +8,8 @@ tensors, for fp32 ones to 8 u (1 + |z| + |z|^3 / 10) (the argument of an exponen
 erfc add some units in the last place); slopes are at most 1.13, second derivatives 1.2. Every output is rounded once.
 """
 import math
+import os
+import subprocess
 
 import pytest
 
@@ -15,6 +17,7 @@ import sdxl_hip as sh
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 DEV = "cuda:0"
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 HALF = {F16: 2.0 ** -11, BF16: 2.0 ** -8, F32: 2.0 ** -24}
@@ -371,3 +374,10 @@ def test_two_calls_at_once():
     for outs, w in zip(got, want):
         for o in outs:
             assert torch.equal(o, w)
+
+
+def test_cpp_group_norm_and_int8_cases():
+    """The C++ host API's group norm and 8-bit linears against host double precision."""
+    exe = os.path.join(ROOT, "sdxl-end2end_amd", "bin", "sdxl_hip_ops_test")
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "group norm and 8-bit cases passed" in r.stdout, r.stdout + r.stderr
