@@ -13,9 +13,9 @@
  * summed about values of its own, so that a mean far from zero costs no digits. Any batch,
  * pixels and channels, any row strides of at least a row; image b follows image b - 1 after
  * pixels * row_stride elements. Tensors need only their element's alignment. Rows shorter than
- * 16 bytes, groups of more than 8 KiB a row, more than 4096 groups or 2^18 images and strides
- * above 2^20 elements take general kernels, several times as long (sdxl_group_norm_i8: rows of
- * more than 20 KiB too).
+ * 16 bytes, groups of more than 8 KiB a row, more than 4096 groups, some millions of images and
+ * strides above 2^20 elements take general kernels, many times as long (sdxl_group_norm_i8: rows
+ * of more than 20 KiB too).
  * A NaN or an infinity in a group makes its rows NaN, and no other group's.
  *
  * All calls are stream-ordered, allocate nothing, never synchronise and may be captured into

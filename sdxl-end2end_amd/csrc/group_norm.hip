@@ -257,7 +257,14 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
         V::unpack(d, v);
 #pragma unroll
         for (int e = 0; e < kV; ++e) v[e] = gn_value<T, kFam>(act, affine.z(e, v[e]));
-        V::store_through(y, V::pack(v));
+        // (in place, the vector that a row's last one overlaps may be written before this one is read: what they share is its)
+        if (at.skip == 0) {
+            V::store_through(y, V::pack(v));
+        } else {
+#pragma unroll
+            for (int e = 0; e < kV; ++e)
+                if (e >= at.skip) ((T*)y)[e] = (T)v[e];
+        }
         y += step_y;
     });
 }
@@ -631,6 +638,8 @@ int64_t vecs_of(const GnParams& p, GnType type, int slab_groups) {
     return ((int64_t)p.group_channels * slab_groups * elem_of(type) + 15) / 16;
 }
 
+constexpr int64_t kMaxColumns = 1 << 22;  // of kMaxThreads threads each: below 2^32
+
 // Threads of a workgroup: of 4 to 8 waves the most whose lanes have work, the most of equals.
 int threads_of(int vecs) {
     int best = 0, best_used = -1;
@@ -733,7 +742,7 @@ int hold_of(const GnParams& p, GnType type, int& slab_groups, int& threads) {
     slab_groups = slab_groups_of(p, type, kHeldBytes);
     const int64_t vecs = vecs_of(p, type, slab_groups);
     if (slab_groups > 1 && p.group_channels < kV && (p.group_channels * 2 != kV || slab_groups * p.group_channels % kV != 0)) return 0;
-    if (vecs > kHeldVecs || p.pixels > (1 << 16) || (int64_t)p.batch * (p.groups / slab_groups) > (1 << 20)) return 0;
+    if (vecs > kHeldVecs || p.pixels > (1 << 16) || (int64_t)p.batch * (p.groups / slab_groups) > kMaxColumns) return 0;
     threads = (int)(vecs * p.pixels < kMaxThreads ? (vecs * p.pixels + 63) / 64 * 64 : kMaxThreads);
     const int rows = threads / (int)vecs, needed = (int)((p.pixels + rows - 1) / rows);
     for (int hold : kHolds)
@@ -744,7 +753,7 @@ int hold_of(const GnParams& p, GnType type, int& slab_groups, int& threads) {
 bool fast_of(const GnParams& p, GnType type) {
     const int slab_groups = slab_groups_of(p, type, kSlabBytes);
     const int64_t vecs = vecs_of(p, type, slab_groups), columns = (int64_t)p.batch * (p.groups / slab_groups);
-    return p.batch > 0 && p.pixels > 0 && p.channels >= 16 / elem_of(type) && vecs <= kMaxThreads && columns <= (1 << 18) &&
+    return p.batch > 0 && p.pixels > 0 && p.channels >= 16 / elem_of(type) && vecs <= kMaxThreads && columns <= kMaxColumns &&
            p.groups <= 4096 && p.pixels < (1 << 28) && p.ld_x <= (1 << 20) && p.ld_y <= (1 << 20) && p.ld_dy <= (1 << 20);
 }
 

@@ -263,6 +263,35 @@ def test_images_of_four_dimensions_and_in_place():
     assert got.data_ptr() == x.data_ptr() and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("P,C,G", [(40, 514, 2), (5000, 514, 2), (3000, 1001, 7), (9000, 45, 3)])
+def test_in_place_where_a_row_ends_inside_a_vector(P, C, G, dtype):
+    """A row's last vector is read over the one before it, which another thread may have written by then."""
+    x = values(1, 2, P, C, std=2.0, mean=3.0, dtype=dtype)
+    gamma, beta = values(2, C, mean=1.0, dtype=dtype), values(3, C, dtype=dtype)
+    want = sh.group_norm(x, gamma, beta, G, activation="silu")
+    for _ in range(5):
+        y = x.clone()
+        sh.group_norm(y, gamma, beta, G, activation="silu", out=y)
+        assert torch.equal(y, want)
+
+
+def test_many_images():
+    """Images of one pixel and of three, hundreds of thousands of them: a workgroup each, or several."""
+    for B, P, C, G in ((300000, 1, 64, 4), (70000, 3, 96, 32)):
+        x = values(1, B, P, C)
+        gamma, beta = values(2, C, mean=1.0), values(3, C)
+        got, stats = sh.group_norm(x, gamma, beta, G, with_stats=True)
+        check_forward(x, gamma, beta, G, "none", 1e-5, got, stats)
+        part = slice(B - 1000, B)
+        q, s = sh.group_norm_i8(x, gamma, beta, G)
+        y = got[part].double()
+        within(q[part].double() * s.view(B, P)[part].double()[..., None], y, 0.51 * s.view(B, P)[part].double()[..., None] + 2 * HALF[F16] * y.abs() + 1e-3, "codes")
+        dx, dgamma, dbeta = sh.group_norm_backward(x, x, gamma, beta, G, stats)
+        one = sh.group_norm_backward(x[part], x[part], gamma, beta, G, stats[part])
+        assert torch.equal(dx[part], one[0])
+
+
 @pytest.mark.parametrize("P", [50, 4000])
 def test_mean_far_from_zero(P):
     """A variance of 1 about a mean of 1000: sums of squares about zero would lose it in fp32."""
