@@ -169,6 +169,8 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
     __syncthreads();
     const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
     const float over_channels = 1.0f / (float)p.group_channels;
+    // pixels of a row of the rows at a time: the first `longer` have one more
+    const int each = count / p.rows_at_once, longer = count - each * p.rows_at_once;
     for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
         const float2* from = parts + g * p.group_channels;
         const int all = rows * p.group_channels;
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
 #pragma unroll 4
         for (int e = lane; e < all; e += p.team) {
             const int r = (int)(((float)e + 0.5f) * over_channels), c = e - r * p.group_channels;  // (e < 2^13: exact)
-            merge.add(from[r * slab.channels + c], (float)share_of(count, r, p.rows_at_once));
+            merge.add(from[r * slab.channels + c], (float)(r < longer ? each + 1 : each));
         }
         const float2 m = merge.finish((float)count * (float)p.group_channels, p.team);
         if (lane == 0) ((float2*)p.partial)[(int64_t)task * p.groups + slab.g0 + g] = m;
@@ -383,6 +385,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_sums_kernel(GnParams p) {
     __syncthreads();
     for (int c = threadIdx.x; c < slab.channels; c += blockDim.x) {
         float2 sum = parts[c];
+#pragma unroll 4
         for (int r = 1; r < rows; ++r) {
             sum.x += parts[r * slab.channels + c].x;
             sum.y += parts[r * slab.channels + c].y;
