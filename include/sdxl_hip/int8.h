@@ -72,6 +72,12 @@ typedef struct sdxl_i8_desc {
 size_t sdxl_linear_i8_workspace_bytes(const sdxl_i8_desc* desc);
 size_t sdxl_gated_linear_i8_workspace_bytes(const sdxl_i8_desc* desc);
 
+/* The kernels that a call of this descriptor runs on the current device (without one: on 256 CUs), on
+ * tensors aligned to 16 bytes: those of sdxl_linear_i8 or (gated 1) sdxl_gated_linear_i8, named as by
+ * sdxl_ff_kernels (feed_forward.h), "quantise; " before the product of 16-bit tokens, " tokens" behind
+ * that which quantises them itself. Text, size and result as there. */
+size_t sdxl_i8_kernels(const sdxl_i8_desc* desc, int32_t gated, char* text, size_t size);
+
 /* out = act((x . w^T) * x_scale * w_scale + bias) + residual: x [m, k] codes with x_scale [m], or
  * 16-bit tokens (x_scale NULL), as if quantised by sdxl_quantize_i8_rows first; w [n, k] codes
  * with w_scale [n]. bias [n] and residual [m, n] are optional (NULL); residual may equal out

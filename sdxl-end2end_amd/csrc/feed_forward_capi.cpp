@@ -259,20 +259,7 @@ sdxl_status backward(const sdxl_ff_desc* d, bool gated, const char* name, const 
                                                        b.sums_alone ? &b.w : nullptr, c.bf16, b.partial, stream), name);
 }
 
-std::string kernel_text(const sdxl_hip::FfChoice& c) {
-    using sdxl_hip::FfKernel;
-    static const char* const tiles[sdxl_hip::kFfTiles] = {"256x320", "256x256", "128x256", "128x192", "128x128", "64x128", "64x64"};
-    static const char* const deep[] = {"32x32/8", "32x32/4", "64x64/4"};
-    const std::string through = c.staged ? " staged" : "";
-    switch (c.kernel) {
-    case FfKernel::kGeneral: break;
-    case FfKernel::kRows: return "rows/" + std::to_string(c.variant) + through;
-    case FfKernel::kDeep: return std::string("deep ") + deep[c.variant] + through;
-    case FfKernel::kTile: return std::string("tile ") + tiles[c.variant];
-    case FfKernel::kStaged: return c.variant == 128 ? "staged 128x128" : "staged 64x64";
-    }
-    return "general";
-}
+using sdxl_hip::kernel_text;
 
 std::string shares_text(int shares) { return shares > 1 ? " in " + std::to_string(shares) + " shares" : ""; }
 

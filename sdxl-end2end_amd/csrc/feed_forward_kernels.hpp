@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <string>
+
 namespace sdxl_hip {
 
 // What a product's epilogue makes of its sums.
@@ -81,6 +83,21 @@ struct FfChoice {
     int variant;
     bool staged;  // rows and deep: operands through registers
 };
+
+// Its name, as sdxl_ff_kernels and sdxl_i8_kernels have it.
+inline std::string kernel_text(const FfChoice& c) {
+    static const char* const tiles[kFfI8Tiles] = {"256x320", "256x256", "128x256", "128x192", "128x128", "64x128", "64x64", "256x192"};
+    static const char* const deep[] = {"32x32/8", "32x32/4", "64x64/4"};
+    const std::string through = c.staged ? " staged" : "";
+    switch (c.kernel) {
+    case FfKernel::kGeneral: break;
+    case FfKernel::kRows: return "rows/" + std::to_string(c.variant) + through;
+    case FfKernel::kDeep: return std::string("deep ") + deep[c.variant] + through;
+    case FfKernel::kTile: return std::string("tile ") + tiles[c.variant];
+    case FfKernel::kStaged: return c.variant == 128 ? "staged 128x128" : "staged 64x64";
+    }
+    return "general";
+}
 
 // Projections and dz, by sizes, strides and alignment.
 FfChoice choose_ff(const FfParams& p, FfEpilogue epilogue, bool j_fp8, int compute_units);

@@ -213,6 +213,27 @@ size_t sdxl_gated_linear_i8_workspace_bytes(const sdxl_i8_desc* d) {
     return workspace_bytes_of(d, true, "sdxl_gated_linear_i8");
 }
 
+size_t sdxl_i8_kernels(const sdxl_i8_desc* d, int32_t gated, char* text, size_t size) {
+    const char* name = "sdxl_i8_kernels";
+    if (text != nullptr && size > 0) text[0] = '\0';
+    Call c;
+    if (gated != 0 && gated != 1) {
+        fail(name, SDXL_STATUS_INVALID_ARGUMENT, "gated must be 0 or 1");
+        return 0;
+    }
+    if (resolve(d, gated == 1, name, c) != SDXL_STATUS_OK || c.m == 0 || c.n == 0) return 0;
+    const auto at = reinterpret_cast<void*>(uintptr_t{256});  // aligned to everything, never followed
+    const bool tokens = quantises(c, d, gated == 1);
+    FfParams p = product_of(c, d, tokens);
+    p.ip = p.jp = p.out = at;
+    const sdxl_hip::FfEpilogue epilogue = gated == 1 ? sdxl_hip::kFfGated : sdxl_hip::kFfLinear;
+    std::string kernels = sdxl_hip::kernel_text(sdxl_hip::choose_ff(p, epilogue, false, sdxl_hip_compute_units()));
+    if (tokens) kernels += " tokens";
+    else if (c.tokens) kernels = "quantise; " + kernels;
+    if (text != nullptr && size > 0) text[kernels.copy(text, size - 1)] = '\0';
+    return kernels.size();
+}
+
 sdxl_status sdxl_linear_i8(const sdxl_i8_desc* d, const void* x, const float* x_scale, const int8_t* w,
                            const float* w_scale, const void* bias, const void* residual, void* out, void* workspace,
                            size_t workspace_bytes, void* stream) {

@@ -74,6 +74,7 @@ INT8_SYMBOLS = (
     "sdxl_layer_norm_i8",
     "sdxl_linear_i8_workspace_bytes",
     "sdxl_gated_linear_i8_workspace_bytes",
+    "sdxl_i8_kernels",
     "sdxl_linear_i8",
     "sdxl_gated_linear_i8",
 )
@@ -269,6 +270,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.sdxl_group_norm_backward.restype = ctypes.c_int
     lib.sdxl_group_norm_backward.argtypes = [ctypes.POINTER(GroupNormDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                              ctypes.c_size_t, vp]
+    lib.sdxl_i8_kernels.restype = ctypes.c_size_t
+    lib.sdxl_i8_kernels.argtypes = [ctypes.POINTER(I8Desc), ctypes.c_int32, ctypes.c_char_p, ctypes.c_size_t]
     lib.sdxl_quantize_i8_rows.restype = ctypes.c_int
     lib.sdxl_quantize_i8_rows.argtypes = [i64, i64, ctypes.c_int32, vp, i64, vp, i64, vp, vp]
     lib.sdxl_layer_norm_i8.restype = ctypes.c_int
@@ -1054,6 +1057,13 @@ def gated_linear_i8(x, w, w_scale, x_scale=None, bias=None, activation: str = "g
     with w_scale [2N], bias [2N]; gate_first: [gate | value]. Other arguments as linear_i8. Returns [M, N]."""
     return _linear_i8("sdxl_gated_linear_i8", True, x, w, w_scale, x_scale, bias, None, activation, gate_first, dtype, out,
                       workspace)
+
+
+def i8_kernels(desc: I8Desc, gated: bool) -> str:
+    """The kernels that a call of this descriptor runs (sdxl_i8_kernels)."""
+    text = ctypes.create_string_buffer(256)
+    load().sdxl_i8_kernels(ctypes.byref(desc), 1 if gated else 0, text, len(text))
+    return text.value.decode()
 
 
 def linear_i8_workspace_bytes(M: int, N: int, K: int, gated: bool = False, dtype: int = F16) -> int:

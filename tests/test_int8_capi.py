@@ -145,3 +145,41 @@ def test_python_refusals():
                 lambda: sh.layer_norm_i8(x, x[0, :32], x[0]), lambda: sh.quantize_i8_rows(x.t())):
         with pytest.raises(sh.SdxlError):
             bad()
+
+
+# sizes (M, N, K) that reach each kernel, of the linear and of the gated form
+KERNELS = {
+    "rows/4": ((1, 9, 16), (2, 9, 48)), "rows/8": ((4, 9, 528), (3, 70, 832)), "rows/16": ((7, 8, 1136), (6, 8, 1072)),
+    "rows/4 staged": ((3, 10, 19), (1, 8, 19)), "rows/8 staged": ((1, 11, 755), (2, 10, 515)), "rows/16 staged": ((6, 15, 1475), (3, 9, 1107)),
+    "deep 32x32/8": ((19, 11, 288), (19, 9, 272)), "deep 32x32/8 staged": ((17, 9, 531), (19, 13, 387)),
+    "deep 32x32/4": ((4604, 39, 656), (36, 2261, 544)), "deep 32x32/4 staged": ((523, 519, 275), (4141, 26, 275)),
+    "deep 64x64/4": ((36, 10747, 4320), (36, 5158, 4192)), "deep 64x64/4 staged": ((392, 1589, 3907), (71, 3777, 2931)),
+    "staged 64x64": ((20, 8, 19), (22, 12, 19)), "staged 128x128": ((1473, 2799, 19), (536, 3385, 19)),
+    "tile 64x64": ((17, 8, 16), (18, 11, 16)), "tile 64x128": ((5538, 338, 16), (262, 3816, 16)),
+    "tile 128x128": ((2589, 823, 2256), (414, 2358, 2096)), "tile 128x192": ((5630, 709, 16), (523, 3759, 16)),
+    "tile 128x256": ((4379, 1353, 16), (1042, 2719, 16)), "tile 256x192": ((3334, 2446, 16), (4189, 995, 16)),
+    "tile 256x256": ((5007, 2429, 16), (2094, 2881, 16)), "tile 256x320": ((4578, 3827, 16), (2105, 3881, 16)),
+    "general": ((9, 33, 15), (70, 9, 7)),
+}
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_sizes_of_kernels(kernel, gated):
+    m, n, k = KERNELS[kernel][gated]
+    for activation in sh.ACTIVATIONS.values():
+        kw = dict(m=m, n=n, k=k, dtype=sh.BF16, activation=activation)
+        assert sh.i8_kernels(desc(**kw), gated) == kernel
+        own = m <= 4 and "rows" in kernel  # up to four tokens are quantised by the product's workgroups
+        assert sh.i8_kernels(desc(**kw, x_dtype=sh.BF16), gated) == (kernel + " tokens" if own else "quantise; " + kernel)
+
+
+def test_kernels_of_no_call():
+    text, lib = ctypes.create_string_buffer(b"x" * 63, 64), sh.load()
+    for d, gated in ((desc(m=0), 0), (desc(n=0), 1), (desc(reserved=1), 0), (desc(), 2)):
+        assert lib.sdxl_i8_kernels(ctypes.byref(d), gated, text, 64) == 0 and text.value == b""
+    assert lib.sdxl_i8_kernels(None, 0, text, 64) == 0
+    whole = sh.i8_kernels(desc(m=40, x_dtype=sh.F16), True)
+    for size in (1, 5, 64):
+        assert lib.sdxl_i8_kernels(ctypes.byref(desc(m=40, x_dtype=sh.F16)), 1, text, size) == len(whole)
+        assert text.value.decode() == whole[:size - 1]

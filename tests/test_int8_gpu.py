@@ -10,6 +10,7 @@ import pytest
 
 import sdxl_hip as sh
 from test_group_norm_gpu import BF16, DEV, F16, HALF, TINY, U, act64, check_forward, normal_form, values, within
+from test_int8_capi import KERNELS
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -105,6 +106,20 @@ def test_tokens_are_quantised_as_by_the_quantiser(i, gated):
     got = fn(x, w, ws, activation="silu")
     check(got, q, xs, w, ws, None, "silu", gated)
     assert torch.equal(got, fn(q, w, ws, x_scale=xs, activation="silu", dtype=dtype))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_each_kernel(kernel, gated):
+    M, N, K = KERNELS[kernel][gated]
+    dtype, features = HALVES[len(kernel) % 2], 2 * N if gated else N
+    tokens, w, ws, bias = values(1, M, K, std=2.0, dtype=dtype), codes(2, features, K), scales(3, features), values(4, features, dtype=dtype)
+    q, xs = sh.quantize_i8_rows(tokens)
+    fn = sh.gated_linear_i8 if gated else sh.linear_i8
+    given = dict(bias=bias, activation="gelu") | ({} if gated else dict(residual=values(5, M, N, dtype=dtype)))
+    got = fn(q, w, ws, x_scale=xs, dtype=dtype, **given)
+    check(got, q, xs, w, ws, bias, "gelu", gated, residual=given.get("residual"))
+    assert torch.equal(got, fn(tokens, w, ws, **given))
 
 
 # widths: one; shorter than a vector; ends inside one; a wave's, several waves', more than registers hold
