@@ -272,41 +272,46 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
 }
 
 // Codes by row. The row's lanes keep their channels' constants: z = x a + b, with b = beta - mean a rounded to 2^-24 of
-// mean a (a 16-bit x itself has 2^-12 of it at best).
+// mean a (a 16-bit x itself has 2^-12 of it at best). Every workgroup merges the parts of all groups, so that eight waves
+// with a row each and a workgroup a CU beat four and two ([1, 16384, 320] fp16, both passes: 16.7 us and 20.8; [2, 1024,
+// 1280] 10.0 and 11.1; sixteen 16.1 and 12.1).
 template <typename T, FfFamily kFam, int kWaves, int kVecs>
-__global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
+__global__ __launch_bounds__(kWaves == 1 ? 512 : 256) void gn_rows_kernel(GnParams p) {
     extern __shared__ __attribute__((aligned(16))) float2 stats[];
     __shared__ float part[4];
     const int task = (int)blockIdx.x;
     const int image = task / p.apply_chunks, chunk = task % p.apply_chunks;
+    constexpr int kRows = kWaves == 1 ? 8 : 1;  // of a workgroup at a time
     const I8Row<kWaves, kVecs> row(p.channels);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
     u32x4 d[kVecs];
+    // (lanes past the row's end: its last vector; past the last row: that one)
     auto fetch = [&](int r) __attribute__((always_inline)) {
-        const char* x = (const char*)p.x + (image * p.pixels + first + r) * p.ld_x * 2;
+        const char* x = (const char*)p.x + (image * p.pixels + first + min(r, count - 1)) * p.ld_x * 2;
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) d[i] = r < count && row.has(i) ? GnVec<T>::load(x + row.column(i) * 2) : u32x4{};
+        for (int i = 0; i < kVecs; ++i) d[i] = GnVec<T>::load(x + row.column(i) * 2);
     };
     int r = (int)threadIdx.x / (64 * kWaves);
     fetch(r);
     merge_stats(p, image, 0, p.groups, p.stats_out != nullptr && chunk == 0, stats);
-    const FfAct act = ff_act(p.activation);
     float a[kVecs][8], b[kVecs][8];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-        if (row.has(i)) {
-            load_channels<T>(p.gamma, row.column(i), a[i]);
-            load_channels<T>(p.beta, row.column(i), b[i]);
+        load_channels<T>(p.gamma, row.column(i), a[i]);
+        load_channels<T>(p.beta, row.column(i), b[i]);
+    }
+    const FfAct act = ff_act(p.activation);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float2 s = stats[group_of(p, row.column(i) + e)];
-                a[i][e] *= s.y;
-                b[i][e] = __builtin_fmaf(-s.x, a[i][e], b[i][e]);
-            }
+    for (int i = 0; i < kVecs; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float2 s = stats[group_of(p, row.column(i) + e)];
+            a[i][e] *= s.y;
+            b[i][e] = __builtin_fmaf(-s.x, a[i][e], b[i][e]);
         }
     }
-    for (; r < count; r += 4 / kWaves) {
+    for (; r < count; r += kRows) {
         float v[kVecs][8];
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
@@ -314,7 +319,7 @@ __global__ __launch_bounds__(256) void gn_rows_kernel(GnParams p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = ff_value<kFam>(act, __builtin_fmaf(v[i][e], a[i][e], b[i][e]));
         }
-        fetch(r + 4 / kWaves);
+        fetch(r + kRows);
         const int64_t at = image * p.pixels + first + r;
         const float scale = row.quantise(v, part, p.q + at * p.ld_q, 0);
         if (row.lane == 0) p.q_scale[at] = scale;
@@ -452,25 +457,25 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     const int64_t step_dx = p.ld_y * p.rows_at_once * (int64_t)sizeof(T);
     GnBatch<4, true> batch;
     batch.load(n, x, step_x, dy, step_dy);
+    GnBackward<T> b;  // (on the way before the merge)
+    b.load(p, image, slab.c0 + at.c0);
     const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
     const float over = 1.0f / ((float)p.pixels * (float)p.group_channels);
     for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
         const float2* from = (const float2*)p.partial + (int64_t)image * p.chunks * p.groups + slab.g0 + g;
-        float a = 0.0f, b = 0.0f;
+        float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll 4
         for (int k = lane; k < p.chunks; k += p.team) {
-            a += from[(int64_t)k * p.groups].x;
-            b += from[(int64_t)k * p.groups].y;
+            s1 += from[(int64_t)k * p.groups].x;
+            s2 += from[(int64_t)k * p.groups].y;
         }
-        a = team_sum(a, p.team);
-        b = team_sum(b, p.team);
-        if (lane == 0) means[g] = float2{a * over, b * over};
+        s1 = team_sum(s1, p.team);
+        s2 = team_sum(s2, p.team);
+        if (lane == 0) means[g] = float2{s1 * over, s2 * over};
     }
     __syncthreads();
     if (n <= 0) return;
     const FfAct act = ff_act(p.activation);
-    GnBackward<T> b;
-    b.load(p, image, slab.c0 + at.c0);
     float a1[kV], a2[kV];  // dx = a dz - a1 - (x - mean) a2
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
@@ -658,10 +663,10 @@ int threads_of(int vecs) {
 
 int team_of(int groups, int threads) { return 64 * groups <= threads ? 64 : 16; }
 
-// Workgroups of the two passes (codes: of the second), and the rounds that a chunk has a multiple of. One workgroup a CU
+// Workgroups of the two passes, and the rounds that a chunk has a multiple of. One workgroup a CU
 // reads fast enough and leaves few parts: [2, 131072, 256] bf16 backward 126 us with 512 and 512, 119 with 256 and 512 or
 // 768, 126 with 256 and 256, 152 with 128 and 512.
-constexpr int kFirstTasks = 256, kSecondTasks = 512, kRowTasks = 512;
+constexpr int kFirstTasks = 256, kSecondTasks = 512;
 constexpr int kBatchRounds = 4;
 
 // `columns` (images by slabs) in chunks of whole rounds of `rows` pixels: `tasks` chunks in all or a little fewer, of
@@ -708,7 +713,7 @@ constexpr int kRowVecs = 5;
 
 template <typename T, FfFamily kFam, int kWaves>
 hipError_t launch_rows_of(const GnParams& p, hipStream_t stream) {
-    const dim3 grid((unsigned)(p.batch * p.apply_chunks)), block(256);
+    const dim3 grid((unsigned)(p.batch * p.apply_chunks)), block(kWaves == 1 ? 512 : 256);
     const size_t lds = (size_t)p.groups * 8;
     switch ((p.vecs + 64 * kWaves - 1) / (64 * kWaves)) {
     case 1: hipLaunchKernelGGL((gn_rows_kernel<T, kFam, kWaves, 1>), grid, block, lds, stream, p); break;
@@ -725,8 +730,7 @@ hipError_t launch_rows(const GnParams& params, GnType type, hipStream_t stream) 
     GnParams p = params;
     p.vecs = (p.channels + 7) / 8;
     const bool wave = p.vecs <= 64 * kRowVecs;
-    p.team = team_of(p.groups, 256);
-    cut_second(p, p.batch, wave ? 4 : 1, kRowTasks, 1);
+    cut_second(p, p.batch, wave ? 8 : 1, wave ? 256 : 512, 1);
     auto launch = [&]<typename T, FfFamily kFam>() {
         return wave ? launch_rows_of<T, kFam, 1>(p, stream) : launch_rows_of<T, kFam, 4>(p, stream);
     };

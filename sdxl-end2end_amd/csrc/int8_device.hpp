@@ -47,7 +47,7 @@ struct __attribute__((packed, aligned(1))) Unaligned8 {
 
 // A row of 16-bit values over kWaves waves (of a workgroup of four), kVecs vectors of 8 a lane: vector `i` of the lane is
 // the row's vector lane_of_row + 64 kWaves i. The row's last vector may overlap the one before; its first `skip` values
-// are that one's.
+// is that one's. Lanes past the row's end hold its last vector again, which changes no maximum.
 template <int kWaves, int kVecs>
 struct I8Row {
     static constexpr int kLanes = 64 * kWaves;
@@ -79,12 +79,10 @@ struct I8Row {
             uint32_t top = 0;  // magnitudes compare as their bits do, NaN above infinity
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
-                if (has(i)) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t m = __float_as_uint(v[i][e]) & 0x7fffffffu;
-                        top = max(top, m <= most ? m : 0);
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t m = __float_as_uint(v[i][e]) & 0x7fffffffu;
+                    top = max(top, m <= most ? m : 0);
                 }
             }
             return __float_as_uint(reduce(__uint_as_float(top), part, [](float a, float b) __attribute__((always_inline)) {

@@ -81,10 +81,16 @@ __global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
         const char* x = (const char*)p.x + r * p.ld_x * 2;
         u32x4 d[kVecs];
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            d[i] = u32x4{};
-            if (row.has(i)) d[i] = ((const Unaligned<2>*)(x + row.column(i) * 2))->v;
+        for (int i = 0; i < kVecs; ++i) d[i] = ((const Unaligned<2>*)(x + row.column(i) * 2))->v;
+        u32x4 g[kNorm ? kVecs : 1], b[kNorm ? kVecs : 1];  // on the way before the sums
+        if constexpr (kNorm) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                g[i] = ((const Unaligned<2>*)((const char*)p.gamma + row.column(i) * 2))->v;
+                b[i] = ((const Unaligned<2>*)((const char*)p.beta + row.column(i) * 2))->v;
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);
         float v[kVecs][8];
 #pragma unroll
         for (int i = 0; i < kVecs; ++i)
@@ -111,14 +117,10 @@ __global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
             const float rstd = 1.0f / __builtin_sqrtf(row.reduce(centred, part, Add{}) / (float)p.cols + p.eps);
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
-                if (row.has(i)) {
-                    const u32x4 g = ((const Unaligned<2>*)((const char*)p.gamma + row.column(i) * 2))->v;
-                    const u32x4 b = ((const Unaligned<2>*)((const char*)p.beta + row.column(i) * 2))->v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[i][2 * e] = __builtin_fmaf((v[i][2 * e] - mean) * rstd, F::lo(g[e]), F::lo(b[e]));
-                        v[i][2 * e + 1] = __builtin_fmaf((v[i][2 * e + 1] - mean) * rstd, F::hi(g[e]), F::hi(b[e]));
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    v[i][2 * e] = __builtin_fmaf((v[i][2 * e] - mean) * rstd, F::lo(g[i][e]), F::lo(b[i][e]));
+                    v[i][2 * e + 1] = __builtin_fmaf((v[i][2 * e + 1] - mean) * rstd, F::hi(g[i][e]), F::hi(b[i][e]));
                 }
             }
         }

@@ -850,12 +850,17 @@ def _gn_common(name, x, gamma, beta, groups, activation):
     return t, batch, pixels, channels, 0 if x.is_contiguous() else _gn_stride(name, "x", x, channels), code, act, index
 
 
+def _new_like(t, x, dtype=None):
+    """A contiguous tensor of x's shape (empty_like takes 1.1 us where empty and new_empty with a shape take 1.7 to 2.2)."""
+    return t.empty_like(x, dtype=dtype) if x.is_contiguous() else t.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
+
+
 def _workspace(name, t, size, workspace, x, index):
     """(pointer, bytes, the tensor to keep) of a workspace that the caller gave, or of one of `size` bytes"""
     if workspace is None:
         if size == 0:
             return None, 0, None
-        workspace = t.empty((size,), dtype=t.uint8, device=x.device)
+        workspace = t.empty(size, dtype=t.uint8, device=x.device)
         return workspace.data_ptr(), size, workspace
     if workspace.get_device() != index or not workspace.is_contiguous():
         raise SdxlError(INVALID_ARGUMENT, f"{name}: workspace must be contiguous and on x's device")
@@ -880,7 +885,7 @@ def group_norm(x, gamma, beta, groups: int, activation: str = "none", eps: float
     t, batch, pixels, channels, ldx, code, act, index = _gn_common(name, x, gamma, beta, groups, activation)
     ldy = 0
     if out is None:
-        out = x.new_empty(x.shape)
+        out = _new_like(t, x)
     else:
         if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index:
             raise SdxlError(INVALID_SHAPE, f"{name}: out must be like x")
@@ -908,9 +913,9 @@ def group_norm_backward(dout, x, gamma, beta, groups: int, stats, activation: st
     desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, 0, lddy, code, act, 0.0, 0)
     lib = load()
     ws, ws_bytes, workspace = _workspace(name, t, lib.packed_sdxl_group_norm_backward_workspace_bytes(desc), workspace, x, index)
-    dx = x.new_empty(x.shape) if need_dx else None
-    dgamma = x.new_empty((channels,)) if need_dgamma else None
-    dbeta = x.new_empty((channels,)) if need_dbeta else None
+    dx = _new_like(t, x) if need_dx else None
+    dgamma = t.empty_like(gamma) if need_dgamma else None
+    dbeta = t.empty_like(beta) if need_dbeta else None
     _ff_call(lib.packed_sdxl_group_norm_backward, index, t, desc, dout.data_ptr(), x.data_ptr(), gamma.data_ptr(),
              beta.data_ptr(), stats.data_ptr(), _ptr(dx), _ptr(dgamma), _ptr(dbeta), ws, ws_bytes)
     return dx, dgamma, dbeta
@@ -922,8 +927,8 @@ def group_norm_i8(x, gamma, beta, groups: int, activation: str = "none", eps: fl
     scales fp32 [rows]) for linear_i8, with with_stats the stats too."""
     name = "sdxl_group_norm_i8"
     t, batch, pixels, channels, ldx, code, act, index = _gn_common(name, x, gamma, beta, groups, activation)
-    q = t.empty(x.shape, dtype=t.int8, device=x.device)
-    scale = t.empty((batch * pixels,), dtype=t.f32, device=x.device)
+    q = _new_like(t, x, t.int8)
+    scale = t.empty(batch * pixels, dtype=t.f32, device=x.device)
     stats = _gn_stats(name, t, None, with_stats, batch, groups, x, index)
     desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, 0, 0, code, act, _f32(eps), 0)
     lib = load()
@@ -962,8 +967,8 @@ def _i8_rows(name, x, gamma, beta, eps):
         _ff_like(name, "gamma", gamma, (cols,), x.dtype, index)
         _ff_like(name, "beta", beta, (cols,), x.dtype, index)
     ldx = 0 if x.is_contiguous() else _gn_stride(name, "x", x, cols)
-    q = t.empty(x.shape, dtype=t.int8, device=x.device)
-    scale = t.empty((rows,), dtype=t.f32, device=x.device)
+    q = _new_like(t, x, t.int8)
+    scale = t.empty(rows, dtype=t.f32, device=x.device)
     lib = load()
     if gamma is not None:
         _ff_call(lib.sdxl_layer_norm_i8, index, t, rows, cols, code, x.data_ptr(), ldx, gamma.data_ptr(), beta.data_ptr(),
@@ -1021,7 +1026,7 @@ def _linear_i8(name, gated, x, w, w_scale, x_scale, bias, residual, activation, 
         _ff_like(name, "residual", residual, (M, N), given, index)
         ldr = 0 if residual.is_contiguous() else _ff_stride(name, "residual", residual)
     if out is None:
-        out = t.empty((M, N), dtype=given, device=x.device)
+        out = t.empty(M, N, dtype=given, device=x.device)
     else:
         _ff_like(name, "out", out, (M, N), given, index)
         ldo = 0 if out.is_contiguous() else _ff_stride(name, "out", out)
