@@ -128,13 +128,19 @@ struct GnMerge {
     }
 };
 
+// Where the first pass leaves a chunk's part of a group: those that a team of the second one merges lie in a run ([1, 16384,
+// 320] fp16 13.4 us; a group's width apart 17.7).
+__device__ __forceinline__ float2* gn_part(const GnParams& p, int image, int group, int chunk) {
+    return (float2*)p.partial + ((int64_t)image * p.groups + group) * p.chunks + chunk;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
     using V = GnVec<T>;
     constexpr int kV = V::kV;
     extern __shared__ __attribute__((aligned(16))) float2 parts[];  // [rows][channels] {mean, sum of squares about it}
     const int column = (int)blockIdx.x % p.columns, chunk = (int)blockIdx.x / p.columns;
-    const int image = column / p.slabs, task = image * p.chunks + chunk;
+    const int image = column / p.slabs;
     const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.chunk_pixels;
     const int count = (int)(p.pixels - first < p.chunk_pixels ? p.pixels - first : p.chunk_pixels);
@@ -181,7 +187,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
             merge.add(from[r * slab.channels + c], (float)(r < longer ? each + 1 : each));
         }
         const float2 m = merge.finish((float)count * (float)p.group_channels, p.team);
-        if (lane == 0) ((float2*)p.partial)[(int64_t)task * p.groups + slab.g0 + g] = m;
+        if (lane == 0) *gn_part(p, image, slab.g0 + g, chunk) = m;
     }
 }
 
@@ -193,10 +199,10 @@ __device__ __forceinline__ void merge_stats(const GnParams& p, int image, int g0
     const float whole = (float)p.chunk_pixels * (float)p.group_channels;
     const float last = (float)(p.pixels - (p.chunks - 1) * p.chunk_pixels) * (float)p.group_channels;
     for (int g = (int)threadIdx.x / kMergeTeam; g < groups; g += teams) {
-        const float2* from = (const float2*)p.partial + (int64_t)image * p.chunks * p.groups + g0 + g;
+        const float2* from = gn_part(p, image, g0 + g, 0);
         GnMerge merge{from[0].x};
 #pragma unroll 4
-        for (int k = lane; k < p.chunks; k += kMergeTeam) merge.add(from[(int64_t)k * p.groups], k == p.chunks - 1 ? last : whole);
+        for (int k = lane; k < p.chunks; k += kMergeTeam) merge.add(from[k], k == p.chunks - 1 ? last : whole);
         const float2 m = merge.finish(values, kMergeTeam);
         if (lane == 0) {
             const float2 s{m.x, 1.0f / __builtin_sqrtf(m.y / values + p.eps)};
@@ -409,24 +415,26 @@ __global__ __launch_bounds__(kMaxThreads) void gn_sums_kernel(GnParams p) {
         }
         a = team_sum(a, p.team);
         b = team_sum(b, p.team);
-        if (lane == 0) ((float2*)p.partial)[(int64_t)task * p.groups + slab.g0 + g] = float2{a, b};
+        if (lane == 0) *gn_part(p, image, slab.g0 + g, chunk) = float2{a, b};
     }
 }
 
 constexpr int kParamChannels = 32;  // of a workgroup that adds up dgamma and dbeta
 
-// dx, and in workgroups of their own, the last ones, dgamma and dbeta.
+// dx, and in workgroups of their own, the last ones (in front they push dx's off their data's XCDs: [8, 1024, 1280] 27.1 us and
+// 24.4), dgamma and dbeta.
 template <typename T, FfFamily kFam>
 __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     using V = GnVec<T>;
     constexpr int kV = V::kV;
     extern __shared__ __attribute__((aligned(16))) float2 means[];
-    const int tasks = p.y != nullptr ? p.apply_chunks * p.columns : 0;
-    if ((int)blockIdx.x >= tasks) {
-        const int c = ((int)blockIdx.x - tasks) * kParamChannels + (int)threadIdx.x % kParamChannels;
+    const int tasks = p.y != nullptr ? p.apply_chunks * p.columns : 0, task = (int)blockIdx.x;
+    if (task >= tasks) {
+        const int c = (task - tasks) * kParamChannels + (int)threadIdx.x % kParamChannels;
         const int lanes = (int)blockDim.x / kParamChannels, lane = (int)threadIdx.x / kParamChannels, parts = p.batch * p.chunks;
         float2 sum{0.0f, 0.0f};
         if (c < p.channels)
+#pragma unroll 8
             for (int k = lane; k < parts; k += lanes) {
                 const float2 a = ((const float2*)p.channel_sums)[(int64_t)k * p.channels + c];
                 sum.x += a.x;
@@ -444,7 +452,7 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
         }
         return;
     }
-    const int column = (int)blockIdx.x % p.columns, chunk = (int)blockIdx.x / p.columns, image = column / p.slabs;
+    const int column = task % p.columns, chunk = task / p.columns, image = column / p.slabs;
     const GnSlab slab = slab_of(p, column % p.slabs);
     const int64_t first = (int64_t)chunk * p.apply_pixels;
     const int count = (int)(p.pixels - first < p.apply_pixels ? p.pixels - first : p.apply_pixels);
@@ -462,12 +470,12 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
     const float over = 1.0f / ((float)p.pixels * (float)p.group_channels);
     for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
-        const float2* from = (const float2*)p.partial + (int64_t)image * p.chunks * p.groups + slab.g0 + g;
+        const float2* from = gn_part(p, image, slab.g0 + g, 0);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll 4
         for (int k = lane; k < p.chunks; k += p.team) {
-            s1 += from[(int64_t)k * p.groups].x;
-            s2 += from[(int64_t)k * p.groups].y;
+            s1 += from[k].x;
+            s2 += from[k].y;
         }
         s1 = team_sum(s1, p.team);
         s2 = team_sum(s2, p.team);
@@ -664,8 +672,8 @@ int threads_of(int vecs) {
 int team_of(int groups, int threads) { return 64 * groups <= threads ? 64 : 16; }
 
 // Workgroups of the two passes, and the rounds that a chunk has a multiple of. One workgroup a CU
-// reads fast enough and leaves few parts: [2, 131072, 256] bf16 backward 126 us with 512 and 512, 119 with 256 and 512 or
-// 768, 126 with 256 and 256, 152 with 128 and 512.
+// reads fast enough and leaves few parts: [2, 16384, 640] fp16 25.9 us with 256 and 512, 26.4 with 512 and 512, 29.5 with 256
+// and 256, 25.1 with 256 and 768; [1, 16384, 320] 13.4, 16.8, 14.1, 13.4.
 constexpr int kFirstTasks = 256, kSecondTasks = 512;
 constexpr int kBatchRounds = 4;
 
@@ -775,8 +783,20 @@ GnPlan gn_plan(const GnParams& p, GnType type, GnCall call) {
     }
     slab_groups = slab_groups_of(p, type, kSlabBytes);
     const int vecs = (int)vecs_of(p, type, slab_groups);
-    const int64_t chunk = chunk_of((int64_t)p.batch * (p.groups / slab_groups), p.pixels, threads_of(vecs) / vecs, kFirstTasks, kBatchRounds);
-    return {true, 0, (int32_t)((p.pixels + chunk - 1) / chunk), chunk};
+    const int64_t columns = (int64_t)p.batch * (p.groups / slab_groups);
+    const int rows = threads_of(vecs) / vecs;
+    auto chunks_of = [&](int64_t chunk) { return (p.pixels + chunk - 1) / chunk; };
+    int64_t chunk = chunk_of(columns, p.pixels, rows, kFirstTasks, kBatchRounds);
+    // The gradients' first pass of 16-bit types, whose slopes keep the vector units busy, takes two workgroups a CU where an
+    // image's parts stay few for it and they come out even: [2, 65536, 640] 162 us (one a CU 175), [2, 16384, 640] 42.8 (46.7), [8,
+    // 1024, 1280] 24.7 (25.8), [2, 4096, 640] 16.7 (17.6). Else: of one column [1, 16384, 320] 23.3 (19.2), of two [2, 131072,
+    // 256] 113.8 (112.7); uneven [2, 6144, 960] 27.6 (25.4); fp32 [4, 4096, 320] 20.5 (19.3).
+    if (call == kGnBackward && type != kGnF32 && columns >= 4) {
+        auto rounds_of = [&](int64_t c) { return (columns * chunks_of(c) + kFirstTasks - 1) / kFirstTasks * c; };
+        const int64_t half = chunk_of(columns, p.pixels, rows, 2 * kFirstTasks, kBatchRounds);
+        if (rounds_of(half) <= rounds_of(chunk)) chunk = half;
+    }
+    return {true, 0, (int32_t)chunks_of(chunk), chunk};
 }
 
 namespace {

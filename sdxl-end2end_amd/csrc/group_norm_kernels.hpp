@@ -16,7 +16,7 @@ struct GnParams {
     float* q_scale;
     const float* stats;    // backward: [batch][groups] {mean, rstd}
     float* stats_out;      // forward, nullable
-    float* partial;        // [batch][chunks][groups] {mean, sum of squares about it}; backward: {sum gamma dz, sum gamma dz n}
+    float* partial;        // [batch][groups][chunks] {mean, sum of squares about it}; backward: {sum gamma dz, sum gamma dz n}
     float* channel_sums;   // backward [batch][chunks][channels] {sum dz, sum dz n}
     int64_t ld_x, ld_y, ld_dy;  // elements
     int64_t ld_q;               // bytes
