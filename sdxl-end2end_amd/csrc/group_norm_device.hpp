@@ -16,8 +16,8 @@ namespace {
 template <typename T, FfFamily kFam>
 __device__ __forceinline__ float gn_value(const FfAct& a, float z) {
     if constexpr (__is_same(T, float) && kFam == kFamErf) {
-        const float zc = __builtin_fmaxf(z, -30.0f);  // (0 there; -infinity too)
-        return zc != zc ? z : zc * (0.5f * erfcf(zc * -0.7071067811865476f));
+        const float zc = z < -30.0f ? -30.0f : z;  // (0 there, -infinity too; NaN stays, which a maximum would drop)
+        return zc * (0.5f * erfcf(zc * -0.7071067811865476f));
     } else {
         return ff_value<kFam>(a, z);
     }

@@ -410,3 +410,23 @@ def test_cpp_group_norm_and_int8_cases():
     exe = os.path.join(ROOT, "sdxl-end2end_amd", "bin", "sdxl_hip_ops_test")
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "group norm and 8-bit cases passed" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("activation", ACTS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_is_not_finite_under_every_activation(dtype, activation, value):
+    """The group's rows are NaN, through one launch, two, and the general kernels (rows below 16 bytes)."""
+    for P, C, G in ((60, 64, 8), (2000, 64, 8), (50, 3, 3)):
+        x = values(1, 2, P, C, dtype=dtype)
+        gamma, beta = values(2, C, mean=1.0, dtype=dtype), values(3, C, dtype=dtype)
+        clean = sh.group_norm(x, gamma, beta, G, activation=activation)
+        group = slice(C // G, 2 * (C // G))
+        x[1, P // 2, C // G + C // G // 2] = value
+        got, stats = sh.group_norm(x, gamma, beta, G, activation=activation, with_stats=True)
+        hit = torch.zeros(2, P, C, dtype=torch.bool, device=DEV)
+        hit[1, :, group] = True
+        assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit]), (P, C)
+        dx, dgamma, _ = sh.group_norm_backward(values(4, 2, P, C, dtype=dtype), x, gamma, beta, G, stats, activation=activation)
+        assert dx[hit].isnan().all() and not dx[~hit].isnan().any(), (P, C)
+        assert torch.equal(dgamma.isnan(), hit[1].any(dim=0)), (P, C)
