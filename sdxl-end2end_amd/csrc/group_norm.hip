@@ -15,13 +15,14 @@
 // chunks as workgroups, whose parts every workgroup of the second pass has to
 // merge ([2, 4096, 960] fp16: 66 us, of which 256 chunks' parts were most).
 //
-// Statistics: a thread sums x - p and (x - p)^2 with p its own first value of the
-// channel, which gives its mean and sum of squares about it; these are merged in
-// the same way about one of the means, M = sum M_i + n_i d_i^2 - (sum n_i d_i)^2 /
-// n with d_i = mean_i - mean_0, first the workgroup's threads in LDS, then the
-// chunks. The value that sums are taken about is one of the n that they are made
-// of, so that its distance from the mean is at most sqrt(M) and the subtraction
-// costs M at most a relative n 2^-24, whatever the mean.
+// Statistics: a thread takes its pixels in batches of eight and sums x - p and (x - p)^2 of a batch, with p the mean of
+// the pixels before it (of the first batch: its first value), then adds the batch to its mean and its sum M of squares
+// about it. Summed about the first value alone, q of n pixels is up to n M where that value lies far from the others, and
+// n roundings of such a q left M off by a relative n^2 2^-24 ([129, 16384, 128] fp32, 1024 pixels a thread, a first value
+// 1000 deviations away: rstd off by 1.7e-3, so by 1.1e-6). About the mean so far a batch's q is at most twice what it adds to M (the first
+// one's eight times). Parts {mean, M} of threads, then of chunks, are merged in the same way: by a lane about its own
+// first part, M = sum M_i + n_i d_i^2 - (sum n_i d_i)^2 / n with d_i = mean_i - mean_0, of as many parts as it has (I of
+// them: M off by a relative 3 (I + 1) (I + 3) 2^-24 at most), then over the lanes of its team about the mean of all.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -88,7 +89,7 @@ struct GnBatch {
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    // f(a's vector, b's) of each, from pixel `first` of the batch on
+    // f(a's vector, b's) of each, from pixel `kFirst` of the batch on
     template <int kFirst = 0, typename Fn>
     __device__ __forceinline__ void visit(int left, Fn&& f) {
 #pragma unroll
@@ -98,9 +99,9 @@ struct GnBatch {
         }
     }
     // the batch that is loaded, after whose start f is called with what follows it, up to n pixels
-    template <int kFirst = 0, typename Fn>
+    template <typename Fn>
     __device__ __forceinline__ void visit_all(int n, const char* from_a, int64_t step_a, const char* from_b, int64_t step_b, Fn&& f) {
-        visit<kFirst>(n, f);
+        visit(n, f);
         while (n > kBatch) {
             n -= kBatch;
             from_a += kBatch * step_a;
@@ -111,20 +112,23 @@ struct GnBatch {
     }
 };
 
-// The mean and centred sum of parts {mean, centred sum} of n values each, as sums about one of the means.
+// The mean and centred sum of parts {mean, centred sum} of n values each, the lane's as sums about the first of them (a lane
+// that has none: any part, of no values).
 struct GnMerge {
-    float about, first = 0.0f, second = 0.0f;
+    float about, values, first = 0.0f, second;
+    __device__ __forceinline__ GnMerge(float2 part, float n) : about(part.x), values(n), second(n > 0.0f ? part.y : 0.0f) {}
     __device__ __forceinline__ void add(float2 part, float n) {
         const float d = part.x - about;
+        values += n;
         first = __builtin_fmaf(d, n, first);
-        second += __builtin_fmaf(d * d, n, part.y);
+        second += __builtin_fmaf(d * d, n, n > 0.0f ? part.y : 0.0f);
     }
-    // of all `values` values, over the team
-    __device__ __forceinline__ float2 finish(float values, int team) {
-        const float f = team_sum(first, team) / values, s = team_sum(second, team);
-        // (negative by rounding where there is no spread; NaN stays)
-        const float m = __builtin_fmaf(-f * values, f, s);
-        return float2{about + f, m < 0.0f ? 0.0f : m};
+    // of all `all` values, over the team; ref: the same mean of a part in every lane
+    __device__ __forceinline__ float2 finish(float all, float ref, int team) const {
+        const float f = values > 0.0f ? first * __builtin_amdgcn_rcpf(values) : 0.0f;
+        const float own = __builtin_fmaf(-first, f, second);  // (negative by rounding where there is no spread; NaN stays)
+        const float d = (about - ref) + f, mean = team_sum(values * d, team) * __builtin_amdgcn_rcpf(all), t = d - mean;
+        return float2{ref + mean, team_sum(__builtin_fmaf(values * t, t, own < 0.0f ? 0.0f : own), team)};
     }
 };
 
@@ -150,11 +154,12 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
         const int64_t step = p.ld_x * p.rows_at_once * (int64_t)sizeof(T);
         const char* x = (const char*)p.x + ((image * p.pixels + first + at.r) * p.ld_x + slab.c0 + at.c0) * (int64_t)sizeof(T);
         const int n = share_of(count, at.r, p.rows_at_once);
-        GnBatch<8, false> batch;
+        constexpr int kBatch = 8;
+        GnBatch<kBatch, false> batch;
         batch.load(n, x, step, nullptr, 0);
         float pivot[kV], s[kV] = {}, q[kV] = {};
         V::unpack(batch.a[0], pivot);
-        batch.visit_all<1>(n, x, step, nullptr, 0, [&](u32x4 d, u32x4) __attribute__((always_inline)) {
+        auto add = [&](u32x4 d, u32x4) __attribute__((always_inline)) {
             float v[kV];
             V::unpack(d, v);
 #pragma unroll
@@ -163,14 +168,41 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
                 s[e] += t;
                 q[e] = __builtin_fmaf(t, t, q[e]);
             }
-        });
-        const float over = 1.0f / (float)n;
-        float2* to = parts + at.r * slab.channels + at.c0;
+        };
+        batch.template visit<1>(n, add);
+        float seen = (float)min(n, kBatch), over = __builtin_amdgcn_rcpf(seen);
+        float mean[kV], squares[kV];  // mean: from the pivot on; squares: about the mean
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-            const float m = s[e] * over, c = __builtin_fmaf(-s[e], m, q[e]);
-            if (e >= at.skip) to[e] = float2{pivot[e] + m, c < 0.0f ? 0.0f : c};
+            mean[e] = s[e] * over;
+            squares[e] = __builtin_fmaf(-s[e], mean[e], q[e]);
         }
+        for (int left = n - kBatch; left > 0; left -= kBatch) {
+            x += kBatch * step;
+            batch.load(left, x, step, nullptr, 0);
+            float off[kV];  // of the pivot from the mean
+#pragma unroll
+            for (int e = 0; e < kV; ++e) {
+                const float to = pivot[e] + mean[e];
+                off[e] = (pivot[e] - to) + mean[e];
+                pivot[e] = to;
+                s[e] = q[e] = 0.0f;
+            }
+            batch.visit(left, add);
+            const float before = seen;
+            seen += (float)min(left, kBatch);
+            over = __builtin_amdgcn_rcpf(seen);
+#pragma unroll
+            for (int e = 0; e < kV; ++e) {
+                const float sum = __builtin_fmaf(before, off[e], s[e]);
+                mean[e] = sum * over;
+                squares[e] += __builtin_fmaf(-sum, mean[e], __builtin_fmaf(before * off[e], off[e], q[e]));
+            }
+        }
+        float2* to = parts + at.r * slab.channels + at.c0;
+#pragma unroll
+        for (int e = 0; e < kV; ++e)
+            if (e >= at.skip) to[e] = float2{pivot[e] + mean[e], squares[e] < 0.0f ? 0.0f : squares[e]};
     }
     __syncthreads();
     const int teams = (int)blockDim.x / p.team, lane = (int)threadIdx.x % p.team;
@@ -180,13 +212,17 @@ __global__ __launch_bounds__(kMaxThreads) void gn_stats_kernel(GnParams p) {
     for (int g = (int)threadIdx.x / p.team; g < slab.groups; g += teams) {
         const float2* from = parts + g * p.group_channels;
         const int all = rows * p.group_channels;
-        GnMerge merge{from[0].x};
+        auto row_of = [&](int e) { return (int)(((float)e + 0.5f) * over_channels); };  // (e < 2^13: exact)
+        auto part = [&](int e, int r) { return from[r * slab.channels + e - r * p.group_channels]; };
+        auto values = [&](int r) { return (float)(r < longer ? each + 1 : each); };
+        const int e0 = min(lane, all - 1), r0 = row_of(e0);
+        GnMerge merge(part(e0, r0), lane < all ? values(r0) : 0.0f);
 #pragma unroll 4
-        for (int e = lane; e < all; e += p.team) {
-            const int r = (int)(((float)e + 0.5f) * over_channels), c = e - r * p.group_channels;  // (e < 2^13: exact)
-            merge.add(from[r * slab.channels + c], (float)(r < longer ? each + 1 : each));
+        for (int e = lane + p.team; e < all; e += p.team) {
+            const int r = row_of(e);
+            merge.add(part(e, r), values(r));
         }
-        const float2 m = merge.finish((float)count * (float)p.group_channels, p.team);
+        const float2 m = merge.finish((float)count * (float)p.group_channels, from[0].x, p.team);
         if (lane == 0) *gn_part(p, image, slab.g0 + g, chunk) = m;
     }
 }
@@ -200,10 +236,19 @@ __device__ __forceinline__ void merge_stats(const GnParams& p, int image, int g0
     const float last = (float)(p.pixels - (p.chunks - 1) * p.chunk_pixels) * (float)p.group_channels;
     for (int g = (int)threadIdx.x / kMergeTeam; g < groups; g += teams) {
         const float2* from = gn_part(p, image, g0 + g, 0);
-        GnMerge merge{from[0].x};
-#pragma unroll 4
-        for (int k = lane; k < p.chunks; k += kMergeTeam) merge.add(from[k], k == p.chunks - 1 ? last : whole);
-        const float2 m = merge.finish(values, kMergeTeam);
+        const float2 own = from[min(lane, p.chunks - 1)];
+        auto of = [&](int k) { return k < p.chunks - 1 ? whole : k == p.chunks - 1 ? last : 0.0f; };
+        GnMerge merge(own, 0.0f);
+        if (p.chunks <= kMergeTeam) merge = GnMerge(own, of(lane));
+        else
+            for (int k = lane; k < p.chunks; k += 4 * kMergeTeam) {
+                float2 part[4];  // on their way together, past the last part that one again, of no values
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[i] = from[min(k + i * kMergeTeam, p.chunks - 1)];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) merge.add(part[i], of(k + i * kMergeTeam));
+            }
+        const float2 m = merge.finish(values, from[0].x, kMergeTeam);
         if (lane == 0) {
             const float2 s{m.x, 1.0f / __builtin_sqrtf(m.y / values + p.eps)};
             stats[g] = s;

@@ -430,3 +430,30 @@ def test_what_is_not_finite_under_every_activation(dtype, activation, value):
         dx, dgamma, _ = sh.group_norm_backward(values(4, 2, P, C, dtype=dtype), x, gamma, beta, G, stats, activation=activation)
         assert dx[hit].isnan().all() and not dx[~hit].isnan().any(), (P, C)
         assert torch.equal(dgamma.isnan(), hit[1].any(dim=0)), (P, C)
+
+
+@pytest.mark.parametrize("far", [30.0, 300.0, 3000.0, 1e5])
+@pytest.mark.parametrize("B,P,C,G,first,rounds,parts,chunks", [(129, 16384, 128, 32, 1, 1024, 4, 1), (1, 262144, 256, 32, 1, 128, 8, 8),
+                                                               (1, 65536, 128, 32, 256, 16, 4, 16), (1, 65536, 128, 32, 4096, 16, 4, 16)])
+def test_digits_of_rstd_where_the_first_values_lie_far_off(B, P, C, G, first, rounds, parts, chunks, far):
+    """One value of a group, or its first pixels, `far` deviations from the others: rstd keeps its digits.
+
+    With M a group's sum of squares about its mean: a thread's batch of 8 has q about a pivot, off by 30 u q (8 terms of
+    two roundings each, the sum's square, their difference); q is at most 8 times what the first batch adds to M (the pivot
+    is one of its values), twice what a later one adds (it is the mean of as many). rounds / 8 batches are added up.
+    A lane merges `parts` threads' parts and then `chunks` chunks' parts, I of them about the first: 3 (I + 3) u of a sum
+    that is at most I + 1 times M (the first is a part of it). The teams' sums and the rest: 32 u. rstd is off by half of it."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(B, P, C, generator=gen, device=DEV)
+    if first == 1:
+        x[:, 0, ::C // G] = far
+    else:
+        x[:, :first] += far
+    _, stats = sh.group_norm(x, torch.ones(C, device=DEV), torch.zeros(C, device=DEV), G, with_stats=True)
+    merged = sum(3 * (i + 3) * (i + 1) for i in (parts, chunks))
+    bound = 0.5 * (240 + rounds / 8 + merged + 32) * U
+    for image, got in zip(x, stats):
+        v = image.double().view(P, G, C // G)
+        mean = v.mean(dim=(0, 2))
+        rstd = ((v - mean.view(1, G, 1)).square().mean(dim=(0, 2)) + 1e-5).rsqrt()
+        within(got[:, 1], rstd, rstd * bound, "rstd")
