@@ -322,8 +322,8 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
     });
 }
 
-// Codes by row. The row's lanes keep their channels' constants: z = x a + b, with b = beta - mean a rounded to 2^-24 of
-// mean a (a 16-bit x itself has 2^-12 of it at best). Every workgroup merges the parts of all groups, so that eight waves
+// Codes by row. The row's lanes keep their channels' constants, of z as sdxl_group_norm forms it. (x a + (beta - mean a) is
+// off by 2^-24 of mean a: up to 0.03 for x = 1000 throughout and eps 1e-6, where z is beta.) Every workgroup merges the parts of all groups, so that eight waves
 // with a row each and a workgroup a CU beat four and two ([1, 16384, 320] fp16, both passes: 16.7 us and 20.8; [2, 1024,
 // 1280] 10.0 and 11.1; sixteen 16.1 and 12.1).
 template <typename T, FfFamily kFam, int kWaves, int kVecs>
@@ -346,21 +346,17 @@ __global__ __launch_bounds__(kWaves == 1 ? 512 : 256) void gn_rows_kernel(GnPara
     int r = (int)threadIdx.x / (64 * kWaves);
     fetch(r);
     merge_stats(p, image, 0, p.groups, p.stats_out != nullptr && chunk == 0, stats);
-    float a[kVecs][8], b[kVecs][8];
+    GnAffine<T> affine[kVecs];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-        load_channels<T>(p.gamma, row.column(i), a[i]);
-        load_channels<T>(p.beta, row.column(i), b[i]);
+        load_channels<T>(p.gamma, row.column(i), affine[i].a);
+        load_channels<T>(p.beta, row.column(i), affine[i].b);
     }
     const FfAct act = ff_act(p.activation);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float2 s = stats[group_of(p, row.column(i) + e)];
-            a[i][e] *= s.y;
-            b[i][e] = __builtin_fmaf(-s.x, a[i][e], b[i][e]);
-        }
+        for (int e = 0; e < 8; ++e) affine[i].set(e, stats[group_of(p, row.column(i) + e)]);
     }
     for (; r < count; r += kRows) {
         float v[kVecs][8];
@@ -368,7 +364,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 512 : 256) void gn_rows_kernel(GnPara
         for (int i = 0; i < kVecs; ++i) {
             GnVec<T>::unpack(d[i], v[i]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = ff_value<kFam>(act, __builtin_fmaf(v[i][e], a[i][e], b[i][e]));
+            for (int e = 0; e < 8; ++e) v[i][e] = ff_value<kFam>(act, affine[i].z(e, v[i][e]));
         }
         fetch(r + kRows);
         const int64_t at = image * p.pixels + first + r;

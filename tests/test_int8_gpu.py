@@ -316,3 +316,15 @@ def test_transformer_entry_captured(B, P):
     check(outs[1], q.view(B * P, C), s, *weights[1], bias[1], "gelu", True)
     q, s = sh.quantize_i8_rows(outs[1])
     check(outs[2], q, s, *weights[2], bias[2], "none", False, residual=outs[0])
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("P,C,G", [(1, 64, 8), (300, 64, 8), (50, 1280, 32), (20, 3200, 4), (9, 6, 3)])
+def test_group_norm_codes_of_constant_groups(P, C, G, dtype):
+    """x - mean is 0, so that z is beta itself, whatever the mean and rstd = 1 / sqrt(eps): codes and scales are beta's."""
+    gamma, beta = values(2, C, mean=1.0, dtype=dtype), values(3, C, dtype=dtype)
+    want_q, want_s = quantized(beta.expand(2, P, C))
+    for value in (3.0, 1000.0, -60000.0 if dtype == F16 else -2.0 ** 26):
+        x = torch.full((2, P, C), value, dtype=dtype, device=DEV)
+        q, s = sh.group_norm_i8(x, gamma, beta, G, eps=1e-6)
+        assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu().float(), want_q), value
