@@ -25,6 +25,7 @@
 // them: M off by a relative 3 (I + 1) (I + 3) 2^-24 at most), then over the lanes of its team about the mean of all.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "group_norm_device.hpp"
@@ -473,23 +474,24 @@ __global__ __launch_bounds__(kMaxThreads) void gn_dx_kernel(GnParams p) {
     if (task >= tasks) {
         const int c = (task - tasks) * kParamChannels + (int)threadIdx.x % kParamChannels;
         const int lanes = (int)blockDim.x / kParamChannels, lane = (int)threadIdx.x / kParamChannels, parts = p.batch * p.chunks;
-        float2 sum{0.0f, 0.0f};
+        double2* const joined = (double2*)means;
+        double2 sum{0.0, 0.0};  // (in 64 bits: a lane may have thousands of images' parts)
         if (c < p.channels)
 #pragma unroll 8
             for (int k = lane; k < parts; k += lanes) {
                 const float2 a = ((const float2*)p.channel_sums)[(int64_t)k * p.channels + c];
-                sum.x += a.x;
-                sum.y += a.y;
+                sum.x += (double)a.x;
+                sum.y += (double)a.y;
             }
-        means[threadIdx.x] = sum;
+        joined[threadIdx.x] = sum;
         __syncthreads();
         if (lane == 0 && c < p.channels) {
             for (int k = 1; k < lanes; ++k) {
-                sum.x += means[k * kParamChannels + threadIdx.x].x;
-                sum.y += means[k * kParamChannels + threadIdx.x].y;
+                sum.x += joined[k * kParamChannels + threadIdx.x].x;
+                sum.y += joined[k * kParamChannels + threadIdx.x].y;
             }
-            if (p.dbeta != nullptr) ((T*)p.dbeta)[c] = (T)sum.x;
-            if (p.dgamma != nullptr) ((T*)p.dgamma)[c] = (T)sum.y;
+            if (p.dbeta != nullptr) ((T*)p.dbeta)[c] = (T)(float)sum.x;
+            if (p.dgamma != nullptr) ((T*)p.dgamma)[c] = (T)(float)sum.y;
         }
         return;
     }
@@ -913,7 +915,7 @@ hipError_t launch_gn_backward(const GnPlan& plan, const GnParams& params, GnType
     if (err != hipSuccess) return err;
     cut_second(p, p.columns, p.rows_at_once, kSecondTasks, kBatchRounds);
     const int64_t grid = (p.y != nullptr ? (int64_t)p.columns * p.apply_chunks : 0) + (parameters ? (p.channels + kParamChannels - 1) / kParamChannels : 0);
-    const size_t lds = (size_t)(p.slab_groups > threads ? p.slab_groups : threads) * 8;
+    const size_t lds = std::max((size_t)p.slab_groups * sizeof(float2), (size_t)threads * sizeof(double2));
     return by_type(type, p.activation, [&]<typename T, FfFamily kFam>() {
         hipLaunchKernelGGL((gn_dx_kernel<T, kFam>), dim3((unsigned)grid), dim3(threads), lds, stream, p);
         return hipGetLastError();

@@ -457,3 +457,22 @@ def test_digits_of_rstd_where_the_first_values_lie_far_off(B, P, C, G, first, ro
         mean = v.mean(dim=(0, 2))
         rstd = ((v - mean.view(1, G, 1)).square().mean(dim=(0, 2)) + 1e-5).rsqrt()
         within(got[:, 1], rstd, rstd * bound, "rstd")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,P,C,G", [(300000, 1, 64, 4), (70000, 3, 96, 32), (100000, 2, 6, 3)])
+def test_parameter_gradients_of_many_images(B, P, C, G, dtype):
+    """dgamma and dbeta of gradients of one sign, over images by the hundred thousand: an image's sums are made in fp32 (P
+    terms), the images' in 64 bits."""
+    x = values(1, B, P, C, dtype=dtype)
+    gamma, beta = values(2, C, mean=1.0, dtype=dtype), values(3, C, dtype=dtype)
+    stats = stats64(x, G, 1e-5)
+    n = (x.double().view(B, P, G, -1) - stats[:, :, 0].double().view(B, 1, G, 1)) * stats[:, :, 1].double().view(B, 1, G, 1)
+    n = n.view(B, P, C)
+    for dy in ((values(4, B, P, C).abs() * 0.1 + 0.05).to(dtype), torch.full_like(x, 0.07)):
+        _, dgamma, dbeta = sh.group_norm_backward(dy, x, gamma, beta, G, stats)
+        d = dy.double()
+        for got, terms_of in ((dbeta, d), (dgamma, d * n)):
+            want, mass = terms_of.sum(dim=(0, 1)), terms_of.abs().sum(dim=(0, 1))
+            err = (P + 8) * U * mass  # P terms, each of three roundings, the image's sum times rstd; 64 bits to fp32
+            within(got, want, err + HALF[dtype] * (want.abs() + err) + TINY[dtype], (B, P, C))
