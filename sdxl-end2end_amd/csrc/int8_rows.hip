@@ -83,7 +83,11 @@ __global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) d[i] = ((const Unaligned<2>*)(x + row.column(i) * 2))->v;
         u32x4 g[kNorm ? kVecs : 1], b[kNorm ? kVecs : 1];  // on the way before the sums
+        // the value that the mean is summed about: of a row of one value the sum is 0 and the mean that value (10239 times
+        // 2047 is not a number of 24 bits: the mean was off by 1.2e-4, and codes of such rows by 7 steps)
+        [[maybe_unused]] T pivot{};
         if constexpr (kNorm) {
+            pivot = *(const T*)x;
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
                 g[i] = ((const Unaligned<2>*)((const char*)p.gamma + row.column(i) * 2))->v;
@@ -102,9 +106,9 @@ __global__ __launch_bounds__(kThreads) void i8_rows_kernel(I8RowsParams p) {
             for (int i = 0; i < kVecs; ++i) {
                 const int skip = row.has(i) ? row.skip(i) : 8;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum += e >= skip ? v[i][e] : 0.0f;
+                for (int e = 0; e < 8; ++e) sum += e >= skip ? v[i][e] - (float)pivot : 0.0f;
             }
-            const float mean = row.reduce(sum, part, Add{}) / (float)p.cols;
+            const float mean = (float)pivot + row.reduce(sum, part, Add{}) / (float)p.cols;
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
                 const int skip = row.has(i) ? row.skip(i) : 8;

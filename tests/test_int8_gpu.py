@@ -328,3 +328,14 @@ def test_group_norm_codes_of_constant_groups(P, C, G, dtype):
         x = torch.full((2, P, C), value, dtype=dtype, device=DEV)
         q, s = sh.group_norm_i8(x, gamma, beta, G, eps=1e-6)
         assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu().float(), want_q), value
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("K", [8, 77, 1280, 2563, 8200, 10239, 10240, 11001])
+def test_layer_norm_codes_of_constant_rows(K, dtype):
+    """x - mean is 0, so that the codes and scales are beta's."""
+    gamma, beta = values(2, K, mean=1.0, dtype=dtype), values(3, K, dtype=dtype)
+    want_q, want_s = quantized(beta.expand(5, K))
+    for value in (3.0, 2047.0, -2047.0 * 32, 0.1):
+        q, s = sh.layer_norm_i8(torch.full((5, K), value, dtype=dtype, device=DEV), gamma, beta)
+        assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu().float(), want_q), value
