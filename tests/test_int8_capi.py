@@ -183,3 +183,25 @@ def test_kernels_of_no_call():
     for size in (1, 5, 64):
         assert lib.sdxl_i8_kernels(ctypes.byref(desc(m=40, x_dtype=sh.F16)), 1, text, size) == len(whole)
         assert text.value.decode() == whole[:size - 1]
+
+
+# sizes that reach the kernels with stages of 128 bytes through more stages than their rings hold (at most four), the last one in part
+DEEP_KERNELS = {
+    "tile 64x64": ((5516, 67, 592), (33, 4162, 720)), "tile 64x128": ((6715, 265, 656), (133, 5494, 592)),
+    "tile 128x128": ((2589, 823, 2256), (414, 2358, 2096)), "tile 128x192": ((6737, 523, 656), (6540, 265, 720)),
+    "tile 128x256": ((6812, 769, 720), (522, 4953, 720)), "tile 256x192": ((5399, 1325, 688), (6543, 522, 720)),
+    "tile 256x256": ((6520, 1745, 592), (1051, 4955, 656)), "tile 256x320": ((6620, 2308, 592), (1281, 5633, 624)),
+    "staged 64x64": ((6412, 66, 715), (33, 4706, 587)), "staged 128x128": ((6551, 529, 651), (279, 5458, 715)),
+}
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kernel", DEEP_KERNELS)
+def test_sizes_of_kernels_in_depth(kernel, gated):
+    m, n, k = DEEP_KERNELS[kernel][gated]
+    assert k > 4 * 128 and k % 128 != 0 and m % 32 != 0
+    assert sh.i8_kernels(desc(m=m, n=n, k=k), gated) == kernel and sh.i8_kernels(desc(m=m, n=n, k=k, dtype=sh.BF16), gated) == kernel
+
+
+def test_every_tile_has_a_size_in_depth():
+    assert set(DEEP_KERNELS) == {k for k in KERNELS if k.startswith(("tile", "staged"))}

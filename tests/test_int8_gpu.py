@@ -10,7 +10,7 @@ import pytest
 
 import sdxl_hip as sh
 from test_group_norm_gpu import BF16, DEV, F16, HALF, TINY, U, act64, check_forward, normal_form, values, within
-from test_int8_capi import KERNELS
+from test_int8_capi import DEEP_KERNELS, KERNELS
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -339,3 +339,17 @@ def test_layer_norm_codes_of_constant_rows(K, dtype):
     for value in (3.0, 2047.0, -2047.0 * 32, 0.1):
         q, s = sh.layer_norm_i8(torch.full((5, K), value, dtype=dtype, device=DEV), gamma, beta)
         assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu().float(), want_q), value
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kernel", DEEP_KERNELS)
+def test_each_tile_in_depth(kernel, gated):
+    """More stages than the ring holds, the last one in part; distinct codes, scales and biases in every place."""
+    M, N, K = DEEP_KERNELS[kernel][gated]
+    for dtype in HALVES:
+        features = 2 * N if gated else N
+        x, xs, w, ws = codes(1, M, K, low=-128), scales(1, M), codes(2, features, K), scales(3, features)
+        bias = values(4, features, dtype=dtype)
+        fn = sh.gated_linear_i8 if gated else sh.linear_i8
+        given = dict(bias=bias, activation="none") | ({} if gated else dict(residual=values(5, M, N, dtype=dtype)))
+        check(fn(x, w, ws, x_scale=xs, dtype=dtype, **given), x, xs, w, ws, bias, "none", gated, residual=given.get("residual"))
