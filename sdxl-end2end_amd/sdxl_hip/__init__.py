@@ -909,6 +909,8 @@ def group_norm_backward(dout, x, gamma, beta, groups: int, stats, activation: st
     if dout.shape != x.shape or dout.dtype != x.dtype or dout.get_device() != index:
         raise SdxlError(INVALID_SHAPE, f"{name}: dout must be like x")
     lddy = 0 if dout.is_contiguous() else _gn_stride(name, "dout", dout, channels)
+    if stats is None:
+        raise SdxlError(INVALID_ARGUMENT, f"{name}: the stats of the forward call are needed")
     _gn_stats(name, t, stats, False, batch, groups, x, index)
     desc = _GROUP_NORM_DESC.pack(batch, pixels, channels, groups, ldx, 0, lddy, code, act, 0.0, 0)
     lib = load()

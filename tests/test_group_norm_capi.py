@@ -135,3 +135,9 @@ def test_python_refusals():
                 lambda: sh.group_norm_i8(x.float(), g.float(), g.float(), 8)):
         with pytest.raises(sh.SdxlError):
             bad()
+
+
+def test_python_gradients_without_statistics():
+    x, g = torch.zeros(2, 4, 64, dtype=torch.float16), torch.zeros(64, dtype=torch.float16)
+    with pytest.raises(sh.SdxlError, match="stats"):
+        sh.group_norm_backward(x, x, g, g, 8, None)
