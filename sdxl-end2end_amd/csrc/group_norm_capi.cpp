@@ -88,6 +88,7 @@ size_t workspace_of(const Call& c, const GnPlan& plan, bool backward) {
 size_t workspace_bytes_of(const sdxl_group_norm_desc* d, sdxl_hip::GnCall call, const char* name) {
     Call c;
     if (resolve(d, name, c) != SDXL_STATUS_OK || c.empty) return 0;
+    if (call == sdxl_hip::kGnRows && c.type == sdxl_hip::kGnF32) return 0;  // (which the call refuses)
     return workspace_of(c, gn_plan(c.p, c.type, call), call == sdxl_hip::kGnBackward);
 }
 

@@ -141,3 +141,8 @@ def test_python_gradients_without_statistics():
     x, g = torch.zeros(2, 4, 64, dtype=torch.float16), torch.zeros(64, dtype=torch.float16)
     with pytest.raises(sh.SdxlError, match="stats"):
         sh.group_norm_backward(x, x, g, g, 8, None)
+
+
+def test_no_workspace_for_codes_of_fp32():
+    assert call("i8", desc(dtype=sh.F32)) == sh.INVALID_SHAPE
+    assert sh.group_norm_workspace_bytes(2, 1 << 17, 64, 8, sh.F32, call="i8") == 0
