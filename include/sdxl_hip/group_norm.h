@@ -10,10 +10,13 @@
  *
  * Types: x, gamma, beta, y, dy and the gradients are fp16, bf16 or fp32 (desc->dtype), the
  * statistics, sums and scales fp32, and every output is rounded once. A group's variance is
- * summed about values of its own, so that a mean far from zero costs no digits. Any batch,
+ * summed about values of its own, so that neither a mean far from zero nor a value far from the
+ * others costs digits; sums of squared distances from the mean have to stay within fp32. Any batch,
  * pixels and channels, any row strides of at least a row; image b follows image b - 1 after
- * pixels * row_stride elements. Tensors need only their element's alignment. Rows shorter than
- * 16 bytes, groups of more than 8 KiB a row, more than 4096 groups, some millions of images and
+ * pixels * row_stride elements. Tensors need only their element's alignment. Kernels work on slabs
+ * of whole groups, as many as the smallest divisor of the groups that makes 512 bytes of a row (all
+ * of a shorter row). Slabs of more than 8 KiB (groups that wide; 37 groups of 256 bytes, which no
+ * divisor cuts), rows shorter than 16 bytes, more than 4096 groups, some millions of images and
  * strides above 2^20 elements take general kernels, many times as long (sdxl_group_norm_i8: rows
  * of more than 20 KiB too).
  * A NaN or an infinity in a group makes its rows NaN, and no other group's.
@@ -52,7 +55,10 @@ typedef struct sdxl_group_norm_desc {
 } sdxl_group_norm_desc;
 
 /* Workspaces of the calls below (parts of the sums), 256-byte aligned; 0 where a call needs none
- * (sdxl_group_norm of small images) and for a descriptor that the call refuses. */
+ * (sdxl_group_norm of small images) and for a descriptor that the call refuses. They hold 8 bytes
+ * for every image, chunk of its pixels (at least one) and group, for the gradients every channel
+ * too: below 2 MiB for the UNet's and the VAE's sizes, but 8 * batch * channels bytes at least,
+ * more than the tensor itself where images have fewer than four pixels of a 16-bit type. */
 size_t sdxl_group_norm_workspace_bytes(const sdxl_group_norm_desc* desc);
 size_t sdxl_group_norm_i8_workspace_bytes(const sdxl_group_norm_desc* desc);
 size_t sdxl_group_norm_backward_workspace_bytes(const sdxl_group_norm_desc* desc);

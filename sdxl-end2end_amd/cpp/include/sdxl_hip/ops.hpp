@@ -109,7 +109,8 @@ public:
 
     // act((input - mean) * rstd * weight + bias) with the statistics of an image's groups, channels
     // last (the spatial transformer's and the residual blocks' norms, unet.cpp:151-181): input
-    // [B, ..., C] fp16, bf16 or fp32, weight and bias [C] of its type.
+    // [B, ..., C] fp16, bf16 or fp32, weight and bias [C] of its type. (The statistics that the
+    // gradients take come from sdxl_group_norm.)
     [[nodiscard]] Tensor group_norm(const Tensor& input, const Tensor& weight, const Tensor& bias, std::size_t groups,
                                     Activation activation = Activation::None, float epsilon = 1.0e-5F) const;
 

@@ -55,6 +55,8 @@ constexpr TileCost kTiles[kFfTiles] = {{256, 320, 1.60f, 0.0f, 15.0f}, {256, 256
 //   256 x 256  gated [8192, 2048] -> 2 x 5456 195 (1.88 POP/s), [16384, 2048] x [2048, 2048] 76-80
 //   256 x 192  [8192, 5120] x [1280, 5120] 66 (256 x 256: 72, 128 x 192: 73)
 //   128 x 256  [2048, 1280] x [3840, 1280] 19 (256 x 256: 25)
+//   128 x 192  [8192, 640] x [640, 640] 11.9 (128 x 256: 13.7, 64 x 128: 14.5), [4096, 2560] x [1280, 2560] 23.5 (25.2, 30.2)
+//   128 x 128  [2048, 5120] x [1280, 5120] 26.7 (64 x 128: 28.6, 128 x 192: 31.9)
 //    64 x 128  [4940, 640] x [640, 640] 9.2 (128 x 128: 10.4)
 //    64 x  64  [154, 1280] x [5120, 1280] 7.7 (32 x 32, shared depth: 10.1)
 // On a whole chip the matrix cores' power holds the long products back, the library's too (8192 cubed 1.97 POP/s).

@@ -832,7 +832,8 @@ GnPlan gn_plan(const GnParams& p, GnType type, GnCall call) {
     int64_t chunk = chunk_of(columns, p.pixels, rows, kFirstTasks, kBatchRounds);
     // The gradients' first pass of 16-bit types, whose slopes keep the vector units busy, takes two workgroups a CU where an
     // image's parts stay few for it and they come out even: [2, 65536, 640] 162 us (one a CU 175), [2, 16384, 640] 42.8 (46.7), [8,
-    // 1024, 1280] 24.7 (25.8), [2, 4096, 640] 16.7 (17.6). Else: of one column [1, 16384, 320] 23.3 (19.2), of two [2, 131072,
+    // 1024, 1280] 24.7 (25.8), [2, 4096, 640] 16.7 (17.6). Three columns, which keep one, would gain or stay: [3, 9216, 320] 26.3
+    // (28.3), [3, 4096, 320] 17.0 (17.7), [3, 16384, 320] 43.7 both. Else: of one column [1, 16384, 320] 23.3 (19.2), of two [2, 131072,
     // 256] 113.8 (112.7); uneven [2, 6144, 960] 27.6 (25.4); fp32 [4, 4096, 320] 20.5 (19.3).
     if (call == kGnBackward && type != kGnF32 && columns >= 4) {
         auto rounds_of = [&](int64_t c) { return (columns * chunks_of(c) + kFirstTasks - 1) / kFirstTasks * c; };

@@ -942,7 +942,8 @@ def group_norm_i8(x, gamma, beta, groups: int, activation: str = "none", eps: fl
 
 def group_norm_workspace_bytes(batch: int, pixels: int, channels: int, groups: int, dtype: int = F16,
                                call: str = "forward") -> int:
-    """Workspace of group_norm ("forward"), group_norm_i8 ("i8") or group_norm_backward ("backward")."""
+    """Workspace of group_norm ("forward"), group_norm_i8 ("i8") or group_norm_backward ("backward") of tensors whose rows
+    are at most 2^20 elements apart."""
     desc = GroupNormDesc(batch=batch, pixels=pixels, channels=channels, groups=groups, dtype=dtype)
     lib = load()
     size = {"forward": lib.sdxl_group_norm_workspace_bytes, "i8": lib.sdxl_group_norm_i8_workspace_bytes,
@@ -1074,7 +1075,7 @@ def i8_kernels(desc: I8Desc, gated: bool) -> str:
 
 
 def linear_i8_workspace_bytes(M: int, N: int, K: int, gated: bool = False, dtype: int = F16) -> int:
-    """Workspace of linear_i8 / gated_linear_i8 with 16-bit tokens."""
+    """Workspace of linear_i8 / gated_linear_i8 with 16-bit tokens, of tensors whose rows are less than 2^20 elements apart."""
     desc = I8Desc(m=M, n=N, k=K, dtype=dtype, x_dtype=dtype)
     lib = load()
     return int((lib.sdxl_gated_linear_i8_workspace_bytes if gated else lib.sdxl_linear_i8_workspace_bytes)(ctypes.byref(desc)))
