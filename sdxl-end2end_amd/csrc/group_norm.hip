@@ -325,8 +325,8 @@ __global__ __launch_bounds__(kMaxThreads) void gn_apply_kernel(GnParams p) {
 
 // Codes by row. The row's lanes keep their channels' constants, of z as sdxl_group_norm forms it. (x a + (beta - mean a) is
 // off by 2^-24 of mean a: up to 0.03 for x = 1000 throughout and eps 1e-6, where z is beta.) Every workgroup merges the parts of all groups, so that eight waves
-// with a row each and a workgroup a CU beat four and two ([1, 16384, 320] fp16, both passes: 16.7 us and 20.8; [2, 1024,
-// 1280] 10.0 and 11.1; sixteen 16.1 and 12.1).
+// with a row each and a workgroup a CU beat four and two ([1, 16384, 320] fp16, both passes: 15.7 us and 18.0; [2, 1024,
+// 1280] 10.4 and 11.1; sixteen 15.1 and, out of registers, 29.2).
 template <typename T, FfFamily kFam, int kWaves, int kVecs>
 __global__ __launch_bounds__(kWaves == 1 ? 512 : 256) void gn_rows_kernel(GnParams p) {
     extern __shared__ __attribute__((aligned(16))) float2 stats[];
